@@ -88,6 +88,30 @@ int qmm_act_planes(int layout, int64_t k, int64_t rows, size_t *codes_off, size_
 int qmm_quantize_act(const float *x, void *xq, int layout, int64_t k, int64_t rows, int64_t stride,
                      int64_t stream);
 
+/* The values a quantized activation stands for, code * scale, as f32, f16 or
+ * bf16 (out_dtype: qmm_x_dtype; out rows k values apart): qmm_dequantize's
+ * counterpart for the planes. */
+int qmm_dequantize_act(const void *xq, int layout, void *out, int out_dtype, int64_t k, int64_t rows, int64_t stream);
+
+/* Residual addition and root-mean-square norm, the result quantized for the
+ * products that read it. Per row, with T the type of x, residual and h
+ * (dtype: qmm_x_dtype):
+ *   h  = T(x + residual)                    (x itself without a residual)
+ *   rs = f32(1 / sqrt(sum h^2 / k + eps))   (the sum in 64 bits)
+ *   y  = f32(f32(h * rs) * w)               (w: k f32 values)
+ * `h` (NULL: not kept) gets the stream, `xq` (NULL: none) the planes of y in
+ * `layout`, equal to qmm_quantize_act's of the f32 y bit for bit, and `y` (NULL:
+ * none; y_dtype) y itself, for what reads plain values (a router). One of xq
+ * and y is given. Strides are in values, at least k; k is a multiple of 4, and
+ * of the layout's block where xq is given. h may be x or residual itself (the
+ * same pointer and stride); otherwise nothing overlaps. A row's result does
+ * not depend on the other rows, nor on their number. One launch. Replaces the
+ * reference's add_rmsnorm (kernels/fused_decode.cu:47-240) and the
+ * quantization in front of its product. */
+int qmm_rms_norm_act(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t r_stride,
+                     const float *w, float eps, void *h, int64_t h_stride, void *xq, int layout, void *y, int y_dtype,
+                     int64_t y_stride, int64_t k, int64_t rows, int64_t stream);
+
 /* Largest `rows` qmm_matvec takes in one launch. */
 int qmm_matvec_max_rows(void);
 
@@ -238,6 +262,20 @@ int qmm_forward_shared(int type, int count, const void *const *w, const int64_t 
                        size_t workspace_bytes, size_t *need, int64_t k, int64_t rows, int launch,
                        int64_t stream);
 
+/* qmm_forward, qmm_forward_shared and (below) qmm_forward_glu from an
+ * activation already quantized in qmm_act_layout(type, rows)
+ * (qmm_rms_norm_act, qmm_quantize_act): the same kernels and, with the
+ * workspace that each plans, the same bits, without the quantizer's launch. The
+ * workspace holds the slots of a K split (and the GLU's two products); *need
+ * can be 0, and without room for the slots a product runs uncut, as
+ * qmm_matmul. xq is read only. Not affected by qmm_set_force_dmmv. */
+int qmm_forward_act(int type, const void *w, const void *xq, float *dst, int64_t ldd, void *workspace,
+                    size_t workspace_bytes, size_t *need, int64_t k, int64_t n, int64_t rows, int launch,
+                    int64_t stream);
+int qmm_forward_shared_act(int type, int count, const void *const *w, const int64_t *n, float *const *dst,
+                           const int64_t *ldd, const void *xq, void *workspace, size_t workspace_bytes, size_t *need,
+                           int64_t k, int64_t rows, int launch, int64_t stream);
+
 /* Gated activations of an MLP: act(gate) * up. */
 enum qmm_glu_act_id {
   QMM_GLU_SILU = 0,       /* gate / (1 + exp(-gate)) * up (fast_math.rs:48-60) */
@@ -261,6 +299,10 @@ enum qmm_glu_act_id {
 int qmm_forward_glu(int type, int act, const void *w_gate, const void *w_up, const float *x, int64_t x_stride,
                     float *dst, int64_t ldd, void *workspace, size_t workspace_bytes, size_t *need, int64_t k,
                     int64_t n, int64_t rows, int launch, int64_t stream);
+
+int qmm_forward_glu_act(int type, int act, const void *w_gate, const void *w_up, const void *xq, float *dst,
+                        int64_t ldd, void *workspace, size_t workspace_bytes, size_t *need, int64_t k, int64_t n,
+                        int64_t rows, int launch, int64_t stream);
 
 /* out[i] = act(gate[i]) * up[i] for n values (f32, on the device). Replaces
  * the reference's fused elementwise ops silu_mul / swiglu_oai_mul
@@ -322,6 +364,77 @@ int qmm_moe_forward_prefill(int type, const void *w, int num_experts, const void
                             const int32_t *sorted_ids, const int32_t *expert_ids, const float *topk_w, int topk,
                             float *dst, int64_t ldd, void *workspace, size_t workspace_bytes, size_t *need,
                             int64_t k, int64_t n, int64_t size_m, int launch, int64_t stream);
+
+/* ---- A paged key/value cache in Q8_0 and the attention over it ------------
+ * Four planes on the device, each 16-byte aligned, `pages` pages of `page`
+ * positions (16, 32, 64, 128 or 256) for kv_heads heads of head_dim values
+ * (64, 96, 128 or 256):
+ *   k_codes  int8 [pages][kv_heads][page][head_dim]
+ *   k_scales f16  [pages][kv_heads][page][head_dim / 32]
+ *   v_codes  int8 [pages][kv_heads][head_dim][page]
+ *   v_scales f16  [pages][kv_heads][head_dim / 32][page]
+ * 1.0625 bytes a value. Keys lie along head_dim and values along the
+ * positions, each along the axis that the attention contracts. Slot s is
+ * position s % page of page s / page; position p of a sequence lies in slot
+ * table[p / page] * page + p % page of its page table. The caller owns the planes and
+ * the tables; a page id outside [0, pages) names no page. */
+typedef struct qmm_cache {
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    int64_t pages;
+    int32_t kv_heads, head_dim, page;
+} qmm_cache;
+
+/* Bytes of a codes plane and of a scales plane (K's and V's alike);
+ * QMM_UNSUPPORTED for sizes not covered. */
+int qmm_cache_plane_bytes(int64_t pages, int kv_heads, int head_dim, int page, size_t *codes, size_t *scales);
+
+/* Quantizes the keys and values of `tokens` tokens into their slots (int64 on
+ * the device). Token t's head h starts at k + t * k_stride + h * k_head_stride
+ * (values of dtype: qmm_x_dtype; v likewise): slices of a fused product's rows
+ * are taken as they are. Per 32 values: the scale amax / 127 (amax over the
+ * finite ones, at most 65468.5: larger values saturate there, so that every
+ * cached value is a finite f16), codes clamp(round(v / scale), -127, 127), NaN
+ * as 0: the wire codec's block (qmm_wire_encode), the scale kept as f16. A slot outside the cache (a
+ * negative one: padding) writes nothing; slots are otherwise distinct, and no other
+ * position of the cache changes. Replaces kv_write_f16 (kernels/kv_append.cu:33). */
+int qmm_cache_write(const qmm_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v,
+                    int64_t v_stride, int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens,
+                    int64_t stream);
+
+/* The keys and values of `tokens` slots, code * scale rounded to out_dtype,
+ * into k and v [tokens][kv_heads][head_dim]. A slot outside the cache reads
+ * as zeros; a slot may be named twice. */
+int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens, void *k, void *v, int out_dtype,
+                   int64_t stream);
+
+/* Causal attention of the new tokens of `seqs` sequences over their cached
+ * positions, the new ones among them (write first, then attend). Sequence b's
+ * new tokens are rows [q_starts[b], q_starts[b + 1]) of q (int32, seqs + 1 of them), its
+ * cached positions 0 .. kv_lens[b] - 1 (int32), its pages the row b of tables
+ * (int32, table_stride apart). Its i-th new token stands at position
+ * pos = kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i and sees the positions j <= pos, with window > 0 those
+ * with j > pos - window only:
+ *   out[row][h] = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h])),
+ *   s_j = scale * q[row][h] . k_j
+ * of kv head h / (heads / kv_heads); without sinks (NULL) their term is
+ * missing. A row that sees no position (or whose pages all name none) is
+ * zero; a position on a page outside the cache counts as not there.
+ * q: [tokens][heads][head_dim], rows q_stride and heads q_head_stride values
+ * apart; out: rows out_stride values apart, heads head_dim. Rows of q that no
+ * sequence holds are left as they were in out. max_q and max_kv bound the sequences' new
+ * tokens and cached positions: the host plans by them (rows past max_q stay as they were, kv_lens is cut
+ * at max_kv and at the table's row). q is scaled and rounded to f16 (to
+ * nearest, saturating at 65504), as are the cache's values and the weights exp(s_j - max);
+ * sums are f32. Any mix of lengths is served by one call; the rows of a
+ * sequence do not depend on the other sequences' data. Plan (launch == 0) and launch as qmm_forward: the
+ * workspace joins the parts of a long context (*need can be 0). Replaces the
+ * reference's decode attention (kernels/decode_attn.cu:257-612) and its paged
+ * attention. */
+int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_stride, int64_t q_head_stride,
+               int64_t tokens, int heads, const int32_t *q_starts, const int32_t *kv_lens, const int32_t *tables,
+               int64_t table_stride, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int64_t window,
+               const float *sinks, void *out, int out_dtype, int64_t out_stride, void *workspace,
+               size_t workspace_bytes, size_t *need, int launch, int64_t stream);
 
 /* ---- GGUF files into device memory --------------------------------------
  * A parsed GGUF file: candle's gguf_file::Content::read

@@ -29,6 +29,16 @@ class QmmError(RuntimeError):
 
 _P, _I64, _I, _SZ, _U64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_uint64
 
+
+class Cache(ctypes.Structure):
+    """qmm_cache: the planes of a paged Q8_0 cache and its sizes."""
+
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("pages", _I64),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page", ctypes.c_int32)]
+
+
+_F, _SZP, _CP = ctypes.c_float, ctypes.POINTER(_SZ), ctypes.POINTER(Cache)
+
 # name -> (restype, argtypes); the exports of include/qmm.h
 SIGNATURES = {
     "qmm_available": (_I, []),
@@ -36,6 +46,17 @@ SIGNATURES = {
     "qmm_act_bytes": (_SZ, [_I, _I64, _I64]),
     "qmm_act_planes": (_I, [_I, _I64, _I64, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
     "qmm_quantize_act": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64]),
+    "qmm_dequantize_act": (_I, [_P, _I, _P, _I, _I64, _I64, _I64]),
+    "qmm_rms_norm_act": (_I, [_P, _I, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I, _P, _I, _I64, _I64, _I64, _I64]),
+    "qmm_forward_act": (_I, [_I, _P, _P, _P, _I64, _P, _SZ, _SZP, _I64, _I64, _I64, _I, _I64]),
+    "qmm_forward_shared_act": (_I, [_I, _I, ctypes.POINTER(_P), ctypes.POINTER(_I64), ctypes.POINTER(_P),
+                                    ctypes.POINTER(_I64), _P, _P, _SZ, _SZP, _I64, _I64, _I, _I64]),
+    "qmm_forward_glu_act": (_I, [_I, _I, _P, _P, _P, _P, _I64, _P, _SZ, _SZP, _I64, _I64, _I64, _I, _I64]),
+    "qmm_cache_plane_bytes": (_I, [_I64, _I, _I, _I, _SZP, _SZP]),
+    "qmm_cache_write": (_I, [_CP, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64]),
+    "qmm_cache_read": (_I, [_CP, _P, _I64, _P, _P, _I, _I64]),
+    "qmm_attend": (_I, [_CP, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _F, _I64, _P, _P, _I,
+                        _I64, _P, _SZ, _SZP, _I, _I64]),
     "qmm_matvec_max_rows": (_I, []),
     "qmm_mmq_few_rows_line": (_I, [_I, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
     "qmm_mmq_max_rows": (_I64, []),

@@ -13,6 +13,7 @@
 #include "../../include/qmm.h"
 #include "qmm_device.h"
 #include "qmm_launch.h"
+#include "value_types.h"
 
 namespace {
 
@@ -62,6 +63,23 @@ void clear_stale_error() { (void)hipGetLastError(); }
 bool shape_ok(int type, int64_t k, int64_t n, int64_t rows) {
   const int qk = block_size(type);
   return qk != 0 && k > 0 && k % qk == 0 && n > 0 && rows > 0 && k <= (int64_t)1 << 30 && n <= ((int64_t)1 << 31) - 1;
+}
+
+// A paged cache's sizes: pages of 16 to 256 positions (a power of two), heads
+// of a dim the attention kernels are built for, planes inside an int64.
+bool cache_shape_ok(int64_t pages, int kv_heads, int head_dim, int page) {
+  const bool hd = head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256;
+  return hd && page >= 16 && page <= 256 && (page & (page - 1)) == 0 && kv_heads >= 1 && kv_heads <= 65535 &&
+         pages >= 1 && pages <= INT32_MAX;
+}
+bool cache_ok(const qmm_cache* c) {
+  return c && cache_shape_ok(c->pages, c->kv_heads, c->head_dim, c->page) && c->k_codes && c->k_scales && c->v_codes &&
+         c->v_scales && ((uintptr_t)c->k_codes & 15) == 0 && ((uintptr_t)c->k_scales & 15) == 0 &&
+         ((uintptr_t)c->v_codes & 15) == 0 && ((uintptr_t)c->v_scales & 15) == 0;
+}
+qmm::CachePlanes planes_of(const qmm_cache& c) {
+  return qmm::CachePlanes{(int8_t*)c.k_codes, (uint16_t*)c.k_scales, (int8_t*)c.v_codes, (uint16_t*)c.v_scales,
+                          c.pages, c.kv_heads, c.head_dim, c.page};
 }
 
 // Compute units of the current device (256 on an MI355X), read once per device.
@@ -565,6 +583,26 @@ int qmm_quantize_act(const float* x, void* xq, int layout, int64_t k, int64_t ro
   return status_of(qmm::launch_act_quantize(layout, x, stride, k, rows, xq, q8k_scale(), (hipStream_t)stream));
 }
 
+int qmm_dequantize_act(const void* xq, int layout, void* out, int out_dtype, int64_t k, int64_t rows, int64_t stream) {
+  if (qmm_act_bytes(layout, k, rows) == 0 || !qmm::value_type_ok(out_dtype) || xq == nullptr || out == nullptr)
+    return QMM_UNSUPPORTED;
+  clear_stale_error();
+  return status_of(qmm::launch_dequantize_act(xq, layout, out, out_dtype, k, rows, (hipStream_t)stream));
+}
+
+int qmm_rms_norm_act(const void* x, int dtype, int64_t x_stride, const void* residual, int64_t r_stride, const float* w,
+                     float eps, void* h, int64_t h_stride, void* xq, int layout, void* y, int y_dtype,
+                     int64_t y_stride, int64_t k, int64_t rows, int64_t stream) {
+  if (!x || !w || !(xq || y) || !qmm::value_type_ok(dtype) || k < 1 || k > (int64_t)1 << 30 || rows < 1 ||
+      x_stride < k || (residual && r_stride < k) || (h && h_stride < k) || !(eps >= 0.0f))
+    return QMM_UNSUPPORTED;
+  if (xq && qmm_act_bytes(layout, k, rows) == 0) return QMM_UNSUPPORTED;
+  if (k % 4 != 0 || (y && (!qmm::value_type_ok(y_dtype) || y_stride < k))) return QMM_UNSUPPORTED;
+  clear_stale_error();
+  return status_of(qmm::launch_rms_norm_act(x, dtype, x_stride, residual, r_stride, w, eps, h, h_stride, xq, layout, y,
+                                            y_dtype, y_stride, k, rows, q8k_scale(), (hipStream_t)stream));
+}
+
 int qmm_matvec_max_rows(void) { return qmm::matvec_max_rows(); }
 
 void qmm_set_force_dmmv(int on) { g_force_dmmv.store(on != 0, std::memory_order_relaxed); }
@@ -676,39 +714,45 @@ int qmm_matmul(int type, const void* w, const void* xq, float* dst, int64_t ldd,
   return launch_product(type, w, n, k, xq, p, layout, rows, dst, ldd, (hipStream_t)stream);
 }
 
-int qmm_forward(int type, const void* w, const float* x, int64_t x_stride, float* dst, int64_t ldd, void* workspace,
-                size_t workspace_bytes, size_t* need, int64_t k, int64_t n, int64_t rows, int launch, int64_t stream) {
-  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || x_stride < k) return QMM_UNSUPPORTED;
+// qmm_forward (pre false: from the f32 activation x, quantized into the
+// workspace) and qmm_forward_act (pre: from the planes at xq, the workspace
+// holding a K split's slots only).
+static int forward_impl(int type, const void* w, bool pre, const void* xq, const float* x, int64_t x_stride, float* dst,
+                        int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k, int64_t n,
+                        int64_t rows, int launch, int64_t stream) {
+  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || (!pre && x_stride < k)) return QMM_UNSUPPORTED;
   const int layout = qmm_act_layout(type, rows);
-  const size_t bytes = qmm::act_bytes(layout, k, rows);
+  const size_t bytes = pre ? 0 : qmm::act_bytes(layout, k, rows);
+  const void* acts = pre ? xq : workspace;
   const hipStream_t st = (hipStream_t)stream;
   // a single-pass GEMM that leaves CUs idle is cut along K when the
   // workspace also holds its split slots (need reports them; with only the
   // activation's bytes it runs uncut)
-  const bool mid = mid_takes(type, w, workspace, n, k, rows);
+  const bool mid = mid_takes(type, w, acts, n, k, rows);
   const size_t split = mid ? qmm::gemm_kq_mid_slot_bytes(one_target(w, n, dst, ldd), k, rows, false)
-                       : sp_takes(type, w, workspace, n, k, rows, st)
+                       : sp_takes(type, w, acts, n, k, rows, st)
                            ? qmm::gemm_q4k_sp_split_bytes(one_target(w, n, dst, ldd), k, rows, (int)cu_count())
                            : 0;
   *need = split ? qmm::align_up(bytes, 256) + split : bytes;
   if (!launch) return QMM_OK;
   if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
-  if (workspace_bytes < bytes || workspace == nullptr) return QMM_WORKSPACE_TOO_SMALL;
-  if (!w || !x || !dst) return QMM_UNSUPPORTED;
+  if (!pre && (workspace_bytes < bytes || workspace == nullptr)) return QMM_WORKSPACE_TOO_SMALL;
+  if (!w || !(pre ? xq : x) || !dst) return QMM_UNSUPPORTED;
+  if (workspace == nullptr) workspace_bytes = 0;
   clear_stale_error();
-  if (g_force_dmmv.load(std::memory_order_relaxed))
+  if (!pre && g_force_dmmv.load(std::memory_order_relaxed))
     return status_of(qmm::launch_dmmv(type, w, n, k, x, x_stride, rows, dst, ldd, st));
-  if (stream_takes(type, k, n, 1, rows) && qmm::mv_q4k_rows_fusable(x, x_stride) &&
-      !matrix_takes(type, w, workspace, n, k, rows, st)) {
+  if (!pre && stream_takes(type, k, n, 1, rows) && qmm::mv_q4k_rows_fusable(x, x_stride) &&
+      !matrix_takes(type, w, acts, n, k, rows, st)) {
     // the activation is quantized inside the product's own launch
     const hipError_t e = launch_stream_targets(type, 1, &w, &n, &dst, &ldd, k, rows, x, x_stride, nullptr, st);
     if (e != hipSuccess) return QMM_DEVICE_ERROR;
     g_matvec_launches.fetch_add(1, std::memory_order_relaxed);
     return QMM_OK;
   }
-  if (qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
+  if (!pre && qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
     return QMM_DEVICE_ERROR;
-  const qmm::ActPlanes p = qmm::act_planes(layout, workspace, k, rows);
+  const qmm::ActPlanes p = qmm::act_planes(layout, (void*)acts, k, rows);
   if (mid && split && workspace_bytes >= *need) {
     if (launch_mid(type, one_target(w, n, dst, ldd), k, p, rows, (char*)workspace + qmm::align_up(bytes, 256), split,
                    nullptr, st) != hipSuccess)
@@ -718,7 +762,7 @@ int qmm_forward(int type, const void* w, const float* x, int64_t x_stride, float
   }
   // Q6_K takes the single-pass GEMM only cut as planned (uncut, a narrow
   // product runs faster on the exact kernel)
-  if (!mid && sp_takes(type, w, workspace, n, k, rows, st) &&
+  if (!mid && sp_takes(type, w, acts, n, k, rows, st) &&
       (type == qmm::T_Q4_K || split == 0 || workspace_bytes >= *need)) {
     const size_t off = qmm::align_up(bytes, 256);
     void* sws = workspace_bytes > off ? (char*)workspace + off : nullptr;
@@ -728,23 +772,38 @@ int qmm_forward(int type, const void* w, const float* x, int64_t x_stride, float
     g_gemm_launches.fetch_add(1, std::memory_order_relaxed);
     return QMM_OK;
   }
-  return launch_product(type, w, n, k, workspace, p, layout, rows, dst, ldd, st);
+  return launch_product(type, w, n, k, acts, p, layout, rows, dst, ldd, st);
 }
 
-int qmm_forward_shared(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
-                       const int64_t* ldd, const float* x, int64_t x_stride, void* workspace, size_t workspace_bytes,
-                       size_t* need, int64_t k, int64_t rows, int launch, int64_t stream) {
-  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || x_stride < k) return QMM_UNSUPPORTED;
+int qmm_forward(int type, const void* w, const float* x, int64_t x_stride, float* dst, int64_t ldd, void* workspace,
+                size_t workspace_bytes, size_t* need, int64_t k, int64_t n, int64_t rows, int launch, int64_t stream) {
+  return forward_impl(type, w, false, nullptr, x, x_stride, dst, ldd, workspace, workspace_bytes, need, k, n, rows,
+                      launch, stream);
+}
+
+int qmm_forward_act(int type, const void* w, const void* xq, float* dst, int64_t ldd, void* workspace,
+                    size_t workspace_bytes, size_t* need, int64_t k, int64_t n, int64_t rows, int launch,
+                    int64_t stream) {
+  return forward_impl(type, w, true, xq, nullptr, 0, dst, ldd, workspace, workspace_bytes, need, k, n, rows, launch,
+                      stream);
+}
+
+// qmm_forward_shared and qmm_forward_shared_act, as forward_impl.
+static int shared_impl(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
+                       const int64_t* ldd, bool pre, const void* xq, const float* x, int64_t x_stride, void* workspace,
+                       size_t workspace_bytes, size_t* need, int64_t k, int64_t rows, int launch, int64_t stream) {
+  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || (!pre && x_stride < k)) return QMM_UNSUPPORTED;
   for (int i = 0; i < count; i++)
     if (!shape_ok(type, k, n[i], rows) || ldd[i] < n[i]) return QMM_UNSUPPORTED;
   const int layout = qmm_act_layout(type, rows);
-  const size_t bytes = qmm::act_bytes(layout, k, rows);
+  const size_t bytes = pre ? 0 : qmm::act_bytes(layout, k, rows);
+  const void* acts = pre ? xq : workspace;
   const hipStream_t st = (hipStream_t)stream;
   // the short-batch kernel's weights share its launches, kMaxTargets each, and
   // so do those of the single-pass GEMM; their split slots follow the
   // activation (one launch's worth, reused launch after launch)
-  auto mid_i = [&](int i) { return mid_takes(type, w[i], workspace, n[i], k, rows); };
-  auto sp_i = [&](int i) { return !mid_i(i) && sp_takes(type, w[i], workspace, n[i], k, rows, st); };
+  auto mid_i = [&](int i) { return mid_takes(type, w[i], acts, n[i], k, rows); };
+  auto sp_i = [&](int i) { return !mid_i(i) && sp_takes(type, w[i], acts, n[i], k, rows, st); };
   size_t split = 0;
   qmm::MvTargets midg{}, spg{};
   for (int i = 0; i <= count; i++) {
@@ -766,11 +825,12 @@ int qmm_forward_shared(int type, int count, const void* const* w, const int64_t*
   *need = split ? qmm::align_up(bytes, 256) + split : bytes;
   if (!launch) return QMM_OK;
   if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
-  if (!x) return QMM_UNSUPPORTED;
+  if (!(pre ? xq : x)) return QMM_UNSUPPORTED;
   for (int i = 0; i < count; i++)
     if (!w[i] || !dst[i]) return QMM_UNSUPPORTED;
   clear_stale_error();
-  if (g_force_dmmv.load(std::memory_order_relaxed)) {
+  if (workspace == nullptr) workspace_bytes = 0;
+  if (!pre && g_force_dmmv.load(std::memory_order_relaxed)) {
     for (int i = 0; i < count; i++)
       if (qmm::launch_dmmv(type, w[i], n[i], k, x, x_stride, rows, dst[i], ldd[i], st) != hipSuccess)
         return QMM_DEVICE_ERROR;
@@ -779,28 +839,29 @@ int qmm_forward_shared(int type, int count, const void* const* w, const int64_t*
   int64_t n_total = 0;
   for (int i = 0; i < count; i++) n_total += n[i];
   const bool room = workspace != nullptr && workspace_bytes >= bytes;
-  bool fused = (room ? stream_takes(type, k, n_total, count, rows) : stream_supported(type, k, rows)) &&
-               qmm::mv_q4k_rows_fusable(x, x_stride);
-  for (int i = 0; fused && i < count; i++) fused = !matrix_takes(type, w[i], workspace, n[i], k, rows, st);
+  bool fused = pre ? stream_from_planes(type, k, rows)
+                   : (room ? stream_takes(type, k, n_total, count, rows) : stream_supported(type, k, rows)) &&
+                         qmm::mv_q4k_rows_fusable(x, x_stride);
+  for (int i = 0; fused && i < count; i++) fused = !matrix_takes(type, w[i], acts, n[i], k, rows, st);
+  const qmm::ActPlanes p = acts ? qmm::act_planes(layout, (void*)acts, k, rows) : qmm::ActPlanes{};
   if (fused) {
-    // one launch per kMaxTargets weights, each quantizing the activation in LDS
+    // one launch per kMaxTargets weights, each quantizing the activation in LDS (or reading its planes)
     for (int i0 = 0; i0 < count; i0 += qmm::kMaxTargets) {
       const int c = count - i0 < qmm::kMaxTargets ? count - i0 : qmm::kMaxTargets;
-      if (launch_stream_targets(type, c, w + i0, n + i0, dst + i0, ldd + i0, k, rows, x, x_stride, nullptr, st) !=
-          hipSuccess)
+      if (launch_stream_targets(type, c, w + i0, n + i0, dst + i0, ldd + i0, k, rows, x, x_stride,
+                                pre ? &p : nullptr, st) != hipSuccess)
         return QMM_DEVICE_ERROR;
       g_matvec_launches.fetch_add(1, std::memory_order_relaxed);
     }
     return QMM_OK;
   }
   // otherwise: the activation quantized once into the workspace, then each product
-  if (workspace_bytes < bytes || workspace == nullptr) return QMM_WORKSPACE_TOO_SMALL;
-  if (qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
+  if (!pre && (workspace_bytes < bytes || workspace == nullptr)) return QMM_WORKSPACE_TOO_SMALL;
+  if (!pre && qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
     return QMM_DEVICE_ERROR;
-  const qmm::ActPlanes p = qmm::act_planes(layout, workspace, k, rows);
   if (!is_kquant(type)) {
     bool gemm = true;
-    for (int i = 0; i < count; i++) gemm = gemm && gemm_takes(type, w[i], workspace, n[i], k, rows, st);
+    for (int i = 0; i < count; i++) gemm = gemm && gemm_takes(type, w[i], acts, n[i], k, rows, st);
     if (gemm) {
       for (int i0 = 0; i0 < count; i0 += qmm::kMaxTargets) {
         if (qmm::launch_gemm_b32(type, targets_of(w, n, dst, ldd, i0, count), k, p, rows, st) != hipSuccess)
@@ -837,33 +898,50 @@ int qmm_forward_shared(int type, int count, const void* const* w, const int64_t*
     } else if (!mid && (type == qmm::T_Q4_K || room_split) && sp_i(i)) {
       add_target(spg, w[i], n[i], dst[i], ldd[i]);
       if (spg.count == qmm::kMaxTargets && !flush(spg, sp_group)) return QMM_DEVICE_ERROR;
-    } else if (!mid && !gemm_takes(type, w[i], workspace, n[i], k, rows, st) &&
-               skinny_takes(type, w[i], workspace, n[i], k, rows, st)) {
+    } else if (!mid && !gemm_takes(type, w[i], acts, n[i], k, rows, st) &&
+               skinny_takes(type, w[i], acts, n[i], k, rows, st)) {
       add_target(grp, w[i], n[i], dst[i], ldd[i]);
       if (grp.count == qmm::kMaxTargets && !flush(grp, few_group)) return QMM_DEVICE_ERROR;
     } else {
-      const int r = launch_product(type, w[i], n[i], k, workspace, p, layout, rows, dst[i], ldd[i], st);
+      const int r = launch_product(type, w[i], n[i], k, acts, p, layout, rows, dst[i], ldd[i], st);
       if (r != QMM_OK) return r;
     }
   }
   return flush(midg, mid_group) && flush(spg, sp_group) && flush(grp, few_group) ? QMM_OK : QMM_DEVICE_ERROR;
 }
 
-int qmm_forward_glu(int type, int act, const void* w_gate, const void* w_up, const float* x, int64_t x_stride,
-                    float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k,
-                    int64_t n, int64_t rows, int launch, int64_t stream) {
+int qmm_forward_shared(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
+                       const int64_t* ldd, const float* x, int64_t x_stride, void* workspace, size_t workspace_bytes,
+                       size_t* need, int64_t k, int64_t rows, int launch, int64_t stream) {
+  return shared_impl(type, count, w, n, dst, ldd, false, nullptr, x, x_stride, workspace, workspace_bytes, need, k,
+                     rows, launch, stream);
+}
+
+int qmm_forward_shared_act(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
+                           const int64_t* ldd, const void* xq, void* workspace, size_t workspace_bytes, size_t* need,
+                           int64_t k, int64_t rows, int launch, int64_t stream) {
+  return shared_impl(type, count, w, n, dst, ldd, true, xq, nullptr, 0, workspace, workspace_bytes, need, k, rows,
+                     launch, stream);
+}
+
+// qmm_forward_glu and qmm_forward_glu_act, as forward_impl.
+static int glu_impl(int type, int act, const void* w_gate, const void* w_up, bool pre, const void* xq, const float* x,
+                    int64_t x_stride, float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need,
+                    int64_t k, int64_t n, int64_t rows, int launch, int64_t stream) {
   if (!shape_ok(type, k, n, rows) || act < QMM_GLU_SILU || act > QMM_GLU_GELU || need == nullptr || ldd < n ||
-      x_stride < k)
+      (!pre && x_stride < k))
     return QMM_UNSUPPORTED;
   // workspace: the quantized activation, then the gate and up products of
   // the two-launch form
   const int layout = qmm_act_layout(type, rows);
-  const size_t abytes = qmm::act_bytes(layout, k, rows);
+  const size_t abytes = pre ? 0 : qmm::act_bytes(layout, k, rows);
+  const void* acts = pre ? xq : workspace;
+  const bool dmmv = !pre && g_force_dmmv.load(std::memory_order_relaxed);
   const size_t obytes = qmm::align_up((size_t)(rows * n) * 4, 256);
   const size_t bytes = abytes + 2 * obytes;
   // in the short-batch kernel's range the GLU adds the products' K-split slots itself, when the
   // workspace holds them
-  const bool mid = mid_takes(type, w_gate, workspace, n, k, rows) && mid_takes(type, w_up, workspace, n, k, rows);
+  const bool mid = mid_takes(type, w_gate, acts, n, k, rows) && mid_takes(type, w_up, acts, n, k, rows);
   const void* w[2] = {w_gate, w_up};
   const int64_t ns[2] = {n, n};
   float* none[2] = {nullptr, nullptr};
@@ -872,24 +950,25 @@ int qmm_forward_glu(int type, int act, const void* w_gate, const void* w_up, con
   *need = aoff + slots > bytes ? aoff + slots : bytes;
   if (!launch) return QMM_OK;
   if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
-  if (!w_gate || !w_up || !x || !dst) return QMM_UNSUPPORTED;
+  if (!w_gate || !w_up || !(pre ? xq : x) || !dst) return QMM_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   clear_stale_error();
-  if (type == qmm::T_Q4_K && !g_force_dmmv.load(std::memory_order_relaxed) && qmm::mv_q4k_glu_supported(k, rows) &&
-      (stream_glu_takes(k, n, rows) || workspace == nullptr || workspace_bytes < bytes) &&
-      qmm::mv_q4k_rows_fusable(x, x_stride) &&
-      !matrix_takes(type, w_gate, workspace, n, k, rows, st) && !matrix_takes(type, w_up, workspace, n, k, rows, st)) {
-    if (qmm::launch_mv_q4k_glu(act, w_gate, w_up, n, k, rows, x, x_stride, nullptr, q8k_scale(), dst, ldd,
-                               cu_count(), st) != hipSuccess)
+  const qmm::ActPlanes p = acts ? qmm::act_planes(layout, (void*)acts, k, rows) : qmm::ActPlanes{};
+  if (type == qmm::T_Q4_K && !dmmv && qmm::mv_q4k_glu_supported(k, rows) &&
+      (pre ? stream_from_planes(type, k, rows)
+           : (stream_glu_takes(k, n, rows) || workspace == nullptr || workspace_bytes < bytes) &&
+                 qmm::mv_q4k_rows_fusable(x, x_stride)) &&
+      !matrix_takes(type, w_gate, acts, n, k, rows, st) && !matrix_takes(type, w_up, acts, n, k, rows, st)) {
+    if (qmm::launch_mv_q4k_glu(act, w_gate, w_up, n, k, rows, x, x_stride, pre ? &p : nullptr,
+                               q8k_scale(), dst, ldd, cu_count(), st) != hipSuccess)
       return QMM_DEVICE_ERROR;
     g_matvec_launches.fetch_add(1, std::memory_order_relaxed);
     return QMM_OK;
   }
   if (workspace_bytes < bytes || workspace == nullptr) return QMM_WORKSPACE_TOO_SMALL;
-  if (mid && workspace_bytes >= aoff + slots && !g_force_dmmv.load(std::memory_order_relaxed)) {
-    if (qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
+  if (mid && workspace_bytes >= aoff + slots && !dmmv) {
+    if (!pre && qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
       return QMM_DEVICE_ERROR;
-    const qmm::ActPlanes p = qmm::act_planes(layout, workspace, k, rows);
     float* parts[2];
     if (launch_mid(type, targets_of(w, ns, none, ns, 0, 2), k, p, rows, (char*)workspace + aoff, slots, parts, st) !=
         hipSuccess)
@@ -900,11 +979,10 @@ int qmm_forward_glu(int type, int act, const void* w_gate, const void* w_up, con
   }
   // the single-pass GEMM, neither weight cut (together they have twice a
   // weight's tiles): gate, up and the GLU in one launch
-  if (type == qmm::T_Q4_K && !g_force_dmmv.load(std::memory_order_relaxed) &&
-      sp_takes(type, w_gate, workspace, n, k, rows, st) && sp_takes(type, w_up, workspace, n, k, rows, st)) {
-    if (qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
+  if (type == qmm::T_Q4_K && !dmmv &&
+      sp_takes(type, w_gate, acts, n, k, rows, st) && sp_takes(type, w_up, acts, n, k, rows, st)) {
+    if (!pre && qmm::launch_act_quantize(layout, x, x_stride, k, rows, workspace, q8k_scale(), st) != hipSuccess)
       return QMM_DEVICE_ERROR;
-    const qmm::ActPlanes p = qmm::act_planes(layout, workspace, k, rows);
     if (qmm::launch_gemm_q4k_sp_glu(act, w_gate, w_up, n, k, p, rows, dst, ldd, st) != hipSuccess)
       return QMM_DEVICE_ERROR;
     g_gemm_launches.fetch_add(1, std::memory_order_relaxed);
@@ -914,10 +992,24 @@ int qmm_forward_glu(int type, int act, const void* w_gate, const void* w_up, con
   float* ubuf = (float*)((char*)gbuf + obytes);
   float* outs[2] = {gbuf, ubuf};
   size_t need2 = 0;
-  const int r = qmm_forward_shared(type, 2, w, ns, outs, ns, x, x_stride, workspace, abytes, &need2, k, rows, 1,
-                                   stream);
+  const int r = shared_impl(type, 2, w, ns, outs, ns, pre, xq, x, x_stride, workspace, abytes, &need2, k, rows, 1,
+                            stream);
   if (r != QMM_OK) return r;
   return status_of(qmm::launch_glu(act, gbuf, n, ubuf, n, dst, ldd, n, rows, st));
+}
+
+int qmm_forward_glu(int type, int act, const void* w_gate, const void* w_up, const float* x, int64_t x_stride,
+                    float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k,
+                    int64_t n, int64_t rows, int launch, int64_t stream) {
+  return glu_impl(type, act, w_gate, w_up, false, nullptr, x, x_stride, dst, ldd, workspace, workspace_bytes, need, k,
+                  n, rows, launch, stream);
+}
+
+int qmm_forward_glu_act(int type, int act, const void* w_gate, const void* w_up, const void* xq, float* dst,
+                        int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k, int64_t n,
+                        int64_t rows, int launch, int64_t stream) {
+  return glu_impl(type, act, w_gate, w_up, true, xq, nullptr, 0, dst, ldd, workspace, workspace_bytes, need, k, n,
+                  rows, launch, stream);
 }
 
 int qmm_glu(int act, const float* gate, const float* up, float* out, int64_t n, int64_t stream) {
@@ -943,6 +1035,68 @@ int qmm_quantize_weights(int type, const float* x, void* w, int64_t nelem, void*
   if (scratch_bytes < qmm::weight_quantize_scratch_bytes(type, nelem)) return QMM_WORKSPACE_TOO_SMALL;
   clear_stale_error();
   return status_of(qmm::launch_weight_quantize(type, x, w, nelem, scratch, (hipStream_t)stream));
+}
+
+int qmm_cache_plane_bytes(int64_t pages, int kv_heads, int head_dim, int page, size_t* codes, size_t* scales) {
+  if (!cache_shape_ok(pages, kv_heads, head_dim, page) || !codes || !scales) return QMM_UNSUPPORTED;
+  *codes = (size_t)pages * (size_t)page * (size_t)kv_heads * (size_t)head_dim;
+  *scales = *codes / 32 * 2;
+  return QMM_OK;
+}
+
+int qmm_cache_write(const qmm_cache* cache, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_stride, int64_t v_head_stride, int dtype, const int64_t* slots, int64_t tokens,
+                    int64_t stream) {
+  if (!cache_ok(cache) || !qmm::value_type_ok(dtype) || tokens < 0 || k_head_stride < cache->head_dim ||
+      v_head_stride < cache->head_dim || k_stride < 0 || v_stride < 0)
+    return QMM_UNSUPPORTED;
+  if (tokens == 0) return QMM_OK;
+  if (!k || !v || !slots) return QMM_UNSUPPORTED;
+  clear_stale_error();
+  return status_of(qmm::launch_cache_write(planes_of(*cache), k, v, dtype, k_stride, k_head_stride, v_stride,
+                                           v_head_stride, slots, tokens, (hipStream_t)stream));
+}
+
+int qmm_cache_read(const qmm_cache* cache, const int64_t* slots, int64_t tokens, void* k, void* v, int out_dtype,
+                   int64_t stream) {
+  if (!cache_ok(cache) || !qmm::value_type_ok(out_dtype) || tokens < 0) return QMM_UNSUPPORTED;
+  if (tokens == 0) return QMM_OK;
+  if (!k || !v || !slots) return QMM_UNSUPPORTED;
+  clear_stale_error();
+  return status_of(
+      qmm::launch_cache_read(planes_of(*cache), slots, tokens, k, v, out_dtype, (hipStream_t)stream));
+}
+
+int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_stride, int64_t q_head_stride,
+               int64_t tokens, int heads, const int32_t* q_starts, const int32_t* kv_lens, const int32_t* tables,
+               int64_t table_stride, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int64_t window,
+               const float* sinks, void* out, int out_dtype, int64_t out_stride, void* workspace,
+               size_t workspace_bytes, size_t* need, int launch, int64_t stream) {
+  if (!cache_ok(cache) || need == nullptr || !qmm::value_type_ok(q_dtype) || !qmm::value_type_ok(out_dtype) ||
+      heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || tokens < 0 || seqs < 0 || seqs > 65535 ||
+      max_q < 0 || max_kv < 0 || table_stride < 0 || window < 0 || q_head_stride < cache->head_dim || q_stride < 0 ||
+      out_stride < (int64_t)heads * cache->head_dim || max_q > INT32_MAX || scale != scale)
+    return QMM_UNSUPPORTED;
+  *need = 0;
+  if (tokens == 0 || seqs == 0 || max_q == 0) return QMM_OK;
+  qmm::AttendArgs a{};
+  a.c = planes_of(*cache);
+  a.q = q; a.out = out; a.q_starts = q_starts; a.kv_lens = kv_lens; a.tables = tables; a.sinks = sinks;
+  a.qs = q_stride; a.qhs = q_head_stride; a.os = out_stride; a.table_stride = table_stride; a.tokens = tokens;
+  a.window = window;
+  a.seqs = (int)seqs; a.heads = heads; a.group = heads / cache->kv_heads;
+  a.max_q = (int)(max_q < tokens ? max_q : tokens);
+  // a sequence's positions lie inside its row of the table
+  const int64_t cap = table_stride > INT32_MAX / cache->page ? INT32_MAX / cache->page * cache->page
+                                                             : table_stride * cache->page;
+  a.max_kv = (int)(max_kv < cap ? max_kv : cap);
+  a.qdt = q_dtype; a.odt = out_dtype; a.scale = scale;
+  *need = qmm::attend_workspace_bytes(a, cu_count());
+  if (!launch) return QMM_OK;
+  if (!q || !out || !q_starts || !kv_lens || (!tables && a.max_kv > 0)) return QMM_UNSUPPORTED;
+  if (*need > 0 && (workspace == nullptr || workspace_bytes < *need)) return QMM_WORKSPACE_TOO_SMALL;
+  clear_stale_error();
+  return status_of(qmm::launch_attend(a, cu_count(), workspace, (hipStream_t)stream));
 }
 
 int qmm_moe_forward(int type, const void* w, int num_experts, const float* x, int64_t x_stride,

@@ -263,6 +263,47 @@ bool gemm_q6k_fits(int64_t n, int64_t k, int64_t rows);
 hipError_t launch_gemm_q6k(const void* w, int64_t n, int64_t k, const ActPlanes& p, int64_t rows, float* dst,
                            int64_t ldd, hipStream_t s);
 
+// Residual addition + root-mean-square norm into the planes of `layout` (xq;
+// null: none), the stream h (null: none) and the normed values y (null:
+// none); and such planes read back (norm.hip). Types: qmm_x_dtype.
+hipError_t launch_rms_norm_act(const void* x, int dtype, int64_t xs, const void* r, int64_t rs, const float* w,
+                               float eps, void* h, int64_t hs, void* xq, int layout, void* y, int ydt, int64_t ys,
+                               int64_t k, int64_t rows, float qmax, hipStream_t st);
+hipError_t launch_dequantize_act(const void* xq, int layout, void* out, int odt, int64_t k, int64_t rows,
+                                 hipStream_t st);
+
+// The paged Q8_0 cache (kv_cache.hip): its planes, writes and reads of slots.
+struct CachePlanes {
+  int8_t* k_codes;
+  uint16_t* k_scales;
+  int8_t* v_codes;
+  uint16_t* v_scales;
+  int64_t pages;
+  int heads, hd, page;
+};
+hipError_t launch_cache_write(const CachePlanes& c, const void* k, const void* v, int dtype, int64_t ks, int64_t khs,
+                              int64_t vs, int64_t vhs, const int64_t* slots, int64_t tokens, hipStream_t st);
+hipError_t launch_cache_read(const CachePlanes& c, const int64_t* slots, int64_t tokens, void* k, void* v, int odt,
+                             hipStream_t st);
+
+// Attention over it (attend.hip). Rows of q and out are qs and os values
+// apart; a q row's heads qhs apart, an out row's hd. `group` query heads
+// share a kv head. window 0: none; sinks null: none.
+struct AttendArgs {
+  CachePlanes c;
+  const void* q;
+  void* out;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  const int32_t* tables;
+  const float* sinks;
+  int64_t qs, qhs, os, table_stride, tokens, window;
+  int seqs, heads, group, max_q, max_kv, qdt, odt;
+  float scale;
+};
+size_t attend_workspace_bytes(const AttendArgs& a, int cus);
+hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st);
+
 // Set-up a first launch would otherwise do (qmm_prepare): the LDS limit of
 // every kernel that asks for more than 64 KiB, on the current device, and
 // the no-allocation scratch's address there.

@@ -1,0 +1,189 @@
+"""A paged key/value cache in Q8_0 and the attention over it (qmm_cache_* and
+qmm_attend): what stands between a decoder layer's q/k/v and o products. The
+reference appends f16 (kernels/kv_append.cu:33) and attends over it with
+kernels/decode_attn.cu:257-612 and its paged attention.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import Cache, QmmError, check, lib
+from .qtensor import _X_DTYPES, on_device
+
+
+class KvCache:
+    """Pages of `page` positions for kv_heads heads of head_dim values, keys
+    and values quantized per 32 values of a head (an f16 scale, 8-bit codes):
+
+      k_codes int8 [pages, kv_heads, page, head_dim], k_scales f16 [.., page, head_dim / 32]
+      v_codes int8 [pages, kv_heads, head_dim, page], v_scales f16 [.., head_dim / 32, page]
+
+    Position p of a sequence lies in slot table[p // page] * page + p % page
+    of its page table. Which pages a sequence has is the caller's to keep."""
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+        if k_codes.dim() != 4:
+            raise ValueError(f"KvCache: k_codes [pages, kv_heads, page, head_dim], not {tuple(k_codes.shape)}")
+        pages, heads, page, hd = k_codes.shape
+        for name, t, shape, dt in (("k_codes", k_codes, (pages, heads, page, hd), torch.int8),
+                                   ("k_scales", k_scales, (pages, heads, page, hd // 32), torch.float16),
+                                   ("v_codes", v_codes, (pages, heads, hd, page), torch.int8),
+                                   ("v_scales", v_scales, (pages, heads, hd // 32, page), torch.float16)):
+            if t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda \
+                    or t.device != k_codes.device or t.data_ptr() % 16:
+                raise ValueError(f"KvCache: {name} must be contiguous, 16-byte aligned {dt} {shape} on one GPU, not "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        _plane_bytes(pages, heads, hd, page)
+        self.planes = (k_codes, k_scales, v_codes, v_scales)
+        self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, hd
+        self.device = k_codes.device
+        self._c = Cache(*(t.data_ptr() for t in self.planes), pages, heads, hd, page)
+        self._ref = ctypes.byref(self._c)
+
+    @staticmethod
+    def alloc(pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> "KvCache":
+        """A cache of zeros: head_dim 64, 96, 128 or 256, page 16 to 256 (a power of two)."""
+        _plane_bytes(pages, kv_heads, head_dim, page)
+        return KvCache(torch.zeros((pages, kv_heads, page, head_dim), dtype=torch.int8, device=device),
+                       torch.zeros((pages, kv_heads, page, head_dim // 32), dtype=torch.float16, device=device),
+                       torch.zeros((pages, kv_heads, head_dim, page), dtype=torch.int8, device=device),
+                       torch.zeros((pages, kv_heads, head_dim // 32, page), dtype=torch.float16, device=device))
+
+    def slots(self, table: torch.Tensor, start: int, count: int) -> torch.Tensor:
+        """The slots (int64) of positions start .. start + count - 1 of the sequence with this page table (1-D)."""
+        p = torch.arange(start, start + count, device=table.device)
+        return table.long()[p // self.page] * self.page + p % self.page
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Quantizes keys and values [tokens, kv_heads, head_dim] (f32, f16 or
+        bf16; the last axis contiguous, the others any distance apart) into
+        `slots` (int64 [tokens]). A negative slot, or one past the cache,
+        writes nothing; the others are distinct."""
+        tokens = slots.numel()
+        self._slots("write", slots)
+        for name, t in (("k", k), ("v", v)):
+            if tuple(t.shape) != (tokens, self.kv_heads, self.head_dim) or t.dtype not in _X_DTYPES \
+                    or t.dtype != k.dtype or t.device != self.device:
+                raise ValueError(f"KvCache.write: {name} [{tokens}, {self.kv_heads}, {self.head_dim}] f32, f16 or bf16 "
+                                 f"on {self.device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+        if tokens == 0:
+            return
+        ks, khs = self._strides("write", "k", k)
+        vs, vhs = self._strides("write", "v", v)
+        with on_device(self.device):
+            check("qmm_cache_write", lib().qmm_cache_write(self._ref, k.data_ptr(), ks, khs, v.data_ptr(), vs, vhs,
+                                                           _X_DTYPES[k.dtype], slots.data_ptr(), tokens,
+                                                           torch.cuda.current_stream().cuda_stream))
+
+    def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values [tokens, kv_heads, head_dim] of `slots` (int64
+        [tokens]) as f16, bf16 or f32; zeros for a slot outside the cache."""
+        self._slots("read", slots)
+        if dtype not in _X_DTYPES:
+            raise ValueError(f"KvCache.read: f32, f16 or bf16, not {dtype}")
+        tokens = slots.numel()
+        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        if tokens:
+            with on_device(self.device):
+                check("qmm_cache_read", lib().qmm_cache_read(self._ref, slots.data_ptr(), tokens, k.data_ptr(),
+                                                             v.data_ptr(), _X_DTYPES[dtype],
+                                                             torch.cuda.current_stream().cuda_stream))
+        return k, v
+
+    def attend(self, q: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor, tables: torch.Tensor,
+               max_q: int, max_kv: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
+               sinks: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """Causal attention of the new tokens q [tokens, heads, head_dim] (f16,
+        bf16 or f32) over the cached positions of their sequences, the new ones
+        among them (write them first). Sequence b's new tokens are rows
+        q_starts[b] .. q_starts[b + 1] - 1, the last of its kv_lens[b] cached
+        positions; tables [seqs, pages a sequence] names its pages (all int32).
+        max_q and max_kv: at least the most new tokens and cached positions of
+        a sequence (max_kv: by default what a row of tables holds); they choose
+        the launch and cut what is longer. scale: by default head_dim ** -0.5.
+        window > 0: a token sees the last `window` positions, its own among
+        them. sinks [heads] f32: a term exp(sink) in each softmax's sum. Rows
+        of q that belong to no sequence are left as they were in `out` (as
+        torch.empty gives them without one). The products run on f16 operands
+        with f32 sums: an f32 q is rounded to f16, as is a bf16 one."""
+        if q.dim() != 3 or q.dtype not in _X_DTYPES or q.device != self.device or q.shape[2] != self.head_dim \
+                or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+            raise ValueError(f"KvCache.attend: q [tokens, a multiple of {self.kv_heads} heads, {self.head_dim}] f16, "
+                             f"bf16 or f32 on {self.device}, not {q.dtype} {tuple(q.shape)} on {q.device}")
+        tokens, heads, hd = q.shape
+        seqs = kv_lens.numel()
+        for name, t, shape in (("q_starts", q_starts, (seqs + 1,)), ("kv_lens", kv_lens, (seqs,))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"KvCache.attend: {name} must be contiguous int32 {shape} on {self.device}, not "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != seqs or tables.device != self.device \
+                or not tables.is_contiguous():
+            raise ValueError(f"KvCache.attend: tables must be contiguous int32 [{seqs}, pages] on {self.device}, not "
+                             f"{tables.dtype} {tuple(tables.shape)} on {tables.device}")
+        if max_q < 0 or window < 0 or (max_kv is not None and max_kv < 0):
+            raise ValueError(f"KvCache.attend: max_q {max_q}, max_kv {max_kv}, window {window}")
+        if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (heads,)
+                                  or sinks.device != self.device or not sinks.is_contiguous()):
+            raise ValueError(f"KvCache.attend: sinks must be {heads} contiguous f32 on {self.device}")
+        if out is None:
+            out = torch.empty((tokens, heads, hd), dtype=out_dtype or q.dtype, device=self.device)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"KvCache.attend: out is {out.dtype}, not {out_dtype}")
+        if tuple(out.shape) != (tokens, heads, hd) or out.dtype not in _X_DTYPES or out.device != self.device \
+                or (tokens and (out.stride(2) != 1 or out.stride(1) != hd)) or (tokens > 1 and out.stride(0) < heads * hd):
+            raise ValueError(f"KvCache.attend: out [{tokens}, {heads}, {hd}] f16, bf16 or f32, rows of consecutive "
+                             f"values, not {out.dtype} {tuple(out.shape)} strides {out.stride()}")
+        if tokens == 0 or seqs == 0:
+            return out
+        qs, qhs = self._strides("attend", "q", q)
+        L, need = lib(), ctypes.c_size_t(0)
+        head = (self._ref, q.data_ptr(), _X_DTYPES[q.dtype], qs, qhs, tokens, heads, q_starts.data_ptr(),
+                kv_lens.data_ptr(), tables.data_ptr(), tables.shape[1], seqs, max_q,
+                tables.shape[1] * self.page if max_kv is None else max_kv, hd ** -0.5 if scale is None else scale,
+                window, sinks.data_ptr() if sinks is not None else None, out.data_ptr(), _X_DTYPES[out.dtype],
+                out.stride(0) if tokens > 1 else heads * hd)
+        with on_device(self.device):
+            st = torch.cuda.current_stream().cuda_stream
+            check("qmm_attend", L.qmm_attend(*head, None, 0, ctypes.byref(need), 0, st))
+            # a buffer a call: stream-ordered, and under capture the graph's own
+            ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
+            check("qmm_attend", L.qmm_attend(*head, ws.data_ptr() if ws is not None else None, need.value,
+                                             ctypes.byref(need), 1, st))
+        return out
+
+    def _slots(self, name: str, slots: torch.Tensor) -> None:
+        if slots.dtype != torch.int64 or slots.dim() != 1 or slots.device != self.device or not slots.is_contiguous():
+            raise ValueError(f"KvCache.{name}: slots must be contiguous int64 [tokens] on {self.device}, not "
+                             f"{slots.dtype} {tuple(slots.shape)} on {slots.device}")
+
+    def _strides(self, name: str, what: str, t: torch.Tensor) -> Tuple[int, int]:
+        """Distances of the tokens and heads of t [tokens, heads, head_dim]."""
+        ts, hs, ds = t.stride()
+        if t.shape[0] <= 1:
+            ts = t.shape[1] * self.head_dim
+        if t.shape[1] <= 1:
+            hs = self.head_dim
+        if ds != 1 or hs < self.head_dim or ts < 0:
+            raise ValueError(f"KvCache.{name}: {what} needs heads of {self.head_dim} consecutive values, not strides "
+                             f"{t.stride()}")
+        return ts, hs
+
+    def __repr__(self) -> str:
+        return f"KvCache[{self.pages} pages of {self.page}, {self.kv_heads} heads of {self.head_dim}; Q8_0]"
+
+
+def _plane_bytes(pages: int, kv_heads: int, head_dim: int, page: int) -> Tuple[int, int]:
+    """Bytes of a codes and of a scales plane; ValueError for sizes not covered."""
+    codes, scales = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    try:
+        check("qmm_cache_plane_bytes", lib().qmm_cache_plane_bytes(pages, kv_heads, head_dim, page,
+                                                                   ctypes.byref(codes), ctypes.byref(scales)))
+    except QmmError:
+        raise ValueError(f"KvCache: {pages} pages of {page} for {kv_heads} heads of {head_dim}: pages of 16 to 256 "
+                         "positions (a power of two), heads of 64, 96, 128 or 256 values") from None
+    return codes.value, scales.value

@@ -16,8 +16,9 @@ import ctypes
 import enum
 import os
 import warnings
+from contextlib import nullcontext
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -55,6 +56,11 @@ def _stream() -> int:
 
 def _ptr(t: torch.Tensor) -> int:
     return t.data_ptr()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one (no switch where it is already)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def fill_normal(n: int, seed: int, mean: float = 0.0, std: float = 1.0, device="cuda") -> torch.Tensor:
@@ -309,6 +315,96 @@ class QTensor:
         return f"QTensor[{list(self.shape)}; {self.dtype.name}]"
 
 
+class QAct:
+    """An activation [..., k] quantized for the products that read it: the
+    planes of qmm_act_planes (codes, scales, sums) in one device buffer, as
+    rms_norm_act and QAct.quantize make them. QMatMul.forward, forward_shared
+    and forward_glu take one in place of the f32 activation where the layout
+    is their weight type's (QAct.layout_of)."""
+
+    def __init__(self, data: torch.Tensor, shape: Sequence[int], layout: int):
+        shape = tuple(int(d) for d in shape)
+        if len(shape) < 1 or layout not in (_lib.ACT_Q8K, _lib.ACT_Q8_0):
+            raise ValueError(f"QAct: shape {shape}, layout {layout}")
+        self.k = shape[-1]
+        self.rows = 1
+        for d in shape[:-1]:
+            self.rows *= d
+        want = lib().qmm_act_bytes(layout, self.k, self.rows) if self.rows else 0
+        if (self.rows and want == 0) or data.dtype != torch.uint8 or data.numel() < want or not data.is_cuda \
+                or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"QAct: {data.numel()} {data.dtype} device bytes for {list(shape)} (want {want}, 16-byte "
+                             "aligned)")
+        self.data_ = data
+        self.shape = shape
+        self.layout = layout
+
+    @staticmethod
+    def layout_of(dtype: GgmlDType) -> int:
+        """The layout that products of a weight type read (qmm_act_layout)."""
+        layout = lib().qmm_act_layout(int(GgmlDType(dtype)), 1)
+        if layout < 0:
+            raise ValueError(f"no quantized activation for {GgmlDType(dtype).name} weights")
+        return layout
+
+    @staticmethod
+    def alloc(shape: Sequence[int], layout: int, device="cuda") -> "QAct":
+        rows = 1
+        for d in shape[:-1]:
+            rows *= int(d)
+        nbytes = lib().qmm_act_bytes(layout, int(shape[-1]), rows) if rows else 0
+        if rows and nbytes == 0:
+            raise ValueError(f"QAct.alloc: rows of {shape[-1]} values are not a whole number of blocks")
+        return QAct(torch.empty(nbytes, dtype=torch.uint8, device=device), shape, layout)
+
+    @staticmethod
+    def quantize(x: torch.Tensor, dtype: GgmlDType) -> "QAct":
+        """x [..., k] f32 as the products of `dtype` weights quantize it (qmm_quantize_act)."""
+        if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous() or x.dim() < 1:
+            raise ValueError("QAct.quantize: a contiguous f32 tensor on the GPU")
+        with on_device(x.device):
+            out = QAct.alloc(x.shape, QAct.layout_of(dtype), x.device)
+            if out.rows:
+                check("qmm_quantize_act", lib().qmm_quantize_act(_ptr(x), _ptr(out.data_), out.layout, out.k, out.rows,
+                                                                 out.k, _stream()))
+        return out
+
+    def planes(self):
+        """(codes int8 [rows, k], scales f32, sums) views (act_planes)."""
+        return act_planes(self.data_, self.layout, self.k, self.rows)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values it stands for, code * scale (qmm_dequantize_act), as f32, f16 or bf16."""
+        if dtype not in _X_DTYPES:
+            raise ValueError(f"QAct.dequantize: f32, f16 or bf16, not {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.data_.device)
+        if out.numel():
+            with on_device(out.device):
+                check("qmm_dequantize_act", lib().qmm_dequantize_act(_ptr(self.data_), self.layout, _ptr(out),
+                                                                     _X_DTYPES[dtype], self.k, self.rows, _stream()))
+        return out
+
+    def dequantize_f16(self) -> torch.Tensor:
+        return self.dequantize(torch.float16)
+
+    def __repr__(self) -> str:
+        return f"QAct[{list(self.shape)}; {'Q8_K' if self.layout == _lib.ACT_Q8K else 'Q8_0'}]"
+
+
+def _check_act(name: str, act: QAct, w: "QTensor") -> None:
+    if len(w.shape) != 2 or act.k != w.shape[1]:
+        raise ValueError(f"{name}: activation {act.shape} incompatible with {w.shape}")
+    if act.layout != QAct.layout_of(w.dtype):
+        raise ValueError(f"{name}: {act!r} is not the layout that {w.dtype.name} products read")
+    if act.data_.device != w.data_.device:
+        raise ValueError(f"{name}: activation on {act.data_.device}, weight on {w.data_.device}")
+
+
+def _act_workspace(need: int, device) -> torch.Tensor:
+    # a buffer a call: stream-ordered, and under capture the graph's own
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+
+
 @dataclass
 class Workspace:
     """The device buffers the products of one weight quantize their activation
@@ -397,8 +493,11 @@ class QMatMul:
         """QMatMul::indexed_moe_forward (mod.rs:1265-1272): QTensor.indexed_moe_forward."""
         return self.qtensor.indexed_moe_forward(x, ids)
 
-    def forward(self, xs: torch.Tensor) -> torch.Tensor:
-        """x [..., k] f32 -> [..., n]; the CustomOp1 shape rules of cpu_fwd (mod.rs:1280-1333)."""
+    def forward(self, xs: Union[torch.Tensor, QAct]) -> torch.Tensor:
+        """x [..., k] f32 -> [..., n]; the CustomOp1 shape rules of cpu_fwd (mod.rs:1280-1333).
+        A QAct in place of x skips the quantizer (qmm_forward_act), with the same bits."""
+        if isinstance(xs, QAct):
+            return self._forward_act(xs)
         if len(self.qtensor.shape) != 2:
             raise ValueError(f"QMatMul::forward: a [n, k] weight, not {self.qtensor.shape}")
         n, k = self.qtensor.shape
@@ -425,11 +524,58 @@ class QMatMul:
 
     __call__ = forward
 
+    def _forward_act(self, act: QAct) -> torch.Tensor:
+        _check_act("QMatMul::forward", act, self.qtensor)
+        n, k = self.qtensor.shape
+        out = torch.empty((*act.shape[:-1], n), dtype=torch.float32, device=act.data_.device)
+        if act.rows == 0:
+            return out
+        L, t, need = lib(), int(self.qtensor.dtype), ctypes.c_size_t(0)
+        with on_device(out.device):
+            st = _stream()
+            head = (t, _ptr(self.qtensor.data_), _ptr(act.data_), _ptr(out), n)
+            check("qmm_forward_act", L.qmm_forward_act(*head, None, 0, ctypes.byref(need), k, n, act.rows, 0, st))
+            buf = _act_workspace(need.value, out.device)
+            check("qmm_forward_act", L.qmm_forward_act(*head, _ptr(buf), need.value, ctypes.byref(need), k, n, act.rows,
+                                                       1, st))
+        return out
+
     @staticmethod
-    def forward_shared(xs: torch.Tensor, ws: Sequence["QMatMul"]) -> List[torch.Tensor]:
+    def _forward_shared_act(act: QAct, ws: Sequence["QMatMul"]) -> List[torch.Tensor]:
+        for w in ws:
+            _check_act("forward_shared", act, w.qtensor)
+        outs = [torch.empty((*act.shape[:-1], w.qtensor.shape[0]), dtype=torch.float32, device=act.data_.device)
+                for w in ws]
+        if act.rows == 0:
+            return outs
+        L, k = lib(), act.k
+        by_type = {}
+        for i, w in enumerate(ws):
+            by_type.setdefault(int(w.qtensor.dtype), []).append(i)
+        with on_device(act.data_.device):
+            st = _stream()
+            for t, idx in by_type.items():
+                cnt = len(idx)
+                wp = (ctypes.c_void_p * cnt)(*[ws[i].qtensor.data_.data_ptr() for i in idx])
+                ns = (ctypes.c_int64 * cnt)(*[ws[i].qtensor.shape[0] for i in idx])
+                dp = (ctypes.c_void_p * cnt)(*[outs[i].data_ptr() for i in idx])
+                need = ctypes.c_size_t(0)
+                head = (t, cnt, wp, ns, dp, ns, _ptr(act.data_))
+                check("qmm_forward_shared_act", L.qmm_forward_shared_act(*head, None, 0, ctypes.byref(need), k,
+                                                                         act.rows, 0, st))
+                buf = _act_workspace(need.value, act.data_.device)
+                check("qmm_forward_shared_act", L.qmm_forward_shared_act(*head, _ptr(buf), need.value,
+                                                                         ctypes.byref(need), k, act.rows, 1, st))
+        return outs
+
+    @staticmethod
+    def forward_shared(xs: Union[torch.Tensor, QAct], ws: Sequence["QMatMul"]) -> List[torch.Tensor]:
         """Several weights against ONE activation, quantized once for all of
         them (mod.rs:1221-1263): one qmm_forward_shared call per group of
-        weights of the same type; a single weight is a plain forward."""
+        weights of the same type; a single weight is a plain forward. A QAct in
+        place of xs is read as it is (every weight's type of its layout)."""
+        if isinstance(xs, QAct):
+            return QMatMul._forward_shared_act(xs, ws)
         if len(ws) <= 1:
             return [w.forward(xs) for w in ws]
         k = ws[0].qtensor.shape[1]
@@ -470,19 +616,22 @@ class QMatMul:
 ACTIVATIONS = {"silu": _lib.GLU_SILU, "swiglu_oai": _lib.GLU_SWIGLU_OAI, "gelu": _lib.GLU_GELU}
 
 
-def forward_glu(xs: torch.Tensor, gate: "QMatMul", up: "QMatMul", activation: str = "silu") -> torch.Tensor:
+def forward_glu(xs: Union[torch.Tensor, QAct], gate: "QMatMul", up: "QMatMul", activation: str = "silu") -> torch.Tensor:
     """act(xs · gateᵀ) * (xs · upᵀ): the gate and up products of an MLP sharing
     one quantized activation and the gated activation between them, written
     once (qmm_forward_glu: one launch for Q4_K at 1-2 rows, long weight rows
     at 2 rows aside, and for its prompts past 128 rows; otherwise the shared
     products and the elementwise GLU). The reference's forward_block
     (src/inference/layers/mod.rs:583-632): forward_shared of ffn_up and
-    ffn_gate, then silu_mul / swiglu_oai_mul / gelu(gate) * up."""
+    ffn_gate, then silu_mul / swiglu_oai_mul / gelu(gate) * up. A QAct in place
+    of xs is read as it is (qmm_forward_glu_act)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
     gq, uq = gate.qtensor, up.qtensor
     if gq.shape != uq.shape or gq.dtype != uq.dtype:
         raise ValueError("forward_glu: gate and up must have one shape and type")
+    if isinstance(xs, QAct):
+        return _forward_glu_act(xs, gq, uq, ACTIVATIONS[activation])
     n, k = gq.shape
     if xs.dim() < 1 or xs.shape[-1] != k:
         raise ValueError(f"input tensor {tuple(xs.shape)} incompatible with k={k}")
@@ -504,6 +653,24 @@ def forward_glu(xs: torch.Tensor, gate: "QMatMul", up: "QMatMul", activation: st
     check("qmm_forward_glu", L.qmm_forward_glu(t, act, gq.data_.data_ptr(), uq.data_.data_ptr(), _ptr(xs), k,
                                                _ptr(out), n, _ptr(buf), buf.numel(), ctypes.byref(need), k, n, rows,
                                                1, st))
+    return out
+
+
+def _forward_glu_act(act: QAct, gq: QTensor, uq: QTensor, activation: int) -> torch.Tensor:
+    _check_act("forward_glu", act, gq)
+    _check_act("forward_glu", act, uq)
+    n, k = gq.shape
+    out = torch.empty((*act.shape[:-1], n), dtype=torch.float32, device=act.data_.device)
+    if act.rows == 0:
+        return out
+    L, t, need = lib(), int(gq.dtype), ctypes.c_size_t(0)
+    with on_device(out.device):
+        st = _stream()
+        head = (t, activation, _ptr(gq.data_), _ptr(uq.data_), _ptr(act.data_), _ptr(out), n)
+        check("qmm_forward_glu_act", L.qmm_forward_glu_act(*head, None, 0, ctypes.byref(need), k, n, act.rows, 0, st))
+        buf = _act_workspace(need.value, out.device)
+        check("qmm_forward_glu_act", L.qmm_forward_glu_act(*head, _ptr(buf), need.value, ctypes.byref(need), k, n,
+                                                           act.rows, 1, st))
     return out
 
 
