@@ -1,11 +1,21 @@
-// attend.h — what the kernels and the entry point of the paged attention
-// share: the arguments, a sequence's bounds and the page of a position.
+// attend.h — what the attention kernels (attend_few.hip, attend_chunk.hip)
+// share: a sequence's bounds, the page of a position, the cache's codes as
+// f16, and the partial results that a context cut into parts leaves.
 #pragma once
 
 #include "qmm_device.h"
 #include "qmm_launch.h"
+#include "value_types.h"
 
 namespace qmm {
+
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = 64;  // positions a step of either kernel takes
 
 // The bounds of sequence b, whatever the device arrays hold: its first row
 // q0, its rows nq (at most max_q, inside the q rows) and its cached positions
@@ -19,10 +29,127 @@ __device__ __forceinline__ void sequence(const AttendArgs& a, int b, int64_t& q0
   kv = n < 0 ? 0 : (n > a.max_kv ? a.max_kv : n);
 }
 
-// The page that holds position j of sequence b, -1 for one outside the cache.
-__device__ __forceinline__ int64_t page_of(const AttendArgs& a, int b, int64_t j) {
-  const int p = a.tables[(int64_t)b * a.table_stride + j / a.c.page];
+// The first position that a row standing at `pos` sees.
+__device__ __forceinline__ int first_seen(const AttendArgs& a, int pos) {
+  return a.window > 0 && a.window <= pos ? pos - (int)a.window + 1 : 0;
+}
+
+// The page that holds position j < kv of sequence b; -1 where j is past kv or
+// the table names no page there.
+__device__ __forceinline__ int page_of(const AttendArgs& a, int b, int j, int kv) {
+  if (j >= kv) return -1;
+  const int p = a.tables[(int64_t)b * a.table_stride + (j >> a.page_bits)];
   return p < 0 || p >= a.c.pages ? -1 : p;
 }
+
+// 4 codes as f16, exactly: a byte b = code + 128 under 0x64 is the f16 1024 + b.
+__device__ __forceinline__ void codes_f16(uint32_t c, h2v& lo, h2v& hi) {
+  const uint32_t x = c ^ 0x80808080u;
+  const h2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  lo = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - off;
+  hi = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - off;
+}
+
+union H8 {
+  h8v v;
+  h2v h[4];
+  uint4 u;
+};
+
+// 8 codes times their scales, each product rounded once to f16: a key's 8
+// share one scale, a value's 8 positions have one each.
+__device__ __forceinline__ h8v key8(uint32_t a, uint32_t b, h2v s) {
+  H8 r;
+  codes_f16(a, r.h[0], r.h[1]);
+  codes_f16(b, r.h[2], r.h[3]);
+#pragma unroll
+  for (int i = 0; i < 4; i++) r.h[i] = r.h[i] * s;
+  return r.v;
+}
+__device__ __forceinline__ h8v value8(uint32_t a, uint32_t b, const uint4& s) {
+  H8 r, d;
+  d.u = s;
+  codes_f16(a, r.h[0], r.h[1]);
+  codes_f16(b, r.h[2], r.h[3]);
+#pragma unroll
+  for (int i = 0; i < 4; i++) r.h[i] = r.h[i] * d.h[i];
+  return r.v;
+}
+__device__ __forceinline__ h2v both(uint32_t f16bits) {
+  return __builtin_bit_cast(h2v, (f16bits & 0xFFFFu) * 0x10001u);
+}
+
+// A query's 8 values at element e, scaled (the softmax runs in powers of two)
+// and rounded once to f16, saturating.
+__device__ __forceinline__ h8v query8(const void* q, int dtype, int64_t e, float f) {
+  h8v r;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float x = (dtype == QMM_X_F32 ? load1<QMM_X_F32>(q, e + i)
+                                        : dtype == QMM_X_F16 ? load1<QMM_X_F16>(q, e + i) : load1<QMM_X_BF16>(q, e + i)) * f;
+    r[i] = (_Float16)(x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x);
+  }
+  return r;
+}
+
+// Scales of 8 positions j0 .. j0 + 7 with those outside [lo, hi) zeroed: what
+// lies there need not be finite, and a weight of zero would not hide it.
+__device__ __forceinline__ uint4 cut_scales(uint4 s, int j0, int lo, int hi) {
+  uint32_t w[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int j = j0 + 2 * i;
+    if (j < lo || j >= hi) w[i] &= 0xFFFF0000u;
+    if (j + 1 < lo || j + 1 >= hi) w[i] &= 0x0000FFFFu;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Partial results: rows of a block (kv head of a sequence, `rows` query rows)
+// for each part of its context: sums of weights times values [part][row][hd],
+// then (largest score, sum of weights) [part][row][2]. A part that a row sees
+// nothing of has the largest score -inf and no valid sums.
+struct AttendParts {
+  float* o;
+  float* ml;
+  int parts, rows, blocks;  // blocks: row blocks of a kv head of a sequence
+};
+__device__ __forceinline__ int64_t part_row(const AttendParts& p, int64_t head_of_seq, int block, int part, int row) {
+  return ((head_of_seq * p.blocks + block) * p.parts + part) * p.rows + row;
+}
+
+// A row's outputs from its sums of weights times values (relative to the
+// largest score `top`) and of weights, the head's sink joined.
+template <int N>
+__device__ __forceinline__ void finish_row(const AttendArgs& a, int head, float top, float sum, const float* acc,
+                                           float* out) {
+  float f = 1.0f;
+  if (a.sinks && sum != 0.0f) {
+    const float sink = a.sinks[head] * kLog2e, mx = fmaxf(top, sink);
+    f = exp2_fast(top - mx);
+    sum = sum * f + exp2_fast(sink - mx);
+  }
+  const float inv = sum == 0.0f ? 0.0f : f / sum;
+#pragma unroll
+  for (int i = 0; i < N; i++) out[i] = sum == 0.0f ? 0.0f : acc[i] * inv;
+}
+
+// 4 outputs at element e.
+__device__ __forceinline__ void store_out4(const AttendArgs& a, int64_t e, const float v[4]) {
+  if (a.out_vec)
+    store4<true>(a.out, a.odt, e, v);
+  else
+    store4<false>(a.out, a.odt, e, v);
+}
+
+// The launches of either kernel over the sequences with lo < rows <= hi query
+// rows a kv head (tokens times group); parts > 1: into `p`.
+hipError_t launch_attend_few(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st);
+hipError_t launch_attend_chunk(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st);
+
+constexpr int kFewRows = 32;     // the most query rows of the few-row kernel
+constexpr int kChunkRows = 128;  // query rows of a workgroup of the chunk kernel
 
 }  // namespace qmm

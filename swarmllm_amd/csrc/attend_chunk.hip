@@ -1,0 +1,277 @@
+// attend_chunk.hip — attention of a prompt's chunk of new tokens over its
+// pages of the cache.
+//
+// What bounds it is the matrix cores and the vector work beside them. A
+// workgroup takes 128 query rows of a kv head (the heads that share it side by
+// side, token after token), 32 a wave, against steps of 64 positions: the
+// step's keys and values are read once for the 128 rows, turned into f16
+// (codes times scales, one rounding) and laid into LDS, the next step's planes
+// in flight meanwhile. Per step a wave computes
+//   S^T = K q^T   (32x32x16: rows positions, columns query rows)
+//   O^T += V^T P^T (rows dims, columns query rows)
+// K row r of a tile is the position whose index has bits 2 and 3 of r
+// exchanged: so a lane's 8 scores of a 16-position step are consecutive
+// positions, and the weights made of them are the second product's operand as
+// they stand. The running maximum, the sum and O's rescaling (only where some
+// maximum grew) belong to the lane's own column.
+#include "attend.h"
+#include "mv_common.h"
+
+namespace qmm {
+
+namespace {
+
+template <int HD>
+struct ChunkSizes {
+  static constexpr int kPieces = kTile * HD / 16;           // 16-code pieces of a step's keys (and values)
+  static constexpr int kEach = (kPieces + 255) / 256;       // a thread's
+  static constexpr int kRow = HD + 8;                       // f16s of a K row in LDS, padded off the next row's banks
+  static constexpr int kVRow = kTile + 8;                   // and of a V row
+  static constexpr int kHalfs = kTile * kRow + HD * kVRow;  // one buffer
+  static constexpr size_t kLds = 2 * kHalfs * sizeof(uint16_t);
+};
+
+// One step's planes in a thread's registers.
+template <int HD>
+struct Staged {
+  uint4 k[ChunkSizes<HD>::kEach], v[ChunkSizes<HD>::kEach], d0[ChunkSizes<HD>::kEach], d1[ChunkSizes<HD>::kEach];
+  uint32_t ks[ChunkSizes<HD>::kEach];
+};
+
+template <int HD>
+__device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int pages, Staged<HD>& s) {
+  using Z = ChunkSizes<HD>;
+  const CachePlanes& c = a.c;
+#pragma unroll
+  for (int i = 0; i < Z::kEach; i++) {
+    const int x = (int)threadIdx.x + 256 * i;
+    const bool on = Z::kPieces % 256 == 0 || x < Z::kPieces;
+    const int row = on ? x / (HD / 16) : 0, e = on ? 16 * (x - row * (HD / 16)) : 0;
+    const int kp = __shfl(pages, row >> 4, kWave), vp = __shfl(pages, x & 3, kWave);
+    const int64_t kr = ((int64_t)(kp < 0 ? 0 : kp) * c.heads + kvh) * c.page + ((j0 + row) & (c.page - 1));
+    s.k[i] = *(const uint4*)(c.k_codes + kr * HD + e);
+    s.ks[i] = c.k_scales[kr * (HD / 32) + (e >> 5)];
+    const int64_t vph = (int64_t)(vp < 0 ? 0 : vp) * c.heads + kvh;
+    const int d = on ? x >> 2 : 0, at = (j0 + 16 * (x & 3)) & (c.page - 1);
+    s.v[i] = *(const uint4*)(c.v_codes + (vph * HD + d) * c.page + at);
+    const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
+    s.d0[i] = *(const uint4*)vs;
+    s.d1[i] = *(const uint4*)(vs + 8);
+  }
+}
+
+// The step's keys and values as f16 into an LDS buffer; [lo, hi): the
+// positions whose values may be used.
+template <int HD>
+__device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int lo, int hi, bool cut, uint16_t* buf) {
+  using Z = ChunkSizes<HD>;
+#pragma unroll
+  for (int i = 0; i < Z::kEach; i++) {
+    const int x = (int)threadIdx.x + 256 * i;
+    const int vp = __shfl(pages, x & 3, kWave);
+    if (Z::kPieces % 256 != 0 && x >= Z::kPieces) continue;
+    const int row = x / (HD / 16), e = 16 * (x - row * (HD / 16));
+    H8 h;
+    const h2v ks = both(s.ks[i]);
+    h.v = key8(s.k[i].x, s.k[i].y, ks);
+    *(uint4*)(buf + row * Z::kRow + e) = h.u;
+    h.v = key8(s.k[i].z, s.k[i].w, ks);
+    *(uint4*)(buf + row * Z::kRow + e + 8) = h.u;
+    uint4 d0 = s.d0[i], d1 = s.d1[i];
+    const int j = j0 + 16 * (x & 3);
+    if (cut) {
+      d0 = cut_scales(d0, j, lo, vp < 0 ? 0 : hi);
+      d1 = cut_scales(d1, j + 8, lo, vp < 0 ? 0 : hi);
+    }
+    uint16_t* vb = buf + kTile * Z::kRow + (x >> 2) * Z::kVRow + 16 * (x & 3);
+    h.v = value8(s.v[i].x, s.v[i].y, d0);
+    *(uint4*)vb = h.u;
+    h.v = value8(s.v[i].z, s.v[i].w, d1);
+    *(uint4*)(vb + 8) = h.u;
+  }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows, AttendParts parts) {
+  using Z = ChunkSizes<HD>;
+  extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
+  const CachePlanes& c = a.c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 31, hi = lane >> 5;
+  const int b = blockIdx.x / c.heads, kvh = blockIdx.x - b * c.heads, part = blockIdx.y;
+  const int block = (int)(gridDim.z - 1 - blockIdx.z);  // the rows that see most first
+  int64_t q0;
+  int nq, kv;
+  sequence(a, b, q0, nq, kv);
+  const int rows = nq * a.group;
+  const int r0 = block * kChunkRows;
+  if (rows <= lo_rows || r0 >= rows) return;
+
+  const int pos0 = kv - nq;
+  const int last_row = rows - 1 < r0 + kChunkRows - 1 ? rows - 1 : r0 + kChunkRows - 1;
+  const int low_pos = pos0 + r0 / a.group, high_pos = pos0 + last_row / a.group;
+  const int lo = first_seen(a, low_pos < 0 ? 0 : low_pos), seen = high_pos + 1;  // [lo, seen): what the rows see
+  const int t0 = lo / kTile, tiles = seen > 0 ? (seen + kTile - 1) / kTile - t0 : 0;
+  const int begin = t0 + (int)((int64_t)tiles * part / parts.parts);
+  const int end = t0 + (int)((int64_t)tiles * (part + 1) / parts.parts);
+
+  // this wave's rows
+  const int r = r0 + 32 * wave + col, qi = r / a.group;
+  const int pos = pos0 + qi;
+  const int wave_low = pos0 + (r0 + 32 * wave) / a.group;
+  const int wave_last = r0 + 32 * wave + 31 < rows - 1 ? r0 + 32 * wave + 31 : rows - 1;
+  const int wave_high = r0 + 32 * wave < rows ? pos0 + wave_last / a.group : -1;  // no rows: sees nothing
+  const int wave_first = first_seen(a, wave_low < 0 ? 0 : wave_low);
+  const int first = first_seen(a, pos);
+  const bool row_on = r < rows;
+  const int64_t row_q = q0 + qi;
+  const int head = kvh * a.group + r - qi * a.group;
+
+  h8v q[HD / 16];
+#pragma unroll
+  for (int s = 0; s < HD / 16; s++)
+    q[s] = row_on ? query8(a.q, a.qdt, row_q * a.qs + (int64_t)head * a.qhs + 16 * s + 8 * hi, a.scale * kLog2e) : h8v{};
+
+  f16v o[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  // lane x < 4 of every wave holds the page of the step's x-th 16 positions
+  auto pages_of = [&](int tile) { return tile < end ? page_of(a, b, tile * kTile + 16 * (lane & 3), kv) : -1; };
+  auto lay_step = [&](const Staged<HD>& s, int tile, int pages, int buf) {
+    const int j0 = tile * kTile;
+    const bool cut = j0 < lo || j0 + kTile > kv || __ballot(pages < 0) != 0;
+    lay<HD>(s, j0, pages, lo, kv, cut, s_buf + buf * Z::kHalfs);
+  };
+
+  Staged<HD> st;
+  int pages = pages_of(begin), next_pages = pages_of(begin + 1);
+  if (begin < end) {
+    fetch<HD>(a, kvh, begin * kTile, pages, st);
+    lay_step(st, begin, pages, 0);
+  }
+  __syncthreads();
+  // K's LDS row of this lane: bits 2 and 3 exchanged
+  const int krow = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
+  for (int tile = begin, cur = 0; tile < end; tile++, cur ^= 1) {
+    const int j0 = tile * kTile;
+    const int after_pages = pages_of(tile + 2);
+    if (tile + 1 < end) fetch<HD>(a, kvh, j0 + kTile, next_pages, st);
+
+    if (j0 <= wave_high && j0 + kTile > wave_first) {
+      const uint16_t* kb = s_buf + cur * Z::kHalfs + krow * Z::kRow + 8 * hi;
+      f16v s[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; d++) {
+          const h8v k = *(const h8v*)(kb + 32 * t * Z::kRow + 16 * d);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[d], s[t], 0, 0, 0);
+        }
+      }
+      const uint64_t absent = __ballot(pages < 0) & 15;
+      if (j0 + kTile - 1 > wave_low || (a.window > 0 && j0 <= (int64_t)wave_high - a.window) || absent) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int x = 32 * t + 16 * (i >> 3) + 8 * hi + (i & 7), j = j0 + x;
+            if (j > pos || j < first || ((absent >> (x >> 4)) & 1)) s[t][i] = -INFINITY;
+          }
+      }
+      float mt = s[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[t][i]);
+      mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
+      if (__ballot(mt > m) != 0) {
+        const float mn = fmaxf(m, mt), f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) o[d] *= f;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      h8v p[4];
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float w = exp2_fast(s[t][i] - base);
+          sum += w;
+          p[2 * t + (i >> 3)][i & 7] = (_Float16)w;
+        }
+      l += sum;
+      const uint16_t* vb = s_buf + cur * Z::kHalfs + kTile * Z::kRow + col * Z::kVRow + 8 * hi;
+#pragma unroll
+      for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const h8v v = *(const h8v*)(vb + 32 * d * Z::kVRow + 16 * t);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[t], o[d], 0, 0, 0);
+        }
+    }
+    if (tile + 1 < end) lay_step(st, tile + 1, next_pages, cur ^ 1);
+    pages = next_pages;
+    next_pages = after_pages;
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32, kWave);
+  if (!row_on) return;
+  if (parts.parts > 1) {
+    const int64_t pr = part_row(parts, (int64_t)blockIdx.x, block, part, r - r0);
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(f4v*)(parts.o + pr * HD + 32 * d + 2 * i + 4 * hi) = f4v{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+    if (hi == 0) {
+      parts.ml[2 * pr] = m;
+      parts.ml[2 * pr + 1] = l;
+    }
+    return;
+  }
+#pragma unroll
+  for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float acc[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+      float out[4];
+      finish_row<4>(a, head, m, l, acc, out);
+      store_out4(a, row_q * a.os + (int64_t)head * HD + 32 * d + 2 * i + 4 * hi, out);
+    }
+}
+
+template <int HD>
+hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
+  if constexpr (ChunkSizes<HD>::kLds > 64 * 1024) {
+    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD>>();
+    if (e != hipSuccess) return e;
+  }
+  const dim3 grid((unsigned)(a.seqs * a.c.heads), (unsigned)p.parts, (unsigned)p.blocks);
+  attend_chunk_kernel<HD><<<grid, 256, ChunkSizes<HD>::kLds, st>>>(a, lo, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attend_chunk(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
+  QMM_NOTE_LAUNCH();
+  switch (a.c.hd) {
+    case 64: return launch_hd<64>(a, lo, p, st);
+    case 96: return launch_hd<96>(a, lo, p, st);
+    case 128: return launch_hd<128>(a, lo, p, st);
+    case 256: return launch_hd<256>(a, lo, p, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace qmm

@@ -1087,10 +1087,14 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   a.seqs = (int)seqs; a.heads = heads; a.group = heads / cache->kv_heads;
   a.max_q = (int)(max_q < tokens ? max_q : tokens);
   // a sequence's positions lie inside its row of the table
-  const int64_t cap = table_stride > INT32_MAX / cache->page ? INT32_MAX / cache->page * cache->page
-                                                             : table_stride * cache->page;
+  constexpr int64_t kMostPositions = (int64_t)1 << 30;
+  if (table_stride > kMostPositions / cache->page) return QMM_UNSUPPORTED;
+  const int64_t cap = table_stride * cache->page;
   a.max_kv = (int)(max_kv < cap ? max_kv : cap);
   a.qdt = q_dtype; a.odt = out_dtype; a.scale = scale;
+  a.out_vec = (uintptr_t)out % (4 * qmm::value_bytes(out_dtype)) == 0 && out_stride % 4 == 0;
+  a.page_bits = __builtin_ctz((unsigned)cache->page);
+  if (!qmm::attend_fits(a)) return QMM_UNSUPPORTED;
   *need = qmm::attend_workspace_bytes(a, cu_count());
   if (!launch) return QMM_OK;
   if (!q || !out || !q_starts || !kv_lens || (!tables && a.max_kv > 0)) return QMM_UNSUPPORTED;

@@ -298,9 +298,11 @@ struct AttendArgs {
   const int32_t* tables;
   const float* sinks;
   int64_t qs, qhs, os, table_stride, tokens, window;
-  int seqs, heads, group, max_q, max_kv, qdt, odt;
+  int seqs, heads, group, max_q, max_kv, qdt, odt, page_bits;
+  bool out_vec;  // out's rows lie at multiples of 4 values
   float scale;
 };
+bool attend_fits(const AttendArgs& a);
 size_t attend_workspace_bytes(const AttendArgs& a, int cus);
 hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st);
 
