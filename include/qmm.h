@@ -423,9 +423,10 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
  * apart; out: rows out_stride values apart, heads head_dim. Rows of q that no
  * sequence holds are left as they were in out. max_q and max_kv bound the sequences' new
  * tokens and cached positions: the host plans by them (rows past max_q stay as they were, kv_lens is cut
- * at max_kv and at the table's row). q is scaled and rounded to f16 (to
- * nearest, saturating at 65504), as are the cache's values and the weights exp(s_j - max);
- * sums are f32. Any mix of lengths is served by one call; the rows of a
+ * at max_kv and at the table's row). The products run on f16
+ * operands with f32 sums: q (an f32 q rounds; all saturate at 65504), the
+ * cache's values code * scale and the weights exp(s_j - max), each rounded
+ * once to nearest. scale is finite (at most 1e30 in size). Any mix of lengths is served by one call; the rows of a
  * sequence do not depend on the other sequences' data. Plan (launch == 0) and launch as qmm_forward: the
  * workspace joins the parts of a long context (*need can be 0). Replaces the
  * reference's decode attention (kernels/decode_attn.cu:257-612) and its paged

@@ -16,6 +16,9 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;  // positions a step of either kernel takes
+// Weights may reach 2^kSlack (f16 holds 2^15) before the running maximum that
+// they are relative to is moved and what is summed so far rescaled.
+constexpr float kSlack = 8.0f;
 
 // The bounds of sequence b, whatever the device arrays hold: its first row
 // q0, its rows nq (at most max_q, inside the q rows) and its cached positions
@@ -79,17 +82,70 @@ __device__ __forceinline__ h2v both(uint32_t f16bits) {
   return __builtin_bit_cast(h2v, (f16bits & 0xFFFFu) * 0x10001u);
 }
 
-// A query's 8 values at element e, scaled (the softmax runs in powers of two)
-// and rounded once to f16, saturating.
-__device__ __forceinline__ h8v query8(const void* q, int dtype, int64_t e, float f) {
-  h8v r;
+// Query row r of a kv head as (new token, head of the group): r / group by a
+// multiplication (rows times group stay below 2^32).
+__device__ __forceinline__ int token_of(const AttendArgs& a, int r) {
+  return a.group_inv ? (int)__umulhi((uint32_t)r, a.group_inv) : r;
+}
+
+// N pieces of 8 of a query's values as f16, piece s from element at(s) on: exact
+// for an f16 query and for a bf16 one of ordinary size; an f32 query rounds
+// once. Past f16's range they saturate. The scale's sign goes with them, its
+// size into the softmax.
+__device__ __forceinline__ _Float16 query_f16(const AttendArgs& a, float x) {
+  x *= a.q_sign;
+  return (_Float16)(x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x);
+}
+template <int N, typename At>
+__device__ __forceinline__ void load_query(const AttendArgs& a, bool on, At at, h8v* q) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float x = (dtype == QMM_X_F32 ? load1<QMM_X_F32>(q, e + i)
-                                        : dtype == QMM_X_F16 ? load1<QMM_X_F16>(q, e + i) : load1<QMM_X_BF16>(q, e + i)) * f;
-    r[i] = (_Float16)(x > 65504.0f ? 65504.0f : x < -65504.0f ? -65504.0f : x);
+  for (int s = 0; s < N; s++) q[s] = h8v{};
+  if (!on) return;
+  if (!a.q_vec) {
+#pragma unroll
+    for (int s = 0; s < N; s++)
+      for (int i = 0; i < 8; i++) {
+        const int64_t e = at(s) + i;
+        q[s][i] = query_f16(a, a.qdt == QMM_X_F32 ? load1<QMM_X_F32>(a.q, e)
+                                                  : a.qdt == QMM_X_F16 ? load1<QMM_X_F16>(a.q, e) : load1<QMM_X_BF16>(a.q, e));
+      }
+  } else if (a.qdt == QMM_X_F32) {
+#pragma unroll
+    for (int s = 0; s < N; s++) {
+      float x[8];
+      load4<QMM_X_F32, true>(a.q, at(s), x);
+      load4<QMM_X_F32, true>(a.q, at(s) + 4, x + 4);
+#pragma unroll
+      for (int i = 0; i < 8; i++) q[s][i] = query_f16(a, x[i]);
+    }
+  } else {
+    H8 r[N];
+#pragma unroll
+    for (int s = 0; s < N; s++) r[s].u = *(const uint4*)((const uint16_t*)a.q + at(s));
+    if (a.qdt == QMM_X_F16) {
+#pragma unroll
+      for (int s = 0; s < N; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[s][i] = query_f16(a, (float)r[s].v[i]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < N; s++) {
+        const uint32_t w[4] = {r[s].u.x, r[s].u.y, r[s].u.z, r[s].u.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[s][i] = query_f16(a, widen<QMM_X_BF16>(w[i >> 1] >> (16 * (i & 1))));
+      }
+    }
   }
-  return r;
+}
+
+// The steps [begin, end) of a part of a row block whose rows see positions
+// [lo, hi): parts of equal length, the last ones shorter or empty.
+__device__ __forceinline__ void part_steps(int lo, int hi, int part, int parts, int& begin, int& end) {
+  const int t0 = lo / kTile, tiles = hi > 0 ? (hi + kTile - 1) / kTile - t0 : 0;
+  const int each = parts > 1 ? (int)(((uint32_t)tiles + parts - 1) / (uint32_t)parts) : tiles;
+  const int first = part * each;
+  begin = t0 + (first < tiles ? first : tiles);
+  end = t0 + (first + each < tiles ? first + each : tiles);
 }
 
 // Scales of 8 positions j0 .. j0 + 7 with those outside [lo, hi) zeroed: what
@@ -149,6 +205,7 @@ __device__ __forceinline__ void store_out4(const AttendArgs& a, int64_t e, const
 hipError_t launch_attend_few(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st);
 hipError_t launch_attend_chunk(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st);
 
+constexpr int kFewWaves = 4;     // waves of a few-row workgroup
 constexpr int kFewRows = 32;     // the most query rows of the few-row kernel
 constexpr int kChunkRows = 128;  // query rows of a workgroup of the chunk kernel
 

@@ -14,35 +14,58 @@ namespace qmm {
 
 namespace {
 
-// 4 dims of a row a thread, over the parts in order.
+// A workgroup joins 64 / (hd / 4) rows: 4 dims a lane, the parts dealt to its
+// 4 waves in turn, their results joined in LDS.
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_rows, int hi_rows, AttendParts p) {
-  const int hd = a.c.hd, per = hd / 4;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t pr = x / per;
-  const int e = 4 * (int)(x - pr * per);
-  const int64_t hb = pr / p.rows;  // (head of a sequence, block)
-  const int row = (int)(pr - hb * p.rows);
-  const int64_t hs = hb / p.blocks;
-  const int block = (int)(hb - hs * p.blocks);
-  const int64_t b = hs / a.c.heads;
-  if (b >= a.seqs) return;
+  __shared__ f4v s_o[4][64];
+  __shared__ float s_m[4][64], s_l[4][64];
+  const int hd = a.c.hd, per = hd / 4, fit = 64 / per;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane / per, e = 4 * (lane - sub * per);
+  // rows of one kv head of a sequence lie block after block
+  const int64_t row_of_head = (int64_t)blockIdx.x * fit + sub;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int block = (int)(row_of_head / p.rows), row = (int)(row_of_head - (int64_t)block * p.rows);
   int64_t q0;
   int nq, kv;
-  sequence(a, (int)b, q0, nq, kv);
-  const int rows = nq * a.group, r = block * p.rows + row;
-  if (rows <= lo_rows || rows > hi_rows || r >= rows) return;
-  float top = -INFINITY;
-  for (int s = 0; s < p.parts; s++) top = fmaxf(top, p.ml[2 * part_row(p, hs, block, s, row)]);
-  const float base = top == -INFINITY ? 0.0f : top;
+  sequence(a, b, q0, nq, kv);
+  const int rows = nq * a.group;
+  const int64_t hs = (int64_t)b * a.c.heads + kvh;
+  const bool on = sub < fit && block < p.blocks && rows > lo_rows && rows <= hi_rows && row_of_head < rows;
+  float top = -INFINITY, sum = 0.0f;
   f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  float sum = 0.0f;
-  for (int s = 0; s < p.parts; s++) {
-    const int64_t i = part_row(p, hs, block, s, row);
-    const float f = exp2_fast(p.ml[2 * i] - base);
-    sum += p.ml[2 * i + 1] * f;
-    acc += *(const f4v*)(p.o + i * hd + e) * f;
+  if (on) {
+    const int64_t i0 = part_row(p, hs, block, wave, row), step = 4 * (int64_t)p.rows;
+    const int n = (p.parts - wave + 3) / 4;
+#pragma unroll 4
+    for (int s = 0; s < n; s++) {
+      const int64_t i = i0 + s * step;
+      const float m = p.ml[2 * i], l = p.ml[2 * i + 1];
+      const f4v o = *(const f4v*)(p.o + i * hd + e);
+      const float mx = fmaxf(top, m), base = mx == -INFINITY ? 0.0f : mx;
+      const float fa = exp2_fast(top - base), fb = exp2_fast(m - base);
+      top = mx;
+      sum = sum * fa + l * fb;
+      acc = acc * fa + o * fb;
+    }
   }
-  const int i = r / a.group, head = (int)(hs - b * a.c.heads) * a.group + r - i * a.group;
+  s_o[wave][lane] = acc;
+  s_m[wave][lane] = top;
+  s_l[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || !on) return;
+#pragma unroll
+  for (int w = 1; w < 4; w++) top = fmaxf(top, s_m[w][lane]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  sum = 0.0f;
+  acc = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float f = exp2_fast(s_m[w][lane] - base);
+    sum += s_l[w][lane] * f;
+    acc += s_o[w][lane] * f;
+  }
+  const int r = (int)row_of_head, i = token_of(a, r), head = kvh * a.group + r - i * a.group;
   float out[4];
   finish_row<4>(a, head, top, sum, (const float*)&acc, out);
   store_out4(a, (q0 + i) * a.os + (int64_t)head * hd + e, out);
@@ -76,8 +99,13 @@ Plan plan_of(const AttendArgs& a, int cus) {
   if (p.few) {
     span = a.max_kv;
     if (a.window > 0 && a.window + p.few / a.group + 1 < span) span = a.window + p.few / a.group + 1;
-    // parts until two workgroups a CU are there, of 4 steps a wave at least
-    p.few_parts = clamp_parts(2 * cus / heads, ((span + kTile - 1) / kTile) / 16);
+    const int64_t tiles = (span + kTile - 1) / kTile;
+    // parts until two workgroups a CU are there, of one step a wave at least,
+    // of four where the CUs have one each without (the join is a launch of
+    // 4 us; graph replays, us: 1 sequence of 2000 in 8 parts 11.1, in 2 18.1;
+    // 4 of 1000 10.6 / 16.2; 16 of 8000 in 4 51.5, in 2 68.1; 32 of 1000 whole
+    // 17.0, in 2 19.5)
+    p.few_parts = clamp_parts(2 * cus / heads, tiles / (heads < cus ? kFewWaves : 4 * kFewWaves));
   }
   return p;
 }
@@ -93,8 +121,10 @@ size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, void* ws, 
 }
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
-  const int64_t threads = (int64_t)a.seqs * a.c.heads * p.blocks * p.rows * (a.c.hd / 4);
-  attend_join_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, st>>>(a, lo, hi, p);
+  const int fit = 64 / (a.c.hd / 4);
+  const int64_t most = (int64_t)a.max_q * a.group, held = (int64_t)p.blocks * p.rows, rows = most < held ? most : held;
+  attend_join_kernel<<<dim3((unsigned)((rows + fit - 1) / fit), (unsigned)a.c.heads, (unsigned)a.seqs), 256, 0, st>>>(
+      a, lo, hi, p);
   return hipGetLastError();
 }
 
@@ -103,8 +133,7 @@ hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipSt
 bool attend_fits(const AttendArgs& a) {
   const int64_t rows = (int64_t)a.max_q * a.group;
   const int64_t heads = (int64_t)a.seqs * a.c.heads;
-  return rows <= (int64_t)65535 * kChunkRows && heads * (rows + kChunkRows) * (a.c.hd / 4) < ((int64_t)1 << 39) &&
-         heads < ((int64_t)1 << 31);
+  return rows <= (int64_t)65535 * kChunkRows && rows * a.group < ((int64_t)1 << 32) && heads < ((int64_t)1 << 31);
 }
 
 size_t attend_workspace_bytes(const AttendArgs& a, int cus) {

@@ -12,8 +12,7 @@
 // K row r of a tile is the position whose index has bits 2 and 3 of r
 // exchanged: so a lane's 8 scores of a 16-position step are consecutive
 // positions, and the weights made of them are the second product's operand as
-// they stand. The running maximum, the sum and O's rescaling (only where some
-// maximum grew) belong to the lane's own column.
+// they stand. The running maximum, the sum and O's rescaling belong to the lane's own column.
 #include "attend.h"
 #include "mv_common.h"
 
@@ -38,37 +37,69 @@ struct Staged {
   uint32_t ks[ChunkSizes<HD>::kEach];
 };
 
-template <int HD>
+// A step's pages. ONE: pages of 64 positions and more, so a step has one, the
+// same for the wave; otherwise lane x < 4 of every wave holds that of the step's
+// x-th 16 positions. -1: none.
+template <bool ONE>
+__device__ __forceinline__ int step_page(const AttendArgs& a, int b, int tile, int end, int kv) {
+  if (tile >= end) return -1;
+  if (ONE) return __builtin_amdgcn_readfirstlane(page_of(a, b, tile * kTile, kv));
+  return page_of(a, b, tile * kTile + 16 * (int)(threadIdx.x & 3), kv);
+}
+
+template <int HD, bool ONE>
 __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int pages, Staged<HD>& s) {
   using Z = ChunkSizes<HD>;
   const CachePlanes& c = a.c;
+  const int8_t* k1 = nullptr;
+  const int8_t* v1 = nullptr;
+  const uint16_t *ks1 = nullptr, *vs1 = nullptr;
+  if constexpr (ONE) {
+    // a step's keys lie side by side, its values in rows of a page
+    const int64_t ph = (int64_t)(pages < 0 ? 0 : pages) * c.heads + kvh;
+    const int at = j0 & (c.page - 1);
+    k1 = c.k_codes + (ph * c.page + at) * HD;
+    ks1 = c.k_scales + (ph * c.page + at) * (HD / 32);
+    v1 = c.v_codes + ph * HD * c.page + at;
+    vs1 = c.v_scales + ph * (HD / 32) * c.page + at;
+  }
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     const int x = (int)threadIdx.x + 256 * i;
     const bool on = Z::kPieces % 256 == 0 || x < Z::kPieces;
-    const int row = on ? x / (HD / 16) : 0, e = on ? 16 * (x - row * (HD / 16)) : 0;
-    const int kp = __shfl(pages, row >> 4, kWave), vp = __shfl(pages, x & 3, kWave);
-    const int64_t kr = ((int64_t)(kp < 0 ? 0 : kp) * c.heads + kvh) * c.page + ((j0 + row) & (c.page - 1));
-    s.k[i] = *(const uint4*)(c.k_codes + kr * HD + e);
-    s.ks[i] = c.k_scales[kr * (HD / 32) + (e >> 5)];
-    const int64_t vph = (int64_t)(vp < 0 ? 0 : vp) * c.heads + kvh;
-    const int d = on ? x >> 2 : 0, at = (j0 + 16 * (x & 3)) & (c.page - 1);
-    s.v[i] = *(const uint4*)(c.v_codes + (vph * HD + d) * c.page + at);
-    const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
-    s.d0[i] = *(const uint4*)vs;
-    s.d1[i] = *(const uint4*)(vs + 8);
+    if constexpr (ONE) {
+      const uint32_t y = on ? x : 0;
+      s.k[i] = *(const uint4*)(k1 + 16 * y);
+      s.ks[i] = ks1[y >> 1];
+      s.v[i] = *(const uint4*)(v1 + (y >> 2) * (uint32_t)c.page + 16 * (y & 3));
+      const uint16_t* vs = vs1 + (y >> 7) * (uint32_t)c.page + 16 * (y & 3);
+      s.d0[i] = *(const uint4*)vs;
+      s.d1[i] = *(const uint4*)(vs + 8);
+    } else {
+      const int row = on ? x / (HD / 16) : 0, e = on ? 16 * (x - row * (HD / 16)) : 0;
+      const int kp = __shfl(pages, row >> 4, kWave), vp = __shfl(pages, x & 3, kWave);
+      const int64_t kr = ((int64_t)(kp < 0 ? 0 : kp) * c.heads + kvh) * c.page + ((j0 + row) & (c.page - 1));
+      s.k[i] = *(const uint4*)(c.k_codes + kr * HD + e);
+      s.ks[i] = c.k_scales[kr * (HD / 32) + (e >> 5)];
+      const int64_t vph = (int64_t)(vp < 0 ? 0 : vp) * c.heads + kvh;
+      const int d = on ? x >> 2 : 0, at = (j0 + 16 * (x & 3)) & (c.page - 1);
+      s.v[i] = *(const uint4*)(c.v_codes + (vph * HD + d) * c.page + at);
+      const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
+      s.d0[i] = *(const uint4*)vs;
+      s.d1[i] = *(const uint4*)(vs + 8);
+    }
   }
 }
 
-// The step's keys and values as f16 into an LDS buffer; [lo, hi): the
-// positions whose values may be used.
-template <int HD>
-__device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int lo, int hi, bool cut, uint16_t* buf) {
+// The step's keys and values as f16 into an LDS buffer. CUT: the values of
+// positions outside [lo, hi), or on no page, are laid as zeros.
+template <int HD, bool ONE, bool CUT>
+__device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int lo, int hi, uint16_t* buf) {
   using Z = ChunkSizes<HD>;
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     const int x = (int)threadIdx.x + 256 * i;
-    const int vp = __shfl(pages, x & 3, kWave);
+    const int vp = !CUT ? 0 : ONE ? pages : __shfl(pages, x & 3, kWave);
     if (Z::kPieces % 256 != 0 && x >= Z::kPieces) continue;
     const int row = x / (HD / 16), e = 16 * (x - row * (HD / 16));
     H8 h;
@@ -78,8 +109,8 @@ __device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int 
     h.v = key8(s.k[i].z, s.k[i].w, ks);
     *(uint4*)(buf + row * Z::kRow + e + 8) = h.u;
     uint4 d0 = s.d0[i], d1 = s.d1[i];
-    const int j = j0 + 16 * (x & 3);
-    if (cut) {
+    if constexpr (CUT) {
+      const int j = j0 + 16 * (x & 3);
       d0 = cut_scales(d0, j, lo, vp < 0 ? 0 : hi);
       d1 = cut_scales(d1, j + 8, lo, vp < 0 ? 0 : hi);
     }
@@ -91,14 +122,14 @@ __device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int 
   }
 }
 
-template <int HD>
+template <int HD, bool ONE>
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows, AttendParts parts) {
   using Z = ChunkSizes<HD>;
   extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
   const CachePlanes& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 31, hi = lane >> 5;
-  const int b = blockIdx.x / c.heads, kvh = blockIdx.x - b * c.heads, part = blockIdx.y;
+  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)c.heads), kvh = blockIdx.x - b * c.heads, part = blockIdx.y;
   const int block = (int)(gridDim.z - 1 - blockIdx.z);  // the rows that see most first
   int64_t q0;
   int nq, kv;
@@ -109,18 +140,17 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
 
   const int pos0 = kv - nq;
   const int last_row = rows - 1 < r0 + kChunkRows - 1 ? rows - 1 : r0 + kChunkRows - 1;
-  const int low_pos = pos0 + r0 / a.group, high_pos = pos0 + last_row / a.group;
+  const int low_pos = pos0 + token_of(a, r0), high_pos = pos0 + token_of(a, last_row);
   const int lo = first_seen(a, low_pos < 0 ? 0 : low_pos), seen = high_pos + 1;  // [lo, seen): what the rows see
-  const int t0 = lo / kTile, tiles = seen > 0 ? (seen + kTile - 1) / kTile - t0 : 0;
-  const int begin = t0 + (int)((int64_t)tiles * part / parts.parts);
-  const int end = t0 + (int)((int64_t)tiles * (part + 1) / parts.parts);
+  int begin, end;
+  part_steps(lo, seen, part, parts.parts, begin, end);
 
   // this wave's rows
-  const int r = r0 + 32 * wave + col, qi = r / a.group;
+  const int r = r0 + 32 * wave + col, qi = token_of(a, r);
   const int pos = pos0 + qi;
-  const int wave_low = pos0 + (r0 + 32 * wave) / a.group;
+  const int wave_low = pos0 + token_of(a, r0 + 32 * wave);
   const int wave_last = r0 + 32 * wave + 31 < rows - 1 ? r0 + 32 * wave + 31 : rows - 1;
-  const int wave_high = r0 + 32 * wave < rows ? pos0 + wave_last / a.group : -1;  // no rows: sees nothing
+  const int wave_high = r0 + 32 * wave < rows ? pos0 + token_of(a, wave_last) : -1;  // no rows: sees nothing
   const int wave_first = first_seen(a, wave_low < 0 ? 0 : wave_low);
   const int first = first_seen(a, pos);
   const bool row_on = r < rows;
@@ -128,9 +158,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
   const int head = kvh * a.group + r - qi * a.group;
 
   h8v q[HD / 16];
-#pragma unroll
-  for (int s = 0; s < HD / 16; s++)
-    q[s] = row_on ? query8(a.q, a.qdt, row_q * a.qs + (int64_t)head * a.qhs + 16 * s + 8 * hi, a.scale * kLog2e) : h8v{};
+  load_query<HD / 16>(a, row_on, [&](int s) { return row_q * a.qs + (int64_t)head * a.qhs + 16 * s + 8 * hi; }, q);
 
   f16v o[HD / 32];
 #pragma unroll
@@ -139,18 +167,19 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  // lane x < 4 of every wave holds the page of the step's x-th 16 positions
-  auto pages_of = [&](int tile) { return tile < end ? page_of(a, b, tile * kTile + 16 * (lane & 3), kv) : -1; };
   auto lay_step = [&](const Staged<HD>& s, int tile, int pages, int buf) {
     const int j0 = tile * kTile;
-    const bool cut = j0 < lo || j0 + kTile > kv || __ballot(pages < 0) != 0;
-    lay<HD>(s, j0, pages, lo, kv, cut, s_buf + buf * Z::kHalfs);
+    uint16_t* to = s_buf + buf * Z::kHalfs;
+    if (j0 < lo || j0 + kTile > kv || __ballot(pages < 0) != 0)
+      lay<HD, ONE, true>(s, j0, pages, lo, kv, to);
+    else
+      lay<HD, ONE, false>(s, j0, pages, lo, kv, to);
   };
 
   Staged<HD> st;
-  int pages = pages_of(begin), next_pages = pages_of(begin + 1);
+  int pages = step_page<ONE>(a, b, begin, end, kv), next_pages = step_page<ONE>(a, b, begin + 1, end, kv);
   if (begin < end) {
-    fetch<HD>(a, kvh, begin * kTile, pages, st);
+    fetch<HD, ONE>(a, kvh, begin * kTile, pages, st);
     lay_step(st, begin, pages, 0);
   }
   __syncthreads();
@@ -158,8 +187,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
   const int krow = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
   for (int tile = begin, cur = 0; tile < end; tile++, cur ^= 1) {
     const int j0 = tile * kTile;
-    const int after_pages = pages_of(tile + 2);
-    if (tile + 1 < end) fetch<HD>(a, kvh, j0 + kTile, next_pages, st);
+    const int after_pages = step_page<ONE>(a, b, tile + 2, end, kv);
+    if (tile + 1 < end) fetch<HD, ONE>(a, kvh, j0 + kTile, next_pages, st);
 
     if (j0 <= wave_high && j0 + kTile > wave_first) {
       const uint16_t* kb = s_buf + cur * Z::kHalfs + krow * Z::kRow + 8 * hi;
@@ -174,7 +203,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
           s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[d], s[t], 0, 0, 0);
         }
       }
-      const uint64_t absent = __ballot(pages < 0) & 15;
+      const uint64_t absent = ONE ? (pages < 0 ? 15 : 0) : __ballot(pages < 0) & 15;
       if (j0 + kTile - 1 > wave_low || (a.window > 0 && j0 <= (int64_t)wave_high - a.window) || absent) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -189,22 +218,24 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[t][i]);
-      mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
-      if (__ballot(mt > m) != 0) {
-        const float mn = fmaxf(m, mt), f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+      // the weights are relative to a maximum that follows the scores only once
+      // one has outgrown it by 2^kSlack (exact in f16 and f32 alike)
+      if (__ballot((mt - m) * a.sc > kSlack) != 0) {
+        mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
+        const float mn = fmaxf(m, mt), f = exp2_fast((m - (mn == -INFINITY ? 0.0f : mn)) * a.sc);
         m = mn;
         l *= f;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) o[d] *= f;
       }
-      const float base = m == -INFINITY ? 0.0f : m;
+      const float bs = m == -INFINITY ? 0.0f : m * a.sc;
       h8v p[4];
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float w = exp2_fast(s[t][i] - base);
+          const float w = exp2_fast(__builtin_fmaf(s[t][i], a.sc, -bs));
           sum += w;
           p[2 * t + (i >> 3)][i & 7] = (_Float16)w;
         }
@@ -234,7 +265,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
       for (int i = 0; i < 16; i += 4)
         *(f4v*)(parts.o + pr * HD + 32 * d + 2 * i + 4 * hi) = f4v{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
     if (hi == 0) {
-      parts.ml[2 * pr] = m;
+      parts.ml[2 * pr] = m * a.sc;
       parts.ml[2 * pr + 1] = l;
     }
     return;
@@ -245,20 +276,26 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
     for (int i = 0; i < 16; i += 4) {
       const float acc[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
       float out[4];
-      finish_row<4>(a, head, m, l, acc, out);
+      finish_row<4>(a, head, m * a.sc, l, acc, out);
       store_out4(a, row_q * a.os + (int64_t)head * HD + 32 * d + 2 * i + 4 * hi, out);
     }
 }
 
-template <int HD>
-hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
+template <int HD, bool ONE>
+hipError_t launch_pages(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
   if constexpr (ChunkSizes<HD>::kLds > 64 * 1024) {
-    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD>>();
+    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD, ONE>>();
     if (e != hipSuccess) return e;
   }
   const dim3 grid((unsigned)(a.seqs * a.c.heads), (unsigned)p.parts, (unsigned)p.blocks);
-  attend_chunk_kernel<HD><<<grid, 256, ChunkSizes<HD>::kLds, st>>>(a, lo, p);
+  attend_chunk_kernel<HD, ONE><<<grid, 256, ChunkSizes<HD>::kLds, st>>>(a, lo, p);
   return hipGetLastError();
+}
+
+template <int HD>
+hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
+  if (a.c.page >= kTile) return launch_pages<HD, true>(a, lo, p, st);
+  return launch_pages<HD, false>(a, lo, p, st);
 }
 
 }  // namespace

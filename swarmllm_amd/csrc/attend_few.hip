@@ -11,7 +11,7 @@
 // of positions 16 g .. 16 g + 15: as they stand they are the second product's
 // operand, and a lane's V operand is 16 consecutive bytes of a V row. No
 // score, key or value passes through LDS; the running maximum, the sum and
-// the rescaling of O all belong to the lane's own column. The 4 waves of a
+// the rescaling of O all belong to the lane's own column. The waves of a
 // workgroup take steps in turn, joined at the end through LDS; a long context
 // is cut into parts of the same kind, joined by attend_join_kernel.
 #include "attend.h"
@@ -26,20 +26,22 @@ struct FewSizes {
   static constexpr int kTail = HD % 64 ? 1 : 0;  // a 32-dim group behind them, 8 dims a lane
   static constexpr int kSteps = HD / 32;       // matrix products of a score
   static constexpr int kDims = HD / 16;        // 16-dim tiles of the output
-  // dims that go through LDS at a time when the waves join
-  static constexpr int kJoin = HD < 128 ? HD : 128;
 };
 
+// NT tiles of 16 query rows.
 template <int HD, int NT>
-__global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_rows, int hi_rows, AttendParts parts) {
+__global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a, int lo_rows, int hi_rows, AttendParts parts) {
   using Z = FewSizes<HD>;
-  constexpr int kJoinRow = Z::kJoin + 4;  // a row of the join buffer, padded off the banks of the next
-  __shared__ float s_o[4][16][kJoinRow];
-  __shared__ float s_m[4][16 * NT], s_l[4][16 * NT];
+  constexpr int W = kFewWaves;
+  constexpr int kJoin = HD < 128 ? HD : 128;  // dims that go through LDS at a time when the waves join
+  static_assert(kJoin % 16 == 0 && HD % kJoin == 0, "whole tiles of 16 dims");
+  constexpr int kJoinRow = kJoin + 4;  // padded off the banks of the next row
+  __shared__ float s_o[W][16][kJoinRow];
+  __shared__ float s_m[W][16 * NT], s_l[W][16 * NT];
   const CachePlanes& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, g = lane >> 4;
-  const int part = blockIdx.y, b = blockIdx.x / c.heads, kvh = blockIdx.x - b * c.heads;
+  const int kvh = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
   int64_t q0;
   int nq, kv;
   sequence(a, b, q0, nq, kv);
@@ -49,26 +51,20 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
   // this workgroup's steps: its part of [first position any row sees, kv)
   const int pos0 = kv - nq;  // of the first new token; negative where it stands before the cache
   const int lo = first_seen(a, pos0 < 0 ? 0 : pos0);
-  const int t0 = lo / kTile, tiles = (kv + kTile - 1) / kTile - t0;
-  const int begin = t0 + (int)((int64_t)tiles * part / parts.parts);
-  const int end = t0 + (int)((int64_t)tiles * (part + 1) / parts.parts);
+  int begin, end;
+  part_steps(lo, kv, part, parts.parts, begin, end);
 
   // queries: lane (column, g) holds the dims its keys' lanes hold
   h8v q[NT][Z::kSteps];
   int pos[NT];
 #pragma unroll
   for (int n = 0; n < NT; n++) {
-    const int r = 16 * n + col, i = r / a.group;
+    const int r = 16 * n + col, i = token_of(a, r);
     pos[n] = pos0 + i;
     const int64_t e = (q0 + i) * a.qs + (int64_t)(kvh * a.group + r - i * a.group) * a.qhs;
-#pragma unroll
-    for (int s = 0; s < Z::kSteps; s++) {
-      const int d = s < 2 * Z::kWide ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 64 * Z::kWide + 8 * g;
-      if (r < rows)
-        q[n][s] = query8(a.q, a.qdt, e + d, a.scale * kLog2e);
-      else
-        q[n][s] = h8v{};
-    }
+    load_query<Z::kSteps>(a, r < rows, [&](int s) {
+      return e + (s < 2 * Z::kWide ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 64 * Z::kWide + 8 * g);
+    }, q[n]);
   }
 
   f4v o[NT][Z::kDims];
@@ -84,7 +80,7 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
   const int ka = col >> 2;  // the 16-position chunk of the lane's K rows; its V chunk is g
   int kp = begin + wave < end ? page_of(a, b, (begin + wave) * kTile + 16 * ka, kv) : -1;
   int vp = begin + wave < end ? page_of(a, b, (begin + wave) * kTile + 16 * g, kv) : -1;
-  for (int tile = begin + wave; tile < end; tile += 4) {
+  for (int tile = begin + wave; tile < end; tile += W) {
     const int j0 = tile * kTile;
     const bool k_there = kp >= 0, v_there = vp >= 0;
     const int64_t kph = (int64_t)(k_there ? kp : 0) * c.heads + kvh, vph = (int64_t)(v_there ? vp : 0) * c.heads + kvh;
@@ -93,38 +89,68 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
     const uint16_t* ks = c.k_scales + (kph * c.page + kat) * (HD / 32);
     const int8_t* vc = c.v_codes + (vph * HD + col) * c.page + vat;
     const uint16_t* vs = c.v_scales + vph * (HD / 32) * c.page + vat;
-    if (tile + 4 < end) {
-      kp = page_of(a, b, j0 + 4 * kTile + 16 * ka, kv);
-      vp = page_of(a, b, j0 + 4 * kTile + 16 * g, kv);
+    if (tile + W < end) {
+      kp = page_of(a, b, j0 + W * kTile + 16 * ka, kv);
+      vp = page_of(a, b, j0 + W * kTile + 16 * g, kv);
     }
     // whether some position of the step is hidden from some row (the same for the wave)
     const bool partial = j0 + kTile - 1 > pos0 || (a.window > 0 && j0 <= (int64_t)kv - 1 - a.window) ||
                          __ballot(!k_there) != 0;
 
+    // the step's planes, all of them in flight at once
+    uint4 wide[4][Z::kWide ? Z::kWide : 1];
+    uint2 tail[4];
+    uint32_t sc[4][Z::kWide + Z::kTail];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int u = 0; u < Z::kWide; u++) wide[t][u] = *(const uint4*)(kc + 4 * t * HD + 64 * u + 16 * g);
+      const uint16_t* kst = ks + 4 * t * (HD / 32);
+      if constexpr (Z::kTail) {
+        tail[t] = *(const uint2*)(kc + 4 * t * HD + 64 * Z::kWide + 8 * g);
+#pragma unroll
+        for (int u = 0; u < Z::kWide; u++) sc[t][u] = kst[2 * u + (g >> 1)];
+        sc[t][Z::kWide] = kst[2 * Z::kWide];
+      } else if constexpr (Z::kWide == 1) {
+        sc[t][0] = *(const uint32_t*)kst >> (16 * (g >> 1));
+      } else if constexpr (Z::kWide == 2) {
+        const uint2 w = *(const uint2*)kst;
+        sc[t][0] = w.x >> (16 * (g >> 1));
+        sc[t][1] = w.y >> (16 * (g >> 1));
+      } else {
+        const uint4 w = *(const uint4*)kst;
+        sc[t][0] = w.x >> (16 * (g >> 1));
+        sc[t][1] = w.y >> (16 * (g >> 1));
+        sc[t][2] = w.z >> (16 * (g >> 1));
+        sc[t][3] = w.w >> (16 * (g >> 1));
+      }
+    }
+    // (the scales of 256 dims would not fit the registers beside their codes)
+    constexpr bool kScalesToo = HD <= 128;
+    uint4 vw[Z::kDims], vd[kScalesToo ? Z::kDims : 1];
+#pragma unroll
+    for (int d = 0; d < Z::kDims; d++) {
+      vw[d] = *(const uint4*)(vc + 16 * d * c.page);
+      if constexpr (kScalesToo) vd[d] = *(const uint4*)(vs + (d >> 1) * c.page + 8 * (d & 1));
+    }
+
     f4v s[NT][4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      uint4 wide[Z::kWide];
-      h2v sc[Z::kWide];
-#pragma unroll
-      for (int u = 0; u < Z::kWide; u++) {
-        wide[u] = *(const uint4*)(kc + 4 * t * HD + 64 * u + 16 * g);
-        sc[u] = both(ks[4 * t * (HD / 32) + 2 * u + (g >> 1)]);
-      }
 #pragma unroll
       for (int n = 0; n < NT; n++) s[n][t] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < Z::kWide; u++) {
-        const h8v k0 = key8(wide[u].x, wide[u].y, sc[u]), k1 = key8(wide[u].z, wide[u].w, sc[u]);
+        const h2v d = both(sc[t][u]);
+        const h8v k0 = key8(wide[t][u].x, wide[t][u].y, d), k1 = key8(wide[t][u].z, wide[t][u].w, d);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][2 * u], s[n][t], 0, 0, 0);
           s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[n][2 * u + 1], s[n][t], 0, 0, 0);
         }
       }
-      if (Z::kTail) {
-        const uint2 w = *(const uint2*)(kc + 4 * t * HD + 64 * Z::kWide + 8 * g);
-        const h8v k0 = key8(w.x, w.y, both(ks[4 * t * (HD / 32) + 2 * Z::kWide]));
+      if constexpr (Z::kTail) {
+        const h8v k0 = key8(tail[t].x, tail[t].y, both(sc[t][Z::kWide]));
 #pragma unroll
         for (int n = 0; n < NT; n++)
           s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][Z::kSteps - 1], s[n][t], 0, 0, 0);
@@ -150,33 +176,41 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) mt = fmaxf(mt, s[n][t][i]);
-      mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
-      mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
-      const float mn = fmaxf(m[n], mt), base = mn == -INFINITY ? 0.0f : mn;
-      const float f = exp2_fast(m[n] - base);
-      m[n] = mn;
+      if (__ballot((mt - m[n]) * a.sc > kSlack) != 0) {
+        mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
+        const float mn = fmaxf(m[n], mt), f = exp2_fast((m[n] - (mn == -INFINITY ? 0.0f : mn)) * a.sc);
+        m[n] = mn;
+        l[n] *= f;
+#pragma unroll
+        for (int d = 0; d < Z::kDims; d++) o[n][d] *= f;
+      }
+      const float bs = m[n] == -INFINITY ? 0.0f : m[n] * a.sc;
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float w = exp2_fast(s[n][t][i] - base);
+          const float w = exp2_fast(__builtin_fmaf(s[n][t][i], a.sc, -bs));
           sum += w;
           p[n][t >> 1][4 * (t & 1) + i] = (_Float16)w;
         }
-      l[n] = l[n] * f + sum;
-#pragma unroll
-      for (int d = 0; d < Z::kDims; d++) o[n][d] *= f;
+      l[n] += sum;
     }
 
     // values
     uint4 d0 = make_uint4(0, 0, 0, 0), d1 = d0;
 #pragma unroll
     for (int d = 0; d < Z::kDims; d++) {
-      const uint4 w = *(const uint4*)(vc + 16 * d * c.page);
+      const uint4 w = vw[d];
       if ((d & 1) == 0) {
-        d0 = *(const uint4*)(vs + (d >> 1) * c.page);
-        d1 = *(const uint4*)(vs + (d >> 1) * c.page + 8);
+        if constexpr (kScalesToo) {
+          d0 = vd[d];
+          d1 = vd[d + 1];
+        } else {
+          d0 = *(const uint4*)(vs + (d >> 1) * c.page);
+          d1 = *(const uint4*)(vs + (d >> 1) * c.page + 8);
+        }
         if (partial) {
           const int hi = v_there ? kv : 0;
           d0 = cut_scales(d0, j0 + 16 * g, lo, hi);
@@ -198,45 +232,45 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
     l[n] += __shfl_xor(l[n], 16, kWave);
     l[n] += __shfl_xor(l[n], 32, kWave);
     if (g == 0) {
-      s_m[wave][16 * n + col] = m[n];
+      s_m[wave][16 * n + col] = m[n] * a.sc;
       s_l[wave][16 * n + col] = l[n];
     }
   }
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int h = 0; h < HD; h += Z::kJoin) {
+    for (int h = 0; h < HD; h += kJoin) {
       __syncthreads();
 #pragma unroll
-      for (int d = 0; d < Z::kJoin / 16; d++) *(f4v*)&s_o[wave][col][16 * d + 4 * g] = o[n][h / 16 + d];
+      for (int d = 0; d < kJoin / 16; d++) *(f4v*)&s_o[wave][col][16 * d + 4 * g] = o[n][h / 16 + d];
       __syncthreads();
       // 4 dims a thread
-      for (int x = threadIdx.x; x < 16 * (Z::kJoin / 4); x += 256) {
-        const int r16 = x / (Z::kJoin / 4), e = 4 * (x - r16 * (Z::kJoin / 4)), r = 16 * n + r16;
+      for (int x = threadIdx.x; x < 16 * (kJoin / 4); x += 64 * W) {
+        const int r16 = x / (kJoin / 4), e = 4 * (x - r16 * (kJoin / 4)), r = 16 * n + r16;
         if (r >= rows) continue;
-        float mw[4], top = -INFINITY, sum = 0.0f;
+        float mw[W], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
           mw[w] = s_m[w][r];
           top = fmaxf(top, mw[w]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
         f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
           const float f = exp2_fast(mw[w] - base);
           sum += s_l[w][r] * f;
           acc += *(const f4v*)&s_o[w][r16][e] * f;
         }
         if (parts.parts > 1) {
-          const int64_t pr = part_row(parts, (int64_t)blockIdx.x, 0, part, r);
+          const int64_t pr = part_row(parts, (int64_t)b * c.heads + kvh, 0, part, r);
           *(f4v*)(parts.o + pr * HD + h + e) = acc;
           if (h + e == 0) {
             parts.ml[2 * pr] = top;
             parts.ml[2 * pr + 1] = sum;
           }
         } else {
-          const int i = r / a.group, head = kvh * a.group + r - i * a.group;
+          const int i = token_of(a, r), head = kvh * a.group + r - i * a.group;
           float out[4];
           finish_row<4>(a, head, top, sum, (const float*)&acc, out);
           store_out4(a, (q0 + i) * a.os + (int64_t)head * HD + h + e, out);
@@ -247,11 +281,11 @@ __global__ __launch_bounds__(256) void attend_few_kernel(AttendArgs a, int lo_ro
 
 template <int HD>
 hipError_t launch_hd(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
-  const dim3 grid((unsigned)(a.seqs * a.c.heads), (unsigned)p.parts);
+  const dim3 grid((unsigned)a.c.heads, (unsigned)p.parts, (unsigned)a.seqs);
   if (hi <= 16)
-    attend_few_kernel<HD, 1><<<grid, 256, 0, st>>>(a, lo, hi, p);
+    attend_few_kernel<HD, 1><<<grid, 64 * kFewWaves, 0, st>>>(a, lo, hi, p);
   else
-    attend_few_kernel<HD, 2><<<grid, 256, 0, st>>>(a, lo, hi, p);
+    attend_few_kernel<HD, 2><<<grid, 64 * kFewWaves, 0, st>>>(a, lo, hi, p);
   return hipGetLastError();
 }
 

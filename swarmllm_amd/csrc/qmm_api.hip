@@ -1075,7 +1075,7 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   if (!cache_ok(cache) || need == nullptr || !qmm::value_type_ok(q_dtype) || !qmm::value_type_ok(out_dtype) ||
       heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || tokens < 0 || seqs < 0 || seqs > 65535 ||
       max_q < 0 || max_kv < 0 || table_stride < 0 || window < 0 || q_head_stride < cache->head_dim || q_stride < 0 ||
-      out_stride < (int64_t)heads * cache->head_dim || max_q > INT32_MAX || scale != scale)
+      out_stride < (int64_t)heads * cache->head_dim || max_q > INT32_MAX || !(scale >= -1e30f && scale <= 1e30f))
     return QMM_UNSUPPORTED;
   *need = 0;
   if (tokens == 0 || seqs == 0 || max_q == 0) return QMM_OK;
@@ -1091,8 +1091,13 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   if (table_stride > kMostPositions / cache->page) return QMM_UNSUPPORTED;
   const int64_t cap = table_stride * cache->page;
   a.max_kv = (int)(max_kv < cap ? max_kv : cap);
-  a.qdt = q_dtype; a.odt = out_dtype; a.scale = scale;
+  a.qdt = q_dtype; a.odt = out_dtype;
+  a.sc = scale == 0.0f ? 1.0f : (scale < 0.0f ? -scale : scale) * 1.4426950408889634f;
+  a.q_sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
+  const int64_t q16 = 16 / qmm::value_bytes(q_dtype);
+  a.q_vec = (uintptr_t)q % 16 == 0 && q_stride % q16 == 0 && q_head_stride % q16 == 0;
   a.out_vec = (uintptr_t)out % (4 * qmm::value_bytes(out_dtype)) == 0 && out_stride % 4 == 0;
+  a.group_inv = a.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + a.group - 1) / a.group) : 0;
   a.page_bits = __builtin_ctz((unsigned)cache->page);
   if (!qmm::attend_fits(a)) return QMM_UNSUPPORTED;
   *need = qmm::attend_workspace_bytes(a, cu_count());

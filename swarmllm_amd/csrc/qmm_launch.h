@@ -299,8 +299,11 @@ struct AttendArgs {
   const float* sinks;
   int64_t qs, qhs, os, table_stride, tokens, window;
   int seqs, heads, group, max_q, max_kv, qdt, odt, page_bits;
+  uint32_t group_inv;  // ceil(2^32 / group), 0 for a group of 1
+  bool q_vec;    // q's heads lie at multiples of 16 bytes
   bool out_vec;  // out's rows lie at multiples of 4 values
-  float scale;
+  float sc;      // |scale| log2(e) (1 for a scale of 0): exp(scale x) = 2^(sc q_sign x)
+  float q_sign;  // the scale's sign: 1, -1 or 0
 };
 bool attend_fits(const AttendArgs& a);
 size_t attend_workspace_bytes(const AttendArgs& a, int cus);

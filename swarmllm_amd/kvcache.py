@@ -6,12 +6,13 @@ kernels/decode_attn.cu:257-612 and its paged attention.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
 
-from ._lib import Cache, QmmError, check, lib
-from .qtensor import _X_DTYPES, on_device
+from ._lib import X_F16, Cache, QmmError, check, lib
+from .qtensor import _X_DTYPES, on_device, raw_stream
 
 
 class KvCache:
@@ -28,19 +29,21 @@ class KvCache:
         if k_codes.dim() != 4:
             raise ValueError(f"KvCache: k_codes [pages, kv_heads, page, head_dim], not {tuple(k_codes.shape)}")
         pages, heads, page, hd = k_codes.shape
+        self.device = k_codes.device
+        ptrs = []
         for name, t, shape, dt in (("k_codes", k_codes, (pages, heads, page, hd), torch.int8),
                                    ("k_scales", k_scales, (pages, heads, page, hd // 32), torch.float16),
                                    ("v_codes", v_codes, (pages, heads, hd, page), torch.int8),
                                    ("v_scales", v_scales, (pages, heads, hd // 32, page), torch.float16)):
-            if t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda \
-                    or t.device != k_codes.device or t.data_ptr() % 16:
+            ptrs.append(t.data_ptr())
+            if t.dtype != dt or t.shape != shape or not t.is_contiguous() or not t.is_cuda \
+                    or t.device != self.device or ptrs[-1] % 16:
                 raise ValueError(f"KvCache: {name} must be contiguous, 16-byte aligned {dt} {shape} on one GPU, not "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
         _plane_bytes(pages, heads, hd, page)
         self.planes = (k_codes, k_scales, v_codes, v_scales)
         self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, hd
-        self.device = k_codes.device
-        self._c = Cache(*(t.data_ptr() for t in self.planes), pages, heads, hd, page)
+        self._c = Cache(*ptrs, pages, heads, hd, page)
         self._ref = ctypes.byref(self._c)
 
     @staticmethod
@@ -65,7 +68,7 @@ class KvCache:
         tokens = slots.numel()
         self._slots("write", slots)
         for name, t in (("k", k), ("v", v)):
-            if tuple(t.shape) != (tokens, self.kv_heads, self.head_dim) or t.dtype not in _X_DTYPES \
+            if t.shape != (tokens, self.kv_heads, self.head_dim) or t.dtype not in _X_DTYPES \
                     or t.dtype != k.dtype or t.device != self.device:
                 raise ValueError(f"KvCache.write: {name} [{tokens}, {self.kv_heads}, {self.head_dim}] f32, f16 or bf16 "
                                  f"on {self.device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -76,7 +79,7 @@ class KvCache:
         with on_device(self.device):
             check("qmm_cache_write", lib().qmm_cache_write(self._ref, k.data_ptr(), ks, khs, v.data_ptr(), vs, vhs,
                                                            _X_DTYPES[k.dtype], slots.data_ptr(), tokens,
-                                                           torch.cuda.current_stream().cuda_stream))
+                                                           raw_stream(self.device)))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values [tokens, kv_heads, head_dim] of `slots` (int64
@@ -91,7 +94,7 @@ class KvCache:
             with on_device(self.device):
                 check("qmm_cache_read", lib().qmm_cache_read(self._ref, slots.data_ptr(), tokens, k.data_ptr(),
                                                              v.data_ptr(), _X_DTYPES[dtype],
-                                                             torch.cuda.current_stream().cuda_stream))
+                                                             raw_stream(self.device)))
         return k, v
 
     def attend(self, q: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor, tables: torch.Tensor,
@@ -118,42 +121,46 @@ class KvCache:
         tokens, heads, hd = q.shape
         seqs = kv_lens.numel()
         for name, t, shape in (("q_starts", q_starts, (seqs + 1,)), ("kv_lens", kv_lens, (seqs,))):
-            if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.device or not t.is_contiguous():
+            if t.dtype != torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
                 raise ValueError(f"KvCache.attend: {name} must be contiguous int32 {shape} on {self.device}, not "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
         if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != seqs or tables.device != self.device \
                 or not tables.is_contiguous():
             raise ValueError(f"KvCache.attend: tables must be contiguous int32 [{seqs}, pages] on {self.device}, not "
                              f"{tables.dtype} {tuple(tables.shape)} on {tables.device}")
+        if out_dtype is not None and out_dtype not in _X_DTYPES:
+            raise ValueError(f"KvCache.attend: out_dtype f16, bf16 or f32, not {out_dtype}")
         if max_q < 0 or window < 0 or (max_kv is not None and max_kv < 0):
             raise ValueError(f"KvCache.attend: max_q {max_q}, max_kv {max_kv}, window {window}")
-        if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (heads,)
+        if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,)
                                   or sinks.device != self.device or not sinks.is_contiguous()):
             raise ValueError(f"KvCache.attend: sinks must be {heads} contiguous f32 on {self.device}")
         if out is None:
             out = torch.empty((tokens, heads, hd), dtype=out_dtype or q.dtype, device=self.device)
         elif out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"KvCache.attend: out is {out.dtype}, not {out_dtype}")
-        if tuple(out.shape) != (tokens, heads, hd) or out.dtype not in _X_DTYPES or out.device != self.device \
-                or (tokens and (out.stride(2) != 1 or out.stride(1) != hd)) or (tokens > 1 and out.stride(0) < heads * hd):
+        elif out.shape != (tokens, heads, hd) or out.dtype not in _X_DTYPES or out.device != self.device \
+                or (tokens and (out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd))) \
+                or (tokens > 1 and out.stride(0) < heads * hd):
             raise ValueError(f"KvCache.attend: out [{tokens}, {heads}, {hd}] f16, bf16 or f32, rows of consecutive "
                              f"values, not {out.dtype} {tuple(out.shape)} strides {out.stride()}")
         if tokens == 0 or seqs == 0:
             return out
         qs, qhs = self._strides("attend", "q", q)
-        L, need = lib(), ctypes.c_size_t(0)
-        head = (self._ref, q.data_ptr(), _X_DTYPES[q.dtype], qs, qhs, tokens, heads, q_starts.data_ptr(),
-                kv_lens.data_ptr(), tables.data_ptr(), tables.shape[1], seqs, max_q,
-                tables.shape[1] * self.page if max_kv is None else max_kv, hd ** -0.5 if scale is None else scale,
-                window, sinks.data_ptr() if sinks is not None else None, out.data_ptr(), _X_DTYPES[out.dtype],
-                out.stride(0) if tokens > 1 else heads * hd)
+        if max_kv is None:
+            max_kv = tables.shape[1] * self.page
         with on_device(self.device):
-            st = torch.cuda.current_stream().cuda_stream
-            check("qmm_attend", L.qmm_attend(*head, None, 0, ctypes.byref(need), 0, st))
+            need = _attend_need(self.device.index, self.pages, self.kv_heads, hd, self.page, tokens, heads,
+                                tables.shape[1], seqs, max_q, max_kv, window)
+            size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
-            ws = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-            check("qmm_attend", L.qmm_attend(*head, ws.data_ptr() if ws is not None else None, need.value,
-                                             ctypes.byref(need), 1, st))
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            check("qmm_attend", lib().qmm_attend(
+                self._ref, q.data_ptr(), _X_DTYPES[q.dtype], qs, qhs, tokens, heads, q_starts.data_ptr(),
+                kv_lens.data_ptr(), tables.data_ptr(), tables.shape[1], seqs, max_q, max_kv,
+                hd ** -0.5 if scale is None else scale, window, None if sinks is None else sinks.data_ptr(),
+                out.data_ptr(), _X_DTYPES[out.dtype], out.stride(0) if tokens > 1 else heads * hd,
+                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(self.device)))
         return out
 
     def _slots(self, name: str, slots: torch.Tensor) -> None:
@@ -177,6 +184,20 @@ class KvCache:
         return f"KvCache[{self.pages} pages of {self.page}, {self.kv_heads} heads of {self.head_dim}; Q8_0]"
 
 
+@functools.lru_cache(maxsize=1024)
+def _attend_need(device: int, pages: int, kv_heads: int, head_dim: int, page: int, tokens: int, heads: int,
+                 table_pages: int, seqs: int, max_q: int, max_kv: int, window: int) -> int:
+    """The workspace bytes that qmm_attend plans on the current device (`device`): by the sizes alone."""
+    some = 256  # any aligned address: planning reads none
+    c, need = Cache(some, some, some, some, pages, kv_heads, head_dim, page), ctypes.c_size_t(0)
+    row = heads * head_dim
+    check("qmm_attend", lib().qmm_attend(ctypes.byref(c), None, X_F16, row, head_dim, tokens, heads, None, None, None,
+                                         table_pages, seqs, max_q, max_kv, 1.0, window, None, None, X_F16, row, None,
+                                         0, ctypes.byref(need), 0, 0))
+    return need.value
+
+
+@functools.lru_cache(maxsize=64)
 def _plane_bytes(pages: int, kv_heads: int, head_dim: int, page: int) -> Tuple[int, int]:
     """Bytes of a codes and of a scales plane; ValueError for sizes not covered."""
     codes, scales = ctypes.c_size_t(0), ctypes.c_size_t(0)

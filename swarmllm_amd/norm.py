@@ -9,7 +9,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import X_F32, check, lib
-from .qtensor import _X_DTYPES, GgmlDType, QAct, on_device
+from .qtensor import _X_DTYPES, GgmlDType, QAct, on_device, raw_stream
 
 
 class NormOut(NamedTuple):
@@ -21,15 +21,14 @@ class NormOut(NamedTuple):
     y: Optional[torch.Tensor]
 
 
-def _rows(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
-    """The distance of t's rows, checked against x (`like`)."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"rms_norm_act: {name} {tuple(t.shape)} {t.dtype} on {t.device}, x is {tuple(like.shape)} "
-                         f"{like.dtype} on {like.device}")
-    k = t.shape[-1]
+def _rows(name: str, t: torch.Tensor, x: torch.Tensor) -> int:
+    """The distance of t's rows, t checked against x."""
+    if t is not x and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+        raise ValueError(f"rms_norm_act: {name} {tuple(t.shape)} {t.dtype} on {t.device}, x is {tuple(x.shape)} "
+                         f"{x.dtype} on {x.device}")
     if t.is_contiguous():
-        return k
-    if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < k:
+        return t.shape[-1]
+    if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         raise ValueError(f"rms_norm_act: {name} needs rows of consecutive values, not strides {t.stride()}")
     return t.stride(0)
 
@@ -45,14 +44,15 @@ def rms_norm_act(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Op
     a tensor to write the stream to, which can be x or residual itself;
     without a residual the stream is x. y_dtype asks for y too, as f32, f16 or
     bf16. The activation equals QAct.quantize of the f32 y bit for bit."""
-    if x.dtype not in _X_DTYPES or not x.is_cuda or x.dim() < 1:
+    code = _X_DTYPES.get(x.dtype)
+    if code is None or not x.is_cuda or x.dim() < 1:
         raise ValueError(f"rms_norm_act: an f32, f16 or bf16 tensor on the GPU, not {x.dtype} on {x.device}")
-    k = x.shape[-1]
+    shape, device = x.shape, x.device
+    k = shape[-1]
     if k < 1 or k % 4:
         raise ValueError(f"rms_norm_act: rows of {k} values (a multiple of 4 is needed)")
-    if weight.dtype != torch.float32 or tuple(weight.shape) != (k,) or weight.device != x.device \
-            or not weight.is_contiguous():
-        raise ValueError(f"rms_norm_act: weight must be {k} contiguous f32 on {x.device}")
+    if weight.dtype != torch.float32 or weight.shape != (k,) or weight.device != device or not weight.is_contiguous():
+        raise ValueError(f"rms_norm_act: weight must be {k} contiguous f32 on {device}")
     if not eps >= 0.0:
         raise ValueError(f"rms_norm_act: eps {eps}")
     if dtype is None and y_dtype is None:
@@ -60,21 +60,24 @@ def rms_norm_act(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Op
     if y_dtype is not None and y_dtype not in _X_DTYPES:
         raise ValueError(f"rms_norm_act: y_dtype f32, f16 or bf16, not {y_dtype}")
     xs = _rows("x", x, x)
-    rs = _rows("residual", residual, x) if residual is not None else 0
-    given = h
+    hp = rp = None
+    rs = hs = k
+    if residual is not None:
+        rp, rs = residual.data_ptr(), _rows("residual", residual, x)
+        if h is None:
+            h = torch.empty(shape, dtype=x.dtype, device=device)
     if h is None:
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else x
-    hs = _rows("h", h, x)
+        h = x
+    else:
+        hp, hs = h.data_ptr(), _rows("h", h, x)
+    act = QAct.alloc(shape, QAct.layout_of(dtype), device) if dtype is not None else None
+    y = torch.empty(shape, dtype=y_dtype, device=device) if y_dtype is not None else None
     rows = x.numel() // k
-    act = QAct.alloc(x.shape, QAct.layout_of(dtype), x.device) if dtype is not None else None
-    y = torch.empty(x.shape, dtype=y_dtype, device=x.device) if y_dtype is not None else None
     if rows:
-        keep = residual is not None or given is not None
-        with on_device(x.device):
+        with on_device(device):
             check("qmm_rms_norm_act", lib().qmm_rms_norm_act(
-                x.data_ptr(), _X_DTYPES[x.dtype], xs, residual.data_ptr() if residual is not None else None, rs,
-                weight.data_ptr(), eps, h.data_ptr() if keep else None, hs,
-                act.data_.data_ptr() if act is not None else None, act.layout if act is not None else 0,
-                y.data_ptr() if y is not None else None, _X_DTYPES[y_dtype] if y is not None else X_F32, k, k, rows,
-                torch.cuda.current_stream().cuda_stream))
+                x.data_ptr(), code, xs, rp, rs, weight.data_ptr(), eps, hp, hs,
+                None if act is None else act.data_.data_ptr(), 0 if act is None else act.layout,
+                None if y is None else y.data_ptr(), X_F32 if y is None else _X_DTYPES[y_dtype], k, k, rows,
+                raw_stream(device)))
     return NormOut(act, h, y)

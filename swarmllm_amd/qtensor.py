@@ -14,6 +14,8 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import functools
+import math
 import os
 import warnings
 from contextlib import nullcontext
@@ -58,9 +60,34 @@ def _ptr(t: torch.Tensor) -> int:
     return t.data_ptr()
 
 
+_HERE = nullcontext()
+
+
 def on_device(device: torch.device):
     """A context in which `device` is the current one (no switch where it is already)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def raw_stream(device: torch.device) -> int:
+    """The hipStream_t of device's current stream (torch.cuda.current_stream
+    makes a Stream object around it: 2 us of a call's 10)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=1024)
+def _act_bytes(layout: int, k: int, rows: int) -> int:
+    """qmm_act_bytes (0 rows: 0); ValueError for rows that are no whole number of blocks."""
+    if rows == 0:
+        return 0
+    n = lib().qmm_act_bytes(layout, k, rows)
+    if n == 0:
+        raise ValueError(f"QAct: rows of {k} values are not a whole number of blocks")
+    return n
+
+
+@functools.lru_cache(maxsize=None)
+def _act_layout(dtype: int) -> int:
+    return lib().qmm_act_layout(dtype, 1)
 
 
 def fill_normal(n: int, seed: int, mean: float = 0.0, std: float = 1.0, device="cuda") -> torch.Tensor:
@@ -326,36 +353,35 @@ class QAct:
         shape = tuple(int(d) for d in shape)
         if len(shape) < 1 or layout not in (_lib.ACT_Q8K, _lib.ACT_Q8_0):
             raise ValueError(f"QAct: shape {shape}, layout {layout}")
-        self.k = shape[-1]
-        self.rows = 1
-        for d in shape[:-1]:
-            self.rows *= d
-        want = lib().qmm_act_bytes(layout, self.k, self.rows) if self.rows else 0
-        if (self.rows and want == 0) or data.dtype != torch.uint8 or data.numel() < want or not data.is_cuda \
-                or not data.is_contiguous() or data.data_ptr() % 16:
+        self._set(data, shape, layout)
+        want = _act_bytes(layout, self.k, self.rows)
+        if data.dtype != torch.uint8 or data.numel() < want or not data.is_cuda or not data.is_contiguous() \
+                or data.data_ptr() % 16:
             raise ValueError(f"QAct: {data.numel()} {data.dtype} device bytes for {list(shape)} (want {want}, 16-byte "
                              "aligned)")
+
+    def _set(self, data, shape, layout) -> None:
         self.data_ = data
         self.shape = shape
         self.layout = layout
+        self.k = shape[-1]
+        self.rows = math.prod(shape[:-1])
 
     @staticmethod
     def layout_of(dtype: GgmlDType) -> int:
         """The layout that products of a weight type read (qmm_act_layout)."""
-        layout = lib().qmm_act_layout(int(GgmlDType(dtype)), 1)
+        layout = _act_layout(int(dtype))
         if layout < 0:
             raise ValueError(f"no quantized activation for {GgmlDType(dtype).name} weights")
         return layout
 
     @staticmethod
     def alloc(shape: Sequence[int], layout: int, device="cuda") -> "QAct":
-        rows = 1
-        for d in shape[:-1]:
-            rows *= int(d)
-        nbytes = lib().qmm_act_bytes(layout, int(shape[-1]), rows) if rows else 0
-        if rows and nbytes == 0:
-            raise ValueError(f"QAct.alloc: rows of {shape[-1]} values are not a whole number of blocks")
-        return QAct(torch.empty(nbytes, dtype=torch.uint8, device=device), shape, layout)
+        shape = tuple(shape)
+        out = QAct.__new__(QAct)  # what __init__ checks holds for a buffer made here
+        out._set(torch.empty(_act_bytes(layout, shape[-1], math.prod(shape[:-1])), dtype=torch.uint8, device=device),
+                 shape, layout)
+        return out
 
     @staticmethod
     def quantize(x: torch.Tensor, dtype: GgmlDType) -> "QAct":
@@ -377,11 +403,13 @@ class QAct:
         """The values it stands for, code * scale (qmm_dequantize_act), as f32, f16 or bf16."""
         if dtype not in _X_DTYPES:
             raise ValueError(f"QAct.dequantize: f32, f16 or bf16, not {dtype}")
-        out = torch.empty(self.shape, dtype=dtype, device=self.data_.device)
-        if out.numel():
-            with on_device(out.device):
-                check("qmm_dequantize_act", lib().qmm_dequantize_act(_ptr(self.data_), self.layout, _ptr(out),
-                                                                     _X_DTYPES[dtype], self.k, self.rows, _stream()))
+        device = self.data_.device
+        out = torch.empty(self.shape, dtype=dtype, device=device)
+        if self.rows:
+            with on_device(device):
+                check("qmm_dequantize_act", lib().qmm_dequantize_act(self.data_.data_ptr(), self.layout, out.data_ptr(),
+                                                                     _X_DTYPES[dtype], self.k, self.rows,
+                                                                     raw_stream(device)))
         return out
 
     def dequantize_f16(self) -> torch.Tensor:
