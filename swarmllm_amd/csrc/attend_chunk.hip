@@ -20,10 +20,17 @@ namespace qmm {
 
 namespace {
 
+// Instruction classes of __builtin_amdgcn_sched_group_barrier.
+constexpr int kMfma = 0x008, kDsRead = 0x100;
+constexpr int kAhead = 4;  // LDS reads of operands in flight ahead of their products
+
 template <int HD>
 struct ChunkSizes {
-  static constexpr int kPieces = kTile * HD / 16;           // 16-code pieces of a step's keys (and values)
-  static constexpr int kEach = (kPieces + 255) / 256;       // a thread's
+  // a step's keys (and values) in items of 32: the 32 dims of a block for one
+  // position, 16 positions of two dims of a block; one scale, 16 scales
+  static constexpr int kItems = kTile * HD / 32;
+  static constexpr bool kHalves = kItems * 2 <= 256;        // half the threads take keys, half values
+  static constexpr int kEach = (kItems + 255) / 256;        // a thread's of either
   static constexpr int kRow = HD + 8;                       // f16s of a K row in LDS, padded off the next row's banks
   static constexpr int kVRow = kTile + 8;                   // and of a V row
   static constexpr int kHalfs = kTile * kRow + HD * kVRow;  // one buffer
@@ -33,9 +40,24 @@ struct ChunkSizes {
 // One step's planes in a thread's registers.
 template <int HD>
 struct Staged {
-  uint4 k[ChunkSizes<HD>::kEach], v[ChunkSizes<HD>::kEach], d0[ChunkSizes<HD>::kEach], d1[ChunkSizes<HD>::kEach];
+  uint4 k[ChunkSizes<HD>::kEach][2], v[ChunkSizes<HD>::kEach][2], d0[ChunkSizes<HD>::kEach], d1[ChunkSizes<HD>::kEach];
   uint32_t ks[ChunkSizes<HD>::kEach];
 };
+
+// A thread's i-th item of keys, or of values; on: whether it has one.
+template <int HD>
+__device__ __forceinline__ int k_item(int i, bool& on) {
+  const int x = (int)threadIdx.x + 256 * i;
+  on = ChunkSizes<HD>::kItems % 256 == 0 || x < ChunkSizes<HD>::kItems;
+  return x;
+}
+template <int HD>
+__device__ __forceinline__ int v_item(int i, bool& on) {
+  if (!ChunkSizes<HD>::kHalves) return k_item<HD>(i, on);
+  const int x = (int)threadIdx.x - 128;
+  on = x >= 0 && x < ChunkSizes<HD>::kItems;
+  return x;
+}
 
 // A step's pages. ONE: pages of 64 positions and more, so a step has one, the
 // same for the wave; otherwise lane x < 4 of every wave holds that of the step's
@@ -65,28 +87,41 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
   }
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
-    const int x = (int)threadIdx.x + 256 * i;
-    const bool on = Z::kPieces % 256 == 0 || x < Z::kPieces;
+    bool k_on, v_on;
+    const int xk = k_item<HD>(i, k_on), xv = v_item<HD>(i, v_on);
+    const int vc = xv & 3, d = 2 * (xv >> 2);  // 16 positions from 16 vc on, dims d and d + 1
     if constexpr (ONE) {
-      const uint32_t y = on ? x : 0;
-      s.k[i] = *(const uint4*)(k1 + 16 * y);
-      s.ks[i] = ks1[y >> 1];
-      s.v[i] = *(const uint4*)(v1 + (y >> 2) * (uint32_t)c.page + 16 * (y & 3));
-      const uint16_t* vs = vs1 + (y >> 7) * (uint32_t)c.page + 16 * (y & 3);
-      s.d0[i] = *(const uint4*)vs;
-      s.d1[i] = *(const uint4*)(vs + 8);
+      if (k_on) {
+        s.k[i][0] = *(const uint4*)(k1 + 32 * (uint32_t)xk);
+        s.k[i][1] = *(const uint4*)(k1 + 32 * (uint32_t)xk + 16);
+        s.ks[i] = ks1[(uint32_t)xk];
+      }
+      if (v_on) {
+        s.v[i][0] = *(const uint4*)(v1 + (uint32_t)d * (uint32_t)c.page + 16 * vc);
+        s.v[i][1] = *(const uint4*)(v1 + (uint32_t)(d + 1) * (uint32_t)c.page + 16 * vc);
+        const uint16_t* vs = vs1 + (uint32_t)(d >> 5) * (uint32_t)c.page + 16 * vc;
+        s.d0[i] = *(const uint4*)vs;
+        s.d1[i] = *(const uint4*)(vs + 8);
+      }
     } else {
-      const int row = on ? x / (HD / 16) : 0, e = on ? 16 * (x - row * (HD / 16)) : 0;
-      const int kp = __shfl(pages, row >> 4, kWave), vp = __shfl(pages, x & 3, kWave);
-      const int64_t kr = ((int64_t)(kp < 0 ? 0 : kp) * c.heads + kvh) * c.page + ((j0 + row) & (c.page - 1));
-      s.k[i] = *(const uint4*)(c.k_codes + kr * HD + e);
-      s.ks[i] = c.k_scales[kr * (HD / 32) + (e >> 5)];
-      const int64_t vph = (int64_t)(vp < 0 ? 0 : vp) * c.heads + kvh;
-      const int d = on ? x >> 2 : 0, at = (j0 + 16 * (x & 3)) & (c.page - 1);
-      s.v[i] = *(const uint4*)(c.v_codes + (vph * HD + d) * c.page + at);
-      const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
-      s.d0[i] = *(const uint4*)vs;
-      s.d1[i] = *(const uint4*)(vs + 8);
+      const int row = xk / (HD / 32), e = 32 * (xk - row * (HD / 32));
+      const int kp = __shfl(pages, (row >> 4) & 3, kWave), vp = __shfl(pages, vc, kWave);
+      if (k_on) {
+        const int64_t kr = ((int64_t)(kp < 0 ? 0 : kp) * c.heads + kvh) * c.page + ((j0 + row) & (c.page - 1));
+        s.k[i][0] = *(const uint4*)(c.k_codes + kr * HD + e);
+        s.k[i][1] = *(const uint4*)(c.k_codes + kr * HD + e + 16);
+        s.ks[i] = c.k_scales[kr * (HD / 32) + (e >> 5)];
+      }
+      if (v_on) {
+        const int64_t vph = (int64_t)(vp < 0 ? 0 : vp) * c.heads + kvh;
+        const int at = (j0 + 16 * vc) & (c.page - 1);
+        const int8_t* v = c.v_codes + (vph * HD + d) * c.page + at;
+        s.v[i][0] = *(const uint4*)v;
+        s.v[i][1] = *(const uint4*)(v + c.page);
+        const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
+        s.d0[i] = *(const uint4*)vs;
+        s.d1[i] = *(const uint4*)(vs + 8);
+      }
     }
   }
 }
@@ -98,27 +133,39 @@ __device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int 
   using Z = ChunkSizes<HD>;
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
-    const int x = (int)threadIdx.x + 256 * i;
-    const int vp = !CUT ? 0 : ONE ? pages : __shfl(pages, x & 3, kWave);
-    if (Z::kPieces % 256 != 0 && x >= Z::kPieces) continue;
-    const int row = x / (HD / 16), e = 16 * (x - row * (HD / 16));
+    bool k_on, v_on;
+    const int xk = k_item<HD>(i, k_on), xv = v_item<HD>(i, v_on);
+    const int vc = xv & 3, d = 2 * (xv >> 2);
+    const int vp = !CUT ? 0 : ONE ? pages : __shfl(pages, vc, kWave);
     H8 h;
-    const h2v ks = both(s.ks[i]);
-    h.v = key8(s.k[i].x, s.k[i].y, ks);
-    *(uint4*)(buf + row * Z::kRow + e) = h.u;
-    h.v = key8(s.k[i].z, s.k[i].w, ks);
-    *(uint4*)(buf + row * Z::kRow + e + 8) = h.u;
-    uint4 d0 = s.d0[i], d1 = s.d1[i];
-    if constexpr (CUT) {
-      const int j = j0 + 16 * (x & 3);
-      d0 = cut_scales(d0, j, lo, vp < 0 ? 0 : hi);
-      d1 = cut_scales(d1, j + 8, lo, vp < 0 ? 0 : hi);
+    if (k_on) {
+      const int row = xk / (HD / 32), e = 32 * (xk - row * (HD / 32));
+      const h2v ks = both(s.ks[i]);
+      uint16_t* kb = buf + row * Z::kRow + e;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        h.v = key8(s.k[i][u].x, s.k[i][u].y, ks);
+        *(uint4*)(kb + 16 * u) = h.u;
+        h.v = key8(s.k[i][u].z, s.k[i][u].w, ks);
+        *(uint4*)(kb + 16 * u + 8) = h.u;
+      }
     }
-    uint16_t* vb = buf + kTile * Z::kRow + (x >> 2) * Z::kVRow + 16 * (x & 3);
-    h.v = value8(s.v[i].x, s.v[i].y, d0);
-    *(uint4*)vb = h.u;
-    h.v = value8(s.v[i].z, s.v[i].w, d1);
-    *(uint4*)(vb + 8) = h.u;
+    if (v_on) {
+      uint4 d0 = s.d0[i], d1 = s.d1[i];
+      if constexpr (CUT) {
+        const int j = j0 + 16 * vc;
+        d0 = cut_scales(d0, j, lo, vp < 0 ? 0 : hi);
+        d1 = cut_scales(d1, j + 8, lo, vp < 0 ? 0 : hi);
+      }
+      uint16_t* vb = buf + kTile * Z::kRow + d * Z::kVRow + 16 * vc;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        h.v = value8(s.v[i][u].x, s.v[i][u].y, d0);
+        *(uint4*)(vb + u * Z::kVRow) = h.u;
+        h.v = value8(s.v[i][u].z, s.v[i][u].w, d1);
+        *(uint4*)(vb + u * Z::kVRow + 8) = h.u;
+      }
+    }
   }
 }
 
@@ -194,15 +241,24 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
       const uint16_t* kb = s_buf + cur * Z::kHalfs + krow * Z::kRow + 8 * hi;
       f16v s[2];
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
+      for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < HD / 16; d++) {
+      for (int d = 0; d < HD / 16; d++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
           const h8v k = *(const h8v*)(kb + 32 * t * Z::kRow + 16 * d);
           s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[d], s[t], 0, 0, 0);
         }
+      // kAhead reads in flight before the first product, then one a product
+      __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+#pragma unroll
+      for (int x = 0; x < HD / 8 - kAhead; x++) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
       const uint64_t absent = ONE ? (pages < 0 ? 15 : 0) : __ballot(pages < 0) & 15;
       if (j0 + kTile - 1 > wave_low || (a.window > 0 && j0 <= (int64_t)wave_high - a.window) || absent) {
 #pragma unroll
@@ -242,12 +298,19 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
       l += sum;
       const uint16_t* vb = s_buf + cur * Z::kHalfs + kTile * Z::kRow + col * Z::kVRow + 8 * hi;
 #pragma unroll
-      for (int d = 0; d < HD / 32; d++)
+      for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int d = 0; d < HD / 32; d++) {
           const h8v v = *(const h8v*)(vb + 32 * d * Z::kVRow + 16 * t);
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[t], o[d], 0, 0, 0);
         }
+      __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 1);
+#pragma unroll
+      for (int x = 0; x < HD / 8 - kAhead; x++) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 1);
     }
     if (tile + 1 < end) lay_step(st, tile + 1, next_pages, cur ^ 1);
     pages = next_pages;
