@@ -170,10 +170,11 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 struct AttendParts {
   float* o;
   float* ml;
-  int parts, rows, blocks;  // blocks: row blocks of a kv head of a sequence
+  int parts, rows;  // query rows of a block
+  int blocks, cut;  // row blocks of a kv head of a sequence; the first `cut` of them are in parts
 };
 __device__ __forceinline__ int64_t part_row(const AttendParts& p, int64_t head_of_seq, int block, int part, int row) {
-  return ((head_of_seq * p.blocks + block) * p.parts + part) * p.rows + row;
+  return ((head_of_seq * p.cut + block) * p.parts + part) * p.rows + row;
 }
 
 // A row's outputs from its sums of weights times values (relative to the
@@ -207,6 +208,5 @@ hipError_t launch_attend_chunk(const AttendArgs& a, int lo, const AttendParts& p
 
 constexpr int kFewWaves = 4;     // waves of a few-row workgroup
 constexpr int kFewRows = 32;     // the most query rows of the few-row kernel
-constexpr int kChunkRows = 128;  // query rows of a workgroup of the chunk kernel
 
 }  // namespace qmm

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   sequence(a, b, q0, nq, kv);
   const int rows = nq * a.group;
   const int64_t hs = (int64_t)b * a.c.heads + kvh;
-  const bool on = sub < fit && block < p.blocks && rows > lo_rows && rows <= hi_rows && row_of_head < rows;
+  const bool on = sub < fit && block < p.cut && rows > lo_rows && rows <= hi_rows && row_of_head < rows;
   float top = -INFINITY, sum = 0.0f;
   f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (on) {
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
 // How a call runs: the sequences of at most `few` query rows a kv head on the
 // few-row kernel (0: none), the others on the chunk kernel.
 struct Plan {
-  int few, few_parts, chunk_blocks, chunk_parts;
+  int few, few_parts, chunk_rows, chunk_blocks, chunk_cut, chunk_parts;
 };
 
 int clamp_parts(int64_t want, int64_t most) {
@@ -82,39 +82,51 @@ int clamp_parts(int64_t want, int64_t most) {
   return (int)(p < 1 ? 1 : p > 64 ? 64 : p);
 }
 
+// Steps that a block of `rows` query rows takes at most.
+int64_t most_steps(const AttendArgs& a, int rows) {
+  int64_t span = a.max_kv;
+  if (a.window > 0 && a.window + rows / a.group + 1 < span) span = a.window + rows / a.group + 1;
+  return (span + kTile - 1) / kTile;
+}
+
 Plan plan_of(const AttendArgs& a, int cus) {
   Plan p{};
   const int64_t rows = (int64_t)a.max_q * a.group, heads = (int64_t)a.seqs * a.c.heads;
-  int64_t span = a.max_kv;  // the positions that a row block's rows see at most
   if (rows > kFewRows) {
-    if (a.window > 0 && a.window + kChunkRows / a.group + 1 < span) span = a.window + kChunkRows / a.group + 1;
-    const int64_t tiles = (span + kTile - 1) / kTile;
-    p.chunk_blocks = (int)((rows + kChunkRows - 1) / kChunkRows);
-    // parts until two workgroups a CU are there, of 8 steps at least
-    p.chunk_parts = clamp_parts(2 * cus / (heads * p.chunk_blocks), tiles / 8);
+    // 256 rows a workgroup lay a step's keys and values down once for 8 waves;
+    // over short contexts twice as many workgroups are worth more (us, 256 /
+    // 128 rows: 512 tokens over 4096 67 / 71, 2 x 2000 over 7777 866 / 937; 1000
+    // over 1000 35 / 32, 8 x 64 over 2000 50 / 48)
+    p.chunk_rows = a.c.hd <= 128 && rows > 256 && most_steps(a, 256) >= 32 ? 256 : 128;
+    p.chunk_blocks = (int)((rows + p.chunk_rows - 1) / p.chunk_rows);
+    const int64_t slots = (int64_t)cus * (p.chunk_rows > 128 || a.c.hd > 128 ? 1 : 2), n = heads * p.chunk_blocks;
+    const int64_t steps = most_steps(a, p.chunk_rows);
+    // parts that fill the CUs, of 8 steps at least: of every block where those
+    // are few, otherwise of what is left behind the last whole round of the CUs
+    const int64_t left = n <= slots ? n : n % slots;
+    p.chunk_parts = left ? clamp_parts(slots / left, steps / 8) : 1;
+    p.chunk_cut = p.chunk_parts > 1 ? (int)((left + heads - 1) / heads) : 0;
+    if (p.chunk_cut == 0) p.chunk_parts = 1;
     if (a.seqs > 1) p.few = 16;  // one-token sequences beside a prompt
   } else {
     p.few = rows <= 16 ? 16 : kFewRows;
   }
   if (p.few) {
-    span = a.max_kv;
-    if (a.window > 0 && a.window + p.few / a.group + 1 < span) span = a.window + p.few / a.group + 1;
-    const int64_t tiles = (span + kTile - 1) / kTile;
     // parts until two workgroups a CU are there, of one step a wave at least,
     // of four where the CUs have one each without (the join is a launch of
     // 4 us; graph replays, us: 1 sequence of 2000 in 8 parts 11.1, in 2 18.1;
     // 4 of 1000 10.6 / 16.2; 16 of 8000 in 4 51.5, in 2 68.1; 32 of 1000 whole
     // 17.0, in 2 19.5)
-    p.few_parts = clamp_parts(2 * cus / heads, tiles / (heads < cus ? kFewWaves : 4 * kFewWaves));
+    p.few_parts = clamp_parts(2 * cus / heads, most_steps(a, p.few) / (heads < cus ? kFewWaves : 4 * kFewWaves));
   }
   return p;
 }
 
 // The partial results at ws: bytes, and where they lie.
-size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, void* ws, AttendParts& p) {
-  p = AttendParts{nullptr, nullptr, parts, rows, blocks};
+size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, void* ws, AttendParts& p) {
+  p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut};
   if (parts <= 1) return 0;
-  const size_t n = (size_t)a.seqs * a.c.heads * blocks * parts * rows;
+  const size_t n = (size_t)a.seqs * a.c.heads * cut * parts * rows;
   p.o = (float*)ws;
   p.ml = p.o + n * a.c.hd;
   return n * (a.c.hd + 2) * sizeof(float);
@@ -122,7 +134,7 @@ size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, void* ws, 
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
   const int fit = 64 / (a.c.hd / 4);
-  const int64_t most = (int64_t)a.max_q * a.group, held = (int64_t)p.blocks * p.rows, rows = most < held ? most : held;
+  const int64_t most = (int64_t)a.max_q * a.group, held = (int64_t)p.cut * p.rows, rows = most < held ? most : held;
   attend_join_kernel<<<dim3((unsigned)((rows + fit - 1) / fit), (unsigned)a.c.heads, (unsigned)a.seqs), 256, 0, st>>>(
       a, lo, hi, p);
   return hipGetLastError();
@@ -133,14 +145,14 @@ hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipSt
 bool attend_fits(const AttendArgs& a) {
   const int64_t rows = (int64_t)a.max_q * a.group;
   const int64_t heads = (int64_t)a.seqs * a.c.heads;
-  return rows <= (int64_t)65535 * kChunkRows && rows * a.group < ((int64_t)1 << 32) && heads < ((int64_t)1 << 31);
+  return rows <= (int64_t)32000 * 128 && rows * a.group < ((int64_t)1 << 32) && heads < ((int64_t)1 << 31);
 }
 
 size_t attend_workspace_bytes(const AttendArgs& a, int cus) {
   const Plan p = plan_of(a, cus);
   AttendParts q;
-  const size_t few = p.few ? parts_at(a, p.few_parts, p.few, 1, nullptr, q) : 0;
-  const size_t chunk = p.chunk_blocks ? parts_at(a, p.chunk_parts, kChunkRows, p.chunk_blocks, nullptr, q) : 0;
+  const size_t few = p.few ? parts_at(a, p.few_parts, p.few, 1, 1, nullptr, q) : 0;
+  const size_t chunk = p.chunk_blocks ? parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, nullptr, q) : 0;
   return few > chunk ? few : chunk;  // one after the other
 }
 
@@ -149,12 +161,12 @@ hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st)
   AttendParts q;
   hipError_t e = hipSuccess;
   if (p.chunk_blocks) {
-    parts_at(a, p.chunk_parts, kChunkRows, p.chunk_blocks, ws, q);
+    parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, ws, q);
     e = launch_attend_chunk(a, p.few, q, st);
     if (e == hipSuccess && q.parts > 1) e = join(a, p.few, INT32_MAX, q, st);
   }
   if (p.few && e == hipSuccess) {
-    parts_at(a, p.few_parts, p.few, 1, ws, q);
+    parts_at(a, p.few_parts, p.few, 1, 1, ws, q);
     e = launch_attend_few(a, 0, p.few, q, st);
     if (e == hipSuccess && q.parts > 1) e = join(a, 0, p.few, q, st);
   }

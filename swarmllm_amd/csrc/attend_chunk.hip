@@ -24,13 +24,14 @@ namespace {
 constexpr int kMfma = 0x008, kDsRead = 0x100;
 constexpr int kAhead = 4;  // LDS reads of operands in flight ahead of their products
 
-template <int HD>
+template <int HD, int W>
 struct ChunkSizes {
   // a step's keys (and values) in items of 32: the 32 dims of a block for one
   // position, 16 positions of two dims of a block; one scale, 16 scales
   static constexpr int kItems = kTile * HD / 32;
-  static constexpr bool kHalves = kItems * 2 <= 256;        // half the threads take keys, half values
-  static constexpr int kEach = (kItems + 255) / 256;        // a thread's of either
+  static constexpr int kThreads = 64 * W;
+  static constexpr bool kHalves = kItems * 2 <= kThreads;   // half the threads take keys, half values
+  static constexpr int kEach = (kItems + kThreads - 1) / kThreads;  // a thread's of either
   static constexpr int kRow = HD + 8;                       // f16s of a K row in LDS, padded off the next row's banks
   static constexpr int kVRow = kTile + 8;                   // and of a V row
   static constexpr int kHalfs = kTile * kRow + HD * kVRow;  // one buffer
@@ -38,26 +39,29 @@ struct ChunkSizes {
 };
 
 // One step's planes in a thread's registers.
-template <int HD>
+template <int HD, int W>
 struct Staged {
-  uint4 k[ChunkSizes<HD>::kEach][2], v[ChunkSizes<HD>::kEach][2], d0[ChunkSizes<HD>::kEach], d1[ChunkSizes<HD>::kEach];
-  uint32_t ks[ChunkSizes<HD>::kEach];
+  uint4 k[ChunkSizes<HD, W>::kEach][2], v[ChunkSizes<HD, W>::kEach][2], d0[ChunkSizes<HD, W>::kEach], d1[ChunkSizes<HD, W>::kEach];
+  uint32_t ks[ChunkSizes<HD, W>::kEach];
 };
 
 // A thread's i-th item of keys, or of values; on: whether it has one.
-template <int HD>
+template <int HD, int W>
 __device__ __forceinline__ int k_item(int i, bool& on) {
-  const int x = (int)threadIdx.x + 256 * i;
-  on = ChunkSizes<HD>::kItems % 256 == 0 || x < ChunkSizes<HD>::kItems;
+  const int x = (int)threadIdx.x + ChunkSizes<HD, W>::kThreads * i;
+  on = ChunkSizes<HD, W>::kItems % ChunkSizes<HD, W>::kThreads == 0 || x < ChunkSizes<HD, W>::kItems;
   return x;
 }
-template <int HD>
+template <int HD, int W>
 __device__ __forceinline__ int v_item(int i, bool& on) {
-  if (!ChunkSizes<HD>::kHalves) return k_item<HD>(i, on);
-  const int x = (int)threadIdx.x - 128;
-  on = x >= 0 && x < ChunkSizes<HD>::kItems;
+  if (!ChunkSizes<HD, W>::kHalves) return k_item<HD, W>(i, on);
+  const int x = (int)threadIdx.x - ChunkSizes<HD, W>::kThreads / 2;
+  on = x >= 0 && x < ChunkSizes<HD, W>::kItems;
   return x;
 }
+
+// The lower dim of item x of values: 16 dims of a block, then the next block's.
+__device__ __forceinline__ int v_dim(int x) { return (x >> 6) * 32 + ((x >> 2) & 15); }
 
 // A step's pages. ONE: pages of 64 positions and more, so a step has one, the
 // same for the wave; otherwise lane x < 4 of every wave holds that of the step's
@@ -65,13 +69,17 @@ __device__ __forceinline__ int v_item(int i, bool& on) {
 template <bool ONE>
 __device__ __forceinline__ int step_page(const AttendArgs& a, int b, int tile, int end, int kv) {
   if (tile >= end) return -1;
-  if (ONE) return __builtin_amdgcn_readfirstlane(page_of(a, b, tile * kTile, kv));
-  return page_of(a, b, tile * kTile + 16 * (int)(threadIdx.x & 3), kv);
+  return page_of(a, b, tile * kTile + (ONE ? 0 : 16 * (int)(threadIdx.x & 3)), kv);
+}
+// ONE: into a scalar register, once the load has surely landed.
+template <bool ONE>
+__device__ __forceinline__ int settled(int page) {
+  return ONE ? __builtin_amdgcn_readfirstlane(page) : page;
 }
 
-template <int HD, bool ONE>
-__device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int pages, Staged<HD>& s) {
-  using Z = ChunkSizes<HD>;
+template <int HD, int W, bool ONE>
+__device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int pages, Staged<HD, W>& s) {
+  using Z = ChunkSizes<HD, W>;
   const CachePlanes& c = a.c;
   const int8_t* k1 = nullptr;
   const int8_t* v1 = nullptr;
@@ -88,8 +96,8 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     bool k_on, v_on;
-    const int xk = k_item<HD>(i, k_on), xv = v_item<HD>(i, v_on);
-    const int vc = xv & 3, d = 2 * (xv >> 2);  // 16 positions from 16 vc on, dims d and d + 1
+    const int xk = k_item<HD, W>(i, k_on), xv = v_item<HD, W>(i, v_on);
+    const int vc = xv & 3, d = v_dim(xv);  // 16 positions from 16 vc on, dims d and d + 16
     if constexpr (ONE) {
       if (k_on) {
         s.k[i][0] = *(const uint4*)(k1 + 32 * (uint32_t)xk);
@@ -98,7 +106,7 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
       }
       if (v_on) {
         s.v[i][0] = *(const uint4*)(v1 + (uint32_t)d * (uint32_t)c.page + 16 * vc);
-        s.v[i][1] = *(const uint4*)(v1 + (uint32_t)(d + 1) * (uint32_t)c.page + 16 * vc);
+        s.v[i][1] = *(const uint4*)(v1 + (uint32_t)(d + 16) * (uint32_t)c.page + 16 * vc);
         const uint16_t* vs = vs1 + (uint32_t)(d >> 5) * (uint32_t)c.page + 16 * vc;
         s.d0[i] = *(const uint4*)vs;
         s.d1[i] = *(const uint4*)(vs + 8);
@@ -117,7 +125,7 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
         const int at = (j0 + 16 * vc) & (c.page - 1);
         const int8_t* v = c.v_codes + (vph * HD + d) * c.page + at;
         s.v[i][0] = *(const uint4*)v;
-        s.v[i][1] = *(const uint4*)(v + c.page);
+        s.v[i][1] = *(const uint4*)(v + 16 * c.page);
         const uint16_t* vs = c.v_scales + (vph * (HD / 32) + (d >> 5)) * c.page + at;
         s.d0[i] = *(const uint4*)vs;
         s.d1[i] = *(const uint4*)(vs + 8);
@@ -128,14 +136,14 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
 
 // The step's keys and values as f16 into an LDS buffer. CUT: the values of
 // positions outside [lo, hi), or on no page, are laid as zeros.
-template <int HD, bool ONE, bool CUT>
-__device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int lo, int hi, uint16_t* buf) {
-  using Z = ChunkSizes<HD>;
+template <int HD, int W, bool ONE, bool CUT>
+__device__ __forceinline__ void lay(const Staged<HD, W>& s, int j0, int pages, int lo, int hi, uint16_t* buf) {
+  using Z = ChunkSizes<HD, W>;
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     bool k_on, v_on;
-    const int xk = k_item<HD>(i, k_on), xv = v_item<HD>(i, v_on);
-    const int vc = xv & 3, d = 2 * (xv >> 2);
+    const int xk = k_item<HD, W>(i, k_on), xv = v_item<HD, W>(i, v_on);
+    const int vc = xv & 3, d = v_dim(xv);
     const int vp = !CUT ? 0 : ONE ? pages : __shfl(pages, vc, kWave);
     H8 h;
     if (k_on) {
@@ -161,36 +169,43 @@ __device__ __forceinline__ void lay(const Staged<HD>& s, int j0, int pages, int 
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         h.v = value8(s.v[i][u].x, s.v[i][u].y, d0);
-        *(uint4*)(vb + u * Z::kVRow) = h.u;
+        *(uint4*)(vb + 16 * u * Z::kVRow) = h.u;
         h.v = value8(s.v[i][u].z, s.v[i][u].w, d1);
-        *(uint4*)(vb + u * Z::kVRow + 8) = h.u;
+        *(uint4*)(vb + 16 * u * Z::kVRow + 8) = h.u;
       }
     }
   }
 }
 
-template <int HD, bool ONE>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows, AttendParts parts) {
-  using Z = ChunkSizes<HD>;
+template <int HD, int W, bool ONE>
+__global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows, AttendParts parts) {
+  using Z = ChunkSizes<HD, W>;
+  constexpr int kRows = 32 * W;
   extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
   const CachePlanes& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 31, hi = lane >> 5;
-  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)c.heads), kvh = blockIdx.x - b * c.heads, part = blockIdx.y;
-  const int block = (int)(gridDim.z - 1 - blockIdx.z);  // the rows that see most first
+  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)c.heads), kvh = blockIdx.x - b * c.heads;
+  // the rows that see most first; behind the whole blocks the parts of those cut
+  const int z = blockIdx.z, cut_z = z - (parts.blocks - parts.cut);
+  const bool whole = cut_z < 0;
+  const int nparts = whole ? 1 : parts.parts;
+  const int down = whole ? 0 : (int)((uint32_t)cut_z / (uint32_t)nparts);
+  const int block = whole ? parts.blocks - 1 - z : parts.cut - 1 - down;
+  const int part = whole ? 0 : cut_z - down * nparts;
   int64_t q0;
   int nq, kv;
   sequence(a, b, q0, nq, kv);
   const int rows = nq * a.group;
-  const int r0 = block * kChunkRows;
+  const int r0 = block * kRows;
   if (rows <= lo_rows || r0 >= rows) return;
 
   const int pos0 = kv - nq;
-  const int last_row = rows - 1 < r0 + kChunkRows - 1 ? rows - 1 : r0 + kChunkRows - 1;
+  const int last_row = rows - 1 < r0 + kRows - 1 ? rows - 1 : r0 + kRows - 1;
   const int low_pos = pos0 + token_of(a, r0), high_pos = pos0 + token_of(a, last_row);
   const int lo = first_seen(a, low_pos < 0 ? 0 : low_pos), seen = high_pos + 1;  // [lo, seen): what the rows see
   int begin, end;
-  part_steps(lo, seen, part, parts.parts, begin, end);
+  part_steps(lo, seen, part, nparts, begin, end);
 
   // this wave's rows
   const int r = r0 + 32 * wave + col, qi = token_of(a, r);
@@ -214,19 +229,20 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  auto lay_step = [&](const Staged<HD>& s, int tile, int pages, int buf) {
+  auto lay_step = [&](const Staged<HD, W>& s, int tile, int pages, int buf) {
     const int j0 = tile * kTile;
     uint16_t* to = s_buf + buf * Z::kHalfs;
     if (j0 < lo || j0 + kTile > kv || __ballot(pages < 0) != 0)
-      lay<HD, ONE, true>(s, j0, pages, lo, kv, to);
+      lay<HD, W, ONE, true>(s, j0, pages, lo, kv, to);
     else
-      lay<HD, ONE, false>(s, j0, pages, lo, kv, to);
+      lay<HD, W, ONE, false>(s, j0, pages, lo, kv, to);
   };
 
-  Staged<HD> st;
-  int pages = step_page<ONE>(a, b, begin, end, kv), next_pages = step_page<ONE>(a, b, begin + 1, end, kv);
+  Staged<HD, W> st;
+  int pages = settled<ONE>(step_page<ONE>(a, b, begin, end, kv));
+  int next_pages = settled<ONE>(step_page<ONE>(a, b, begin + 1, end, kv));
   if (begin < end) {
-    fetch<HD, ONE>(a, kvh, begin * kTile, pages, st);
+    fetch<HD, W, ONE>(a, kvh, begin * kTile, pages, st);
     lay_step(st, begin, pages, 0);
   }
   __syncthreads();
@@ -235,7 +251,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
   for (int tile = begin, cur = 0; tile < end; tile++, cur ^= 1) {
     const int j0 = tile * kTile;
     const int after_pages = step_page<ONE>(a, b, tile + 2, end, kv);
-    if (tile + 1 < end) fetch<HD, ONE>(a, kvh, j0 + kTile, next_pages, st);
+    if (tile + 1 < end) fetch<HD, W, ONE>(a, kvh, j0 + kTile, next_pages, st);
 
     if (j0 <= wave_high && j0 + kTile > wave_first) {
       const uint16_t* kb = s_buf + cur * Z::kHalfs + krow * Z::kRow + 8 * hi;
@@ -314,13 +330,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
     }
     if (tile + 1 < end) lay_step(st, tile + 1, next_pages, cur ^ 1);
     pages = next_pages;
-    next_pages = after_pages;
+    next_pages = settled<ONE>(after_pages);
     __syncthreads();
   }
 
   l += __shfl_xor(l, 32, kWave);
   if (!row_on) return;
-  if (parts.parts > 1) {
+  if (nparts > 1) {
     const int64_t pr = part_row(parts, (int64_t)blockIdx.x, block, part, r - r0);
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
@@ -344,21 +360,23 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void attend_chunk_kernel(Att
     }
 }
 
-template <int HD, bool ONE>
+template <int HD, int W, bool ONE>
 hipError_t launch_pages(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
-  if constexpr (ChunkSizes<HD>::kLds > 64 * 1024) {
-    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD, ONE>>();
+  if constexpr (ChunkSizes<HD, W>::kLds > 64 * 1024) {
+    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD, W, ONE>>();
     if (e != hipSuccess) return e;
   }
-  const dim3 grid((unsigned)(a.seqs * a.c.heads), (unsigned)p.parts, (unsigned)p.blocks);
-  attend_chunk_kernel<HD, ONE><<<grid, 256, ChunkSizes<HD>::kLds, st>>>(a, lo, p);
+  const dim3 grid((unsigned)(a.seqs * a.c.heads), 1, (unsigned)(p.blocks + p.cut * (p.parts - 1)));
+  attend_chunk_kernel<HD, W, ONE><<<grid, 64 * W, ChunkSizes<HD, W>::kLds, st>>>(a, lo, p);
   return hipGetLastError();
 }
 
 template <int HD>
 hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
-  if (a.c.page >= kTile) return launch_pages<HD, true>(a, lo, p, st);
-  return launch_pages<HD, false>(a, lo, p, st);
+  if constexpr (HD <= 128)
+    if (p.rows > 128)
+      return a.c.page >= kTile ? launch_pages<HD, 8, true>(a, lo, p, st) : launch_pages<HD, 8, false>(a, lo, p, st);
+  return a.c.page >= kTile ? launch_pages<HD, 4, true>(a, lo, p, st) : launch_pages<HD, 4, false>(a, lo, p, st);
 }
 
 }  // namespace
