@@ -113,11 +113,15 @@ Plan plan_of(const AttendArgs& a, int cus) {
   }
   if (p.few) {
     // parts until two workgroups a CU are there, of one step a wave at least,
-    // of four where the CUs have one each without (the join is a launch of
-    // 4 us; graph replays, us: 1 sequence of 2000 in 8 parts 11.1, in 2 18.1;
-    // 4 of 1000 10.6 / 16.2; 16 of 8000 in 4 51.5, in 2 68.1; 32 of 1000 whole
-    // 17.0, in 2 19.5)
-    p.few_parts = clamp_parts(2 * cus / heads, most_steps(a, p.few) / (heads < cus ? kFewWaves : 4 * kFewWaves));
+    // of four where the CUs have one each without, and none up to two steps a
+    // wave (the join is a launch of 4 us, as much again for the host; graph
+    // replays, us: 1 sequence of 500 whole 11.3, in 2 parts 10.8; of 2000 in 8
+    // 11.1, in 2 18.1; 4 of 1000 in 4 10.6, whole 16.2; 16 of 8000 in 4 51.5, in 2
+    // 68.1; 32 of 1000 whole 17.0, in 2 19.5)
+    const int64_t steps = most_steps(a, p.few);
+    p.few_parts = steps <= 2 * kFewWaves
+                      ? 1
+                      : clamp_parts(2 * cus / heads, steps / (heads < cus ? kFewWaves : 4 * kFewWaves));
   }
   return p;
 }

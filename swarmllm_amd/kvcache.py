@@ -67,18 +67,18 @@ class KvCache:
         writes nothing; the others are distinct."""
         tokens = slots.numel()
         self._slots("write", slots)
-        for name, t in (("k", k), ("v", v)):
-            if t.shape != (tokens, self.kv_heads, self.head_dim) or t.dtype not in _X_DTYPES \
-                    or t.dtype != k.dtype or t.device != self.device:
-                raise ValueError(f"KvCache.write: {name} [{tokens}, {self.kv_heads}, {self.head_dim}] f32, f16 or bf16 "
-                                 f"on {self.device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+        shape, code = (tokens, self.kv_heads, self.head_dim), _X_DTYPES.get(k.dtype)
+        if code is None or k.shape != shape or v.shape != shape or v.dtype != k.dtype or k.device != self.device \
+                or v.device != self.device:
+            raise ValueError(f"KvCache.write: k and v {list(shape)} in f32, f16 or bf16 on {self.device}, not {k.dtype} "
+                             f"{tuple(k.shape)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
         if tokens == 0:
             return
         ks, khs = self._strides("write", "k", k)
         vs, vhs = self._strides("write", "v", v)
         with on_device(self.device):
             check("qmm_cache_write", lib().qmm_cache_write(self._ref, k.data_ptr(), ks, khs, v.data_ptr(), vs, vhs,
-                                                           _X_DTYPES[k.dtype], slots.data_ptr(), tokens,
+                                                           code, slots.data_ptr(), tokens,
                                                            raw_stream(self.device)))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -114,54 +114,64 @@ class KvCache:
         of q that belong to no sequence are left as they were in `out` (as
         torch.empty gives them without one). The products run on f16 operands
         with f32 sums: an f32 q is rounded to f16, as is a bf16 one."""
-        if q.dim() != 3 or q.dtype not in _X_DTYPES or q.device != self.device or q.shape[2] != self.head_dim \
-                or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+        device = self.device
+        q_type = _X_DTYPES.get(q.dtype)
+        if q.dim() != 3 or q_type is None or q.device != device or q.shape[2] != self.head_dim or q.shape[1] < 1 \
+                or q.shape[1] % self.kv_heads:
             raise ValueError(f"KvCache.attend: q [tokens, a multiple of {self.kv_heads} heads, {self.head_dim}] f16, "
-                             f"bf16 or f32 on {self.device}, not {q.dtype} {tuple(q.shape)} on {q.device}")
+                             f"bf16 or f32 on {device}, not {q.dtype} {tuple(q.shape)} on {q.device}")
         tokens, heads, hd = q.shape
         seqs = kv_lens.numel()
-        for name, t, shape in (("q_starts", q_starts, (seqs + 1,)), ("kv_lens", kv_lens, (seqs,))):
-            if t.dtype != torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
-                raise ValueError(f"KvCache.attend: {name} must be contiguous int32 {shape} on {self.device}, not "
-                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != seqs or tables.device != self.device \
-                or not tables.is_contiguous():
-            raise ValueError(f"KvCache.attend: tables must be contiguous int32 [{seqs}, pages] on {self.device}, not "
-                             f"{tables.dtype} {tuple(tables.shape)} on {tables.device}")
-        if out_dtype is not None and out_dtype not in _X_DTYPES:
-            raise ValueError(f"KvCache.attend: out_dtype f16, bf16 or f32, not {out_dtype}")
+        self._int32("q_starts", q_starts, (seqs + 1,))
+        self._int32("kv_lens", kv_lens, (seqs,))
+        if tables.dim() != 2:
+            raise ValueError(f"KvCache.attend: tables [{seqs}, pages a sequence], not {tuple(tables.shape)}")
+        pages = tables.shape[1]
+        self._int32("tables", tables, (seqs, pages))
         if max_q < 0 or window < 0 or (max_kv is not None and max_kv < 0):
             raise ValueError(f"KvCache.attend: max_q {max_q}, max_kv {max_kv}, window {window}")
-        if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,)
-                                  or sinks.device != self.device or not sinks.is_contiguous()):
-            raise ValueError(f"KvCache.attend: sinks must be {heads} contiguous f32 on {self.device}")
+        if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (heads,) or sinks.device != device
+                                  or not sinks.is_contiguous()):
+            raise ValueError(f"KvCache.attend: sinks must be {heads} contiguous f32 on {device}")
+        out_stride = heads * hd
         if out is None:
-            out = torch.empty((tokens, heads, hd), dtype=out_dtype or q.dtype, device=self.device)
-        elif out_dtype is not None and out.dtype != out_dtype:
-            raise ValueError(f"KvCache.attend: out is {out.dtype}, not {out_dtype}")
-        elif out.shape != (tokens, heads, hd) or out.dtype not in _X_DTYPES or out.device != self.device \
-                or (tokens and (out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd))) \
-                or (tokens > 1 and out.stride(0) < heads * hd):
-            raise ValueError(f"KvCache.attend: out [{tokens}, {heads}, {hd}] f16, bf16 or f32, rows of consecutive "
-                             f"values, not {out.dtype} {tuple(out.shape)} strides {out.stride()}")
+            out_type = q_type if out_dtype is None else _X_DTYPES.get(out_dtype)
+            if out_type is None:
+                raise ValueError(f"KvCache.attend: out_dtype f16, bf16 or f32, not {out_dtype}")
+            out = torch.empty((tokens, heads, hd), dtype=out_dtype or q.dtype, device=device)
+        else:
+            out_type = _X_DTYPES.get(out.dtype)
+            if out_type is None or (out_dtype is not None and out.dtype != out_dtype) or out.device != device \
+                    or out.shape != (tokens, heads, hd) \
+                    or (tokens and (out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd))) \
+                    or (tokens > 1 and out.stride(0) < out_stride):
+                raise ValueError(f"KvCache.attend: out [{tokens}, {heads}, {hd}] {out_dtype or 'f16, bf16 or f32'}, "
+                                 f"rows of consecutive values, not {out.dtype} {tuple(out.shape)} strides "
+                                 f"{out.stride()}")
+            if tokens > 1:
+                out_stride = out.stride(0)
         if tokens == 0 or seqs == 0:
             return out
         qs, qhs = self._strides("attend", "q", q)
         if max_kv is None:
-            max_kv = tables.shape[1] * self.page
-        with on_device(self.device):
-            need = _attend_need(self.device.index, self.pages, self.kv_heads, hd, self.page, tokens, heads,
-                                tables.shape[1], seqs, max_q, max_kv, window)
+            max_kv = pages * self.page
+        with on_device(device):
+            need = _attend_need(device.index, self.pages, self.kv_heads, hd, self.page, tokens, heads, pages, seqs,
+                                max_q, max_kv, window)
             size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             check("qmm_attend", lib().qmm_attend(
-                self._ref, q.data_ptr(), _X_DTYPES[q.dtype], qs, qhs, tokens, heads, q_starts.data_ptr(),
-                kv_lens.data_ptr(), tables.data_ptr(), tables.shape[1], seqs, max_q, max_kv,
-                hd ** -0.5 if scale is None else scale, window, None if sinks is None else sinks.data_ptr(),
-                out.data_ptr(), _X_DTYPES[out.dtype], out.stride(0) if tokens > 1 else heads * hd,
-                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(self.device)))
+                self._ref, q.data_ptr(), q_type, qs, qhs, tokens, heads, q_starts.data_ptr(), kv_lens.data_ptr(),
+                tables.data_ptr(), pages, seqs, max_q, max_kv, hd ** -0.5 if scale is None else scale, window,
+                None if sinks is None else sinks.data_ptr(), out.data_ptr(), out_type, out_stride,
+                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device)))
         return out
+
+    def _int32(self, name: str, t: torch.Tensor, shape) -> None:
+        if t.dtype != torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"KvCache.attend: {name} must be contiguous int32 {shape} on {self.device}, not {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
 
     def _slots(self, name: str, slots: torch.Tensor) -> None:
         if slots.dtype != torch.int64 or slots.dim() != 1 or slots.device != self.device or not slots.is_contiguous():

@@ -64,12 +64,13 @@ def rms_norm_act(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Op
     rs = hs = k
     if residual is not None:
         rp, rs = residual.data_ptr(), _rows("residual", residual, x)
-        if h is None:
-            h = torch.empty(shape, dtype=x.dtype, device=device)
-    if h is None:
-        h = x
-    else:
+    if h is not None:
         hp, hs = h.data_ptr(), _rows("h", h, x)
+    elif residual is not None:
+        h = torch.empty(shape, dtype=x.dtype, device=device)
+        hp = h.data_ptr()
+    else:
+        h = x
     act = QAct.alloc(shape, QAct.layout_of(dtype), device) if dtype is not None else None
     y = torch.empty(shape, dtype=y_dtype, device=device) if y_dtype is not None else None
     rows = x.numel() // k
