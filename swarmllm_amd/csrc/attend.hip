@@ -14,16 +14,16 @@ namespace qmm {
 
 namespace {
 
-// A workgroup joins 64 / (hd / 4) rows: 4 dims a lane, the parts dealt to its
-// 4 waves in turn, their results joined in LDS.
+// A wave joins 64 / (hd / 4) rows, 4 dims a lane. G == 4: the parts of those
+// rows are dealt to the workgroup's 4 waves in turn and joined in LDS (many
+// parts); G == 1: each wave takes all parts of rows of its own.
+template <int G>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_rows, int hi_rows, AttendParts p) {
-  __shared__ f4v s_o[4][64];
-  __shared__ float s_m[4][64], s_l[4][64];
   const int hd = a.c.hd, per = hd / 4, fit = 64 / per;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int sub = lane / per, e = 4 * (lane - sub * per);
+  const int sub = lane / per, e = 4 * (lane - sub * per), first = G > 1 ? wave : 0;
   // rows of one kv head of a sequence lie block after block
-  const int64_t row_of_head = (int64_t)blockIdx.x * fit + sub;
+  const int64_t row_of_head = ((int64_t)blockIdx.x * (4 / G) + (G > 1 ? 0 : wave)) * fit + sub;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int block = (int)(row_of_head / p.rows), row = (int)(row_of_head - (int64_t)block * p.rows);
   int64_t q0;
@@ -35,8 +35,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   float top = -INFINITY, sum = 0.0f;
   f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (on) {
-    const int64_t i0 = part_row(p, hs, block, wave, row), step = 4 * (int64_t)p.rows;
-    const int n = (p.parts - wave + 3) / 4;
+    const int64_t i0 = part_row(p, hs, block, first, row), step = G * (int64_t)p.rows;
+    const int n = (p.parts - first + G - 1) / G;
 #pragma unroll 4
     for (int s = 0; s < n; s++) {
       const int64_t i = i0 + s * step;
@@ -49,22 +49,27 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
       acc = acc * fa + o * fb;
     }
   }
-  s_o[wave][lane] = acc;
-  s_m[wave][lane] = top;
-  s_l[wave][lane] = sum;
-  __syncthreads();
-  if (wave != 0 || !on) return;
+  if constexpr (G > 1) {
+    __shared__ f4v s_o[G][64];
+    __shared__ float s_m[G][64], s_l[G][64];
+    s_o[wave][lane] = acc;
+    s_m[wave][lane] = top;
+    s_l[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-  for (int w = 1; w < 4; w++) top = fmaxf(top, s_m[w][lane]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  sum = 0.0f;
-  acc = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = 1; w < G; w++) top = fmaxf(top, s_m[w][lane]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+    acc = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float f = exp2_fast(s_m[w][lane] - base);
-    sum += s_l[w][lane] * f;
-    acc += s_o[w][lane] * f;
+    for (int w = 0; w < G; w++) {
+      const float f = exp2_fast(s_m[w][lane] - base);
+      sum += s_l[w][lane] * f;
+      acc += s_o[w][lane] * f;
+    }
   }
+  if (!on) return;
   const int r = (int)row_of_head, i = token_of(a, r), head = kvh * a.group + r - i * a.group;
   float out[4];
   finish_row<4>(a, head, top, sum, (const float*)&acc, out);
@@ -137,10 +142,16 @@ size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, v
 }
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
-  const int fit = 64 / (a.c.hd / 4);
+  // (us, parts dealt to 4 waves / all to one: 512 tokens' 64 blocks in 4 parts
+  // 11.9 / 8.5, one sequence's 32 rows in 32 parts 4.5 / 7)
+  const bool deal = p.parts > 8;
+  const int fit = 64 / (a.c.hd / 4) * (deal ? 1 : 4);
   const int64_t most = (int64_t)a.max_q * a.group, held = (int64_t)p.cut * p.rows, rows = most < held ? most : held;
-  attend_join_kernel<<<dim3((unsigned)((rows + fit - 1) / fit), (unsigned)a.c.heads, (unsigned)a.seqs), 256, 0, st>>>(
-      a, lo, hi, p);
+  const dim3 grid((unsigned)((rows + fit - 1) / fit), (unsigned)a.c.heads, (unsigned)a.seqs);
+  if (deal)
+    attend_join_kernel<4><<<grid, 256, 0, st>>>(a, lo, hi, p);
+  else
+    attend_join_kernel<1><<<grid, 256, 0, st>>>(a, lo, hi, p);
   return hipGetLastError();
 }
 

@@ -83,6 +83,22 @@ def test_long_contexts_joined_from_parts(new, n):
     run([new, 1], [n, 7], 4, 1, 64, 16, BF16, seed=n, sinks=True)
 
 
+@pytest.mark.parametrize("hd,page", [(64, 16), (64, 64), (96, 128), (128, 32), (128, 64)])
+@pytest.mark.parametrize("window", [0, 2100])
+def test_chunks_of_several_rounds_of_the_cus(hd, page, window):
+    """More blocks of 256 rows than CUs (64 kv heads, 5 blocks of each): the
+    first blocks in parts, the others whole, and a one-token sequence beside."""
+    run([1100], [2400], 64, 64, hd, page, F16, window=window, seed=hd)
+    run([300, 1, 290], [2300, 2100, 2048], 16, 4, hd, page, BF16, window=window, seed=hd, sinks=True)
+
+
+@pytest.mark.parametrize("new,n", [(65, 2047), (520, 2049), (100, 10000)])
+def test_blocks_of_128_and_256_rows(new, n):
+    """Both sides of the lines between the two (rows past 256, contexts past 2048)."""
+    for heads, kv_heads in ((4, 1), (2, 1), (12, 4)):
+        run([new], [n], heads, kv_heads, 128, 64, F16, seed=n)
+
+
 def test_rows_that_see_nothing():
     """kv_len under the new tokens (the first rows stand before position 0), no cached positions at all, tables of no page."""
     for new, kvl in (([1, 4, 3], [0, 2, 0]), ([40, 33], [7, 0])):
