@@ -105,9 +105,7 @@ int qmm_dequantize_act(const void *xq, int layout, void *out, int out_dtype, int
  * and y is given. Strides are in values, at least k; k is a multiple of 4, and
  * of the layout's block where xq is given. h may be x or residual itself (the
  * same pointer and stride); otherwise nothing overlaps. A row's result does
- * not depend on the other rows, nor on their number. One launch. Replaces the
- * reference's add_rmsnorm (kernels/fused_decode.cu:47-240) and the
- * quantization in front of its product. */
+ * not depend on the other rows, nor on their number. One launch. */
 int qmm_rms_norm_act(const void *x, int dtype, int64_t x_stride, const void *residual, int64_t r_stride,
                      const float *w, float eps, void *h, int64_t h_stride, void *xq, int layout, void *y, int y_dtype,
                      int64_t y_stride, int64_t k, int64_t rows, int64_t stream);
@@ -376,8 +374,8 @@ int qmm_moe_forward_prefill(int type, const void *w, int num_experts, const void
  * 1.0625 bytes a value. Keys lie along head_dim and values along the
  * positions, each along the axis that the attention contracts. Slot s is
  * position s % page of page s / page; position p of a sequence lies in slot
- * table[p / page] * page + p % page of its page table. The caller owns the planes and
- * the tables; a page id outside [0, pages) names no page. */
+ * table[p / page] * page + p % page of its page table. The caller owns the
+ * planes and the tables; a page id outside [0, pages) names no page. */
 typedef struct qmm_cache {
     void *k_codes, *k_scales, *v_codes, *v_scales;
     int64_t pages;
@@ -394,9 +392,9 @@ int qmm_cache_plane_bytes(int64_t pages, int kv_heads, int head_dim, int page, s
  * are taken as they are. Per 32 values: the scale amax / 127 (amax over the
  * finite ones, at most 65468.5: larger values saturate there, so that every
  * cached value is a finite f16), codes clamp(round(v / scale), -127, 127), NaN
- * as 0: the wire codec's block (qmm_wire_encode), the scale kept as f16. A slot outside the cache (a
- * negative one: padding) writes nothing; slots are otherwise distinct, and no other
- * position of the cache changes. Replaces kv_write_f16 (kernels/kv_append.cu:33). */
+ * as 0: the wire codec's block (qmm_wire_encode), the scale kept as f16. A
+ * slot outside the cache (a negative one: padding) writes nothing; the others
+ * are distinct, and no other position of the cache changes. */
 int qmm_cache_write(const qmm_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v,
                     int64_t v_stride, int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens,
                     int64_t stream);
@@ -409,11 +407,11 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
 
 /* Causal attention of the new tokens of `seqs` sequences over their cached
  * positions, the new ones among them (write first, then attend). Sequence b's
- * new tokens are rows [q_starts[b], q_starts[b + 1]) of q (int32, seqs + 1 of them), its
- * cached positions 0 .. kv_lens[b] - 1 (int32), its pages the row b of tables
- * (int32, table_stride apart). Its i-th new token stands at position
- * pos = kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i and sees the positions j <= pos, with window > 0 those
- * with j > pos - window only:
+ * new tokens are rows [q_starts[b], q_starts[b + 1]) of q (int32, seqs + 1 of
+ * them), its cached positions 0 .. kv_lens[b] - 1 (int32), its pages the row b
+ * of tables (int32, table_stride apart). Its i-th new token stands at position
+ * pos = kv_lens[b] - (q_starts[b + 1] - q_starts[b]) + i and sees the
+ * positions j <= pos, with window > 0 those with j > pos - window only:
  *   out[row][h] = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sinks[h])),
  *   s_j = scale * q[row][h] . k_j
  * of kv head h / (heads / kv_heads); without sinks (NULL) their term is
@@ -421,16 +419,17 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
  * zero; a position on a page outside the cache counts as not there.
  * q: [tokens][heads][head_dim], rows q_stride and heads q_head_stride values
  * apart; out: rows out_stride values apart, heads head_dim. Rows of q that no
- * sequence holds are left as they were in out. max_q and max_kv bound the sequences' new
- * tokens and cached positions: the host plans by them (rows past max_q stay as they were, kv_lens is cut
- * at max_kv and at the table's row). The products run on f16
- * operands with f32 sums: q (an f32 q rounds; all saturate at 65504), the
- * cache's values code * scale and the weights exp(s_j - max), each rounded
- * once to nearest. scale is finite (at most 1e30 in size). Any mix of lengths is served by one call; the rows of a
- * sequence do not depend on the other sequences' data. Plan (launch == 0) and launch as qmm_forward: the
- * workspace joins the parts of a long context (*need can be 0). Replaces the
- * reference's decode attention (kernels/decode_attn.cu:257-612) and its paged
- * attention. */
+ * sequence holds are left as they were in out. max_q and max_kv bound the
+ * sequences' new tokens and cached positions: the host plans by them (rows
+ * past max_q stay as they were, a kv_lens past max_kv or past the table's row
+ * counts as that). The products run on f16 operands with f32 sums: q (an f32 q
+ * rounds; all saturate at 65504), the cache's values code * scale and the
+ * weights, each rounded once to nearest. scale is finite (at most 1e30 in
+ * size). Any mix of lengths is served by one call; the rows of a sequence do
+ * not depend on the other sequences' data. Plan (launch == 0) and launch as
+ * qmm_forward: the workspace joins the parts of a long context (*need can be
+ * 0). On a stream being captured the first call of a process wants qmm_prepare
+ * before it, as a product's. */
 int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_stride, int64_t q_head_stride,
                int64_t tokens, int heads, const int32_t *q_starts, const int32_t *kv_lens, const int32_t *tables,
                int64_t table_stride, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int64_t window,

@@ -2,9 +2,9 @@
 // pages of the cache.
 //
 // What bounds it is the matrix cores and the vector work beside them. A
-// workgroup takes 128 query rows of a kv head (the heads that share it side by
-// side, token after token), 32 a wave, against steps of 64 positions: the
-// step's keys and values are read once for the 128 rows, turned into f16
+// workgroup takes 128 or 256 query rows of a kv head (the heads that share it
+// side by side, token after token), 32 a wave, against steps of 64 positions:
+// the step's keys and values are read once for all the rows, turned into f16
 // (codes times scales, one rounding) and laid into LDS, the next step's planes
 // in flight meanwhile. Per step a wave computes
 //   S^T = K q^T   (32x32x16: rows positions, columns query rows)
@@ -12,7 +12,19 @@
 // K row r of a tile is the position whose index has bits 2 and 3 of r
 // exchanged: so a lane's 8 scores of a 16-position step are consecutive
 // positions, and the weights made of them are the second product's operand as
-// they stand. The running maximum, the sum and O's rescaling belong to the lane's own column.
+// they stand. The running maximum, the sum and O's rescaling belong to the
+// lane's own column.
+//
+// Two prompts' chunks of 2000 tokens over 7777 (64 query heads on 8 of 128 dims)
+// take 866 us, 0.77 PFLOP/s; a library product of 8192^3 reaches 1.15. The
+// products, the softmax's and the conversions' vector instructions (about 290 a
+// wave and step with 128 rows a workgroup, 230 with 256) and the LDS reads (32
+// operands of 1 KiB a wave and step) each take a third to a half of a step and
+// overlap only between the two waves of a SIMD. Tried and slower: a step's
+// scores beside the weights of the one before (the second set of scores spills
+// at 256 registers), steps of 32 positions, 64 rows a wave (accumulators past 256
+// registers are copied back and forth each step), and products and vector
+// instructions interleaved by hand.
 #include "attend.h"
 #include "mv_common.h"
 
@@ -41,8 +53,9 @@ struct ChunkSizes {
 // One step's planes in a thread's registers.
 template <int HD, int W>
 struct Staged {
-  uint4 k[ChunkSizes<HD, W>::kEach][2], v[ChunkSizes<HD, W>::kEach][2], d0[ChunkSizes<HD, W>::kEach], d1[ChunkSizes<HD, W>::kEach];
-  uint32_t ks[ChunkSizes<HD, W>::kEach];
+  static constexpr int kEach = ChunkSizes<HD, W>::kEach;
+  uint4 k[kEach][2], v[kEach][2], d0[kEach], d1[kEach];
+  uint32_t ks[kEach];
 };
 
 // A thread's i-th item of keys, or of values; on: whether it has one.
@@ -178,7 +191,8 @@ __device__ __forceinline__ void lay(const Staged<HD, W>& s, int j0, int pages, i
 }
 
 template <int HD, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows, AttendParts parts) {
+__global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows,
+                                                                                         AttendParts parts) {
   using Z = ChunkSizes<HD, W>;
   constexpr int kRows = 32 * W;
   extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];

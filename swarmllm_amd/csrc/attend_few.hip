@@ -14,6 +14,13 @@
 // the rescaling of O all belong to the lane's own column. The waves of a
 // workgroup take steps in turn, joined at the end through LDS; a long context
 // is cut into parts of the same kind, joined by attend_join_kernel.
+//
+// 64 sequences of 4000 tokens (64 query heads on 8 of 128 dims) take 88 us, 420 MB
+// at 4.8 TB/s, a copy's rate; 16 of 8000, ragged, 47 and 4.7 us of join. Few
+// short sequences are bound by the chain of one step (bounds, page, planes, some
+// 850 vector instructions, join): one of 500 tokens takes 11 us. The loads of a
+// step's keys and values are all issued before its first product: with the
+// values' loaded behind the scores the 16 sequences took 71 us.
 #include "attend.h"
 
 namespace qmm {

@@ -1,7 +1,5 @@
 """A paged key/value cache in Q8_0 and the attention over it (qmm_cache_* and
-qmm_attend): what stands between a decoder layer's q/k/v and o products. The
-reference appends f16 (kernels/kv_append.cu:33) and attends over it with
-kernels/decode_attn.cu:257-612 and its paged attention.
+qmm_attend): what stands between a decoder layer's q/k/v and o products.
 """
 from __future__ import annotations
 

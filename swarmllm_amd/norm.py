@@ -1,6 +1,6 @@
 """Residual addition and root-mean-square norm into the 8-bit activation that
 a product reads (qmm_rms_norm_act): the step in front of a decoder layer's
-products (the reference's add_rmsnorm, kernels/fused_decode.cu:47-240).
+products.
 """
 from __future__ import annotations
 
