@@ -21,15 +21,17 @@ constexpr int kTile = 64;  // positions a step of either kernel takes
 constexpr float kSlack = 8.0f;
 
 // The bounds of sequence b, whatever the device arrays hold: its first row
-// q0, its rows nq (at most max_q, inside the q rows) and its cached positions
-// kv (inside its table).
-__device__ __forceinline__ void sequence(const AttendArgs& a, int b, int64_t& q0, int& nq, int& kv) {
+// q0, its rows nq (at most max_q, inside the q rows), its cached positions kv
+// (inside its table) and the first row's position pos0 (negative where it
+// stands before the cache).
+__device__ __forceinline__ void sequence(const AttendArgs& a, int b, int64_t& q0, int& nq, int& kv, int& pos0) {
   const int64_t s = a.q_starts[b], e = a.q_starts[b + 1];
   q0 = s < 0 ? 0 : (s > a.tokens ? a.tokens : s);
   const int64_t q1 = e < q0 ? q0 : (e > a.tokens ? a.tokens : e);
   nq = q1 - q0 > a.max_q ? a.max_q : (int)(q1 - q0);
   const int n = a.kv_lens[b];
   kv = n < 0 ? 0 : (n > a.max_kv ? a.max_kv : n);
+  pos0 = kv - (int)(q1 - q0);  // rows past max_q count
 }
 
 // The first position that a row standing at `pos` sees.

@@ -25,8 +25,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int block = (int)(row_of_head / p.rows), row = (int)(row_of_head - (int64_t)block * p.rows);
   int64_t q0;
-  int nq, kv;
-  sequence(a, b, q0, nq, kv);
+  int nq, kv, pos0;
+  sequence(a, b, q0, nq, kv, pos0);
   const int rows = nq * a.group;
   const int64_t hs = (int64_t)b * a.c.heads + kvh;
   const bool on = sub < fit && block < p.cut && rows > lo_rows && rows <= hi_rows && row_of_head < rows;

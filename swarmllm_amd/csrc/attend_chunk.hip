@@ -208,13 +208,12 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
   const int block = whole ? parts.blocks - 1 - z : parts.cut - 1 - down;
   const int part = whole ? 0 : cut_z - down * nparts;
   int64_t q0;
-  int nq, kv;
-  sequence(a, b, q0, nq, kv);
+  int nq, kv, pos0;
+  sequence(a, b, q0, nq, kv, pos0);
   const int rows = nq * a.group;
   const int r0 = block * kRows;
   if (rows <= lo_rows || r0 >= rows) return;
 
-  const int pos0 = kv - nq;
   const int last_row = rows - 1 < r0 + kRows - 1 ? rows - 1 : r0 + kRows - 1;
   const int low_pos = pos0 + token_of(a, r0), high_pos = pos0 + token_of(a, last_row);
   const int lo = first_seen(a, low_pos < 0 ? 0 : low_pos), seen = high_pos + 1;  // [lo, seen): what the rows see

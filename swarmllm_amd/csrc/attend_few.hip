@@ -50,13 +50,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
   const int col = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x, part = blockIdx.y, b = blockIdx.z;
   int64_t q0;
-  int nq, kv;
-  sequence(a, b, q0, nq, kv);
+  int nq, kv, pos0;
+  sequence(a, b, q0, nq, kv, pos0);
   const int rows = nq * a.group;
   if (rows <= lo_rows || rows > hi_rows) return;  // another launch's (or none)
 
   // this workgroup's steps: its part of [first position any row sees, kv)
-  const int pos0 = kv - nq;  // of the first new token; negative where it stands before the cache
   const int lo = first_seen(a, pos0 < 0 ? 0 : pos0);
   int begin, end;
   part_steps(lo, kv, part, parts.parts, begin, end);

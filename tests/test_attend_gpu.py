@@ -245,3 +245,16 @@ def test_refusals():
     assert kv.attend(q[:0], starts[:1] * 0, lens[:0], tables[:0], max_q=0).shape == (0, 4, 64)
     out = torch.full_like(q, 3.0)
     assert (kv.attend(q, starts[:1], lens[:0], tables[:0], max_q=2, out=out) == 3).all()
+
+
+@pytest.mark.parametrize("new,most", [(5, 3), (40, 7), (300, 40), (600, 290)])
+def test_rows_past_max_q_are_left_and_move_no_other(new, most):
+    """Positions go by q_starts and kv_lens alone: the rows inside max_q are those of a call that has them all."""
+    kv, q, starts, lens, tables, _ = batch([new, 1], [new + 900, 300], 8, 2, 64, 32, F16, seed=new)
+    want, tol = attend64(kv, q, starts, lens, tables, 0.125)
+    out = torch.full_like(q, 7.0)
+    kv.attend(q, starts, lens, tables, max_q=most, out=out)
+    inside = torch.arange(new + 1, device="cuda")
+    inside = (inside < most) | (inside == new)
+    check(out[inside], want[inside], tol[inside])
+    assert (out[~inside] == 7).all()
