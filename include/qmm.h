@@ -90,7 +90,7 @@ int qmm_quantize_act(const float *x, void *xq, int layout, int64_t k, int64_t ro
 
 /* The values a quantized activation stands for, code * scale, as f32, f16 or
  * bf16 (out_dtype: qmm_x_dtype; out rows k values apart): qmm_dequantize's
- * counterpart for the planes. */
+ * counterpart for the planes (xq 16-byte aligned). */
 int qmm_dequantize_act(const void *xq, int layout, void *out, int out_dtype, int64_t k, int64_t rows, int64_t stream);
 
 /* Residual addition and root-mean-square norm, the result quantized for the
@@ -99,10 +99,10 @@ int qmm_dequantize_act(const void *xq, int layout, void *out, int out_dtype, int
  *   h  = T(x + residual)                    (x itself without a residual)
  *   rs = f32(1 / sqrt(sum h^2 / k + eps))   (the sum in 64 bits)
  *   y  = f32(f32(h * rs) * w)               (w: k f32 values)
- * `h` (NULL: not kept) gets the stream, `xq` (NULL: none) the planes of y in
- * `layout`, equal to qmm_quantize_act's of the f32 y bit for bit, and `y` (NULL:
- * none; y_dtype) y itself, for what reads plain values (a router). One of xq
- * and y is given. Strides are in values, at least k; k is a multiple of 4, and
+ * `h` (NULL: not kept) gets the stream, `xq` (NULL: none; 16-byte aligned)
+ * the planes of y in `layout`, equal to qmm_quantize_act's of the f32 y bit for
+ * bit, and `y` (NULL: none; y_dtype) y itself, for what reads plain values (a
+ * router). One of xq and y is given. Strides are in values, at least k; k is a multiple of 4, and
  * of the layout's block where xq is given. h may be x or residual itself (the
  * same pointer and stride); otherwise nothing overlaps. A row's result does
  * not depend on the other rows, nor on their number. One launch. */
@@ -262,9 +262,9 @@ int qmm_forward_shared(int type, int count, const void *const *w, const int64_t 
 
 /* qmm_forward, qmm_forward_shared and (below) qmm_forward_glu from an
  * activation already quantized in qmm_act_layout(type, rows)
- * (qmm_rms_norm_act, qmm_quantize_act): the same kernels and, with the
- * workspace that each plans, the same bits, without the quantizer's launch. The
- * workspace holds the slots of a K split (and the GLU's two products); *need
+ * (qmm_rms_norm_act, qmm_quantize_act), 16-byte aligned: the same kernels and,
+ * with the workspace that each plans, the same bits, without the quantizer's
+ * launch. The workspace holds the slots of a K split (and the GLU's two products); *need
  * can be 0, and without room for the slots a product runs uncut, as
  * qmm_matmul. xq is read only. Not affected by qmm_set_force_dmmv. */
 int qmm_forward_act(int type, const void *w, const void *xq, float *dst, int64_t ldd, void *workspace,
@@ -427,9 +427,8 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
  * weights, each rounded once to nearest. scale is finite (at most 1e30 in
  * size). Any mix of lengths is served by one call; the rows of a sequence do
  * not depend on the other sequences' data. Plan (launch == 0) and launch as
- * qmm_forward: the workspace joins the parts of a long context (*need can be
- * 0). On a stream being captured the first call of a process wants qmm_prepare
- * before it, as a product's. */
+ * qmm_forward: the workspace (16-byte aligned) joins the parts of a long
+ * context (*need can be 0). */
 int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_stride, int64_t q_head_stride,
                int64_t tokens, int heads, const int32_t *q_starts, const int32_t *kv_lens, const int32_t *tables,
                int64_t table_stride, int64_t seqs, int64_t max_q, int64_t max_kv, float scale, int64_t window,
@@ -592,8 +591,9 @@ size_t qmm_read_floor_sink_bytes(void);
 int qmm_read_floor(const void *a, size_t a_bytes, const void *b, size_t b_bytes, void *sink, int64_t stream);
 
 /* Fault injection, host side (the reference's fail_the_next_mmq_allocation,
- * quantized/cuda.rs:972-991): the next qmm_forward launch returns
- * QMM_NO_ROOM without enqueuing anything, once. */
+ * quantized/cuda.rs:972-991): the next launch of qmm_forward (or
+ * of another call with a workspace that its plan sizes) returns QMM_NO_ROOM
+ * without enqueuing anything, once. */
 void qmm_fail_next_launch(void);
 
 /* Synthetic data: `n` f32 values from N(mean, std) on the device,

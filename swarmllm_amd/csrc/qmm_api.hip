@@ -65,6 +65,9 @@ bool shape_ok(int type, int64_t k, int64_t n, int64_t rows) {
   return qk != 0 && k > 0 && k % qk == 0 && n > 0 && rows > 0 && k <= (int64_t)1 << 30 && n <= ((int64_t)1 << 31) - 1;
 }
 
+// As the planes of an activation or a cache, or partial results, have to lie.
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
 // A paged cache's sizes: pages of 16 to 256 positions (a power of two), heads
 // of a dim the attention kernels are built for, planes inside an int64.
 bool cache_shape_ok(int64_t pages, int kv_heads, int head_dim, int page) {
@@ -74,8 +77,7 @@ bool cache_shape_ok(int64_t pages, int kv_heads, int head_dim, int page) {
 }
 bool cache_ok(const qmm_cache* c) {
   return c && cache_shape_ok(c->pages, c->kv_heads, c->head_dim, c->page) && c->k_codes && c->k_scales && c->v_codes &&
-         c->v_scales && ((uintptr_t)c->k_codes & 15) == 0 && ((uintptr_t)c->k_scales & 15) == 0 &&
-         ((uintptr_t)c->v_codes & 15) == 0 && ((uintptr_t)c->v_scales & 15) == 0;
+         c->v_scales && aligned16(c->k_codes) && aligned16(c->k_scales) && aligned16(c->v_codes) && aligned16(c->v_scales);
 }
 qmm::CachePlanes planes_of(const qmm_cache& c) {
   return qmm::CachePlanes{(int8_t*)c.k_codes, (uint16_t*)c.k_scales, (int8_t*)c.v_codes, (uint16_t*)c.v_scales,
@@ -242,8 +244,6 @@ bool mmq_allows(int64_t rows) {
   const MmqPolicy& pol = mmq_policy();
   return pol.on && rows <= pol.max_rows;
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Q4_K and Q6_K at 17-128 rows and Q6_K's up to 256 that the single-pass GEMM
 // does not take (gemm_kq_mid.hip): the weight cut along K.
@@ -584,7 +584,8 @@ int qmm_quantize_act(const float* x, void* xq, int layout, int64_t k, int64_t ro
 }
 
 int qmm_dequantize_act(const void* xq, int layout, void* out, int out_dtype, int64_t k, int64_t rows, int64_t stream) {
-  if (qmm_act_bytes(layout, k, rows) == 0 || !qmm::value_type_ok(out_dtype) || xq == nullptr || out == nullptr)
+  if (qmm_act_bytes(layout, k, rows) == 0 || !qmm::value_type_ok(out_dtype) || xq == nullptr || !aligned16(xq) ||
+      out == nullptr)
     return QMM_UNSUPPORTED;
   clear_stale_error();
   return status_of(qmm::launch_dequantize_act(xq, layout, out, out_dtype, k, rows, (hipStream_t)stream));
@@ -596,7 +597,7 @@ int qmm_rms_norm_act(const void* x, int dtype, int64_t x_stride, const void* res
   if (!x || !w || !(xq || y) || !qmm::value_type_ok(dtype) || k < 1 || k > (int64_t)1 << 30 || rows < 1 ||
       x_stride < k || (residual && r_stride < k) || (h && h_stride < k) || !(eps >= 0.0f))
     return QMM_UNSUPPORTED;
-  if (xq && qmm_act_bytes(layout, k, rows) == 0) return QMM_UNSUPPORTED;
+  if (xq && (qmm_act_bytes(layout, k, rows) == 0 || !aligned16(xq))) return QMM_UNSUPPORTED;
   if (k % 4 != 0 || (y && (!qmm::value_type_ok(y_dtype) || y_stride < k))) return QMM_UNSUPPORTED;
   clear_stale_error();
   return status_of(qmm::launch_rms_norm_act(x, dtype, x_stride, residual, r_stride, w, eps, h, h_stride, xq, layout, y,
@@ -720,7 +721,8 @@ int qmm_matmul(int type, const void* w, const void* xq, float* dst, int64_t ldd,
 static int forward_impl(int type, const void* w, bool pre, const void* xq, const float* x, int64_t x_stride, float* dst,
                         int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k, int64_t n,
                         int64_t rows, int launch, int64_t stream) {
-  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || (!pre && x_stride < k)) return QMM_UNSUPPORTED;
+  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || (pre ? !aligned16(xq) : x_stride < k))
+    return QMM_UNSUPPORTED;
   const int layout = qmm_act_layout(type, rows);
   const size_t bytes = pre ? 0 : qmm::act_bytes(layout, k, rows);
   const void* acts = pre ? xq : workspace;
@@ -792,7 +794,8 @@ int qmm_forward_act(int type, const void* w, const void* xq, float* dst, int64_t
 static int shared_impl(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
                        const int64_t* ldd, bool pre, const void* xq, const float* x, int64_t x_stride, void* workspace,
                        size_t workspace_bytes, size_t* need, int64_t k, int64_t rows, int launch, int64_t stream) {
-  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || (!pre && x_stride < k)) return QMM_UNSUPPORTED;
+  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || (pre ? !aligned16(xq) : x_stride < k))
+    return QMM_UNSUPPORTED;
   for (int i = 0; i < count; i++)
     if (!shape_ok(type, k, n[i], rows) || ldd[i] < n[i]) return QMM_UNSUPPORTED;
   const int layout = qmm_act_layout(type, rows);
@@ -929,7 +932,7 @@ static int glu_impl(int type, int act, const void* w_gate, const void* w_up, boo
                     int64_t x_stride, float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need,
                     int64_t k, int64_t n, int64_t rows, int launch, int64_t stream) {
   if (!shape_ok(type, k, n, rows) || act < QMM_GLU_SILU || act > QMM_GLU_GELU || need == nullptr || ldd < n ||
-      (!pre && x_stride < k))
+      (pre ? !aligned16(xq) : x_stride < k))
     return QMM_UNSUPPORTED;
   // workspace: the quantized activation, then the gate and up products of
   // the two-launch form
@@ -1102,7 +1105,8 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   if (!qmm::attend_fits(a)) return QMM_UNSUPPORTED;
   *need = qmm::attend_workspace_bytes(a, cu_count());
   if (!launch) return QMM_OK;
-  if (!q || !out || !q_starts || !kv_lens || (!tables && a.max_kv > 0)) return QMM_UNSUPPORTED;
+  if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
+  if (!q || !out || !q_starts || !kv_lens || (!tables && a.max_kv > 0) || !aligned16(workspace)) return QMM_UNSUPPORTED;
   if (*need > 0 && (workspace == nullptr || workspace_bytes < *need)) return QMM_WORKSPACE_TOO_SMALL;
   clear_stale_error();
   return status_of(qmm::launch_attend(a, cu_count(), workspace, (hipStream_t)stream));

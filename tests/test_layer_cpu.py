@@ -142,3 +142,25 @@ def test_products_of_planes_plan_the_slots_alone(t, k, n, rows):
     assert L.qmm_forward_act(3, P, P, P, n, None, 0, ctypes.byref(b), k, n, rows, 0, 0) == QMM_UNSUPPORTED
     assert L.qmm_forward_glu_act(t, 5, P, P, P, P, n, None, 0, ctypes.byref(b), k, n, rows, 0, 0) == QMM_UNSUPPORTED
     assert L.qmm_forward_shared_act(t, 0, None, None, None, None, P, None, 0, ctypes.byref(b), k, rows, 0, 0) == QMM_UNSUPPORTED
+
+
+def test_addresses_off_16_bytes_are_refused():
+    """The planes of an activation and the partial results of a context are read and written 16 bytes at a time."""
+    odd = ctypes.c_void_p(4096 + 8)
+    assert norm(xq=odd) == QMM_UNSUPPORTED
+    L, n = lib(), need()
+    assert L.qmm_dequantize_act(odd, _lib.ACT_Q8K, P, X_F16, 512, 1, 0) == QMM_UNSUPPORTED
+    assert L.qmm_forward_act(12, P, odd, P, 64, None, 0, ctypes.byref(n), 512, 64, 1, 0, 0) == QMM_UNSUPPORTED
+    assert L.qmm_forward_glu_act(12, 0, P, P, odd, P, 64, None, 0, ctypes.byref(n), 512, 64, 1, 0, 0) == QMM_UNSUPPORTED
+    one, w, d = (ctypes.c_int64 * 1)(64), (ctypes.c_void_p * 1)(4096), (ctypes.c_void_p * 1)(4096)
+    assert L.qmm_forward_shared_act(12, 1, w, one, d, one, odd, None, 0, ctypes.byref(n), 512, 1, 0, 0) == QMM_UNSUPPORTED
+    long = dict(seqs=1, tokens=1, max_q=1, max_kv=3200)
+    want = attend(**long)[1]
+    assert attend(launch=1, ws=odd, ws_bytes=want, **long) == (QMM_UNSUPPORTED, want)
+
+
+def test_attend_takes_the_injected_fault():
+    lib().qmm_fail_next_launch()
+    assert attend(max_kv=512)[0] == QMM_OK  # a plan does not
+    assert attend(max_kv=512, launch=1, q=None)[0] == _lib.QMM_NO_ROOM
+    assert attend(max_kv=512, launch=1, q=None)[0] == QMM_UNSUPPORTED  # once

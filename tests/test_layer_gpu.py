@@ -4,6 +4,10 @@ rms_norm_act with the residual -> gate/up + GLU from its planes -> down. Each
 step is held to its own definition on the inputs it was given; a captured
 decode step replays with the eager step's bits, graphs and streams beside each
 other do not disturb each other."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -199,3 +203,53 @@ def test_results_do_not_change_from_call_to_call_nor_with_the_batch():
     first = kv.attend(q, s, l, t, max_q=3)
     for _ in range(5):
         assert torch.equal(kv.attend(q, s, l, t, max_q=3), first)
+
+
+FIRST_CALLS_CAPTURED = """
+import torch
+from swarmllm_amd import GgmlDType, KvCache, rms_norm_act
+g = torch.Generator(device="cuda")
+g.manual_seed(5)
+x = torch.randn(600, 8 * 128, generator=g, device="cuda")
+w = torch.ones(8 * 128, device="cuda")
+kv = KvCache.alloc(60, 2, 128, 64)
+tables = torch.randperm(60, generator=g, device="cuda").view(1, 60).int()
+slots = kv.slots(tables[0], 3000, 600)
+past = torch.randn(3000, 2, 128, generator=g, device="cuda")
+starts = torch.tensor([0, 600], device="cuda", dtype=torch.int32)
+lens = torch.tensor([3600], device="cuda", dtype=torch.int32)
+old = kv.slots(tables[0], 0, 3000)
+
+def step():
+    n = rms_norm_act(x, w, 1e-5, dtype=GgmlDType.Q4K, y_dtype=torch.float16)
+    q = n.act.dequantize_f16().view(600, 8, 128)
+    kv.write(past, past, old)
+    kv.write(q[:, :2], q[:, 2:4], slots)
+    k, v = kv.read(slots)
+    return n.y, q, k, v, kv.attend(q, starts, lens, tables, max_q=600), kv.attend(q[599:], starts // 600, lens, tables, max_q=1)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    first = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in first]
+for a, b in zip(got, step()):
+    assert a.dtype == b.dtype and a.isfinite().all() and torch.equal(a, b)
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, first))
+print("captured first calls equal eager ones")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """Each entry point's first call of a process may be a captured one (no
+    qmm_prepare before it): what a first launch sets up, more than 64 KiB of
+    LDS for 256 query rows a workgroup among it, is allowed under capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=root + (os.pathsep + os.environ["PYTHONPATH"] if os.environ.get("PYTHONPATH") else ""))
+    res = subprocess.run([sys.executable, "-u", "-c", FIRST_CALLS_CAPTURED], env=env, cwd=root, capture_output=True,
+                         text=True, timeout=100)
+    assert res.returncode == 0 and "captured first calls equal" in res.stdout, res.stdout[-2000:] + res.stderr[-2000:]
