@@ -6,6 +6,13 @@
 //   s_j = scale * q . k_j,  o = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m))
 // over the positions j of the sequence with pos - window < j <= pos, m their
 // largest s_j. A row that no position is left to is zero.
+//
+// q, keys (code * scale), values and weights are f16 operands of the matrix
+// cores, each rounded once; scores, maxima, sums and outputs are f32. The
+// rounding, 2^-11 of a value, is an eighth of the half step that a code's own
+// rounding leaves (1 / 254 of its block's largest); f16 outputs end 4e-4 to
+// 5e-4 from 64 bits (an exact sum's rounding: 2e-4). f32 operands run at a 16th
+// of the rate.
 #include "attend.h"
 
 namespace qmm {

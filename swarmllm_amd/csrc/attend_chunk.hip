@@ -16,8 +16,8 @@
 // lane's own column.
 //
 // Two prompts' chunks of 2000 tokens over 7777 (64 query heads on 8 of 128 dims)
-// take 866 us, 0.77 PFLOP/s; a library product of 8192^3 reaches 1.15. The
-// products, the softmax's and the conversions' vector instructions (about 290 a
+// take 866-888 us, 0.76 PFLOP/s; a library product of 8192^3 reaches 1.15. The
+// products (matrix cores busy 43% of the CUs' cycles), the softmax's and the conversions' vector instructions (about 290 a
 // wave and step with 128 rows a workgroup, 230 with 256) and the LDS reads (32
 // operands of 1 KiB a wave and step) each take a third to a half of a step and
 // overlap only between the two waves of a SIMD. Tried and slower: a step's
