@@ -174,6 +174,8 @@ struct AttendParts {
   float* ml;
   int parts, rows;  // query rows of a block
   int blocks, cut;  // row blocks of a kv head of a sequence; the first `cut` of them are in parts
+  int4* split;      // shares (attend_chunk.hip): the block that each leaves unfinished
+  int shares;       // 0: none
 };
 __device__ __forceinline__ int64_t part_row(const AttendParts& p, int64_t head_of_seq, int block, int part, int row) {
   return ((head_of_seq * p.cut + block) * p.parts + part) * p.rows + row;
@@ -202,6 +204,11 @@ __device__ __forceinline__ void store_out4(const AttendArgs& a, int64_t e, const
   else
     store4<false>(a.out, a.odt, e, v);
 }
+
+constexpr int kShareRows = 256;  // query rows of a block that shares may split
+// Partial results of share w: slot 2 w for a block that a share before it
+// began, 2 w + 1 for one that it leaves to the next.
+__device__ __forceinline__ int64_t share_row(int slot, int row) { return (int64_t)slot * kShareRows + row; }
 
 // The launches of either kernel over the sequences with lo < rows <= hi query
 // rows a kv head (tokens times group); parts > 1: into `p`.

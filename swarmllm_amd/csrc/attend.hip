@@ -81,10 +81,43 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   store_out4(a, (q0 + i) * a.os + (int64_t)head * hd + e, out);
 }
 
+// A block that shares have split: its pieces from the share that began it to
+// the one that ended it. 4 dims a lane, 64 / (hd / 4) rows a wave.
+__global__ __launch_bounds__(256) void attend_join_shares_kernel(AttendArgs a, AttendParts p) {
+  const int w = blockIdx.x;
+  const int4 split = p.split[w];
+  if (split.w < 0) return;
+  const int hd = a.c.hd, per = hd / 4, fit = 64 / per;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane / per, e = 4 * (lane - sub * per), row = (blockIdx.y * 4 + wave) * fit + sub;
+  const int b = split.x, kvh = split.y, r = split.z * kShareRows + row;
+  int64_t q0;
+  int nq, kv, pos0;
+  sequence(a, b, q0, nq, kv, pos0);
+  if (sub >= fit || row >= kShareRows || r >= nq * a.group) return;
+  float top = -INFINITY, sum = 0.0f;
+  f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int v = w; v <= split.w; v++) {
+    const int64_t i = share_row(v == w ? 2 * w + 1 : 2 * v, row);
+    const float m = p.ml[2 * i], l = p.ml[2 * i + 1];
+    const f4v o = *(const f4v*)(p.o + i * hd + e);
+    const float mx = fmaxf(top, m), base = mx == -INFINITY ? 0.0f : mx;
+    const float fa = exp2_fast(top - base), fb = exp2_fast(m - base);
+    top = mx;
+    sum = sum * fa + l * fb;
+    acc = acc * fa + o * fb;
+  }
+  const int i = token_of(a, r), head = kvh * a.group + r - i * a.group;
+  float out[4];
+  finish_row<4>(a, head, top, sum, (const float*)&acc, out);
+  store_out4(a, (q0 + i) * a.os + (int64_t)head * hd + e, out);
+}
+
 // How a call runs: the sequences of at most `few` query rows a kv head on the
 // few-row kernel (0: none), the others on the chunk kernel.
 struct Plan {
-  int few, few_parts, chunk_rows, chunk_blocks, chunk_cut, chunk_parts;
+  int few, few_parts, chunk_rows, chunk_blocks, chunk_cut, chunk_parts, shares;
 };
 
 int clamp_parts(int64_t want, int64_t most) {
@@ -103,20 +136,31 @@ Plan plan_of(const AttendArgs& a, int cus) {
   Plan p{};
   const int64_t rows = (int64_t)a.max_q * a.group, heads = (int64_t)a.seqs * a.c.heads;
   if (rows > kFewRows) {
-    // 256 rows a workgroup lay a step's keys and values down once for 8 waves;
+    // blocks of 256 rows lay a step's keys and values down once for 8 waves;
     // over short contexts twice as many workgroups are worth more (us, 256 /
-    // 128 rows: 512 tokens over 4096 67 / 71, 2 x 2000 over 7777 866 / 937; 1000
+    // 128 rows: 512 tokens over 4096 67 / 71, 2000 and 1333 over 7777 and 5832 866 / 937; 1000
     // over 1000 35 / 32, 8 x 64 over 2000 50 / 48)
-    p.chunk_rows = a.c.hd <= 128 && rows > 256 && most_steps(a, 256) >= 32 ? 256 : 128;
+    p.chunk_rows = a.c.hd <= 128 && rows > kShareRows && most_steps(a, kShareRows) >= 32 ? kShareRows : 128;
     p.chunk_blocks = (int)((rows + p.chunk_rows - 1) / p.chunk_rows);
     const int64_t slots = (int64_t)cus * (p.chunk_rows > 128 || a.c.hd > 128 ? 1 : 2), n = heads * p.chunk_blocks;
-    const int64_t steps = most_steps(a, p.chunk_rows);
-    // parts that fill the CUs, of 8 steps at least: of every block where those
-    // are few, otherwise of what is left behind the last whole round of the CUs
-    const int64_t left = n <= slots ? n : n % slots;
-    p.chunk_parts = left ? clamp_parts(slots / left, steps / 8) : 1;
-    p.chunk_cut = p.chunk_parts > 1 ? (int)((left + heads - 1) / heads) : 0;
-    if (p.chunk_cut == 0) p.chunk_parts = 1;
+    const double work = (double)(a.max_kv + 1024) * a.group * (double)n;  // in 64 bits
+    if (p.chunk_rows == kShareRows && n > slots && n < 6 * slots && work < 1e17) {
+      // a few rounds of the CUs: equal shares, so that the last round is whole and
+      // sequences shorter than max_q and max_kv leave no CU idle (us, shares /
+      // blocks: 2000 and 1333 tokens over 7777 and 5832 751 / 887; all of one length
+      // 0 to 3 % slower: 2 x 2000 over 7777 985 / 981, 4000 over 7777 831 / 809). Many
+      // rounds fill up by themselves, and their short blocks' beginnings count
+      // more (7777 over 7777 1338 / 1083); fewer blocks than CUs are cut evenly
+      // (512 over 4096 76 / 56).
+      p.shares = cus;
+    } else {
+      // parts that fill the CUs, of 8 steps at least: of every block where those
+      // are few, otherwise of what is left behind the last whole round of the CUs
+      const int64_t left = n <= slots ? n : n % slots;
+      p.chunk_parts = left ? clamp_parts(slots / left, most_steps(a, p.chunk_rows) / 8) : 1;
+      p.chunk_cut = p.chunk_parts > 1 ? (int)((left + heads - 1) / heads) : 0;
+      if (p.chunk_cut == 0) p.chunk_parts = 1;
+    }
     if (a.seqs > 1) p.few = 16;  // one-token sequences beside a prompt
   } else {
     p.few = rows <= 16 ? 16 : kFewRows;
@@ -138,12 +182,21 @@ Plan plan_of(const AttendArgs& a, int cus) {
 
 // The partial results at ws: bytes, and where they lie.
 size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, void* ws, AttendParts& p) {
-  p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut};
+  p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut, nullptr, 0};
   if (parts <= 1) return 0;
   const size_t n = (size_t)a.seqs * a.c.heads * cut * parts * rows;
   p.o = (float*)ws;
   p.ml = p.o + n * a.c.hd;
   return n * (a.c.hd + 2) * sizeof(float);
+}
+
+// And those of `shares`.
+size_t shares_at(const AttendArgs& a, int shares, void* ws, AttendParts& p) {
+  p = AttendParts{(float*)ws, nullptr, 1, kShareRows, 0, 0, nullptr, shares};
+  const size_t n = (size_t)2 * shares * kShareRows;
+  p.ml = p.o + n * a.c.hd;
+  p.split = (int4*)(p.ml + 2 * n);
+  return n * (a.c.hd + 2) * sizeof(float) + shares * sizeof(int4);
 }
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
@@ -172,7 +225,7 @@ size_t attend_workspace_bytes(const AttendArgs& a, int cus) {
   const Plan p = plan_of(a, cus);
   AttendParts q;
   const size_t few = p.few ? parts_at(a, p.few_parts, p.few, 1, 1, nullptr, q) : 0;
-  const size_t chunk = p.chunk_blocks ? parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, nullptr, q) : 0;
+  const size_t chunk = p.shares ? shares_at(a, p.shares, nullptr, q) : p.chunk_blocks ? parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, nullptr, q) : 0;
   return few > chunk ? few : chunk;  // one after the other
 }
 
@@ -180,7 +233,15 @@ hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st)
   const Plan p = plan_of(a, cus);
   AttendParts q;
   hipError_t e = hipSuccess;
-  if (p.chunk_blocks) {
+  if (p.shares) {
+    shares_at(a, p.shares, ws, q);
+    e = launch_attend_chunk(a, p.few, q, st);
+    if (e == hipSuccess) {
+      const int rows = 4 * (64 / (a.c.hd / 4));
+      attend_join_shares_kernel<<<dim3((unsigned)p.shares, (unsigned)((kShareRows + rows - 1) / rows)), 256, 0, st>>>(a, q);
+      e = hipGetLastError();
+    }
+  } else if (p.chunk_blocks) {
     parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, ws, q);
     e = launch_attend_chunk(a, p.few, q, st);
     if (e == hipSuccess && q.parts > 1) e = join(a, p.few, INT32_MAX, q, st);

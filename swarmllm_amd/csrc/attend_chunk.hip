@@ -15,12 +15,12 @@
 // they stand. The running maximum, the sum and O's rescaling belong to the
 // lane's own column.
 //
-// Two prompts' chunks of 2000 tokens over 7777 (64 query heads on 8 of 128 dims)
-// take 866-888 us, 0.76 PFLOP/s; a library product of 8192^3 reaches 1.15. The
-// products (matrix cores busy 43% of the CUs' cycles), the softmax's and the conversions' vector instructions (about 290 a
-// wave and step with 128 rows a workgroup, 230 with 256) and the LDS reads (32
-// operands of 1 KiB a wave and step) each take a third to a half of a step and
-// overlap only between the two waves of a SIMD. Tried and slower: a step's
+// Chunks of 2000 and 1333 tokens over 7777 and 5832 (64 query heads on 8 of 128
+// dims) take 751-763 us, 0.88 PFLOP/s; a library product of 8192^3 reaches 1.15.
+// The products, the softmax's and the conversions' vector instructions (about
+// 290 a wave and step with 128 rows a workgroup, 235 with 256) and the LDS reads
+// (32 operands of 1 KiB a wave and step) each take a third to a half of a step
+// and overlap only between the two waves of a SIMD. Tried and slower: a step's
 // scores beside the weights of the one before (the second set of scores spills
 // at 256 registers), steps of 32 positions, 64 rows a wave (accumulators past 256
 // registers are copied back and forth each step), and products and vector
@@ -31,6 +31,24 @@
 namespace qmm {
 
 namespace {
+
+// A kernel's arguments, all of them.
+struct ChunkCall {
+  AttendArgs a;
+  AttendParts parts;
+  int lo_rows;
+};
+
+// Read afresh where they are wanted: 60 registers of arguments that live through
+// a block's steps would push what a step needs out of the scalar registers
+// (into lanes of vector registers and back, 136 moves a step).
+__device__ __forceinline__ ChunkCall call_args() {
+  auto p = (const __attribute__((address_space(4))) ChunkCall*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  ChunkCall c;
+  __builtin_memcpy(&c, (const ChunkCall*)p, sizeof c);
+  return c;
+}
 
 // Instruction classes of __builtin_amdgcn_sched_group_barrier.
 constexpr int kMfma = 0x008, kDsRead = 0x100;
@@ -60,15 +78,15 @@ struct Staged {
 
 // A thread's i-th item of keys, or of values; on: whether it has one.
 template <int HD, int W>
-__device__ __forceinline__ int k_item(int i, bool& on) {
-  const int x = (int)threadIdx.x + ChunkSizes<HD, W>::kThreads * i;
+__device__ __forceinline__ int k_item(int tid, int i, bool& on) {
+  const int x = tid + ChunkSizes<HD, W>::kThreads * i;
   on = ChunkSizes<HD, W>::kItems % ChunkSizes<HD, W>::kThreads == 0 || x < ChunkSizes<HD, W>::kItems;
   return x;
 }
 template <int HD, int W>
-__device__ __forceinline__ int v_item(int i, bool& on) {
-  if (!ChunkSizes<HD, W>::kHalves) return k_item<HD, W>(i, on);
-  const int x = (int)threadIdx.x - ChunkSizes<HD, W>::kThreads / 2;
+__device__ __forceinline__ int v_item(int tid, int i, bool& on) {
+  if (!ChunkSizes<HD, W>::kHalves) return k_item<HD, W>(tid, i, on);
+  const int x = tid - ChunkSizes<HD, W>::kThreads / 2;
   on = x >= 0 && x < ChunkSizes<HD, W>::kItems;
   return x;
 }
@@ -79,19 +97,22 @@ __device__ __forceinline__ int v_dim(int x) { return (x >> 6) * 32 + ((x >> 2) &
 // A step's pages. ONE: pages of 64 positions and more, so a step has one, the
 // same for the wave; otherwise lane x < 4 of every wave holds that of the step's
 // x-th 16 positions. -1: none.
+// The table's entry (-1 behind the last), looked at only in settled() so
+// that nothing waits for it meanwhile.
 template <bool ONE>
-__device__ __forceinline__ int step_page(const AttendArgs& a, int b, int tile, int end, int kv) {
-  if (tile >= end) return -1;
-  return page_of(a, b, tile * kTile + (ONE ? 0 : 16 * (int)(threadIdx.x & 3)), kv);
+__device__ __forceinline__ int step_page(const AttendArgs& a, int tid, int b, int tile, int end, int kv) {
+  const int j = tile * kTile + (ONE ? 0 : 16 * (tid & 3));
+  return tile < end && j < kv ? a.tables[(int64_t)b * a.table_stride + (j >> a.page_bits)] : -1;
 }
-// ONE: into a scalar register, once the load has surely landed.
+// ONE: into a scalar register.
 template <bool ONE>
-__device__ __forceinline__ int settled(int page) {
+__device__ __forceinline__ int settled(const AttendArgs& a, int page) {
+  if (page >= a.c.pages) page = -1;
   return ONE ? __builtin_amdgcn_readfirstlane(page) : page;
 }
 
 template <int HD, int W, bool ONE>
-__device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int pages, Staged<HD, W>& s) {
+__device__ __forceinline__ void fetch(const AttendArgs& a, int tid, int kvh, int j0, int pages, Staged<HD, W>& s) {
   using Z = ChunkSizes<HD, W>;
   const CachePlanes& c = a.c;
   const int8_t* k1 = nullptr;
@@ -109,7 +130,7 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     bool k_on, v_on;
-    const int xk = k_item<HD, W>(i, k_on), xv = v_item<HD, W>(i, v_on);
+    const int xk = k_item<HD, W>(tid, i, k_on), xv = v_item<HD, W>(tid, i, v_on);
     const int vc = xv & 3, d = v_dim(xv);  // 16 positions from 16 vc on, dims d and d + 16
     if constexpr (ONE) {
       if (k_on) {
@@ -150,12 +171,12 @@ __device__ __forceinline__ void fetch(const AttendArgs& a, int kvh, int j0, int 
 // The step's keys and values as f16 into an LDS buffer. CUT: the values of
 // positions outside [lo, hi), or on no page, are laid as zeros.
 template <int HD, int W, bool ONE, bool CUT>
-__device__ __forceinline__ void lay(const Staged<HD, W>& s, int j0, int pages, int lo, int hi, uint16_t* buf) {
+__device__ __forceinline__ void lay(const Staged<HD, W>& s, int tid, int j0, int pages, int lo, int hi, uint16_t* buf) {
   using Z = ChunkSizes<HD, W>;
 #pragma unroll
   for (int i = 0; i < Z::kEach; i++) {
     bool k_on, v_on;
-    const int xk = k_item<HD, W>(i, k_on), xv = v_item<HD, W>(i, v_on);
+    const int xk = k_item<HD, W>(tid, i, k_on), xv = v_item<HD, W>(tid, i, v_on);
     const int vc = xv & 3, d = v_dim(xv);
     const int vp = !CUT ? 0 : ONE ? pages : __shfl(pages, vc, kWave);
     H8 h;
@@ -190,50 +211,33 @@ __device__ __forceinline__ void lay(const Staged<HD, W>& s, int j0, int pages, i
   }
 }
 
+// The steps of one block of 32 W query rows of kv head kvh of sequence b: its
+// rows from r0 on, steps [begin, end) of those that its rows see. Partial rows
+// from part_at on, or (-1) the outputs themselves. Ends with the workgroup's
+// waves past their last use of LDS.
 template <int HD, int W, bool ONE>
-__global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chunk_kernel(AttendArgs a, int lo_rows,
-                                                                                         AttendParts parts) {
+__device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0, int rows, int kv, int pos0, int r0,
+                                             int lo, int begin, int end, int64_t part_at, uint16_t* s_buf) {
   using Z = ChunkSizes<HD, W>;
-  constexpr int kRows = 32 * W;
-  extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
-  const CachePlanes& c = a.c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const ChunkCall call = call_args();
+  const AttendArgs& a0 = call.a;
+  const int lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, hi = lane >> 5;
-  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)c.heads), kvh = blockIdx.x - b * c.heads;
-  // the rows that see most first; behind the whole blocks the parts of those cut
-  const int z = blockIdx.z, cut_z = z - (parts.blocks - parts.cut);
-  const bool whole = cut_z < 0;
-  const int nparts = whole ? 1 : parts.parts;
-  const int down = whole ? 0 : (int)((uint32_t)cut_z / (uint32_t)nparts);
-  const int block = whole ? parts.blocks - 1 - z : parts.cut - 1 - down;
-  const int part = whole ? 0 : cut_z - down * nparts;
-  int64_t q0;
-  int nq, kv, pos0;
-  sequence(a, b, q0, nq, kv, pos0);
-  const int rows = nq * a.group;
-  const int r0 = block * kRows;
-  if (rows <= lo_rows || r0 >= rows) return;
-
-  const int last_row = rows - 1 < r0 + kRows - 1 ? rows - 1 : r0 + kRows - 1;
-  const int low_pos = pos0 + token_of(a, r0), high_pos = pos0 + token_of(a, last_row);
-  const int lo = first_seen(a, low_pos < 0 ? 0 : low_pos), seen = high_pos + 1;  // [lo, seen): what the rows see
-  int begin, end;
-  part_steps(lo, seen, part, nparts, begin, end);
 
   // this wave's rows
-  const int r = r0 + 32 * wave + col, qi = token_of(a, r);
+  const int r = r0 + 32 * wave + col, qi = token_of(a0, r);
   const int pos = pos0 + qi;
-  const int wave_low = pos0 + token_of(a, r0 + 32 * wave);
+  const int wave_low = pos0 + token_of(a0, r0 + 32 * wave);
   const int wave_last = r0 + 32 * wave + 31 < rows - 1 ? r0 + 32 * wave + 31 : rows - 1;
-  const int wave_high = r0 + 32 * wave < rows ? pos0 + token_of(a, wave_last) : -1;  // no rows: sees nothing
-  const int wave_first = first_seen(a, wave_low < 0 ? 0 : wave_low);
-  const int first = first_seen(a, pos);
+  const int wave_high = r0 + 32 * wave < rows ? pos0 + token_of(a0, wave_last) : -1;  // no rows: sees nothing
+  const int wave_first = first_seen(a0, wave_low < 0 ? 0 : wave_low);
+  const int first = first_seen(a0, pos);
   const bool row_on = r < rows;
   const int64_t row_q = q0 + qi;
-  const int head = kvh * a.group + r - qi * a.group;
+  const int head = kvh * a0.group + r - qi * a0.group;
 
   h8v q[HD / 16];
-  load_query<HD / 16>(a, row_on, [&](int s) { return row_q * a.qs + (int64_t)head * a.qhs + 16 * s + 8 * hi; }, q);
+  load_query<HD / 16>(a0, row_on, [&](int s) { return row_q * a0.qs + (int64_t)head * a0.qhs + 16 * s + 8 * hi; }, q);
 
   f16v o[HD / 32];
 #pragma unroll
@@ -241,21 +245,23 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
 #pragma unroll
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
+  const ChunkCall in_steps = call_args();
+  const AttendArgs& a = in_steps.a;
 
   auto lay_step = [&](const Staged<HD, W>& s, int tile, int pages, int buf) {
     const int j0 = tile * kTile;
     uint16_t* to = s_buf + buf * Z::kHalfs;
     if (j0 < lo || j0 + kTile > kv || __ballot(pages < 0) != 0)
-      lay<HD, W, ONE, true>(s, j0, pages, lo, kv, to);
+      lay<HD, W, ONE, true>(s, tid, j0, pages, lo, kv, to);
     else
-      lay<HD, W, ONE, false>(s, j0, pages, lo, kv, to);
+      lay<HD, W, ONE, false>(s, tid, j0, pages, lo, kv, to);
   };
 
   Staged<HD, W> st;
-  int pages = settled<ONE>(step_page<ONE>(a, b, begin, end, kv));
-  int next_pages = settled<ONE>(step_page<ONE>(a, b, begin + 1, end, kv));
+  int pages = settled<ONE>(a, step_page<ONE>(a, tid, b, begin, end, kv));
+  int next_pages = settled<ONE>(a, step_page<ONE>(a, tid, b, begin + 1, end, kv));
   if (begin < end) {
-    fetch<HD, W, ONE>(a, kvh, begin * kTile, pages, st);
+    fetch<HD, W, ONE>(a, tid, kvh, begin * kTile, pages, st);
     lay_step(st, begin, pages, 0);
   }
   __syncthreads();
@@ -263,8 +269,8 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
   const int krow = (col & 19) | ((col & 4) << 1) | ((col & 8) >> 1);
   for (int tile = begin, cur = 0; tile < end; tile++, cur ^= 1) {
     const int j0 = tile * kTile;
-    const int after_pages = step_page<ONE>(a, b, tile + 2, end, kv);
-    if (tile + 1 < end) fetch<HD, W, ONE>(a, kvh, j0 + kTile, next_pages, st);
+    const int after_pages = step_page<ONE>(a, tid, b, tile + 2, end, kv);
+    if (tile + 1 < end) fetch<HD, W, ONE>(a, tid, kvh, j0 + kTile, next_pages, st);
 
     if (j0 <= wave_high && j0 + kTile > wave_first) {
       const uint16_t* kb = s_buf + cur * Z::kHalfs + krow * Z::kRow + 8 * hi;
@@ -343,21 +349,23 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
     }
     if (tile + 1 < end) lay_step(st, tile + 1, next_pages, cur ^ 1);
     pages = next_pages;
-    next_pages = settled<ONE>(after_pages);
+    next_pages = settled<ONE>(a, after_pages);
     __syncthreads();
   }
 
   l += __shfl_xor(l, 32, kWave);
   if (!row_on) return;
-  if (nparts > 1) {
-    const int64_t pr = part_row(parts, (int64_t)blockIdx.x, block, part, r - r0);
+  const ChunkCall after = call_args();
+  if (part_at >= 0) {
+    const AttendParts& parts = after.parts;
+    const int64_t pr = part_at + r - r0;
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         *(f4v*)(parts.o + pr * HD + 32 * d + 2 * i + 4 * hi) = f4v{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
     if (hi == 0) {
-      parts.ml[2 * pr] = m * a.sc;
+      parts.ml[2 * pr] = m * after.a.sc;
       parts.ml[2 * pr + 1] = l;
     }
     return;
@@ -368,28 +376,263 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
     for (int i = 0; i < 16; i += 4) {
       const float acc[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
       float out[4];
-      finish_row<4>(a, head, m * a.sc, l, acc, out);
-      store_out4(a, row_q * a.os + (int64_t)head * HD + 32 * d + 2 * i + 4 * hi, out);
+      finish_row<4>(after.a, head, m * after.a.sc, l, acc, out);
+      store_out4(after.a, row_q * after.a.os + (int64_t)head * HD + 32 * d + 2 * i + 4 * hi, out);
     }
 }
 
+// What the rows of a block see: positions [lo, seen).
+__device__ __forceinline__ void block_sees(const AttendArgs& a, int rows, int pos0, int r0, int block_rows, int& lo,
+                                           int& seen) {
+  const int last_row = rows - 1 < r0 + block_rows - 1 ? rows - 1 : r0 + block_rows - 1;
+  const int low = pos0 + token_of(a, r0);
+  lo = first_seen(a, low < 0 ? 0 : low);
+  seen = pos0 + token_of(a, last_row) + 1;
+}
+
+// A workgroup a block of 32 W rows, or a part of one.
 template <int HD, int W, bool ONE>
-hipError_t launch_pages(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
-  if constexpr (ChunkSizes<HD, W>::kLds > 64 * 1024) {
-    const hipError_t e = set_max_dynamic_lds<attend_chunk_kernel<HD, W, ONE>>();
+__global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chunk_kernel(ChunkCall call) {
+  constexpr int kRows = 32 * W;
+  const AttendArgs& a = call.a;
+  const AttendParts& parts = call.parts;
+  extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
+  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)a.c.heads), kvh = blockIdx.x - b * a.c.heads;
+  // the rows that see most first; behind the whole blocks the parts of those cut
+  const int z = blockIdx.z, cut_z = z - (parts.blocks - parts.cut);
+  const bool whole = cut_z < 0;
+  const int nparts = whole ? 1 : parts.parts;
+  const int down = whole ? 0 : (int)((uint32_t)cut_z / (uint32_t)nparts);
+  const int block = whole ? parts.blocks - 1 - z : parts.cut - 1 - down;
+  const int part = whole ? 0 : cut_z - down * nparts;
+  int64_t q0;
+  int nq, kv, pos0;
+  sequence(a, b, q0, nq, kv, pos0);
+  const int rows = nq * a.group, r0 = block * kRows;
+  if (rows <= call.lo_rows || r0 >= rows) return;
+  int lo, seen, begin, end;
+  block_sees(a, rows, pos0, r0, kRows, lo, seen);
+  part_steps(lo, seen, part, nparts, begin, end);
+  attend_block<HD, W, ONE>(threadIdx.x, b, kvh, q0, rows, kv, pos0, r0, lo, begin, end,
+                           nparts > 1 ? part_row(parts, (int64_t)blockIdx.x, block, part, 0) : -1, s_buf);
+}
+
+// The blocks of 256 rows of a sequence's kv head as lengths of work: block j's
+// is first + more * j (the positions that its rows see, times the group, and
+// four steps more for its beginning and end). An estimate: all that the shares
+// ask of it is that every workgroup finds the same.
+struct BlockWork {
+  int64_t first;
+  int more, blocks;
+  __device__ __forceinline__ int64_t before(int j) const { return first * j + (int64_t)more * j * (j - 1) / 2; }
+};
+__device__ __forceinline__ BlockWork block_work(const AttendArgs& a, int nq, int kv, int pos0, int lo_rows) {
+  const int rows = nq * a.group;
+  BlockWork w;
+  w.blocks = rows <= lo_rows ? 0 : (rows + kShareRows - 1) / kShareRows;
+  const bool cut = a.window > 0 && a.window < kv;
+  w.more = cut ? 0 : kShareRows;
+  w.first = (int64_t)((cut ? (int)a.window : pos0 < 0 ? 0 : pos0) + 4 * kTile) * a.group + kShareRows;
+  return w;
+}
+
+// Where a share stands: in LDS, for a step wants the scalar registers itself.
+struct ShareAt {
+  int64_t wave[8];
+  int64_t each, u, end;  // a share's length, the place of the piece at hand, the share's end
+  int64_t base;          // the work before sequence b
+  int b, kvh, block;     // the piece's (b: -1 behind a sequence's last block)
+};
+
+// The sequence whose work place u falls into (s.b) and the work before it
+// (s.base). START: u is that of share w of n, found with the share's length and
+// end. Every thread of the workgroup calls; ends with a barrier.
+template <bool START>
+__device__ __forceinline__ void find_sequence(const ChunkCall& c, int tid, int w, ShareAt& s) {
+  const AttendArgs& a = c.a;
+  const int lane = tid & 63, wv = tid >> 6;
+  int64_t u = START ? -1 : s.u, all = 0;
+  // the work of all sequences, then (START) the place among them: in one pass where 512 threads have one each
+  for (int pass = START && a.seqs > 512 ? 0 : 1; pass < 2; pass++) {
+    all = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 512) {
+      int64_t mine = 0;
+      if (b0 + tid < a.seqs) {
+        int64_t q0;
+        int nq, kv, pos0;
+        sequence(a, b0 + tid, q0, nq, kv, pos0);
+        const BlockWork bw = block_work(a, nq, kv, pos0, c.lo_rows);
+        mine = bw.before(bw.blocks) * a.c.heads;
+      }
+      int64_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t t = __shfl_up(upto, d, kWave);
+        if (lane >= d) upto += t;
+      }
+      __syncthreads();
+      if (lane == 63) s.wave[wv] = upto;
+      __syncthreads();
+      int64_t before = all;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (i < wv) before += s.wave[i];
+        all += s.wave[i];
+      }
+      before += upto - mine;
+      if (START && pass == 1 && u < 0) {
+        // 8 steps of a block at least
+        const int64_t least = (int64_t)8 * kTile * a.group, even = (all + c.parts.shares - 1) / c.parts.shares;
+        const int64_t each = even < least ? least : even;
+        u = w * each;
+        if (tid == 0) {
+          s.each = each;
+          s.u = u;
+          s.end = u + each < all ? u + each : all;
+        }
+      }
+      if (u >= before && u < before + mine) {
+        s.b = b0 + tid;
+        s.base = before;
+      }
+    }
+    if (START && pass == 0) {
+      const int64_t least = (int64_t)8 * kTile * a.group, even = (all + c.parts.shares - 1) / c.parts.shares;
+      const int64_t each = even < least ? least : even;
+      u = w * each;
+      if (tid == 0) {
+        s.each = each;
+        s.u = u;
+        s.end = u + each < all ? u + each : all;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return ((int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+// A place x of a block's work (its length `work`) as one of its steps, at least 3
+// steps from either end of the block or on it.
+__device__ __forceinline__ int step_at(int64_t x, int64_t work, int steps) {
+  const int s = (int)((double)x * steps / (double)work);
+  return s < 3 ? 0 : steps - s < 3 ? steps : s;
+}
+
+// The blocks of 256 rows of all sequences and kv heads in a row, dealt to the
+// workgroups in equal lengths of work: a share begins and ends inside a block
+// as it falls, and what it leaves of one is joined by attend_join_shares_kernel
+// (attend.hip). Ragged batches so keep all CUs busy to the end: chunks of 2000
+// and 1333 tokens over 7777 and 5832, 840 blocks of 71 to 122 steps, took 887 us
+// a block a workgroup.
+template <int HD, bool ONE>
+__global__ __launch_bounds__(512, 1) void attend_shares_kernel(ChunkCall) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
+  ShareAt& s = *(ShareAt*)(s_buf + 2 * ChunkSizes<HD, 8>::kHalfs);  // behind the two buffers
+  for (bool start = true;; start = false) {
+    const ChunkCall call = call_args();
+    const AttendArgs& a = call.a;
+    // (anew each time: what follows from it would live through the steps from outside the loop, 38 registers)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    // neighbours in the row on one XCD (workgroups go to the 8 in turn): they share keys and values
+    const int n = call.parts.shares, id = blockIdx.x, w = n % 8 == 0 ? (id & 7) * (n / 8) + (id >> 3) : id;
+    bool found = start;
+    if (start) {
+      if (tid == 0) call.parts.split[w] = make_int4(0, 0, 0, -1);
+      find_sequence<true>(call, tid, w, s);
+    } else {
+      __syncthreads();
+    }
+    const int64_t u = uniform(s.u), u1 = uniform(s.end), each = uniform(s.each);
+    if (u >= u1) return;
+    if (!start && __builtin_amdgcn_readfirstlane(s.b) < 0) {
+      find_sequence<false>(call, tid, w, s);
+      found = true;
+    }
+    const int b = __builtin_amdgcn_readfirstlane(s.b);
+    int64_t q0;
+    int nq, kv, pos0;
+    sequence(a, b, q0, nq, kv, pos0);
+    q0 = uniform(q0);  // (read through vector registers: what a block's steps take from these is scalar)
+    nq = __builtin_amdgcn_readfirstlane(nq);
+    kv = __builtin_amdgcn_readfirstlane(kv);
+    pos0 = __builtin_amdgcn_readfirstlane(pos0);
+    const BlockWork bw = block_work(a, nq, kv, pos0, call.lo_rows);
+    int kvh, block;
+    int64_t from = u;
+    if (found) {
+      const int64_t per_head = bw.before(bw.blocks), in = u - uniform(s.base);
+      kvh = (int)(in / per_head);
+      const int64_t at = in - kvh * per_head;
+      block = 0;
+      for (int d = 1 << (31 - __builtin_clz(bw.blocks)); d; d >>= 1)
+        if (block + d < bw.blocks && bw.before(block + d) <= at) block += d;
+      from = u - at + bw.before(block);
+    } else {
+      kvh = s.kvh;
+      block = s.block;
+    }
+    kvh = __builtin_amdgcn_readfirstlane(kvh);
+    block = __builtin_amdgcn_readfirstlane(block);
+    const int64_t work = bw.first + (int64_t)bw.more * block, to = from + work;
+    const int rows = nq * a.group, r0 = block * kShareRows;
+    int lo, seen, t0, t1;
+    block_sees(a, rows, pos0, r0, kShareRows, lo, seen);
+    part_steps(lo, seen, 0, 1, t0, t1);
+    const int steps = t1 - t0;
+    const int begin = __builtin_amdgcn_readfirstlane(start ? step_at(u - from, work, steps) : 0);
+    const int end = __builtin_amdgcn_readfirstlane(to <= u1 ? steps : step_at(u1 - from, work, steps));
+    __syncthreads();
+    if (tid == 0) {
+      const bool head_left = block + 1 < bw.blocks, left = head_left || kvh + 1 < a.c.heads;
+      s.u = to;
+      s.block = head_left ? block + 1 : 0;
+      s.kvh = head_left ? kvh : kvh + 1;
+      if (!left) s.b = -1;
+      if (begin == 0 && end > 0 && end < steps) {
+        int64_t last = (to - 1) / each;  // the share that takes the block's last steps
+        while (step_at(last * each - from, work, steps) == steps) last--;
+        call.parts.split[w] = make_int4(b, kvh, block, (int)last);
+      }
+    }
+    // (a boundary moved to the block's first or last step leaves a share nothing of it)
+    if (steps > 0 && (begin == steps || (begin == 0 && end == 0))) continue;
+    const int64_t part_at = begin == 0 && end == steps ? -1 : share_row(begin > 0 ? 2 * w : 2 * w + 1, 0);
+    attend_block<HD, 8, ONE>(tid, b, kvh, q0, rows, kv, pos0, r0, lo, t0 + begin, t0 + end, part_at, s_buf);
+  }
+}
+
+template <int HD, int W, size_t kMore, auto Kernel>
+hipError_t launch_pages(const dim3& grid, const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
+  constexpr size_t kLds = ChunkSizes<HD, W>::kLds + kMore;
+  static_assert(ChunkSizes<HD, W>::kLds % alignof(ShareAt) == 0, "where the search's place lies");
+  if constexpr (kLds > 64 * 1024) {
+    const hipError_t e = set_max_dynamic_lds<Kernel>();
     if (e != hipSuccess) return e;
   }
-  const dim3 grid((unsigned)(a.seqs * a.c.heads), 1, (unsigned)(p.blocks + p.cut * (p.parts - 1)));
-  attend_chunk_kernel<HD, W, ONE><<<grid, 64 * W, ChunkSizes<HD, W>::kLds, st>>>(a, lo, p);
+  Kernel<<<grid, 64 * W, kLds, st>>>(ChunkCall{a, p, lo});
   return hipGetLastError();
 }
 
 template <int HD>
 hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
-  if constexpr (HD <= 128)
+  const bool one = a.c.page >= kTile;
+  const dim3 grid((unsigned)(a.seqs * a.c.heads), 1, (unsigned)(p.blocks + p.cut * (p.parts - 1)));
+  if constexpr (HD <= 128) {
+    const dim3 shares((unsigned)p.shares);
+    if (p.shares)
+      return one ? launch_pages<HD, 8, sizeof(ShareAt), attend_shares_kernel<HD, true>>(shares, a, lo, p, st)
+                 : launch_pages<HD, 8, sizeof(ShareAt), attend_shares_kernel<HD, false>>(shares, a, lo, p, st);
     if (p.rows > 128)
-      return a.c.page >= kTile ? launch_pages<HD, 8, true>(a, lo, p, st) : launch_pages<HD, 8, false>(a, lo, p, st);
-  return a.c.page >= kTile ? launch_pages<HD, 4, true>(a, lo, p, st) : launch_pages<HD, 4, false>(a, lo, p, st);
+      return one ? launch_pages<HD, 8, 0, attend_chunk_kernel<HD, 8, true>>(grid, a, lo, p, st)
+                 : launch_pages<HD, 8, 0, attend_chunk_kernel<HD, 8, false>>(grid, a, lo, p, st);
+  }
+  return one ? launch_pages<HD, 4, 0, attend_chunk_kernel<HD, 4, true>>(grid, a, lo, p, st)
+             : launch_pages<HD, 4, 0, attend_chunk_kernel<HD, 4, false>>(grid, a, lo, p, st);
 }
 
 }  // namespace

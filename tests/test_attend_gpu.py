@@ -258,3 +258,39 @@ def test_rows_past_max_q_are_left_and_move_no_other(new, most):
     inside = (inside < most) | (inside == new)
     check(out[inside], want[inside], tol[inside])
     assert (out[~inside] == 7).all()
+
+
+@pytest.mark.parametrize("hd,page,dtype", [(64, 16, F16), (64, 64, BF16), (96, 32, BF16), (128, 64, F16), (128, 16, BF16)])
+@pytest.mark.parametrize("window,sinks", [(0, False), (0, True), (2100, False)])
+def test_blocks_in_equal_shares(hd, page, dtype, window, sinks):
+    """480 blocks of 256 rows by the longest sequence, 200 and some in fact: chunks, a prompt without a past, one
+    whose first rows stand before the cache, a few-token and an absent sequence, whole tables' pages apart."""
+    run([1100, 1, 700, 0, 300, 430], [2300, 2100, 700, 40, 2600, 200], 20, 20, hd, page, dtype, window=window,
+        sinks=sinks, seed=hd + page)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(12, 4), (40, 8), (24, 2)])
+def test_shares_of_shared_heads(heads, kv_heads):
+    """Groups of 3, 5 and 12: blocks that end inside a token's heads."""
+    new = [2100, 900, 1500] if kv_heads == 2 else [1500, 2000, 40, 1000] * (2 if kv_heads == 4 else 1)
+    kvl = [n + 100 * i for i, n in enumerate(new)]
+    kvl[0] += 1500
+    run(new, kvl, heads, kv_heads, 64, 64, F16, seed=heads)
+
+
+def test_more_sequences_than_threads_beside_a_prompt():
+    """A search of several rounds: prompts among 700 sequences of one token, and of none."""
+    new, kvl = [1] * 700, [1 + i % 70 for i in range(700)]
+    for i, (n, k) in {3: (500, 2200), 511: (300, 300), 512: (290, 2000), 600: (0, 9), 699: (512, 2100)}.items():
+        new[i], kvl[i] = n, k
+    per = 2200 // 256 + 1
+    kv, g = filled(per * 5 + 700, 1, 64, 256, 3)
+    tables = torch.full((700, per), -1, dtype=torch.int32, device="cuda")
+    tables[:, 0] = torch.arange(700, dtype=torch.int32, device="cuda")
+    for x, i in enumerate((3, 511, 512, 600, 699)):
+        tables[i] = torch.arange(700 + x * per, 700 + (x + 1) * per, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([sum(new[:b]) for b in range(701)], dtype=torch.int32, device="cuda")
+    lens = torch.tensor(kvl, dtype=torch.int32, device="cuda")
+    q = (1.5 * torch.randn(sum(new), 1, 64, generator=g, device="cuda")).half()
+    got = kv.attend(q, starts, lens, tables, max_q=512)
+    check(got, *attend64(kv, q, starts, lens, tables, 0.125))
