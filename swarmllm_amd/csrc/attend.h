@@ -19,6 +19,12 @@ constexpr int kTile = 64;  // positions a step of either kernel takes
 // Weights may reach 2^kSlack (f16 holds 2^15) before the running maximum that
 // they are relative to is moved and what is summed so far rescaled.
 constexpr float kSlack = 8.0f;
+// Weights are 2^(s sc - m sc), m the maximum they are relative to. Up to this
+// size m sc is rounded by 2^-17 at most and one fused multiply-add a weight
+// does it; where some row's is larger the scores are taken as s - m first, for
+// the rounding grows with m sc (from 2^28 on by 16 and more: weights past f16,
+// or all of them zero) and ends in an infinity.
+constexpr float kFar = 256.0f;
 
 // The bounds of sequence b, whatever the device arrays hold: its first row
 // q0, its rows nq (at most max_q, inside the q rows), its cached positions kv
@@ -167,8 +173,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // Partial results: rows of a block (kv head of a sequence, `rows` query rows)
 // for each part of its context: sums of weights times values [part][row][hd],
-// then (largest score, sum of weights) [part][row][2]. A part that a row sees
-// nothing of has the largest score -inf and no valid sums.
+// then (the score that they are relative to, as the product gives it, and the
+// sum of weights) [part][row][2]; that score is -inf in a part that a row sees
+// nothing of.
 struct AttendParts {
   float* o;
   float* ml;
@@ -181,15 +188,23 @@ __device__ __forceinline__ int64_t part_row(const AttendParts& p, int64_t head_o
   return ((head_of_seq * p.cut + block) * p.parts + part) * p.rows + row;
 }
 
-// A row's outputs from its sums of weights times values (relative to the
-// largest score `top`) and of weights, the head's sink joined.
+// What sums relative to score m count for beside ones relative to `base`
+// (finite). The scores meet before the scale, whose product with either may
+// pass f32's range.
+__device__ __forceinline__ float weight_of(const AttendArgs& a, float m, float base) {
+  return exp2_fast((m - base) * a.sc);
+}
+
+// A row's outputs from its sums of weights times values (relative to score
+// `top`) and of weights, the head's sink joined.
 template <int N>
 __device__ __forceinline__ void finish_row(const AttendArgs& a, int head, float top, float sum, const float* acc,
                                            float* out) {
   float f = 1.0f;
   if (a.sinks && sum != 0.0f) {
-    const float sink = a.sinks[head] * kLog2e, mx = fmaxf(top, sink);
-    f = exp2_fast(top - mx);
+    const float at = fminf(fmaxf(top * a.sc, -3e38f), 3e38f);  // finite
+    const float sink = a.sinks[head] * kLog2e, mx = fmaxf(at, sink);
+    f = exp2_fast(at - mx);
     sum = sum * f + exp2_fast(sink - mx);
   }
   const float inv = sum == 0.0f ? 0.0f : f / sum;

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
       const float m = p.ml[2 * i], l = p.ml[2 * i + 1];
       const f4v o = *(const f4v*)(p.o + i * hd + e);
       const float mx = fmaxf(top, m), base = mx == -INFINITY ? 0.0f : mx;
-      const float fa = exp2_fast(top - base), fb = exp2_fast(m - base);
+      const float fa = weight_of(a, top, base), fb = weight_of(a, m, base);
       top = mx;
       sum = sum * fa + l * fb;
       acc = acc * fa + o * fb;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
     acc = f4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < G; w++) {
-      const float f = exp2_fast(s_m[w][lane] - base);
+      const float f = weight_of(a, s_m[w][lane], base);
       sum += s_l[w][lane] * f;
       acc += s_o[w][lane] * f;
     }
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void attend_join_shares_kernel(AttendArgs a, A
     const float m = p.ml[2 * i], l = p.ml[2 * i + 1];
     const f4v o = *(const f4v*)(p.o + i * hd + e);
     const float mx = fmaxf(top, m), base = mx == -INFINITY ? 0.0f : mx;
-    const float fa = exp2_fast(top - base), fb = exp2_fast(m - base);
+    const float fa = weight_of(a, top, base), fb = weight_of(a, m, base);
     top = mx;
     sum = sum * fa + l * fb;
     acc = acc * fa + o * fb;

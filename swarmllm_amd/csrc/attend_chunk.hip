@@ -245,6 +245,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
 #pragma unroll
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
+  bool far = false;  // some row's maximum is past kFar (the same for the wave)
   const ChunkCall in_steps = call_args();
   const AttendArgs& a = in_steps.a;
 
@@ -313,13 +314,22 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
       // one has outgrown it by 2^kSlack (exact in f16 and f32 alike)
       if (__ballot((mt - m) * a.sc > kSlack) != 0) {
         mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
-        const float mn = fmaxf(m, mt), f = exp2_fast((m - (mn == -INFINITY ? 0.0f : mn)) * a.sc);
+        const float mn = fmaxf(m, mt), to = mn == -INFINITY ? 0.0f : mn, f = weight_of(a, m, to);
+        far = __ballot(fabsf(to) * a.sc > kFar) != 0;
         m = mn;
         l *= f;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) o[d] *= f;
       }
-      const float bs = m == -INFINITY ? 0.0f : m * a.sc;
+      const float to = m == -INFINITY ? 0.0f : m;
+      float bs = to * a.sc;
+      if (__builtin_expect(far, 0)) {
+        bs = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[t][i] -= to;
+      }
       h8v p[4];
       float sum = 0.0f;
 #pragma unroll
@@ -365,7 +375,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
       for (int i = 0; i < 16; i += 4)
         *(f4v*)(parts.o + pr * HD + 32 * d + 2 * i + 4 * hi) = f4v{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
     if (hi == 0) {
-      parts.ml[2 * pr] = m * after.a.sc;
+      parts.ml[2 * pr] = m;
       parts.ml[2 * pr + 1] = l;
     }
     return;
@@ -376,7 +386,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
     for (int i = 0; i < 16; i += 4) {
       const float acc[4] = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
       float out[4];
-      finish_row<4>(after.a, head, m * after.a.sc, l, acc, out);
+      finish_row<4>(after.a, head, m, l, acc, out);
       store_out4(after.a, row_q * after.a.os + (int64_t)head * HD + 32 * d + 2 * i + 4 * hi, out);
     }
 }

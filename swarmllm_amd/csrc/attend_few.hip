@@ -75,8 +75,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
 
   f4v o[NT][Z::kDims];
   float m[NT], l[NT];
+  bool far[NT];  // some row's maximum is past kFar (the same for the wave)
 #pragma unroll
   for (int n = 0; n < NT; n++) {
+    far[n] = false;
     m[n] = -INFINITY;
     l[n] = 0.0f;
 #pragma unroll
@@ -185,13 +187,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
       if (__ballot((mt - m[n]) * a.sc > kSlack) != 0) {
         mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
         mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
-        const float mn = fmaxf(m[n], mt), f = exp2_fast((m[n] - (mn == -INFINITY ? 0.0f : mn)) * a.sc);
+        const float mn = fmaxf(m[n], mt), to = mn == -INFINITY ? 0.0f : mn, f = weight_of(a, m[n], to);
+        far[n] = __ballot(fabsf(to) * a.sc > kFar) != 0;
         m[n] = mn;
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < Z::kDims; d++) o[n][d] *= f;
       }
-      const float bs = m[n] == -INFINITY ? 0.0f : m[n] * a.sc;
+      const float to = m[n] == -INFINITY ? 0.0f : m[n];
+      float bs = to * a.sc;
+      if (__builtin_expect(far[n], 0)) {
+        bs = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[n][t][i] -= to;
+      }
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 4; t++)
@@ -238,7 +249,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
     l[n] += __shfl_xor(l[n], 16, kWave);
     l[n] += __shfl_xor(l[n], 32, kWave);
     if (g == 0) {
-      s_m[wave][16 * n + col] = m[n] * a.sc;
+      s_m[wave][16 * n + col] = m[n];
       s_l[wave][16 * n + col] = l[n];
     }
   }
@@ -264,7 +275,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
         f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < W; w++) {
-          const float f = exp2_fast(mw[w] - base);
+          const float f = weight_of(a, mw[w], base);
           sum += s_l[w][r] * f;
           acc += *(const f4v*)&s_o[w][r16][e] * f;
         }
