@@ -205,7 +205,7 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int head, float 
     const float at = fminf(fmaxf(top * a.sc, -3e38f), 3e38f);  // finite
     const float sink = a.sinks[head] * kLog2e, mx = fmaxf(at, sink);
     f = exp2_fast(at - mx);
-    sum = sum * f + exp2_fast(sink - mx);
+    sum = sum * f + (sink == mx ? 1.0f : exp2_fast(sink - mx));  // (an infinite sink less itself is NaN)
   }
   const float inv = sum == 0.0f ? 0.0f : f / sum;
 #pragma unroll

@@ -81,3 +81,15 @@ def test_queries_and_keys_in_the_thousands(new, n):
     q.fill_(4000.0)
     q[:, 1::2] = -4000.0
     check_exact_scores(kv, q, starts, lens, tables, 0.0883883461356163, max_q=new)
+
+
+@pytest.mark.parametrize("new,n", [(1, 90), (1, 9000), (40, 600), (40, 5000)])
+def test_sinks_past_the_largest_number(new, n):
+    """A sink that is infinite, or is so in the exponent's base, takes all of a row's weight; one below every number none."""
+    kv, q, starts, lens, tables, _ = batch([new], [n], 4, 2, 64, 64, F32, seed=n)
+    none = kv.attend(q, starts, lens, tables, max_q=new)
+    inf = float("inf")
+    got = kv.attend(q, starts, lens, tables, max_q=new, sinks=torch.tensor([inf, 3e38, -inf, -3e38], device="cuda"))
+    assert (got[:, :2] == 0).all() and torch.equal(got[:, 2:], none[:, 2:])
+    far = kv.attend(q, starts, lens, tables, max_q=new, scale=2.0**99, sinks=torch.full((4,), inf, device="cuda"))
+    assert (far == 0).all()
