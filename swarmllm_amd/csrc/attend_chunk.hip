@@ -244,7 +244,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
   for (int d = 0; d < HD / 32; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, bs = 0.0f;  // bs: m sc, what the weights' exponents are less (0: none yet, or far)
   bool far = false;  // some row's maximum is past kFar (the same for the wave)
   const ChunkCall in_steps = call_args();
   const AttendArgs& a = in_steps.a;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
         for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[t][i]);
       // the weights are relative to a maximum that follows the scores only once
       // one has outgrown it by 2^kSlack (exact in f16 and f32 alike)
-      if (__ballot((mt - m) * a.sc > kSlack) != 0) {
+      if (__ballot((mt - m) * a.sc > kSlack) != 0 || far) {
         mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
         const float mn = fmaxf(m, mt), to = mn == -INFINITY ? 0.0f : mn, f = weight_of(a, m, to);
         far = __ballot(fabsf(to) * a.sc > kFar) != 0;
@@ -320,15 +320,12 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
         l *= f;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) o[d] *= f;
-      }
-      const float to = m == -INFINITY ? 0.0f : m;
-      float bs = to * a.sc;
-      if (__builtin_expect(far, 0)) {
-        bs = 0.0f;
+        bs = far ? 0.0f : to * a.sc;
+        if (far)
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+          for (int t = 0; t < 2; t++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[t][i] -= to;
+            for (int i = 0; i < 16; i++) s[t][i] -= to;
       }
       h8v p[4];
       float sum = 0.0f;

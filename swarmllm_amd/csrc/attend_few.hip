@@ -74,13 +74,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
   }
 
   f4v o[NT][Z::kDims];
-  float m[NT], l[NT];
+  float m[NT], l[NT], bs[NT];  // bs: m sc, what the weights' exponents are less (0: none yet, or far)
   bool far[NT];  // some row's maximum is past kFar (the same for the wave)
 #pragma unroll
   for (int n = 0; n < NT; n++) {
     far[n] = false;
     m[n] = -INFINITY;
-    l[n] = 0.0f;
+    l[n] = bs[n] = 0.0f;
 #pragma unroll
     for (int d = 0; d < Z::kDims; d++) o[n][d] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) mt = fmaxf(mt, s[n][t][i]);
-      if (__ballot((mt - m[n]) * a.sc > kSlack) != 0) {
+      if (__ballot((mt - m[n]) * a.sc > kSlack) != 0 || far[n]) {
         mt = fmaxf(mt, __shfl_xor(mt, 16, kWave));
         mt = fmaxf(mt, __shfl_xor(mt, 32, kWave));
         const float mn = fmaxf(m[n], mt), to = mn == -INFINITY ? 0.0f : mn, f = weight_of(a, m[n], to);
@@ -193,22 +193,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < Z::kDims; d++) o[n][d] *= f;
-      }
-      const float to = m[n] == -INFINITY ? 0.0f : m[n];
-      float bs = to * a.sc;
-      if (__builtin_expect(far[n], 0)) {
-        bs = 0.0f;
+        bs[n] = far[n] ? 0.0f : to * a.sc;
+        if (far[n])
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+          for (int t = 0; t < 4; t++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) s[n][t][i] -= to;
+            for (int i = 0; i < 4; i++) s[n][t][i] -= to;
       }
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float w = exp2_fast(__builtin_fmaf(s[n][t][i], a.sc, -bs));
+          const float w = exp2_fast(__builtin_fmaf(s[n][t][i], a.sc, -bs[n]));
           sum += w;
           p[n][t >> 1][4 * (t & 1) + i] = (_Float16)w;
         }
