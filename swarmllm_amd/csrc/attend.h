@@ -172,7 +172,7 @@ __device__ __forceinline__ uint4 cut_scales(uint4 s, int j0, int lo, int hi) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Partial results: rows of a block (kv head of a sequence, `rows` query rows)
-// for each part of its context: sums of weights times values [part][row][hd],
+// for each part of its context: sums of weights times values [cut_index][part][row][hd],
 // then (the score that they are relative to, as the product gives it, and the
 // sum of weights) [part][row][2]; that score is -inf in a part that a row sees
 // nothing of.
@@ -180,12 +180,19 @@ struct AttendParts {
   float* o;
   float* ml;
   int parts, rows;  // query rows of a block
-  int blocks, cut;  // row blocks of a kv head of a sequence; the first `cut` of them are in parts
+  int blocks, cut;  // row blocks of a kv head of a sequence; blocks that are in parts
+  int cut_rows, cut_more;  // those: every head's first cut_rows, and the next of the last cut_more heads
   int4* split;      // shares (attend_chunk.hip): the block that each leaves unfinished
   int shares;       // 0: none
 };
-__device__ __forceinline__ int64_t part_row(const AttendParts& p, int64_t head_of_seq, int block, int part, int row) {
-  return ((head_of_seq * p.cut + block) * p.parts + part) * p.rows + row;
+// The place of a block among those in parts (every head's first cut_rows, then
+// the last heads' next); -1: it is whole.
+__device__ __forceinline__ int cut_index(const AttendArgs& a, const AttendParts& p, int head_of_seq, int block) {
+  const int heads = a.seqs * a.c.heads, x = head_of_seq - (heads - p.cut_more);
+  return block < p.cut_rows ? head_of_seq * p.cut_rows + block : block == p.cut_rows && x >= 0 ? heads * p.cut_rows + x : -1;
+}
+__device__ __forceinline__ int64_t part_row(const AttendParts& p, int cut_index, int part, int row) {
+  return ((int64_t)cut_index * p.parts + part) * p.rows + row;
 }
 
 // What sums relative to score m count for beside ones relative to `base`

@@ -27,7 +27,6 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   const int hd = a.c.hd, per = hd / 4, fit = 64 / per;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane / per, e = 4 * (lane - sub * per), first = G > 1 ? wave : 0;
-  // rows of one kv head of a sequence lie block after block
   const int64_t row_of_head = ((int64_t)blockIdx.x * (4 / G) + (G > 1 ? 0 : wave)) * fit + sub;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int block = (int)(row_of_head / p.rows), row = (int)(row_of_head - (int64_t)block * p.rows);
@@ -35,12 +34,12 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   int nq, kv, pos0;
   sequence(a, b, q0, nq, kv, pos0);
   const int rows = nq * a.group;
-  const int64_t hs = (int64_t)b * a.c.heads + kvh;
-  const bool on = sub < fit && block < p.cut && rows > lo_rows && rows <= hi_rows && row_of_head < rows;
+  const int cut = cut_index(a, p, b * a.c.heads + kvh, block);
+  const bool on = sub < fit && cut >= 0 && rows > lo_rows && rows <= hi_rows && row_of_head < rows;
   float top = -INFINITY, sum = 0.0f;
   f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
   if (on) {
-    const int64_t i0 = part_row(p, hs, block, first, row), step = G * (int64_t)p.rows;
+    const int64_t i0 = part_row(p, cut, first, row), step = G * (int64_t)p.rows;
     const int n = (p.parts - first + G - 1) / G;
 #pragma unroll 4
     for (int s = 0; s < n; s++) {
@@ -155,11 +154,13 @@ Plan plan_of(const AttendArgs& a, int cus) {
       p.shares = cus;
     } else {
       // parts that fill the CUs, of 8 steps at least: of every block where those
-      // are few, otherwise of what is left behind the last whole round of the CUs
+      // are few, otherwise of what is left behind the last whole round of the CUs,
+      // those blocks alone, so that the parts are never more than a round holds
+      // (65 sequences of 5 tokens over 8192, 64 heads on 8 of 128, leave 8 blocks:
+      // 301 us, 381 with that block of all 520 heads cut, over 554 MB of partial results)
       const int64_t left = n <= slots ? n : n % slots;
       p.chunk_parts = left ? clamp_parts(slots / left, most_steps(a, p.chunk_rows) / 8) : 1;
-      p.chunk_cut = p.chunk_parts > 1 ? (int)((left + heads - 1) / heads) : 0;
-      if (p.chunk_cut == 0) p.chunk_parts = 1;
+      p.chunk_cut = p.chunk_parts > 1 ? (int)left : 0;
     }
     if (a.seqs > 1) p.few = 16;  // one-token sequences beside a prompt
   } else {
@@ -180,11 +181,12 @@ Plan plan_of(const AttendArgs& a, int cus) {
   return p;
 }
 
-// The partial results at ws: bytes, and where they lie.
+// The partial results at ws of the last `cut` blocks: bytes, and where they lie.
 size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, void* ws, AttendParts& p) {
-  p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut, nullptr, 0};
+  const int heads = a.seqs * a.c.heads;
+  p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut, cut / heads, cut % heads, nullptr, 0};
   if (parts <= 1) return 0;
-  const size_t n = (size_t)a.seqs * a.c.heads * cut * parts * rows;
+  const size_t n = (size_t)cut * parts * rows;
   p.o = (float*)ws;
   p.ml = p.o + n * a.c.hd;
   return n * (a.c.hd + 2) * sizeof(float);
@@ -192,7 +194,7 @@ size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, v
 
 // And those of `shares`.
 size_t shares_at(const AttendArgs& a, int shares, void* ws, AttendParts& p) {
-  p = AttendParts{(float*)ws, nullptr, 1, kShareRows, 0, 0, nullptr, shares};
+  p = AttendParts{(float*)ws, nullptr, 1, kShareRows, 0, 0, 0, 0, nullptr, shares};
   const size_t n = (size_t)2 * shares * kShareRows;
   p.ml = p.o + n * a.c.hd;
   p.split = (int4*)(p.ml + 2 * n);
@@ -204,7 +206,8 @@ hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipSt
   // blocks 11.9 / 7.8, 31 of one token's 32 heads 4.2 / 5.1, 64 of them 5.2 / 10.9)
   const bool deal = p.parts > 8;
   const int fit = 64 / (a.c.hd / 4) * (deal ? 1 : 4);
-  const int64_t most = (int64_t)a.max_q * a.group, held = (int64_t)p.cut * p.rows, rows = most < held ? most : held;
+  const int64_t heads = (int64_t)a.seqs * a.c.heads, most = (int64_t)a.max_q * a.group;
+  const int64_t held = (p.cut + heads - 1) / heads * p.rows, rows = most < held ? most : held;
   const dim3 grid((unsigned)((rows + fit - 1) / fit), (unsigned)a.c.heads, (unsigned)a.seqs);
   if (deal)
     attend_join_kernel<4><<<grid, 256, 0, st>>>(a, lo, hi, p);
@@ -224,7 +227,7 @@ bool attend_fits(const AttendArgs& a) {
 size_t attend_workspace_bytes(const AttendArgs& a, int cus) {
   const Plan p = plan_of(a, cus);
   AttendParts q;
-  const size_t few = p.few ? parts_at(a, p.few_parts, p.few, 1, 1, nullptr, q) : 0;
+  const size_t few = p.few ? parts_at(a, p.few_parts, p.few, 1, a.seqs * a.c.heads, nullptr, q) : 0;
   const size_t chunk = p.shares ? shares_at(a, p.shares, nullptr, q) : p.chunk_blocks ? parts_at(a, p.chunk_parts, p.chunk_rows, p.chunk_blocks, p.chunk_cut, nullptr, q) : 0;
   return few > chunk ? few : chunk;  // one after the other
 }
@@ -247,7 +250,7 @@ hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st)
     if (e == hipSuccess && q.parts > 1) e = join(a, p.few, INT32_MAX, q, st);
   }
   if (p.few && e == hipSuccess) {
-    parts_at(a, p.few_parts, p.few, 1, 1, ws, q);
+    parts_at(a, p.few_parts, p.few, 1, a.seqs * a.c.heads, ws, q);
     e = launch_attend_few(a, 0, p.few, q, st);
     if (e == hipSuccess && q.parts > 1) e = join(a, 0, p.few, q, st);
   }

@@ -404,14 +404,28 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
   const AttendArgs& a = call.a;
   const AttendParts& parts = call.parts;
   extern __shared__ __attribute__((aligned(16))) uint16_t s_buf[];
-  const int b = (int)((uint32_t)blockIdx.x / (uint32_t)a.c.heads), kvh = blockIdx.x - b * a.c.heads;
-  // the rows that see most first; behind the whole blocks the parts of those cut
-  const int z = blockIdx.z, cut_z = z - (parts.blocks - parts.cut);
-  const bool whole = cut_z < 0;
-  const int nparts = whole ? 1 : parts.parts;
-  const int down = whole ? 0 : (int)((uint32_t)cut_z / (uint32_t)nparts);
-  const int block = whole ? parts.blocks - 1 - z : parts.cut - 1 - down;
-  const int part = whole ? 0 : cut_z - down * nparts;
+  // the rows that see most first, every head's block in a row of the grid; then
+  // the parts of the rows of blocks that are cut, and last what a row cut for its
+  // last heads only has more than the first parts, which stand in that row
+  const int heads = gridDim.x, z = blockIdx.z, top = parts.blocks - parts.cut_rows;
+  int hs = blockIdx.x, block = parts.blocks - 1 - z, part = 0, nparts = 1;
+  if (z < top) {
+    if (z == top - 1 && hs >= heads - parts.cut_more) nparts = parts.parts;
+  } else {
+    nparts = parts.parts;
+    const int row = z - top, down = (int)((uint32_t)row / (uint32_t)nparts);
+    part = row - down * nparts;
+    block = parts.cut_rows - 1 - down;
+    if (block < 0) {
+      const uint32_t at = (uint32_t)(row - parts.cut_rows * nparts) * heads + hs, more = parts.cut_more;
+      if (at >= more * (nparts - 1)) return;  // the grid's last row
+      const uint32_t n = at / more;
+      part = 1 + (int)n;
+      block = parts.cut_rows;
+      hs = heads - (int)(more - (at - n * more));
+    }
+  }
+  const int b = (int)((uint32_t)hs / (uint32_t)a.c.heads), kvh = hs - b * a.c.heads;
   int64_t q0;
   int nq, kv, pos0;
   sequence(a, b, q0, nq, kv, pos0);
@@ -421,7 +435,7 @@ __global__ __launch_bounds__(64 * W, HD > 128 || W > 4 ? 1 : 2) void attend_chun
   block_sees(a, rows, pos0, r0, kRows, lo, seen);
   part_steps(lo, seen, part, nparts, begin, end);
   attend_block<HD, W, ONE>(threadIdx.x, b, kvh, q0, rows, kv, pos0, r0, lo, begin, end,
-                           nparts > 1 ? part_row(parts, (int64_t)blockIdx.x, block, part, 0) : -1, s_buf);
+                           nparts > 1 ? part_row(parts, cut_index(a, parts, hs, block), part, 0) : -1, s_buf);
 }
 
 // The blocks of 256 rows of a sequence's kv head as lengths of work: block j's
@@ -628,7 +642,8 @@ hipError_t launch_pages(const dim3& grid, const AttendArgs& a, int lo, const Att
 template <int HD>
 hipError_t launch_hd(const AttendArgs& a, int lo, const AttendParts& p, hipStream_t st) {
   const bool one = a.c.page >= kTile;
-  const dim3 grid((unsigned)(a.seqs * a.c.heads), 1, (unsigned)(p.blocks + p.cut * (p.parts - 1)));
+  const int64_t heads = (int64_t)a.seqs * a.c.heads, more = (int64_t)p.cut_more * (p.parts - 1);
+  const dim3 grid((unsigned)heads, 1, (unsigned)(p.blocks + p.cut_rows * (p.parts - 1) + (more + heads - 1) / heads));
   if constexpr (HD <= 128) {
     const dim3 shares((unsigned)p.shares);
     if (p.shares)

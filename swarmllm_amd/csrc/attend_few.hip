@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
           acc += *(const f4v*)&s_o[w][r16][e] * f;
         }
         if (parts.parts > 1) {
-          const int64_t pr = part_row(parts, (int64_t)b * c.heads + kvh, 0, part, r);
+          const int64_t pr = part_row(parts, b * c.heads + kvh, part, r);
           *(f4v*)(parts.o + pr * HD + h + e) = acc;
           if (h + e == 0) {
             parts.ml[2 * pr] = top;

@@ -164,3 +164,16 @@ def test_attend_takes_the_injected_fault():
     assert attend(max_kv=512)[0] == QMM_OK  # a plan does not
     assert attend(max_kv=512, launch=1, q=None)[0] == _lib.QMM_NO_ROOM
     assert attend(max_kv=512, launch=1, q=None)[0] == QMM_UNSUPPORTED  # once
+
+
+@pytest.mark.parametrize("heads,hd", [(64, 128), (8, 256), (40, 64)])
+@pytest.mark.parametrize("max_kv", [2000, 8192, 32768])
+def test_partial_results_stay_within_a_round_of_the_cus(heads, hd, max_kv):
+    """However many blocks stand behind the last whole round, their parts are no more than a round holds: 512
+    workgroups of 128 query rows, or twice 256 of 256 in equal shares, a row's sums and its two numbers each."""
+    most = 2 * 256 * 256 * (hd + 2) * 4 + 256 * 16
+    for new in (5, 33, 40, 130, 700):
+        for seqs in (1, 2, 31, 32, 33, 51, 63, 64, 65, 66, 127, 128, 129, 192, 200, 256, 257, 1025, 8193):
+            st, got = attend(cache(pages=10**6, hd=hd), seqs=seqs, tokens=seqs * new, max_q=new, heads=heads,
+                             max_kv=max_kv, table_stride=512, q_stride=heads * hd, q_head=hd, out_stride=heads * hd)
+            assert st == QMM_OK and got <= most, (seqs, new, got)
