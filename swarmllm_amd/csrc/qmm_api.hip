@@ -1086,7 +1086,6 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   a.c = planes_of(*cache);
   a.q = q; a.out = out; a.q_starts = q_starts; a.kv_lens = kv_lens; a.tables = tables; a.sinks = sinks;
   a.qs = q_stride; a.qhs = q_head_stride; a.os = out_stride; a.table_stride = table_stride; a.tokens = tokens;
-  a.window = window;
   a.seqs = (int)seqs; a.heads = heads; a.group = heads / cache->kv_heads;
   a.max_q = (int)(max_q < tokens ? max_q : tokens);
   // a sequence's positions lie inside its row of the table
@@ -1094,6 +1093,7 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   if (table_stride > kMostPositions / cache->page) return QMM_UNSUPPORTED;
   const int64_t cap = table_stride * cache->page;
   a.max_kv = (int)(max_kv < cap ? max_kv : cap);
+  a.window = window < a.max_kv ? window : 0;  // a longer one hides nothing (and must not pass 64 bits in the plan)
   a.qdt = q_dtype; a.odt = out_dtype;
   a.sc = scale == 0.0f ? 1.0f : (scale < 0.0f ? -scale : scale) * 1.4426950408889634f;
   a.q_sign = scale == 0.0f ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;

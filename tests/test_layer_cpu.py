@@ -177,3 +177,14 @@ def test_partial_results_stay_within_a_round_of_the_cus(heads, hd, max_kv):
             st, got = attend(cache(pages=10**6, hd=hd), seqs=seqs, tokens=seqs * new, max_q=new, heads=heads,
                              max_kv=max_kv, table_stride=512, q_stride=heads * hd, q_head=hd, out_stride=heads * hd)
             assert st == QMM_OK and got <= most, (seqs, new, got)
+
+
+@pytest.mark.parametrize("shape", [dict(seqs=1, tokens=1, max_q=1), dict(seqs=1, tokens=512, max_q=512),
+                                   dict(seqs=2, tokens=4000, max_q=2000), dict(seqs=16, tokens=16, max_q=1)])
+def test_a_window_past_the_context_plans_as_none(shape):
+    """The largest number is a caller's way to say "no window"."""
+    for max_kv in (700, 3200):
+        none = attend(max_kv=max_kv, **shape)
+        assert none[0] == QMM_OK
+        for window in (max_kv, 2**31, 2**62, 2**63 - 1):
+            assert attend(max_kv=max_kv, window=window, **shape) == none
