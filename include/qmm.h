@@ -264,9 +264,10 @@ int qmm_forward_shared(int type, int count, const void *const *w, const int64_t 
  * activation already quantized in qmm_act_layout(type, rows)
  * (qmm_rms_norm_act, qmm_quantize_act), 16-byte aligned: the same kernels and,
  * with the workspace that each plans, the same bits, without the quantizer's
- * launch. The workspace holds the slots of a K split (and the GLU's two products); *need
- * can be 0, and without room for the slots a product runs uncut, as
- * qmm_matmul. xq is read only. Not affected by qmm_set_force_dmmv. */
+ * launch. The workspace, 16-byte aligned too, holds the slots of a K split (and
+ * the GLU's two products); *need can be 0, and without room for the slots a
+ * product runs uncut, as qmm_matmul. xq is read only. Not affected by
+ * qmm_set_force_dmmv. */
 int qmm_forward_act(int type, const void *w, const void *xq, float *dst, int64_t ldd, void *workspace,
                     size_t workspace_bytes, size_t *need, int64_t k, int64_t n, int64_t rows, int launch,
                     int64_t stream);

@@ -721,7 +721,7 @@ int qmm_matmul(int type, const void* w, const void* xq, float* dst, int64_t ldd,
 static int forward_impl(int type, const void* w, bool pre, const void* xq, const float* x, int64_t x_stride, float* dst,
                         int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k, int64_t n,
                         int64_t rows, int launch, int64_t stream) {
-  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || (pre ? !aligned16(xq) : x_stride < k))
+  if (!shape_ok(type, k, n, rows) || need == nullptr || ldd < n || (pre ? !aligned16(xq) || !aligned16(workspace) : x_stride < k))
     return QMM_UNSUPPORTED;
   const int layout = qmm_act_layout(type, rows);
   const size_t bytes = pre ? 0 : qmm::act_bytes(layout, k, rows);
@@ -794,7 +794,7 @@ int qmm_forward_act(int type, const void* w, const void* xq, float* dst, int64_t
 static int shared_impl(int type, int count, const void* const* w, const int64_t* n, float* const* dst,
                        const int64_t* ldd, bool pre, const void* xq, const float* x, int64_t x_stride, void* workspace,
                        size_t workspace_bytes, size_t* need, int64_t k, int64_t rows, int launch, int64_t stream) {
-  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || (pre ? !aligned16(xq) : x_stride < k))
+  if (count < 1 || !w || !n || !dst || !ldd || need == nullptr || (pre ? !aligned16(xq) || !aligned16(workspace) : x_stride < k))
     return QMM_UNSUPPORTED;
   for (int i = 0; i < count; i++)
     if (!shape_ok(type, k, n[i], rows) || ldd[i] < n[i]) return QMM_UNSUPPORTED;
@@ -932,7 +932,7 @@ static int glu_impl(int type, int act, const void* w_gate, const void* w_up, boo
                     int64_t x_stride, float* dst, int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need,
                     int64_t k, int64_t n, int64_t rows, int launch, int64_t stream) {
   if (!shape_ok(type, k, n, rows) || act < QMM_GLU_SILU || act > QMM_GLU_GELU || need == nullptr || ldd < n ||
-      (pre ? !aligned16(xq) : x_stride < k))
+      (pre ? !aligned16(xq) || !aligned16(workspace) : x_stride < k))
     return QMM_UNSUPPORTED;
   // workspace: the quantized activation, then the gate and up products of
   // the two-launch form

@@ -188,3 +188,23 @@ def test_a_window_past_the_context_plans_as_none(shape):
         assert none[0] == QMM_OK
         for window in (max_kv, 2**31, 2**62, 2**63 - 1):
             assert attend(max_kv=max_kv, window=window, **shape) == none
+
+
+@pytest.mark.parametrize("t,k,n,rows", [(12, 4096, 4096, 1), (12, 14336, 4096, 77), (14, 14336, 4096, 100), (8, 4096, 4096, 9)])
+def test_a_workspace_of_products_off_16_bytes_is_refused(t, k, n, rows):
+    """The slots of a K split and the GLU's products lie at its start and go 16 bytes at a time."""
+    L, size = lib(), need()
+    one, w, d = (ctypes.c_int64 * 1)(n), (ctypes.c_void_p * 1)(4096), (ctypes.c_void_p * 1)(4096)
+    for at in (4097, 4100, 4104):
+        odd = ctypes.c_void_p(at)
+        for launch in (0, 1):
+            # (w and xq missing where the call would launch: nothing may reach the device here)
+            x, wp = (None, None) if launch else (P, P)
+            for room in (0, 2**40):
+                assert L.qmm_forward_act(t, P, P, P, n, odd, room, ctypes.byref(size), k, n, rows, 0, 0) == QMM_UNSUPPORTED
+                assert L.qmm_forward_act(t, wp, x, P, n, odd, room, ctypes.byref(size), k, n, rows, launch, 0) == QMM_UNSUPPORTED
+                assert L.qmm_forward_shared_act(t, 1, w, one, d, one, x, odd, room, ctypes.byref(size), k, rows, launch, 0) == QMM_UNSUPPORTED
+                assert L.qmm_forward_glu_act(t, 0, wp, wp, x, P, n, odd, room, ctypes.byref(size), k, n, rows, launch, 0) == QMM_UNSUPPORTED
+    assert L.qmm_forward_act(t, P, P, P, n, P, 2**40, ctypes.byref(size), k, n, rows, 0, 0) == QMM_OK
+    assert L.qmm_forward_glu_act(t, 0, P, P, P, P, n, P, 2**40, ctypes.byref(size), k, n, rows, 0, 0) == QMM_OK
+    assert L.qmm_forward_shared_act(t, 1, w, one, d, one, P, P, 2**40, ctypes.byref(size), k, rows, 0, 0) == QMM_OK
