@@ -5,9 +5,11 @@
 // T), ss = sum h^2, rs = f32(1 / sqrt(ss / k + eps)), y = f32(f32(h * rs) * w),
 // and the codes, scales and sums of y as the activation quantizers write them
 // (q8k_block_wave, q8_0_code): the planes equal qmm_quantize_act's of y bit
-// for bit. The sum runs in 64 bits, so rs, and with it a row's codes, does not
-// depend on the order of the sum: every launch shape below gives the same
-// bits. Built without FP contraction, which would join h * rs * w otherwise.
+// for bit. The sum runs in 64 bits, and in one order for all the launch shapes
+// that a row length can take (each of 16 sums takes every 16th block of 256
+// values, a lane's values in turn, then the lanes', then the sums from the first
+// on), so a row's bits do not follow from its batch. Built without FP
+// contraction, which would join h * rs * w otherwise.
 //
 // A lane holds 4 consecutive values, a wave a 256-value block at a time (16-
 // or 8-byte loads, whole lines), so a Q8_K block is one wave's and a Q8_0
@@ -41,6 +43,18 @@ __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
   return v;
+}
+
+// Four sums over the wave's lanes in wave_sum64's order; lanes 16 j and up
+// hold that of v[j].
+__device__ __forceinline__ double wave_sums64(const double v[4], int lane) {
+  const bool b5 = lane & 32, b4 = lane & 16;
+  const double a0 = (b5 ? v[2] : v[0]) + __shfl_xor(b5 ? v[0] : v[2], 32, kWave);
+  const double a1 = (b5 ? v[3] : v[1]) + __shfl_xor(b5 ? v[1] : v[3], 32, kWave);
+  double s = (b4 ? a1 : a0) + __shfl_xor(b4 ? a0 : a1, 16, kWave);
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor(s, m, kWave);
+  return s;
 }
 
 // The 4 values at element e of a row (h as stored: rounded to T), and h out.
@@ -112,8 +126,10 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void rms_norm_act_kernel(
   const int64_t row = (int64_t)blockIdx.x * kRows + wave / WPR;
   const bool row_on = row < a.rows;  // no early return: the waves of a row meet at a barrier
   constexpr int kHeld = NB ? NB : 1;
+  constexpr int kSums = WPR == 4 ? 4 : 1;  // 16 of a row that more than one wave takes
+  static_assert(WPR == 1 || WPR * kSums == 16, "the same 16 in each shape");
   float h[kHeld][4];
-  double ss = 0.0;
+  double sums[kSums] = {};
   const int64_t e0 = (int64_t)sub * 256 + 4 * lane;
   if (row_on) {
     if (NB) {
@@ -128,7 +144,8 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void rms_norm_act_kernel(
         if (e < a.k) {
           if (a.h) store4<VEC>(a.h, T, row * a.hs + e, h[b]);
 #pragma unroll
-          for (int i = 0; i < 4; i++) ss = __builtin_fma((double)h[b][i], (double)h[b][i], ss);
+          for (int i = 0; i < 4; i++)
+            sums[b % kSums] = __builtin_fma((double)h[b][i], (double)h[b][i], sums[b % kSums]);
         }
       }
     } else {
@@ -136,18 +153,22 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void rms_norm_act_kernel(
         load_h<T, VEC>(a, row, e, h[0]);
         if (a.h) store4<VEC>(a.h, T, row * a.hs + e, h[0]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) ss = __builtin_fma((double)h[0][i], (double)h[0][i], ss);
+        for (int i = 0; i < 4; i++) sums[0] = __builtin_fma((double)h[0][i], (double)h[0][i], sums[0]);
       }
     }
   }
-  ss = wave_sum64(ss);
+  double ss;
+  if constexpr (kSums == 4)
+    ss = wave_sums64(sums, lane);
+  else
+    ss = wave_sum64(sums[0]);
   if (WPR > 1) {
     __shared__ double s_ss[16];
-    if (lane == 0) s_ss[wave] = ss;
+    if ((lane & (64 / kSums - 1)) == 0) s_ss[sub + WPR * (lane / (64 / kSums))] = ss;
     __syncthreads();
     ss = 0.0;
 #pragma unroll
-    for (int i = 0; i < WPR; i++) ss += s_ss[wave - sub + i];
+    for (int i = 0; i < 16; i++) ss += s_ss[i];
   }
   if (!row_on) return;
   const float rs = (float)(1.0 / sqrt(ss / (double)a.k + (double)a.eps));
