@@ -426,8 +426,13 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
  * counts as that). The products run on f16 operands with f32 sums: q (an f32 q
  * rounds; all saturate at 65504), the cache's values code * scale and the
  * weights, each rounded once to nearest. scale is finite (at most 1e30 in
- * size). Any mix of lengths is served by one call; the rows of a sequence do
- * not depend on the other sequences' data. Plan (launch == 0) and launch as
+ * size). Any mix of lengths is served by one call. A sequence's rows do not
+ * depend on the other sequences' queries, keys, values and pages, and are the same
+ * bits from call to call. Where its sums are split, and so the last bits of a row
+ * (all within the roundings above), follows from the launch that the host plans
+ * by the call's sizes (seqs, tokens, max_q, max_kv, window) and, in a call with more than 256 query rows a
+ * kv head (max_q times heads / kv_heads), from the other sequences' q_starts and
+ * kv_lens too. Plan (launch == 0) and launch as
  * qmm_forward: the workspace (16-byte aligned) joins the parts of a long
  * context (*need can be 0). */
 int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_stride, int64_t q_head_stride,

@@ -111,7 +111,10 @@ class KvCache:
         them. sinks [heads] f32: a term exp(sink) in each softmax's sum. Rows
         of q that belong to no sequence are left as they were in `out` (as
         torch.empty gives them without one). The products run on f16 operands
-        with f32 sums: an f32 q is rounded to f16, as is a bf16 one."""
+        with f32 sums: an f32 q is rounded to f16, as is a bf16 one. A row does
+        not depend on the other sequences' values; its last bits can follow from
+        max_q, max_kv, the number of sequences and, past 256 query rows a kv
+        head, the other sequences' lengths, by which the sums are split."""
         device = self.device
         q_type = _X_DTYPES.get(q.dtype)
         if q.dim() != 3 or q_type is None or q.device != device or q.shape[2] != self.head_dim or q.shape[1] < 1 \
