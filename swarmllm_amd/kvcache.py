@@ -54,7 +54,11 @@ class KvCache:
                        torch.zeros((pages, kv_heads, head_dim // 32, page), dtype=torch.float16, device=device))
 
     def slots(self, table: torch.Tensor, start: int, count: int) -> torch.Tensor:
-        """The slots (int64) of positions start .. start + count - 1 of the sequence with this page table (1-D)."""
+        """The slots (int64) of positions start .. start + count - 1 of the sequence with this page table (1-D),
+        all of them inside it. A page id outside the cache gives slots outside it."""
+        if table.dim() != 1 or start < 0 or count < 0 or start + count > table.numel() * self.page:
+            raise ValueError(f"KvCache.slots: positions {start} .. {start + count - 1} of a table {tuple(table.shape)} of "
+                             f"pages of {self.page}")
         p = torch.arange(start, start + count, device=table.device)
         return table.long()[p // self.page] * self.page + p % self.page
 

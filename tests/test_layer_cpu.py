@@ -208,3 +208,21 @@ def test_a_workspace_of_products_off_16_bytes_is_refused(t, k, n, rows):
     assert L.qmm_forward_act(t, P, P, P, n, P, 2**40, ctypes.byref(size), k, n, rows, 0, 0) == QMM_OK
     assert L.qmm_forward_glu_act(t, 0, P, P, P, P, n, P, 2**40, ctypes.byref(size), k, n, rows, 0, 0) == QMM_OK
     assert L.qmm_forward_shared_act(t, 1, w, one, d, one, P, P, 2**40, ctypes.byref(size), k, rows, 0, 0) == QMM_OK
+
+
+def test_slots_stay_inside_the_table():
+    """A position behind the last page would index past the table, on the device; one before the first wraps around."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from swarmllm_amd import KvCache
+
+    kv, table = SimpleNamespace(page=16), torch.tensor([5, 0, -1, 9], dtype=torch.int32)
+    assert KvCache.slots(kv, table, 14, 4).tolist() == [94, 95, 0, 1]
+    assert KvCache.slots(kv, table, 0, 64).numel() == 64 and KvCache.slots(kv, table, 64, 0).numel() == 0
+    assert (KvCache.slots(kv, table, 32, 16) < 0).all()  # no page: padding
+    for t, start, count in ((table, 64, 1), (table, 60, 5), (table, -1, 2), (table, 0, -1), (table[:0], 0, 1),
+                            (table.view(2, 2), 0, 4), (table, 2**40, 1)):
+        with pytest.raises(ValueError):
+            KvCache.slots(kv, t, start, count)
