@@ -16,10 +16,14 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;  // positions a step of either kernel takes
-// Weights may reach 2^kSlack (f16 holds 2^15) before the running maximum that
+// Weights may reach 2^kSlack (lifted, f16 holds 2^15) before the running maximum that
 // they are relative to is moved and what is summed so far rescaled.
 constexpr float kSlack = 8.0f;
-// Weights are 2^(s sc - m sc), m the maximum they are relative to. Up to this
+// Weights are lifted by 2^kLift, which leaves again with the division by their
+// sum: f16 holds them down to 2^-31 of the largest and not to 2^-24 only (a
+// million positions of 2^-25.5 beside one of 1 are 2 % of a row's output).
+constexpr float kLift = 7.0f;
+// Weights are 2^(s sc - m sc + kLift), m the maximum they are relative to. Up to this
 // size m sc is rounded by 2^-17 at most and one fused multiply-add a weight
 // does it; where some row's is larger the scores are taken as s - m first, for
 // the rounding grows with m sc (from 2^28 on by 16 and more: weights past f16,
@@ -212,7 +216,7 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int head, float 
     const float at = fminf(fmaxf(top * a.sc, -3e38f), 3e38f);  // finite
     const float sink = a.sinks[head] * kLog2e, mx = fmaxf(at, sink);
     f = exp2_fast(at - mx);
-    sum = sum * f + (sink == mx ? 1.0f : exp2_fast(sink - mx));  // (an infinite sink less itself is NaN)
+    sum = sum * f + exp2_fast(sink == mx ? kLift : sink - mx + kLift);  // (an infinite sink less itself is NaN)
   }
   const float inv = sum == 0.0f ? 0.0f : f / sum;
 #pragma unroll

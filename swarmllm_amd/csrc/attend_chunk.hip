@@ -244,7 +244,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
   for (int d = 0; d < HD / 32; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f, bs = 0.0f;  // bs: m sc, what the weights' exponents are less (0: none yet, or far)
+  float m = -INFINITY, l = 0.0f, bs = 0.0f;  // bs: m sc - kLift, what the weights' exponents are less (far: m is taken off before)
   bool far = false;  // some row's maximum is past kFar (the same for the wave)
   const ChunkCall in_steps = call_args();
   const AttendArgs& a = in_steps.a;
@@ -320,7 +320,7 @@ __device__ __forceinline__ void attend_block(int tid, int b, int kvh, int64_t q0
         l *= f;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++) o[d] *= f;
-        bs = far ? 0.0f : to * a.sc;
+        bs = far ? -kLift : __builtin_fmaf(to, a.sc, -kLift);
         if (far)
 #pragma unroll
           for (int t = 0; t < 2; t++)

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
   }
 
   f4v o[NT][Z::kDims];
-  float m[NT], l[NT], bs[NT];  // bs: m sc, what the weights' exponents are less (0: none yet, or far)
+  float m[NT], l[NT], bs[NT];  // bs: m sc - kLift, what the weights' exponents are less (far: m is taken off before)
   bool far[NT];  // some row's maximum is past kFar (the same for the wave)
 #pragma unroll
   for (int n = 0; n < NT; n++) {
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attend_few_kernel(AttendArgs a
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < Z::kDims; d++) o[n][d] *= f;
-        bs[n] = far[n] ? 0.0f : to * a.sc;
+        bs[n] = far[n] ? -kLift : __builtin_fmaf(to, a.sc, -kLift);
         if (far[n])
 #pragma unroll
           for (int t = 0; t < 4; t++)

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from layer_reference import attend64, rounding
+from swarmllm_amd import KvCache
 from test_attend_gpu import BF16, F16, F32, batch
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +94,40 @@ def test_sinks_past_the_largest_number(new, n):
     assert (got[:, :2] == 0).all() and torch.equal(got[:, 2:], none[:, 2:])
     far = kv.attend(q, starts, lens, tables, max_q=new, scale=2.0**99, sinks=torch.full((4,), inf, device="cuda"))
     assert (far == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 33])
+def test_many_small_weights_beside_a_large_one(new):
+    """2^20 positions of a weight of 2^-25.5 behind one of 1: together 2 % of the row, and each under half the smallest
+    f16. 64 sequences of 8 kv heads on the same pages, so that none is cut in parts that would each find a maximum of
+    its own. The weak weights are exact to 2^-32 (half the smallest f16, the weights lifted by 2^7)."""
+    n, seqs, page = 2**20, 64, 256
+    kv = KvCache.alloc(n // page, 8, 64, page)
+    kv.planes[1].fill_(1.0)
+    kv.planes[3].fill_(2.0**-7)
+    kv.planes[0][..., 0] = -51
+    kv.planes[0][0, :, 0, 0] = 0
+    v = torch.randint(-127, 128, (8, 64), device="cuda", dtype=torch.int8)
+    first = torch.randint(-127, 128, (8, 64), device="cuda", dtype=torch.int8)
+    kv.planes[2][:] = v[None, :, :, None]
+    kv.planes[2][0, :, :, 0] = first
+    q = torch.zeros(seqs * new, 8, 64, device="cuda")
+    q[..., 0] = 1.0
+    scale = 0.34657359  # ln 2 / 2 (as an f32 number): 51 of it are 25.5 powers of two
+    scale32 = torch.tensor(scale, dtype=torch.float32).double()
+    starts = torch.arange(seqs + 1, device="cuda", dtype=torch.int32) * new
+    lens = torch.full((seqs,), n, device="cuda", dtype=torch.int32)
+    tables = torch.arange(n // page, device="cuda", dtype=torch.int32).expand(seqs, -1).contiguous()
+    got = kv.attend(q, starts, lens, tables, max_q=new, scale=scale)
+    w = torch.exp(-51.0 * scale32.cuda())
+    weak = w * (n - new + torch.arange(new, device="cuda").double()).repeat(seqs)[:, None, None]
+    want = (first.double() + weak * v.double()) * 2.0**-7 / (1 + weak)
+    size = (first.double().abs() + weak * v.double().abs()) * 2.0**-7 / (1 + weak)
+    # 2^-11 a value and a weight, 2^-15 the exponents and joins, a weak weight 2^-32. The matrix instructions add 8
+    # positions' products to a sum at a time and round it to nearest, by at most 2^-24 of itself, each time (16 products of
+    # 1/16, 3/16 and 5/16 of a step of the sum add 0, 4 and 4 steps: two eights of 1/2, 3/2 and 5/2, to even). That is n / 8
+    # times for a chunk's row and n / 32 times in each of the four waves of few rows, and up to 64 more in joins; here all to
+    # one side, for each addition is the same 8 weights of 2^-18.5 (1.4 |v| / |first| of the sum's steps). 0.8 % of a row, 0.2
+    adds = (n / 8 if new > 32 else n / 32) + 64
+    tol = (2 * 2.0**-11 * (1 + 2.0**-11) + 2.0**-15 + 2.0**-24 * adds) * size + 2.0**-32 * n
+    assert ((got.double() - want).abs() <= tol + rounding(F32) * want.abs()).all(), float(((got.double() - want).abs() - tol).max())
