@@ -395,7 +395,8 @@ int qmm_cache_plane_bytes(int64_t pages, int kv_heads, int head_dim, int page, s
  * cached value is a finite f16), codes clamp(round(v / scale), -127, 127), NaN
  * as 0: the wire codec's block (qmm_wire_encode), the scale kept as f16. A
  * slot outside the cache (a negative one: padding) writes nothing; the others
- * are distinct, and no other position of the cache changes. */
+ * are distinct, and no other position of the cache changes. At most 2^29 tokens
+ * a call (qmm_cache_read alike). */
 int qmm_cache_write(const qmm_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v,
                     int64_t v_stride, int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens,
                     int64_t stream);
@@ -426,7 +427,7 @@ int qmm_cache_read(const qmm_cache *cache, const int64_t *slots, int64_t tokens,
  * counts as that). The products run on f16 operands with f32 sums: q (an f32 q
  * rounds; all saturate at 65504), the cache's values code * scale and the
  * weights, each rounded once to nearest. scale is finite (at most 1e30 in
- * size). Any mix of lengths is served by one call. A sequence's rows do not
+ * size); seqs times kv_heads is below 2^23. Any mix of lengths is served by one call. A sequence's rows do not
  * depend on the other sequences' queries, keys, values and pages, and are the same
  * bits from call to call. Where its sums are split, and so the last bits of a row
  * (all within the roundings above), follows from the launch that the host plans

@@ -221,7 +221,8 @@ hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipSt
 bool attend_fits(const AttendArgs& a) {
   const int64_t rows = (int64_t)a.max_q * a.group;
   const int64_t heads = (int64_t)a.seqs * a.c.heads;
-  return rows <= (int64_t)32000 * 128 && rows * a.group < ((int64_t)1 << 32) && heads < ((int64_t)1 << 31);
+  return rows <= (int64_t)32000 * 128 && rows * a.group < ((int64_t)1 << 32) &&
+         heads < ((int64_t)1 << 23);  // workgroups of 512 threads in a launch's x, which wraps at 2^32
 }
 
 size_t attend_workspace_bytes(const AttendArgs& a, int cus) {

@@ -398,7 +398,6 @@ hipError_t launch_write_type(const CachePlanes& c, const void* k, const void* v,
 hipError_t launch_cache_write(const CachePlanes& c, const void* k, const void* v, int dtype, int64_t ks, int64_t khs,
                               int64_t vs, int64_t vhs, const int64_t* slots, int64_t tokens, hipStream_t st) {
   QMM_NOTE_LAUNCH();
-  if (tokens > ((int64_t)1 << 36)) return hipErrorInvalidValue;  // a grid of 2^30 workgroups
   switch (dtype) {
     case QMM_X_F32: return launch_write_type<QMM_X_F32>(c, k, v, ks, khs, vs, vhs, slots, tokens, st);
     case QMM_X_F16: return launch_write_type<QMM_X_F16>(c, k, v, ks, khs, vs, vhs, slots, tokens, st);
@@ -410,7 +409,6 @@ hipError_t launch_cache_write(const CachePlanes& c, const void* k, const void* v
 hipError_t launch_cache_read(const CachePlanes& c, const int64_t* slots, int64_t tokens, void* k, void* v, int odt,
                              hipStream_t st) {
   QMM_NOTE_LAUNCH();
-  if (tokens > ((int64_t)1 << 36)) return hipErrorInvalidValue;
   const int vec = (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0;
   if (few_values(c, tokens))
     cache_read_token_kernel<<<token_grid(c, tokens, 8), 256, 0, st>>>(c, slots, k, v, odt, vec);

@@ -123,7 +123,7 @@ template <int T, int LAYOUT, int WPR, int NB, bool VEC>
 __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void rms_norm_act_kernel(NormArgs a, int ydt) {
   constexpr int kRows = WPR < 4 ? 4 / WPR : 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % WPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + wave / WPR;
+  const int64_t row = wide_block() * kRows + wave / WPR;
   const bool row_on = row < a.rows;  // no early return: the waves of a row meet at a barrier
   constexpr int kHeld = NB ? NB : 1;
   constexpr int kSums = WPR == 4 ? 4 : 1;  // 16 of a row that more than one wave takes
@@ -196,8 +196,8 @@ template <int T, int LAYOUT, int WPR, int NB>
 hipError_t launch_vec(const NormArgs& a, int ydt, bool vec, hipStream_t st) {
   constexpr int kRows = WPR < 4 ? 4 / WPR : 1;
   const int64_t groups = (a.rows + kRows - 1) / kRows;
-  if (groups >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)groups), block(WPR < 4 ? 256 : WPR * 64);
+  if (groups >= ((int64_t)1 << 36)) return hipErrorInvalidValue;
+  const dim3 grid = wide_grid(groups), block(WPR < 4 ? 256 : WPR * 64);
   if (vec)
     rms_norm_act_kernel<T, LAYOUT, WPR, NB, true><<<grid, block, 0, st>>>(a, ydt);
   else
@@ -229,7 +229,7 @@ template <int LAYOUT>
 __global__ __launch_bounds__(256) void dequantize_act_kernel(const int8_t* __restrict__ codes,
                                                              const float* __restrict__ d, void* __restrict__ out,
                                                              int odt, int vec, int64_t n) {
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const int64_t e = (wide_block() * 256 + threadIdx.x) * 8;
   if (e >= n) return;
   const uint2 c = *(const uint2*)(codes + e);
   const float s = d[e >> (LAYOUT == ACT_Q8K ? 8 : 5)];
@@ -283,12 +283,12 @@ hipError_t launch_dequantize_act(const void* xq, int layout, void* out, int odt,
   QMM_NOTE_LAUNCH();
   const ActPlanes p = act_planes(layout, (void*)xq, k, rows);
   const int64_t n = k * rows, groups = (n + 2047) / 2048;
-  if (groups >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
+  if (groups >= ((int64_t)1 << 36)) return hipErrorInvalidValue;
   const int vec = (uintptr_t)out % 16 == 0;
   if (layout == ACT_Q8K)
-    dequantize_act_kernel<ACT_Q8K><<<dim3((unsigned)groups), 256, 0, st>>>(p.codes, p.d, out, odt, vec, n);
+    dequantize_act_kernel<ACT_Q8K><<<wide_grid(groups), 256, 0, st>>>(p.codes, p.d, out, odt, vec, n);
   else
-    dequantize_act_kernel<ACT_Q8_0><<<dim3((unsigned)groups), 256, 0, st>>>(p.codes, p.d, out, odt, vec, n);
+    dequantize_act_kernel<ACT_Q8_0><<<wide_grid(groups), 256, 0, st>>>(p.codes, p.d, out, odt, vec, n);
   return hipGetLastError();
 }
 

@@ -79,6 +79,8 @@ bool cache_ok(const qmm_cache* c) {
   return c && cache_shape_ok(c->pages, c->kv_heads, c->head_dim, c->page) && c->k_codes && c->k_scales && c->v_codes &&
          c->v_scales && aligned16(c->k_codes) && aligned16(c->k_scales) && aligned16(c->v_codes) && aligned16(c->v_scales);
 }
+// Tokens of a cache write or read: 2^23 workgroups of 64 (a launch's threads stay below 2^32).
+constexpr int64_t kMostCacheTokens = (int64_t)1 << 29;
 qmm::CachePlanes planes_of(const qmm_cache& c) {
   return qmm::CachePlanes{(int8_t*)c.k_codes, (uint16_t*)c.k_scales, (int8_t*)c.v_codes, (uint16_t*)c.v_scales,
                           c.pages, c.kv_heads, c.head_dim, c.page};
@@ -1050,7 +1052,8 @@ int qmm_cache_plane_bytes(int64_t pages, int kv_heads, int head_dim, int page, s
 int qmm_cache_write(const qmm_cache* cache, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v,
                     int64_t v_stride, int64_t v_head_stride, int dtype, const int64_t* slots, int64_t tokens,
                     int64_t stream) {
-  if (!cache_ok(cache) || !qmm::value_type_ok(dtype) || tokens < 0 || k_head_stride < cache->head_dim ||
+  if (!cache_ok(cache) || !qmm::value_type_ok(dtype) || tokens < 0 || tokens > kMostCacheTokens ||
+      k_head_stride < cache->head_dim ||
       v_head_stride < cache->head_dim || k_stride < 0 || v_stride < 0)
     return QMM_UNSUPPORTED;
   if (tokens == 0) return QMM_OK;
@@ -1062,7 +1065,7 @@ int qmm_cache_write(const qmm_cache* cache, const void* k, int64_t k_stride, int
 
 int qmm_cache_read(const qmm_cache* cache, const int64_t* slots, int64_t tokens, void* k, void* v, int out_dtype,
                    int64_t stream) {
-  if (!cache_ok(cache) || !qmm::value_type_ok(out_dtype) || tokens < 0) return QMM_UNSUPPORTED;
+  if (!cache_ok(cache) || !qmm::value_type_ok(out_dtype) || tokens < 0 || tokens > kMostCacheTokens) return QMM_UNSUPPORTED;
   if (tokens == 0) return QMM_OK;
   if (!k || !v || !slots) return QMM_UNSUPPORTED;
   clear_stale_error();

@@ -10,6 +10,14 @@ namespace qmm {
 inline __host__ __device__ int value_bytes(int dtype) { return dtype == QMM_X_F32 ? 4 : 2; }
 inline bool value_type_ok(int dtype) { return dtype == QMM_X_F16 || dtype == QMM_X_BF16 || dtype == QMM_X_F32; }
 
+// A launch's threads in x stay below 2^32 (a larger grid wraps around without an
+// error): up to 2^21 workgroups in x, of any size, and y for the rest.
+inline dim3 wide_grid(int64_t groups) {
+  const int64_t x = groups < ((int64_t)1 << 21) ? groups : (int64_t)1 << 21;
+  return dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+}
+__device__ __forceinline__ int64_t wide_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // bf16 bits of v, to nearest even; NaN stays a (quiet) NaN.
 __device__ __forceinline__ uint16_t f2bf(float v) {
   const uint32_t u = __float_as_uint(v);

@@ -226,3 +226,14 @@ def test_slots_stay_inside_the_table():
                             (table.view(2, 2), 0, 4), (table, 2**40, 1)):
         with pytest.raises(ValueError):
             KvCache.slots(kv, t, start, count)
+
+
+def test_calls_of_more_threads_than_a_launch_takes_are_refused():
+    """Past 2^32 threads in x a grid wraps around without an error."""
+    L, r = lib(), ctypes.byref(cache())
+    for tokens in (2**29 + 1, 2**40):
+        assert L.qmm_cache_write(r, None, 1024, 128, None, 1024, 128, X_F32, None, tokens, 0) == QMM_UNSUPPORTED
+        assert L.qmm_cache_read(r, None, tokens, None, None, X_F16, 0) == QMM_UNSUPPORTED
+    many = dict(heads=256, q_stride=256 * 128, out_stride=256 * 128, max_kv=512)
+    assert attend(cache(heads=256), seqs=2**15, tokens=2**15, max_q=1, **many)[0] == QMM_UNSUPPORTED
+    assert attend(cache(heads=256), seqs=2**15 - 1, tokens=2**15, max_q=1, **many)[0] == QMM_OK

@@ -62,3 +62,17 @@ def test_the_order_of_the_sum_does_not_follow_from_the_batch(k):
     assert (many.y == one.y).all()
     for a, b in zip(one.act.planes(), many.act.planes()):
         assert (a[0] == b).all()
+
+
+def test_more_rows_than_a_launch_has_threads_in_one_direction():
+    """2^26 rows of a wave each, and some."""
+    rows = 2**26 + 5
+    x = torch.arange(rows, device="cuda", dtype=torch.int32).remainder_(251).add_(1).float()[:, None].repeat(1, 4)
+    x[:, 1] = 0.5
+    out = rms_norm_act(x, torch.ones(4, device="cuda"), 0.0, dtype=None, y_dtype=torch.float32)
+    for part in (slice(0, 2000), slice(2**25 - 1000, 2**25 + 1000), slice(rows - 2000, rows)):
+        h = x[part].double()
+        want = h / h.square().mean(1, keepdim=True).sqrt()
+        assert ((out.y[part].double() - want).abs() <= 3.001 * 2.0**-24 * want).all()
+    # and no row is another's
+    assert torch.equal(out.y[:251].repeat(3, 1), out.y[251 * 2**17: 251 * (2**17 + 3)])
