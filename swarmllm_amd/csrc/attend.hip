@@ -27,6 +27,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, int lo_r
   const int hd = a.c.hd, per = hd / 4, fit = 64 / per;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane / per, e = 4 * (lane - sub * per), first = G > 1 ? wave : 0;
+  // rows of one kv head of a sequence, block after block
   const int64_t row_of_head = ((int64_t)blockIdx.x * (4 / G) + (G > 1 ? 0 : wave)) * fit + sub;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int block = (int)(row_of_head / p.rows), row = (int)(row_of_head - (int64_t)block * p.rows);
@@ -181,24 +182,24 @@ Plan plan_of(const AttendArgs& a, int cus) {
   return p;
 }
 
-// The partial results at ws of the last `cut` blocks: bytes, and where they lie.
+// The partial results of `cut` blocks at ws: bytes, and where they lie.
 size_t parts_at(const AttendArgs& a, int parts, int rows, int blocks, int cut, void* ws, AttendParts& p) {
   const int heads = a.seqs * a.c.heads;
   p = AttendParts{nullptr, nullptr, parts, rows, blocks, cut, cut / heads, cut % heads, nullptr, 0};
   if (parts <= 1) return 0;
   const size_t n = (size_t)cut * parts * rows;
   p.o = (float*)ws;
-  p.ml = p.o + n * a.c.hd;
+  p.ml = (float*)((uintptr_t)ws + n * a.c.hd * sizeof(float));  // (integers: a plan has no workspace)
   return n * (a.c.hd + 2) * sizeof(float);
 }
 
 // And those of `shares`.
 size_t shares_at(const AttendArgs& a, int shares, void* ws, AttendParts& p) {
   p = AttendParts{(float*)ws, nullptr, 1, kShareRows, 0, 0, 0, 0, nullptr, shares};
-  const size_t n = (size_t)2 * shares * kShareRows;
-  p.ml = p.o + n * a.c.hd;
-  p.split = (int4*)(p.ml + 2 * n);
-  return n * (a.c.hd + 2) * sizeof(float) + shares * sizeof(int4);
+  const size_t n = (size_t)2 * shares * kShareRows, sums = n * (a.c.hd + 2) * sizeof(float);
+  p.ml = (float*)((uintptr_t)ws + n * a.c.hd * sizeof(float));
+  p.split = (int4*)((uintptr_t)ws + sums);
+  return sums + shares * sizeof(int4);
 }
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
