@@ -11,8 +11,8 @@
 // cores, each rounded once; scores, maxima, sums and outputs are f32. The
 // rounding, 2^-11 of a value, is an eighth of the half step that a code's own
 // rounding leaves (1 / 254 of its block's largest); f16 outputs end 4e-4 to
-// 5e-4 from 64 bits (an exact sum's rounding: 2e-4). f32 operands run at a 16th
-// of the rate.
+// 5e-4 from 64 bits (an exact sum's rounding: 2e-4), f32 ones from f32 queries
+// 5.4e-4 to 5.6e-4. f32 operands run at a 16th of the rate.
 #include "attend.h"
 
 namespace qmm {
@@ -138,8 +138,9 @@ Plan plan_of(const AttendArgs& a, int cus) {
   if (rows > kFewRows) {
     // blocks of 256 rows lay a step's keys and values down once for 8 waves;
     // over short contexts twice as many workgroups are worth more (us, 256 /
-    // 128 rows: 512 tokens over 4096 67 / 71, 2000 and 1333 over 7777 and 5832 866 / 937; 1000
-    // over 1000 35 / 32, 8 x 64 over 2000 50 / 48)
+    // 128 rows: 512 tokens over 4096, 32 heads on 8 of 128 dims, 67 / 71; 2000 and 1333 over
+    // 7777 and 5832, 64 on 8 of 128, 866 / 937; 1000 over 1000, 32 on 8 of 64, 35 / 32; 8 x 64
+    // over 2000, 64 on 8 of 64, 50 / 48)
     p.chunk_rows = a.c.hd <= 128 && rows > kShareRows && most_steps(a, kShareRows) >= 32 ? kShareRows : 128;
     p.chunk_blocks = (int)((rows + p.chunk_rows - 1) / p.chunk_rows);
     const int64_t slots = (int64_t)cus * (p.chunk_rows > 128 || a.c.hd > 128 ? 1 : 2), n = heads * p.chunk_blocks;
@@ -147,11 +148,11 @@ Plan plan_of(const AttendArgs& a, int cus) {
     if (p.chunk_rows == kShareRows && n > slots && n < 6 * slots && work < 1e17) {
       // a few rounds of the CUs: equal shares, so that the last round is whole and
       // sequences shorter than max_q and max_kv leave no CU idle (us, shares /
-      // blocks: 2000 and 1333 tokens over 7777 and 5832 751 / 887; all of one length
+      // blocks, 64 heads on 8 of 128 dims: 2000 and 1333 tokens over 7777 and 5832 751 / 887; all of one length
       // 0 to 3 % slower: 2 x 2000 over 7777 985 / 981, 4000 over 7777 831 / 809). Many
       // rounds fill up by themselves, and their short blocks' beginnings count
       // more (7777 over 7777 1338 / 1083); fewer blocks than CUs are cut evenly
-      // (512 over 4096 76 / 56).
+      // (512 over 4096, 32 heads on 8, 76 / 56).
       p.shares = cus;
     } else {
       // parts that fill the CUs, of 8 steps at least: of every block where those
@@ -171,7 +172,7 @@ Plan plan_of(const AttendArgs& a, int cus) {
     // parts until two workgroups a CU are there, of one step a wave at least,
     // of four where the CUs have one each without, and none up to two steps a
     // wave (the join is a launch of 4 us, as much again for the host; graph
-    // replays, us: 1 sequence of 500 whole 11.3, in 2 parts 10.8; of 2000 in 8
+    // replays, us, 32 heads on 8 of 128 dims, the 16 64 on 8: 1 sequence of 500 whole 11.3, in 2 parts 10.8; of 2000 in 8
     // 11.1, in 2 18.1; 4 of 1000 in 4 10.6, whole 16.2; 16 of 8000 in 4 51.5, in 2
     // 68.1; 32 of 1000 whole 17.0, in 2 19.5)
     const int64_t steps = most_steps(a, p.few);
@@ -203,7 +204,7 @@ size_t shares_at(const AttendArgs& a, int shares, void* ws, AttendParts& p) {
 }
 
 hipError_t join(const AttendArgs& a, int lo, int hi, const AttendParts& p, hipStream_t st) {
-  // (us, parts dealt to 4 waves / all to one wave: 4 parts of 512 tokens' 64
+  // (us, parts dealt to 4 waves / all to one wave, 32 heads on 8 of 128 dims: 4 parts of 512 tokens' 64
   // blocks 11.9 / 7.8, 31 of one token's 32 heads 4.2 / 5.1, 64 of them 5.2 / 10.9)
   const bool deal = p.parts > 8;
   const int fit = 64 / (a.c.hd / 4) * (deal ? 1 : 4);

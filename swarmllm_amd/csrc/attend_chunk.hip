@@ -16,7 +16,8 @@
 // lane's own column.
 //
 // Chunks of 2000 and 1333 tokens over 7777 and 5832 (64 query heads on 8 of 128
-// dims) take 751-763 us, 0.88 PFLOP/s; a library product of 8192^3 reaches 1.15.
+// dims) take 741-781 us from card to card, 0.86-0.90 PFLOP/s; a library product of 8192^3
+// reaches 1.15.
 // The products, the softmax's and the conversions' vector instructions (about
 // 290 a wave and step with 128 rows a workgroup, 235 with 256) and the LDS reads
 // (32 operands of 1 KiB a wave and step) each take a third to a half of a step

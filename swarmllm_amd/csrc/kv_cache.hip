@@ -17,7 +17,7 @@
 // 16 consecutive positions (a prompt's do but at its ends) a lane moves them
 // as one 16-byte piece; other tokens go a byte at a time. 32768 tokens of 8 x
 // 128 values read back as f16 in 46 us (206 MB at 4.5 TB/s; a byte at a time
-// 136 us), 2000 tokens' f32 rows written in 10.4 us (18.3) and read in 7.1 (11.2).
+// 136 us), 2000 tokens' f32 rows written in 10.1-10.9 us (18.3) and read in 6-7 (11.2).
 // A few tokens (a decode step's) take kernels of their own, a token a workgroup
 // and nothing between its slot and its stores: 8 tokens 3.7 us each way, 8 on
 // the tiles.

@@ -15,8 +15,8 @@
 // or 8-byte loads, whole lines), so a Q8_K block is one wave's and a Q8_0
 // block 8 lanes'. A row stays in registers between its two passes, so what
 // bounds a batch is its bytes: 2000 rows of 8192 f32 values with a residual take
-// 49 us, 213 MB at 4.35 TB/s (a copy reaches 4.8). One row of 4096 takes 3.6 us
-// (an empty launch 2.6), 77 of 2880 bf16 values 4.8.
+// 49-51 us, 213 MB at 4.2-4.35 TB/s (a copy reaches 4.8). One row of 4096 takes
+// 3.9-4.2 us (an empty launch 2.6), 77 of 2880 bf16 values 4.6-5.5.
 #include "../../include/qmm.h"
 #include "qmm_device.h"
 #include "qmm_launch.h"
