@@ -5,6 +5,7 @@
 // fused decode kernel's.
 #include "glu_act.h"
 #include "qmm_launch.h"
+#include "value_types.h"
 
 namespace qmm {
 
@@ -14,7 +15,7 @@ template <int ACT>
 __global__ __launch_bounds__(256) void glu_kernel(const float* __restrict__ gate, int64_t ldg,
                                                   const float* __restrict__ up, int64_t ldu, float* __restrict__ out,
                                                   int64_t ldo, int64_t n, int64_t rows) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = wide_block() * 256 + threadIdx.x;
   if (i >= n * rows) return;
   const int64_t r = i / n, c = i - r * n;
   out[r * ldo + c] = glu_act<ACT>(gate[r * ldg + c], up[r * ldu + c]);
@@ -82,8 +83,8 @@ template <int ACT>
 hipError_t launch(const float* gate, int64_t ldg, const float* up, int64_t ldu, float* out, int64_t ldo, int64_t n,
                   int64_t rows, hipStream_t st) {
   const int64_t total = n * rows;
-  if ((total + 255) / 256 >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
-  glu_kernel<ACT><<<dim3((unsigned)((total + 255) / 256)), 256, 0, st>>>(gate, ldg, up, ldu, out, ldo, n, rows);
+  if ((total + 255) / 256 >= ((int64_t)1 << 36)) return hipErrorInvalidValue;
+  glu_kernel<ACT><<<wide_grid((total + 255) / 256), 256, 0, st>>>(gate, ldg, up, ldu, out, ldo, n, rows);
   return hipGetLastError();
 }
 

@@ -211,6 +211,7 @@ hipError_t launch_act_quantize(int layout, const float* x, int64_t stride, int64
       act_q8k_kernel<false><<<grid, 256, 0, st>>>(x, stride, k, rows, p.codes, p.d, (int16_t*)p.sums, q8k_scale);
   } else {
     const int64_t threads = rows * (k / 32) * 8;
+    if (threads >= ((int64_t)1 << 32) - 256) return hipErrorInvalidValue;  // what a launch takes in x
     const dim3 grid((unsigned)((threads + 255) / 256));
     if (vec)
       q8_0_kernel<true, false><<<grid, 256, 0, st>>>(x, stride, k, rows, p.codes, p.d, (int32_t*)p.sums, nullptr);
