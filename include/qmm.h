@@ -442,6 +442,94 @@ int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_str
                const float *sinks, void *out, int out_dtype, int64_t out_stride, void *workspace,
                size_t workspace_bytes, size_t *need, int launch, int64_t stream);
 
+/* ---- A batch of many requests ---------------------------------------------
+ * The page tables of a batch's sequences, on the device: the caller's arrays.
+ *   tables      int32 [seqs][table_stride]: the first row_pages of a row name
+ *               the sequence's pages, -1 where it has none
+ *   lens        int32 [seqs]: the positions it holds (qmm_attend's kv_lens)
+ *   free_pages  int32 [pool]: a stack of the pages that no sequence has; what
+ *               lies past its count has no meaning
+ *   free_count  int32 [1]
+ * page: positions of a page (16, 32, 64, 128 or 256). A page is one sequence's.
+ * At most 4096 sequences, fewer than 2^31 entries of tables, 2^30 positions a
+ * sequence. */
+typedef struct qmm_pages {
+    int32_t *tables, *lens, *free_pages, *free_count;
+    int64_t table_stride, row_pages, pool;
+    int32_t seqs, page;
+} qmm_pages;
+
+/* One step of them. Sequence b, in order: its length is cut to keep[b] (NULL:
+ * none is; a keep below 0 or past the length cuts nothing) and the pages past
+ * it go onto the stack; then it takes pages for fresh[b] more tokens (NULL or
+ * below 0: none) off it. The pages that a step puts back are the first that it
+ * takes, in the order of sequences and pages, so a step that cuts what the one
+ * before added leaves the same tables. The rows of the batch are numbered
+ * sequence after sequence: q_starts [seqs + 1] (qmm_attend's) is the running sum
+ * of fresh, at most `tokens`, and of row t
+ *   slots[t]      the cache slot of its position (qmm_cache_write's), int64
+ *   positions[t]  its position in the sequence (NULL: not wanted)
+ *   seq[t]        its sequence (NULL: not wanted)
+ * A sequence is extended by all of its new tokens or by none: by none where its
+ * rows would pass `tokens`, its positions its row of the table, or its pages
+ * those that are left, and then no later sequence takes a page either. taken
+ * [seqs] says by how many. A row of a sequence that is not extended has slot
+ * and position -1, a row past the last sequence's has sequence -1 too. Tables,
+ * lengths and stack are updated in place. One launch up to 4096 tokens, two
+ * past them. */
+int qmm_pages_step(const qmm_pages *pages, const int32_t *keep, const int32_t *fresh, int64_t tokens,
+                   int32_t *q_starts, int32_t *taken, int64_t *slots, int32_t *positions, int32_t *seq,
+                   int64_t stream);
+
+/* Low-rank adapters of many requests beside `count` (at most 4) products of
+ * one activation: for row r with i = ids[r] (int32 on the device)
+ *   out[r][j] = y[r][j] + scales[i] * sum_q (sum_e x[r][e] a[i][q][e]) b[i][j][q]
+ * of each projection; a row whose id is outside [0, slots) keeps its y. x:
+ * rows x k (x_dtype: qmm_x_dtype, rows x_stride values apart, k a multiple of
+ * 32); a [slots][rank][k] and b [slots][n][rank] of w_dtype (qmm_x_dtype), each
+ * 16-byte aligned, rank a multiple of 8 up to 128 (an adapter of a lower rank
+ * has zeros); scales [slots] f32 (NULL: 1); y and out f32. out may be y itself
+ * (the same pointer and stride); otherwise nothing overlaps. Values of x and of
+ * the adapters enter as they are, sums are f32. Where x's sums are split, and
+ * so a row's last bits, follows from rows, k and count. An adapter's values reach its own
+ * rows only. Plan (launch == 0) and launch as qmm_forward: the workspace
+ * (16-byte aligned) holds x's products with a. Two launches. At most 2^20 rows. */
+typedef struct qmm_adapter {
+    const void *a, *b;
+    const float *scales;
+    const float *y;
+    float *out;
+    int64_t n, y_stride, out_stride;
+    int32_t rank;
+} qmm_adapter;
+int qmm_adapters_add(int count, const qmm_adapter *adapters, int slots, int w_dtype, const void *x, int x_dtype,
+                     int64_t x_stride, const int32_t *ids, int64_t k, int64_t rows, void *workspace,
+                     size_t workspace_bytes, size_t *need, int launch, int64_t stream);
+
+/* A token for each row of logits [rows][vocab] (dtype: qmm_x_dtype, rows
+ * `stride` values apart; vocab at most 2^19) from a uniform number u[row] in
+ * [0, 1) (f32). Settings of each row, each array NULL for off in all rows:
+ *   temperature (f32): weights exp((x - max x) / temperature); 0, below it or
+ *     NaN: the largest logit's token (NULL: 1)
+ *   top_k (int32): the k largest logits stay; off below 1 and from vocab on
+ *   top_p (f32): of those the fewest, largest first, whose weight reaches
+ *     top_p of theirs (the first always); off from 1 on and for NaN
+ *   min_p (f32): of those the ones whose weight is min_p of the largest one's
+ *     at least; off at 0, below it and for NaN, past 1 as 1
+ * Equal logits count by their index, the lowest first. The token is the first,
+ * by index, of the ones that stay at which the running sum of their weights
+ * passes u times the total (u past 1 as 1, below 0 or NaN as 0). ids (int32) gets the token and
+ * probs (NULL: not wanted) its weight over the total (1 without temperature).
+ * A NaN logit counts as -inf, a logit of -inf is never drawn; a row of nothing
+ * else gives -1 (qmm_gather_rows' "no row") and 0. Where a logit is +inf, those
+ * alone are drawn, equally. Weights are relative to the largest, in 64 bits; weights
+ * below 2^-60 may count as 0 where a setting is on. A row's token follows from
+ * the row, its settings and vocab alone. Plan and
+ * launch as qmm_forward (workspace 16-byte aligned). Two launches. At most 65535 rows. */
+int qmm_sample(const void *logits, int dtype, int64_t stride, const float *u, const float *temperature,
+               const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *probs, int64_t vocab,
+               int64_t rows, void *workspace, size_t workspace_bytes, size_t *need, int launch, int64_t stream);
+
 /* ---- GGUF files into device memory --------------------------------------
  * A parsed GGUF file: candle's gguf_file::Content::read
  * (quantized/gguf_file.rs:415-487): header (magic "GGUF", versions 1-3),

@@ -37,6 +37,20 @@ class Cache(ctypes.Structure):
                 ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page", ctypes.c_int32)]
 
 
+class Pages(ctypes.Structure):
+    """qmm_pages: the page tables of a batch's sequences and their free pages."""
+
+    _fields_ = [("tables", _P), ("lens", _P), ("free_pages", _P), ("free_count", _P), ("table_stride", _I64),
+                ("row_pages", _I64), ("pool", _I64), ("seqs", ctypes.c_int32), ("page", ctypes.c_int32)]
+
+
+class Adapter(ctypes.Structure):
+    """qmm_adapter: the adapters beside one product, and its output."""
+
+    _fields_ = [("a", _P), ("b", _P), ("scales", _P), ("y", _P), ("out", _P), ("n", _I64), ("y_stride", _I64),
+                ("out_stride", _I64), ("rank", ctypes.c_int32)]
+
+
 _F, _SZP, _CP = ctypes.c_float, ctypes.POINTER(_SZ), ctypes.POINTER(Cache)
 
 # name -> (restype, argtypes); the exports of include/qmm.h
@@ -57,6 +71,10 @@ SIGNATURES = {
     "qmm_cache_read": (_I, [_CP, _P, _I64, _P, _P, _I, _I64]),
     "qmm_attend": (_I, [_CP, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _F, _I64, _P, _P, _I,
                         _I64, _P, _SZ, _SZP, _I, _I64]),
+    "qmm_pages_step": (_I, [ctypes.POINTER(Pages), _P, _P, _I64, _P, _P, _P, _P, _P, _I64]),
+    "qmm_adapters_add": (_I, [_I, ctypes.POINTER(Adapter), _I, _I, _P, _I, _I64, _P, _I64, _I64, _P, _SZ, _SZP, _I,
+                              _I64]),
+    "qmm_sample": (_I, [_P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _SZ, _SZP, _I, _I64]),
     "qmm_matvec_max_rows": (_I, []),
     "qmm_mmq_few_rows_line": (_I, [_I, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
     "qmm_mmq_max_rows": (_I64, []),

@@ -1115,6 +1115,80 @@ int qmm_attend(const qmm_cache* cache, const void* q, int q_dtype, int64_t q_str
   return status_of(qmm::launch_attend(a, cu_count(), workspace, (hipStream_t)stream));
 }
 
+int qmm_pages_step(const qmm_pages* pages, const int32_t* keep, const int32_t* fresh, int64_t tokens, int32_t* q_starts,
+                   int32_t* taken, int64_t* slots, int32_t* positions, int32_t* seq, int64_t stream) {
+  if (!pages || pages->seqs < 0 || pages->seqs > qmm::pages_most_seqs() || tokens < 0 || tokens > kMostCacheTokens ||
+      pages->page < 16 || pages->page > 256 || (pages->page & (pages->page - 1)) != 0 || pages->row_pages < 0 ||
+      pages->table_stride < pages->row_pages || pages->pool < 0 || pages->pool > INT32_MAX ||
+      pages->row_pages > ((int64_t)1 << 30) / pages->page ||
+      (int64_t)pages->seqs * pages->row_pages > INT32_MAX || !pages->free_count || !q_starts ||
+      (pages->row_pages > 0 && pages->seqs > 0 && !pages->tables) || (pages->pool > 0 && !pages->free_pages) ||
+      (pages->seqs > 0 && (!pages->lens || !taken)) || (tokens > 0 && !slots))
+    return QMM_UNSUPPORTED;
+  qmm::PagesArgs a{};
+  a.tables = pages->tables; a.lens = pages->lens; a.free_pages = pages->free_pages; a.free_count = pages->free_count;
+  a.keep = keep; a.fresh = fresh; a.q_starts = q_starts; a.taken = taken; a.slots = slots; a.positions = positions;
+  a.seq = seq; a.table_stride = pages->table_stride; a.row_pages = pages->row_pages; a.pool = pages->pool;
+  a.tokens = tokens; a.seqs = pages->seqs; a.page = pages->page;
+  clear_stale_error();
+  return status_of(qmm::launch_pages_step(a, (hipStream_t)stream));
+}
+
+int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dtype, const void* x, int x_dtype,
+                     int64_t x_stride, const int32_t* ids, int64_t k, int64_t rows, void* workspace,
+                     size_t workspace_bytes, size_t* need, int launch, int64_t stream) {
+  if (count < 1 || count > qmm::kMaxTargets || !adapters || slots < 0 || !qmm::value_type_ok(w_dtype) ||
+      !qmm::value_type_ok(x_dtype) || need == nullptr || k < 32 || k % 32 != 0 || k > (int64_t)1 << 30 ||
+      x_stride < k || rows < 0 || rows > (int64_t)1 << 20)
+    return QMM_UNSUPPORTED;
+  qmm::LoraArgs a{};
+  a.x = x; a.ids = ids; a.xs = x_stride; a.k = k; a.rows = rows; a.count = count; a.slots = slots;
+  a.x_vec = aligned16(x) && x_stride * qmm::value_bytes(x_dtype) % 16 == 0;
+  for (int i = 0; i < count; i++) {
+    const qmm_adapter& d = adapters[i];
+    if (d.n < 1 || d.n > INT32_MAX || d.rank < 8 || d.rank > qmm::lora_most_rank() || d.rank % 8 != 0 ||
+        d.y_stride < d.n || d.out_stride < d.n || (d.y == d.out && d.y && d.y_stride != d.out_stride) ||
+        !aligned16(d.a) || !aligned16(d.b))
+      return QMM_UNSUPPORTED;
+    qmm::LoraTarget& t = a.t[i];
+    t.a = d.a; t.b = d.b; t.scales = d.scales; t.y = d.y; t.out = d.out;
+    t.n = d.n; t.ldy = d.y_stride; t.ldo = d.out_stride; t.rank = d.rank;
+    t.vec = aligned16(d.y) && aligned16(d.out) && d.y_stride % 4 == 0 && d.out_stride % 4 == 0;
+  }
+  *need = 0;
+  if (rows == 0) return QMM_OK;
+  *need = qmm::lora_plan(a, workspace, cu_count());
+  if (!launch) return QMM_OK;
+  if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
+  if (!x || !ids || !aligned16(workspace)) return QMM_UNSUPPORTED;
+  for (int i = 0; i < count; i++)
+    if (!a.t[i].y || !a.t[i].out || (slots > 0 && (!a.t[i].a || !a.t[i].b))) return QMM_UNSUPPORTED;
+  if (workspace == nullptr || workspace_bytes < *need) return QMM_WORKSPACE_TOO_SMALL;
+  clear_stale_error();
+  return status_of(qmm::launch_lora(a, x_dtype, w_dtype, (hipStream_t)stream));
+}
+
+int qmm_sample(const void* logits, int dtype, int64_t stride, const float* u, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int32_t* ids, float* probs, int64_t vocab,
+               int64_t rows, void* workspace, size_t workspace_bytes, size_t* need, int launch, int64_t stream) {
+  if (!qmm::value_type_ok(dtype) || need == nullptr || vocab < 1 || vocab > qmm::sample_most_vocab() || stride < vocab ||
+      rows < 0 || rows > 65535)
+    return QMM_UNSUPPORTED;
+  *need = 0;
+  if (rows == 0) return QMM_OK;
+  qmm::SampleArgs a{};
+  a.logits = logits; a.u = u; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+  a.ids = ids; a.probs = probs; a.stride = stride; a.rows = (int)rows; a.vocab = (int)vocab;
+  a.vec = (uintptr_t)logits % (4 * qmm::value_bytes(dtype)) == 0 && stride % 4 == 0;
+  *need = qmm::sample_plan(a, workspace);
+  if (!launch) return QMM_OK;
+  if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
+  if (!logits || !u || !ids || !aligned16(workspace)) return QMM_UNSUPPORTED;
+  if (workspace == nullptr || workspace_bytes < *need) return QMM_WORKSPACE_TOO_SMALL;
+  clear_stale_error();
+  return status_of(qmm::launch_sample(a, dtype, (hipStream_t)stream));
+}
+
 int qmm_moe_forward(int type, const void* w, int num_experts, const float* x, int64_t x_stride,
                     const int32_t* sorted_ids, const int32_t* expert_ids, const float* topk_w, int topk, float* dst,
                     int64_t ldd, void* workspace, size_t workspace_bytes, size_t* need, int64_t k, int64_t n,

@@ -309,6 +309,73 @@ bool attend_fits(const AttendArgs& a);
 size_t attend_workspace_bytes(const AttendArgs& a, int cus);
 hipError_t launch_attend(const AttendArgs& a, int cus, void* ws, hipStream_t st);
 
+// A step of a batch's page tables (pages.hip). keep, fresh, positions and seq
+// may be null.
+struct PagesArgs {
+  int32_t* tables;
+  int32_t* lens;
+  int32_t* free_pages;
+  int32_t* free_count;
+  const int32_t* keep;
+  const int32_t* fresh;
+  int32_t* q_starts;
+  int32_t* taken;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* seq;
+  int64_t table_stride, row_pages, pool, tokens;
+  int seqs, page;
+};
+int pages_most_seqs();
+hipError_t launch_pages_step(const PagesArgs& a, hipStream_t st);
+
+// Low-rank adapters beside up to kMaxTargets products of one activation
+// (lora.hip). mid: the partial results of x A^T, [splits][rows][rank] at
+// places of a workspace that lora_plan sets out (its bytes returned; 16-byte
+// aligned). vec: y's and out's rows lie at 16 bytes.
+struct LoraTarget {
+  const void* a;
+  const void* b;
+  const float* scales;  // may be null: 1
+  const float* y;
+  float* out;  // y itself, or apart from it
+  float* mid;
+  int64_t n, ldy, ldo;
+  int rank;
+  bool vec;
+};
+struct LoraArgs {
+  LoraTarget t[kMaxTargets];
+  const void* x;
+  const int32_t* ids;
+  int64_t xs, k, rows;
+  int count, slots, splits;
+  bool x_vec;  // x's rows lie at 16 bytes
+};
+int lora_most_rank();
+size_t lora_plan(LoraArgs& a, void* ws, int cus);
+hipError_t launch_lora(const LoraArgs& a, int xdt, int wdt, hipStream_t st);
+
+// One token a row from its logits (sample.hip). Settings may be null (off).
+struct SampleArgs {
+  const void* logits;
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int32_t* ids;
+  float* probs;  // may be null
+  float* maxima;   // workspace: [rows][4 chunks] the groups' largest logits
+  double* masses;  // and [rows][chunks] the chunks' weights
+  int64_t stride;
+  int rows, vocab;
+  bool vec;  // the logits' rows lie at 4 values
+};
+int64_t sample_most_vocab();
+size_t sample_plan(SampleArgs& a, void* ws);
+hipError_t launch_sample(const SampleArgs& a, int dtype, hipStream_t st);
+
 // Set-up a first launch would otherwise do (qmm_prepare): the LDS limit of
 // every kernel that asks for more than 64 KiB, on the current device, and
 // the no-allocation scratch's address there.
