@@ -16,26 +16,57 @@ namespace {
 
 typedef float f4v __attribute__((ext_vector_type(4)));
 
-// Values [i, i + N) of an array of type T, N * its size a multiple of 8 bytes.
-// VEC: at 8 * that size's alignment; otherwise a value at a time.
-template <int T, int N, bool VEC>
-__device__ __forceinline__ void load_values(const void* p, int64_t i, float* v) {
-#pragma unroll
-  for (int e = 0; e < N; e += 4) load4<T, VEC>(p, i + e, v + e);
-}
+constexpr int kMostRank = 128;
 
-// The rows of a tile that `id` holds: lanes whose row is of the adapter next in
-// turn. `left` has a bit for each of the tile's 16 rows still to be served.
-struct Turn {
-  uint32_t left;
-  __device__ __forceinline__ explicit Turn(int id) { left = (uint32_t)__ballot(id >= 0) & 0xFFFFu; }
-  // the next adapter (the same for the wave), its rows taken off
-  __device__ __forceinline__ int next(int id) {
-    const int a = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-    left &= ~(uint32_t)__ballot(id == a);
-    return a;
+// 8 values as they lie in memory, on their way to registers.
+template <int T>
+struct Raw {
+  uint4 u[T == QMM_X_F32 ? 2 : 1];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if (VEC) {
+      const uint4* q = (const uint4*)((const char*)p + i * (T == QMM_X_F32 ? 4 : 2));
+      u[0] = q[0];
+      if (T == QMM_X_F32) u[sizeof(u) / 16 - 1] = q[1];
+    } else if (T == QMM_X_F32) {
+      const uint32_t* q = (const uint32_t*)p + i;
+      u[0] = make_uint4(q[0], q[1], q[2], q[3]);
+      u[sizeof(u) / 16 - 1] = make_uint4(q[4], q[5], q[6], q[7]);
+    } else {
+      const uint16_t* q = (const uint16_t*)p + i;
+      u[0] = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16,
+                        q[6] | (uint32_t)q[7] << 16);
+    }
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (T == QMM_X_F32) {
+        const uint4 h = u[sizeof(u) / 16 - 1];
+        const uint32_t z[4] = {h.x, h.y, h.z, h.w};
+        v[e] = __uint_as_float(w[e]);
+        v[4 + e] = __uint_as_float(z[e]);
+      } else {
+        v[2 * e] = widen<T>(w[e] & 0xFFFFu);
+        v[2 * e + 1] = widen<T>(w[e] >> 16);
+      }
+    }
   }
 };
+
+// Values [i, i + N) of an array of type T, N 4 or 8. VEC: at an address that is
+// a multiple of their size (of 16 bytes at most); otherwise a value at a time.
+template <int T, int N, bool VEC>
+__device__ __forceinline__ void load_values(const void* p, int64_t i, float* v) {
+  if constexpr (N == 8) {
+    Raw<T> r;
+    r.template load<VEC>(p, i);
+    r.values(v);
+  } else {
+    load4<T, VEC>(p, i, v);
+  }
+}
 
 // The adapter of row r, -1 without one.
 __device__ __forceinline__ int id_of(const LoraArgs& a, int64_t r) {
@@ -43,157 +74,400 @@ __device__ __forceinline__ int id_of(const LoraArgs& a, int64_t r) {
   return id >= 0 && id < a.slots ? id : -1;
 }
 
-constexpr int kDownWaves = 4;
+// ---- rows one by one (decode batches: few rows of one adapter) --------------
 
-// 16 rows x all ranks over one part of k: lane (row, g) holds ranks 4 g .. 4 g + 3 of each 16.
+// The products of a row of x with `J` rows of A, rows `lda` apart, over the
+// 8-value units first, first + step, ... of k; lanes take units in turn.
+template <int XT, int WT, bool VEC, int J>
+__device__ __forceinline__ void dots(const void* x, int64_t xi, const void* w, int64_t wi, int64_t lda, int first, int step,
+                                     int units, float* sum) {
+#pragma unroll
+  for (int j = 0; j < J; j++) sum[j] = 0.0f;
+#pragma unroll 4
+  for (int u = first; u < units; u += step) {
+    float v[8];
+    load_values<XT, 8, VEC>(x, xi + 8 * u, v);
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      float a[8];
+      load_values<WT, 8, true>(w, wi + j * lda + 8 * u, a);
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum[j] = fmaf(a[e], v[e], sum[j]);
+    }
+  }
+}
+
+constexpr int kRowThreads = 512, kRowOut = 1024;
+
+// kRowOut outputs of one row. FUSED: with the row's products with A, which each
+// workgroup of the row makes for itself; otherwise they come from mid.
+template <int XT, int WT, bool VEC, bool FUSED>
+__global__ __launch_bounds__(kRowThreads) void lora_row_kernel(LoraArgs a) {
+  __shared__ float s_mid[kMostRank];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const LoraTarget& t = a.t[blockIdx.z];
+  const int64_t n0 = (int64_t)blockIdx.x * kRowOut, row = blockIdx.y;
+  if (n0 >= t.n) return;
+  const int id = id_of(a, row);
+  if (id >= 0) {
+    const float scale = t.scales ? t.scales[id] : 1.0f;
+    if (FUSED) {
+      constexpr int J = 2;  // of a multiple of 8
+      for (int j = J * wave; j < t.rank; j += J * (kRowThreads / 64)) {
+        float sum[J];
+        dots<XT, WT, VEC, J>(a.x, row * a.xs, t.a, ((int64_t)id * t.rank + j) * a.k, a.k, lane, 64, (int)(a.k / 8), sum);
+#pragma unroll
+        for (int i = 0; i < J; i++) {
+          const float v = wave_sum(sum[i]);
+          if (lane == 0) s_mid[j + i] = v * scale;
+        }
+      }
+    } else {
+      for (int j = tid; j < t.rank; j += kRowThreads) s_mid[j] = t.mid[row * t.rank + j] * scale;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kRowOut / kRowThreads; i++) {
+    const int64_t n = n0 + i * kRowThreads + tid;
+    if (n >= t.n) break;
+    float v = t.y[row * t.ldy + n];
+    if (id >= 0) {
+      const int64_t at = ((int64_t)id * t.n + n) * t.rank;
+      float sum = 0.0f;
+#pragma unroll 2
+      for (int j = 0; j < t.rank; j += 8) {
+        float b[8];
+        load_values<WT, 8, true>(t.b, at + j, b);
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fmaf(b[e], s_mid[j + e], sum);
+      }
+      v += sum;
+    } else if (t.y == t.out) {
+      return;
+    }
+    t.out[row * t.ldo + n] = v;
+  }
+}
+
+// A row's products with 4 rows of A, k dealt to the workgroup's waves.
+template <int XT, int WT, bool VEC>
+__global__ __launch_bounds__(256) void lora_row_down_kernel(LoraArgs a) {
+  constexpr int J = 4;
+  __shared__ float s_part[4][J];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const LoraTarget& t = a.t[blockIdx.z];
+  const int64_t row = blockIdx.y;
+  const int j0 = J * blockIdx.x, id = id_of(a, row);
+  if (j0 >= t.rank || id < 0) return;
+  float sum[J];
+  dots<XT, WT, VEC, J>(a.x, row * a.xs, t.a, ((int64_t)id * t.rank + j0) * a.k, a.k, threadIdx.x, 256, (int)(a.k / 8), sum);
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const float v = wave_sum(sum[j]);
+    if (lane == 0) s_part[wave][j] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < J)
+    t.mid[row * t.rank + j0 + threadIdx.x] =
+        (s_part[0][threadIdx.x] + s_part[1][threadIdx.x]) + (s_part[2][threadIdx.x] + s_part[3][threadIdx.x]);
+}
+
+// ---- tiles of rows on the matrix cores (prompts) ----------------------------
+
+constexpr int kTile = 32, kMostSlots = 4096;
+constexpr int down_waves(int rt) { return rt > 4 ? 4 : 8; }  // 64 KiB of LDS where they join
+
+// Rows with one adapter together, in tiles of kTile: a tile's adapter in whose
+// (-1: rows without one; kNoTile: past the last tile), its rows in order (-1:
+// none). Which place a row has in its adapter's tiles does not matter: a row's
+// results come from its own column of the matrix products.
+constexpr int kNoTile = -2;
+__global__ __launch_bounds__(1024) void lora_tiles_kernel(LoraArgs a, int tiles, int with_none) {
+  extern __shared__ int32_t s_count[];  // [slots + 1] rows of an adapter, then the places given out
+  int32_t* const s_first = s_count + a.slots + 1;  // [slots + 1] its first tile
+  __shared__ int32_t s_waves[16];
+  const int n = a.slots + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < n; i += 1024) s_count[i] = 0;
+  __syncthreads();
+  for (int64_t r = tid; r < a.rows; r += 1024) {
+    const int id = id_of(a, r);
+    if (id >= 0 || with_none) atomicAdd(&s_count[id >= 0 ? id : a.slots], 1);
+  }
+  __syncthreads();
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += 1024) {
+    const int i = i0 + tid, count = i < n ? s_count[i] : 0, mine = (count + kTile - 1) / kTile;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += up;
+    }
+    if (lane == 63) s_waves[wave] = sum;
+    __syncthreads();
+    int before = base, all = 0;
+    for (int w = 0; w < 16; w++) {
+      if (w < wave) before += s_waves[w];
+      all += s_waves[w];
+    }
+    const int first = before + sum - mine;
+    if (i < n) {
+      s_first[i] = first;
+      s_count[i] = 0;
+      for (int t = 0; t < mine; t++) a.whose[first + t] = i < a.slots ? i : -1;
+      for (int r = count; r < mine * kTile; r++) a.order[first * kTile + r] = -1;
+    }
+    base += all;
+    __syncthreads();
+  }
+  for (int t = base + tid; t < tiles; t += 1024) a.whose[t] = kNoTile;
+  for (int64_t r = tid; r < a.rows; r += 1024) {
+    const int id = id_of(a, r);
+    if (id < 0 && !with_none) continue;
+    const int i = id >= 0 ? id : a.slots;
+    a.order[s_first[i] * kTile + atomicAdd(&s_count[i], 1)] = (int32_t)r;
+  }
+}
+
+// A tile's rows x all ranks over one part of k, its steps of 32 dealt to the
+// waves: lane (row, g) holds ranks 4 g .. 4 g + 3 of each 16 for rows `col` and
+// 16 + col.
 template <int XT, int WT, int RT, bool VEC>
-__global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs a) {
-  constexpr int R = 16 * RT;
-  __shared__ float s_part[kDownWaves][16][R + 4];
+__global__ __launch_bounds__(64 * down_waves(RT)) void lora_down_kernel(LoraArgs a) {
+  constexpr int R = 16 * RT, W = down_waves(RT);
+  __shared__ float s_part[W][16][R + 4];
+  const int who = a.whose[blockIdx.x];
+  if (who < 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const LoraTarget& t = a.t[blockIdx.z];
-  const int64_t row = (int64_t)blockIdx.x * 16 + col;
-  const int id = id_of(a, row);
+  const int32_t* rows = a.order + (int64_t)blockIdx.x * kTile;
   const int64_t steps = a.k / 32;
   const int64_t begin = steps * blockIdx.y / a.splits, end = steps * (blockIdx.y + 1) / a.splits;
-  const int64_t xrow = (row < a.rows ? row : a.rows - 1) * a.xs;
-  for (Turn turn(id); turn.left;) {
-    const int who = turn.next(id);
-    f4v acc[RT];
+  int64_t xrow[2], arow[RT];
 #pragma unroll
-    for (int i = 0; i < RT; i++) acc[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t s = begin + wave; s < end; s += kDownWaves) {
-      const int64_t e = 32 * s + 8 * g;
-      float x[8];
-      load_values<XT, 8, VEC>(a.x, xrow + e, x);
+  for (int h = 0; h < 2; h++) xrow[h] = (int64_t)max(0, rows[16 * h + col]) * a.xs + 8 * g;
 #pragma unroll
-      for (int i = 0; i < RT; i++) {
-        float w[8];
-        const int j = 16 * i + col;
-        load_values<WT, 8, true>(t.a, ((int64_t)who * t.rank + (j < t.rank ? j : t.rank - 1)) * a.k + e, w);
-#pragma unroll
-        for (int q = 0; q < 8; q++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[q], x[q], acc[i], 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < RT; i++) *(f4v*)&s_part[wave][col][16 * i + 4 * g] = acc[i];
-    __syncthreads();
-    for (int x = threadIdx.x; x < 16 * R; x += 64 * kDownWaves) {
-      const int r = x / R, j = x - r * R;
-      const int64_t at = (int64_t)blockIdx.x * 16 + r;
-      if (j < t.rank && id_of(a, at) == who) {
-        float v = s_part[0][r][j];
-#pragma unroll
-        for (int w = 1; w < kDownWaves; w++) v += s_part[w][r][j];
-        t.mid[(blockIdx.y * a.rows + at) * t.rank + j] = v;
-      }
-    }
-    __syncthreads();
+  for (int i = 0; i < RT; i++) {
+    const int j = 16 * i + col;
+    arow[i] = ((int64_t)who * t.rank + (j < t.rank ? j : t.rank - 1)) * a.k + 8 * g;
   }
-}
-
-constexpr int kUpWaves = 4, kUpTiles = 4;
-
-// 16 rows x 64 outputs a wave: lane (row, g) holds outputs 4 g .. 4 g + 3 of each 16.
-template <int WT, int RT>
-__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const LoraTarget& t = a.t[blockIdx.z];
-  const int64_t n0 = ((int64_t)blockIdx.x * kUpWaves + wave) * 16 * kUpTiles;
-  if (n0 >= t.n) return;
-  const int64_t row = (int64_t)blockIdx.y * 16 + col;
-  const int id = id_of(a, row);
-  const bool in = row < a.rows;
-  f4v y[kUpTiles];
+  f4v acc[2][RT];
 #pragma unroll
-  for (int i = 0; i < kUpTiles; i++) {
-    const int64_t n = n0 + 16 * i + 4 * g;
-    y[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-    if (!in) continue;
-    if (t.vec && n + 4 <= t.n) {
-      y[i] = *(const f4v*)(t.y + row * t.ldy + n);
-    } else {
+  for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int v = 0; v < 4; v++)
-        if (n + v < t.n) y[i][v] = t.y[row * t.ldy + n + v];
-    }
-  }
-  for (Turn turn(id); turn.left;) {
-    const int who = turn.next(id);
-    const float scale = t.scales ? t.scales[who] : 1.0f;
-    f4v acc[kUpTiles];
+    for (int i = 0; i < RT; i++) acc[h][i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+  // two steps in flight; past the last one it is loaded again
+  Raw<XT> x[2][2];
+  Raw<WT> w[2][RT];
+  auto load = [&](int b, int64_t s) {
+    s = s < end ? s : end - 1;
 #pragma unroll
-    for (int i = 0; i < kUpTiles; i++) acc[i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int h = 0; h < 2; h++) x[b][h].template load<VEC>(a.x, xrow[h] + 32 * s);
+#pragma unroll
+    for (int i = 0; i < RT; i++) w[b][i].template load<true>(t.a, arow[i] + 32 * s);
+  };
+  auto multiply = [&](int b) {
+    float xv[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; h++) x[b][h].values(xv[h]);
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-      const int j = 16 * i + 4 * g;
-      if (16 * i >= t.rank) break;
-      f4v m = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (id == who && j < t.rank) {
-        for (int s = 0; s < a.splits; s++) m += *(const f4v*)(t.mid + (s * a.rows + row) * t.rank + j);
-        m *= scale;
-      }
+      float wv[8];
+      w[b][i].values(wv);
 #pragma unroll
-      for (int c = 0; c < kUpTiles; c++) {
-        const int64_t n = n0 + 16 * c + col;
-        float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j < t.rank && n < t.n) load4<WT, true>(t.b, ((int64_t)who * t.n + n) * t.rank + j, w);
+      for (int q = 0; q < 8; q++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[q], m[q], acc[c], 0, 0, 0);
-      }
+        for (int h = 0; h < 2; h++)
+          acc[h][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[q], xv[h][q], acc[h][i], 0, 0, 0);
     }
-    // an adapter's values reach its own rows only
-    if (id == who) {
-#pragma unroll
-      for (int i = 0; i < kUpTiles; i++) y[i] += acc[i];
-    }
+  };
+  if (begin + wave < end) load(0, begin + wave);
+  for (int64_t s = begin + wave; s < end; s += 2 * W) {
+    load(1, s + W);
+    multiply(0);
+    load(0, s + 2 * W);
+    if (s + W < end) multiply(1);
   }
-  if (!in || (id < 0 && t.y == t.out)) return;
 #pragma unroll
-  for (int i = 0; i < kUpTiles; i++) {
-    const int64_t n = n0 + 16 * i + 4 * g;
-    if (t.vec && n + 4 <= t.n) {
-      *(f4v*)(t.out + row * t.ldo + n) = y[i];
-    } else {
+  for (int h = 0; h < 2; h++) {
+    if (h) __syncthreads();
 #pragma unroll
-      for (int v = 0; v < 4; v++)
-        if (n + v < t.n) t.out[row * t.ldo + n + v] = y[i][v];
+    for (int i = 0; i < RT; i++) *(f4v*)&s_part[wave][col][16 * i + 4 * g] = acc[h][i];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 16 * R; at += 64 * W) {
+      const int r = at / R, j = at - r * R, row = rows[16 * h + r];
+      if (row >= 0 && j < t.rank) {
+        float v = s_part[0][r][j];
+#pragma unroll
+        for (int q = 1; q < W; q++) v += s_part[q][r][j];
+        t.mid[(blockIdx.y * a.rows + row) * t.rank + j] = v;
+      }
     }
   }
 }
 
-int64_t tiles_of(int64_t rows) { return (rows + 15) / 16; }
+// The parts of k added, in the first one's place.
+__global__ __launch_bounds__(256) void lora_join_kernel(LoraArgs a) {
+  const LoraTarget& t = a.t[blockIdx.y];
+  const int64_t n = a.rows * t.rank, i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (i >= n) return;
+  f4v v = *(const f4v*)(t.mid + i);
+#pragma unroll 4
+  for (int s = 1; s < a.splits; s++) v += *(const f4v*)(t.mid + s * n + i);
+  *(f4v*)(t.mid + i) = v;
+}
 
+constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlocks = 2;
+
+__device__ __forceinline__ f4v load_row4(const LoraTarget& t, const float* p, int64_t n) {
+  if (t.vec && n + 4 <= t.n) return *(const f4v*)(p + n);
+  f4v y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int v = 0; v < 4; v++)
+    if (n + v < t.n) y[v] = p[n + v];
+  return y;
+}
+__device__ __forceinline__ void store_row4(const LoraTarget& t, float* p, int64_t n, f4v y) {
+  if (t.vec && n + 4 <= t.n) {
+    *(f4v*)(p + n) = y;
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < 4; v++)
+    if (n + v < t.n) p[n + v] = y[v];
+}
+
+// A tile's rows x 64 outputs a wave at a time, kUpBlocks times: lane (row, g)
+// holds outputs 4 g .. 4 g + 3 of each 16 for rows `col` and 16 + col, and takes
+// the ranks U g .. U g + U - 1 of each of S runs of 4 U.
+template <int WT, int U, int S>
+__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a) {
+  const int who = a.whose[blockIdx.y];
+  const LoraTarget& t = a.t[blockIdx.z];
+  if (who == kNoTile || (who < 0 && t.y == t.out)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int64_t first = ((int64_t)blockIdx.x * kUpBlocks * kUpWaves + wave) * 16 * kUpTiles;
+  const int32_t* rows = a.order + (int64_t)blockIdx.y * kTile;
+  const int64_t row[2] = {rows[col], rows[16 + col]};
+  const float scale = who >= 0 && t.scales ? t.scales[who] : 1.0f;
+  float m[2][S][U];
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      const int j = 4 * U * s + U * g;
+      if (who >= 0 && row[h] >= 0 && j < t.rank) {
+        load_values<QMM_X_F32, U, true>(t.mid, row[h] * t.rank + j, m[h][s]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < U; q++) m[h][s][q] = 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < U; q++) m[h][s][q] *= scale;
+    }
+  for (int blk = 0; blk < kUpBlocks; blk++) {
+    const int64_t n0 = first + (int64_t)blk * kUpWaves * 16 * kUpTiles;
+    if (n0 >= t.n) break;
+    f4v y[2][kUpTiles];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int c = 0; c < kUpTiles; c++)
+        y[h][c] = row[h] >= 0 ? load_row4(t, t.y + row[h] * t.ldy, n0 + 16 * c + 4 * g) : f4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < kUpTiles; c++) {
+      f4v acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      if (who >= 0) {
+        const int64_t n = n0 + 16 * c + col, at = ((int64_t)who * t.n + (n < t.n ? n : t.n - 1)) * t.rank;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          const int j = 4 * U * s + U * g;
+          float w[U];
+          load_values<WT, U, true>(t.b, at + (j < t.rank ? j : 0), w);
+          if (j >= t.rank) {
+#pragma unroll
+            for (int q = 0; q < U; q++) w[q] = 0.0f;
+          }
+#pragma unroll
+          for (int q = 0; q < U; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[q], m[h][s][q], acc[h], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        if (row[h] >= 0) store_row4(t, t.out + row[h] * t.ldo, n0 + 16 * c + 4 * g, y[h][c] + acc[h]);
+    }
+  }
+}
+
+// Tiles that the rows can make: whole ones, and one begun for each adapter and for none.
+int64_t tiles_of(const LoraArgs& a) {
+  return (a.rows + kTile - 1) / kTile + (a.slots + 1 < a.rows ? a.slots + 1 : a.rows);
+}
+
+// How a call runs.
+enum Form { kFused, kRows, kTiles };
+
+Form form_of(const LoraArgs& a) {
+  int rank = 0;
+  for (int i = 0; i < a.count; i++) rank = rank > a.t[i].rank ? rank : a.t[i].rank;
+  if (a.rows > 64) return kTiles;
+  return rank * a.k <= (int64_t)1 << 17 ? kFused : kRows;
+}
+
+// Parts of k: until two workgroups a CU are there, of 4 steps a wave at least.
 int splits_of(const LoraArgs& a, int cus) {
-  const int64_t groups = tiles_of(a.rows) * a.count, most = a.k / 512;
+  if (form_of(a) != kTiles) return 1;
+  const int64_t groups = (a.rows + kTile - 1) / kTile * a.count, most = a.k / 1024;
   int64_t s = 2 * cus / groups;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
-template <int XT, int WT, int RT>
-hipError_t launch_ranks(const LoraArgs& a, hipStream_t st) {
-  int64_t widest = 0;
-  for (int i = 0; i < a.count; i++) widest = widest > a.t[i].n ? widest : a.t[i].n;
-  const int64_t tiles = tiles_of(a.rows), wide = 16 * kUpTiles * kUpWaves;
-  const dim3 down((unsigned)tiles, (unsigned)a.splits, (unsigned)a.count);
-  if (a.x_vec)
-    lora_down_kernel<XT, WT, RT, true><<<down, 64 * kDownWaves, 0, st>>>(a);
-  else
-    lora_down_kernel<XT, WT, RT, false><<<down, 64 * kDownWaves, 0, st>>>(a);
-  const dim3 up((unsigned)((widest + wide - 1) / wide), (unsigned)tiles, (unsigned)a.count);
-  lora_up_kernel<WT, RT><<<up, 64 * kUpWaves, 0, st>>>(a);
+template <int XT, int WT, int RT, bool VEC>
+hipError_t launch_tiles(const LoraArgs& a, int64_t widest, int64_t rank, hipStream_t st) {
+  const int64_t tiles = tiles_of(a), wide = 16 * kUpTiles * kUpWaves * kUpBlocks;
+  int with_none = 0;
+  for (int i = 0; i < a.count; i++) with_none |= a.t[i].y != a.t[i].out;
+  lora_tiles_kernel<<<1, 1024, 2 * (a.slots + 1) * sizeof(int32_t), st>>>(a, (int)tiles, with_none);
+  lora_down_kernel<XT, WT, RT, VEC><<<dim3((unsigned)tiles, (unsigned)a.splits, (unsigned)a.count), 64 * down_waves(RT), 0, st>>>(a);
+  if (a.splits > 1)
+    lora_join_kernel<<<dim3((unsigned)((a.rows * rank + 1023) / 1024), (unsigned)a.count), 256, 0, st>>>(a);
+  constexpr int U = RT == 1 ? 4 : 8, S = RT == 1 ? 1 : RT / 2;
+  lora_up_kernel<WT, U, S><<<dim3((unsigned)((widest + wide - 1) / wide), (unsigned)tiles, (unsigned)a.count),
+                             64 * kUpWaves, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <int XT, int WT, bool VEC>
+hipError_t launch_form(const LoraArgs& a, hipStream_t st) {
+  int64_t widest = 0, rank = 0;
+  for (int i = 0; i < a.count; i++) {
+    widest = widest > a.t[i].n ? widest : a.t[i].n;
+    rank = rank > a.t[i].rank ? rank : a.t[i].rank;
+  }
+  const Form form = form_of(a);
+  if (form == kTiles) {
+    if (rank <= 16) return launch_tiles<XT, WT, 1, VEC>(a, widest, rank, st);
+    if (rank <= 32) return launch_tiles<XT, WT, 2, VEC>(a, widest, rank, st);
+    if (rank <= 64) return launch_tiles<XT, WT, 4, VEC>(a, widest, rank, st);
+    return launch_tiles<XT, WT, 8, VEC>(a, widest, rank, st);
+  }
+  const dim3 grid((unsigned)((widest + kRowOut - 1) / kRowOut), (unsigned)a.rows, (unsigned)a.count);
+  if (form == kFused) {
+    lora_row_kernel<XT, WT, VEC, true><<<grid, kRowThreads, 0, st>>>(a);
+  } else {
+    lora_row_down_kernel<XT, WT, VEC><<<dim3((unsigned)(rank / 4), (unsigned)a.rows, (unsigned)a.count), 256, 0, st>>>(a);
+    lora_row_kernel<XT, WT, VEC, false><<<grid, kRowThreads, 0, st>>>(a);
+  }
   return hipGetLastError();
 }
 
 template <int XT, int WT>
 hipError_t launch_types(const LoraArgs& a, hipStream_t st) {
-  int rank = 0;
-  for (int i = 0; i < a.count; i++) rank = rank > a.t[i].rank ? rank : a.t[i].rank;
-  if (rank <= 16) return launch_ranks<XT, WT, 1>(a, st);
-  if (rank <= 32) return launch_ranks<XT, WT, 2>(a, st);
-  if (rank <= 64) return launch_ranks<XT, WT, 4>(a, st);
-  return launch_ranks<XT, WT, 8>(a, st);
+  return a.x_vec ? launch_form<XT, WT, true>(a, st) : launch_form<XT, WT, false>(a, st);
 }
 
 template <int XT>
@@ -207,7 +481,8 @@ hipError_t launch_x(const LoraArgs& a, int wdt, hipStream_t st) {
 
 }  // namespace
 
-int lora_most_rank() { return 128; }
+int lora_most_rank() { return kMostRank; }
+int lora_most_slots() { return kMostSlots; }
 
 size_t lora_plan(LoraArgs& a, void* ws, int cus) {
   a.splits = splits_of(a, cus);
@@ -215,6 +490,12 @@ size_t lora_plan(LoraArgs& a, void* ws, int cus) {
   for (int i = 0; i < a.count; i++) {
     a.t[i].mid = (float*)((uintptr_t)ws + at);
     at += align_up((size_t)a.splits * a.rows * a.t[i].rank * sizeof(float), 16);
+  }
+  if (form_of(a) == kTiles) {
+    a.order = (int32_t*)((uintptr_t)ws + at);
+    at += tiles_of(a) * kTile * sizeof(int32_t);
+    a.whose = (int32_t*)((uintptr_t)ws + at);
+    at += align_up(tiles_of(a) * sizeof(int32_t), 16);
   }
   return at;
 }

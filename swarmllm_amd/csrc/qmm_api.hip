@@ -1137,7 +1137,7 @@ int qmm_pages_step(const qmm_pages* pages, const int32_t* keep, const int32_t* f
 int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dtype, const void* x, int x_dtype,
                      int64_t x_stride, const int32_t* ids, int64_t k, int64_t rows, void* workspace,
                      size_t workspace_bytes, size_t* need, int launch, int64_t stream) {
-  if (count < 1 || count > qmm::kMaxTargets || !adapters || slots < 0 || !qmm::value_type_ok(w_dtype) ||
+  if (count < 1 || count > qmm::kMaxTargets || !adapters || slots < 0 || slots > qmm::lora_most_slots() || !qmm::value_type_ok(w_dtype) ||
       !qmm::value_type_ok(x_dtype) || need == nullptr || k < 32 || k % 32 != 0 || k > (int64_t)1 << 30 ||
       x_stride < k || rows < 0 || rows > (int64_t)1 << 20)
     return QMM_UNSUPPORTED;

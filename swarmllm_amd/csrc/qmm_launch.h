@@ -348,11 +348,14 @@ struct LoraArgs {
   LoraTarget t[kMaxTargets];
   const void* x;
   const int32_t* ids;
+  int32_t* order;  // the rows tile by tile, and the tiles' adapters (many rows)
+  int32_t* whose;
   int64_t xs, k, rows;
   int count, slots, splits;
   bool x_vec;  // x's rows lie at 16 bytes
 };
 int lora_most_rank();
+int lora_most_slots();
 size_t lora_plan(LoraArgs& a, void* ws, int cus);
 hipError_t launch_lora(const LoraArgs& a, int xdt, int wdt, hipStream_t st);
 

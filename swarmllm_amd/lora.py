@@ -19,7 +19,7 @@ class Adapters:
     """The adapters of one projection [n, k]: a [slots, rank, k] and b [slots, n,
     rank] of one type (f32, f16 or bf16), scales [slots] f32 (None: 1). rank is a
     multiple of 8 up to 128; an adapter of a lower rank has zeros behind it. k is a
-    multiple of 32."""
+    multiple of 32, slots at most 4096."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: Optional[torch.Tensor] = None):
         if a.dim() != 3 or b.dim() != 3 or a.dtype not in _X_DTYPES or a.shape[0] != b.shape[0] \
@@ -34,9 +34,10 @@ class Adapters:
                     or t.data_ptr() % 16:
                 raise ValueError(f"Adapters: {name} must be contiguous, 16-byte aligned {a.dtype} on one GPU, not "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        if self.rank < 8 or self.rank > 128 or self.rank % 8 or self.k < 32 or self.k % 32 or self.n < 1:
-            raise ValueError(f"Adapters: rank {self.rank} (a multiple of 8 up to 128) for a projection [{self.n}, {self.k}] "
-                             "(k a multiple of 32)")
+        if self.rank < 8 or self.rank > 128 or self.rank % 8 or self.k < 32 or self.k % 32 or self.n < 1 \
+                or self.slots > 4096:
+            raise ValueError(f"Adapters: {self.slots} of rank {self.rank} (at most 4096, a multiple of 8 up to 128) for a "
+                             f"projection [{self.n}, {self.k}] (k a multiple of 32)")
         if scales is not None and (scales.dtype != torch.float32 or scales.shape != (self.slots,)
                                    or scales.device != self.device or not scales.is_contiguous()):
             raise ValueError(f"Adapters: scales must be {self.slots} contiguous f32 on {self.device}")
@@ -84,7 +85,7 @@ class Adapters:
         if rows == 0:
             return outs
         with on_device(device):
-            need = _need(device.index, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
+            need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
             ws = torch.empty(need, dtype=torch.uint8, device=device)
@@ -107,12 +108,12 @@ def _rows(name: str, t: torch.Tensor, width: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _need(device: int, k: int, rows: int, sizes: Tuple[Tuple[int, int], ...]) -> int:
+def _need(device: int, slots: int, k: int, rows: int, sizes: Tuple[Tuple[int, int], ...]) -> int:
     """The workspace bytes that qmm_adapters_add plans on the current device (`device`): by the sizes alone."""
     c, need = (Adapter * len(sizes))(), ctypes.c_size_t(0)
     for i, (n, rank) in enumerate(sizes):
         c[i] = Adapter(None, None, None, None, None, n, n, n, rank)
-    check("qmm_adapters_add", lib().qmm_adapters_add(len(sizes), c, 1, _X_DTYPES[torch.float32], None,
+    check("qmm_adapters_add", lib().qmm_adapters_add(len(sizes), c, slots, _X_DTYPES[torch.float32], None,
                                                      _X_DTYPES[torch.float32], k, None, k, rows, None, 0,
                                                      ctypes.byref(need), 0, 0))
     return need.value
