@@ -38,6 +38,10 @@ struct Raw {
                         q[6] | (uint32_t)q[7] << 16);
     }
   }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(u) / 16); i++) u[i] = make_uint4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ void values(float* v) const {
     const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
 #pragma unroll
@@ -54,6 +58,40 @@ struct Raw {
     }
   }
 };
+
+// A value as a sum of bf16 ones, each the leading 8 bits of what those before it
+// leave: 1 for a bf16 value, 2 for f16, 3 for f32, and nothing left.
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+template <int T>
+constexpr int kPieces = T == QMM_X_BF16 ? 1 : T == QMM_X_F16 ? 2 : 3;
+// the upper halves of a and b, side by side
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+template <int N>
+__device__ __forceinline__ void pieces_of(float v[8], b8v out[N]) {
+#pragma unroll
+  for (int p = 0; p < N; p++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = upper_halves(v[2 * e], v[2 * e + 1]);
+    out[p] = __builtin_bit_cast(b8v, make_uint4(w[0], w[1], w[2], w[3]));
+    if (p + 1 < N) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+    }
+  }
+}
+template <int T>
+__device__ __forceinline__ void pieces_of(const Raw<T>& r, b8v out[kPieces<T>]) {
+  if constexpr (T == QMM_X_BF16) {
+    out[0] = __builtin_bit_cast(b8v, r.u[0]);
+  } else {
+    float v[8];
+    r.values(v);
+    pieces_of<kPieces<T>>(v, out);
+  }
+}
 
 // Values [i, i + N) of an array of type T, N 4 or 8. VEC: at an address that is
 // a multiple of their size (of 16 bytes at most); otherwise a value at a time.
@@ -176,13 +214,34 @@ __global__ __launch_bounds__(256) void lora_row_down_kernel(LoraArgs a) {
 // ---- tiles of rows on the matrix cores (prompts) ----------------------------
 
 constexpr int kTile = 32, kMostSlots = 4096;
-constexpr int down_waves(int rt) { return rt > 4 ? 4 : 8; }  // 64 KiB of LDS where they join
+// Waves of a down workgroup: few where registers leave a CU 12 waves or fewer (two
+// workgroups of 8 would not fit, three of 4 do), and as 64 KiB of LDS allow.
+constexpr int down_waves(int rt, int wt) { return rt > 4 && wt == QMM_X_F32 ? 2 : rt > 1 ? 4 : 8; }
 
 // Rows with one adapter together, in tiles of kTile: a tile's adapter in whose
 // (-1: rows without one; kNoTile: past the last tile), its rows in order (-1:
 // none). Which place a row has in its adapter's tiles does not matter: a row's
 // results come from its own column of the matrix products.
-constexpr int kNoTile = -2;
+constexpr int kNoTile = -2, kEarly = 4;
+
+// A place among the rows of adapter id (-1: none is wanted), one addition for
+// each adapter that a wave's rows have.
+__device__ __forceinline__ int take_places(int id, int32_t* count) {
+  const int lane = threadIdx.x & 63;
+  int place = -1;
+  uint64_t left = __ballot(id >= 0);
+  while (left) {
+    const int lead = __builtin_ctzll(left), who = __builtin_amdgcn_readlane(id, lead);
+    const uint64_t same = __ballot(id == who);
+    int first = 0;
+    if (lane == lead) first = atomicAdd(&count[who], __popcll(same));
+    first = __builtin_amdgcn_readlane(first, lead);
+    if (id == who) place = first + __popcll(same & (((uint64_t)1 << lane) - 1));
+    left &= ~same;
+  }
+  return place;
+}
+
 __global__ __launch_bounds__(1024) void lora_tiles_kernel(LoraArgs a, int tiles, int with_none) {
   extern __shared__ int32_t s_count[];  // [slots + 1] rows of an adapter, then the places given out
   int32_t* const s_first = s_count + a.slots + 1;  // [slots + 1] its first tile
@@ -190,10 +249,16 @@ __global__ __launch_bounds__(1024) void lora_tiles_kernel(LoraArgs a, int tiles,
   const int n = a.slots + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < n; i += 1024) s_count[i] = 0;
   __syncthreads();
-  for (int64_t r = tid; r < a.rows; r += 1024) {
+  auto id_at = [&](int64_t r) {
     const int id = id_of(a, r);
-    if (id >= 0 || with_none) atomicAdd(&s_count[id >= 0 ? id : a.slots], 1);
-  }
+    return id < 0 && with_none && r < a.rows ? a.slots : id;
+  };
+  int early[kEarly];  // the ids of the first rows, read once
+#pragma unroll
+  for (int e = 0; e < kEarly; e++) early[e] = id_at(e * 1024 + tid);
+#pragma unroll
+  for (int e = 0; e < kEarly; e++) (void)take_places(early[e], s_count);
+  for (int64_t r = kEarly * 1024; r < a.rows; r += 1024) (void)take_places(id_at(r + tid), s_count);
   __syncthreads();
   int base = 0;
   for (int i0 = 0; i0 < n; i0 += 1024) {
@@ -222,35 +287,62 @@ __global__ __launch_bounds__(1024) void lora_tiles_kernel(LoraArgs a, int tiles,
     __syncthreads();
   }
   for (int t = base + tid; t < tiles; t += 1024) a.whose[t] = kNoTile;
-  for (int64_t r = tid; r < a.rows; r += 1024) {
-    const int id = id_of(a, r);
-    if (id < 0 && !with_none) continue;
-    const int i = id >= 0 ? id : a.slots;
-    a.order[s_first[i] * kTile + atomicAdd(&s_count[i], 1)] = (int32_t)r;
+  auto put = [&](int64_t r, int id) {
+    const int place = take_places(id, s_count);
+    if (place >= 0) a.order[s_first[id] * kTile + place] = (int32_t)r;
+  };
+#pragma unroll
+  for (int e = 0; e < kEarly; e++) put(e * 1024 + tid, early[e]);
+  for (int64_t r = kEarly * 1024; r < a.rows; r += 1024) put(r + tid, id_at(r + tid));
+}
+
+// 16 bytes of a row.
+template <int T, bool VEC>
+__device__ __forceinline__ uint4 load16(const void* p, int64_t i) {
+  if (VEC) return *(const uint4*)((const char*)p + i * (T == QMM_X_F32 ? 4 : 2));
+  if (T == QMM_X_F32) {
+    const uint32_t* q = (const uint32_t*)p + i;
+    return make_uint4(q[0], q[1], q[2], q[3]);
   }
+  const uint16_t* q = (const uint16_t*)p + i;
+  return make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16,
+                    q[6] | (uint32_t)q[7] << 16);
 }
 
 // A tile's rows x all ranks over one part of k, its steps of 32 dealt to the
 // waves: lane (row, g) holds ranks 4 g .. 4 g + 3 of each 16 for rows `col` and
-// 16 + col.
+// 16 + col. x and A come in whole lines (consecutive lanes in one row) and change
+// lanes in LDS of the wave's own: loaded as the products take them, a lane a row,
+// every 16 bytes were a line looked up.
 template <int XT, int WT, int RT, bool VEC>
-__global__ __launch_bounds__(64 * down_waves(RT)) void lora_down_kernel(LoraArgs a) {
-  constexpr int R = 16 * RT, W = down_waves(RT);
-  __shared__ float s_part[W][16][R + 4];
-  const int who = a.whose[blockIdx.x];
+__global__ __launch_bounds__(64 * down_waves(RT, WT)) void lora_down_kernel(LoraArgs a, int tiles) {
+  constexpr int R = 16 * RT, W = down_waves(RT, WT);
+  // 16-byte chunks of a row's step, and loads a lane
+  constexpr int C = XT == QMM_X_F32 ? 8 : 4, I = kTile * C / 64, WC = WT == QMM_X_F32 ? 8 : 4, WI = R * WC / 64;
+  constexpr int kWaveBytes = 16 * (kTile * (C + 1) + R * (WC + 1)), kPartBytes = 16 * (R + 4) * 4;
+  __shared__ __attribute__((aligned(16))) char s_mem[W * (kWaveBytes > kPartBytes ? kWaveBytes : kPartBytes)];
+  uint4 (*const s_x)[C + 1] = (uint4 (*)[C + 1])(s_mem + kWaveBytes * (threadIdx.x >> 6));
+  uint4 (*const s_w)[WC + 1] = (uint4 (*)[WC + 1])(s_x + kTile);
+  float (*const s_part)[16][R + 4] = (float (*)[16][R + 4]) s_mem;
+  // parts of k in eights: a part's tiles one after another on one XCD, whose L2 then holds the part's A
+  const int turn = blockIdx.x >> 3;
+  const int tile = a.splits % 8 ? (int)blockIdx.x % tiles : turn % tiles;
+  const int part = a.splits % 8 ? (int)blockIdx.x / tiles : (int)(blockIdx.x & 7) + 8 * (turn / tiles);
+  const int who = a.whose[tile];
   if (who < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const LoraTarget& t = a.t[blockIdx.z];
-  const int32_t* rows = a.order + (int64_t)blockIdx.x * kTile;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const LoraTarget& t = a.t[blockIdx.y];
+  const int32_t* rows = a.order + (int64_t)tile * kTile;
   const int64_t steps = a.k / 32;
-  const int64_t begin = steps * blockIdx.y / a.splits, end = steps * (blockIdx.y + 1) / a.splits;
-  int64_t xrow[2], arow[RT];
+  const int64_t begin = steps * part / a.splits, end = steps * (part + 1) / a.splits;
+  int64_t xrow[I], arow[WI];
 #pragma unroll
-  for (int h = 0; h < 2; h++) xrow[h] = (int64_t)max(0, rows[16 * h + col]) * a.xs + 8 * g;
+  for (int i = 0; i < I; i++)
+    xrow[i] = (int64_t)max(0, rows[64 / C * i + lane / C]) * a.xs + 32 / C * (lane % C);
 #pragma unroll
-  for (int i = 0; i < RT; i++) {
-    const int j = 16 * i + col;
-    arow[i] = ((int64_t)who * t.rank + (j < t.rank ? j : t.rank - 1)) * a.k + 8 * g;
+  for (int i = 0; i < WI; i++) {
+    const int j = 64 / WC * i + lane / WC;
+    arow[i] = ((int64_t)who * t.rank + (j < t.rank ? j : t.rank - 1)) * a.k + 32 / WC * (lane % WC);
   }
   f4v acc[2][RT];
 #pragma unroll
@@ -258,32 +350,52 @@ __global__ __launch_bounds__(64 * down_waves(RT)) void lora_down_kernel(LoraArgs
 #pragma unroll
     for (int i = 0; i < RT; i++) acc[h][i] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
   // two steps in flight; past the last one it is loaded again
-  Raw<XT> x[2][2];
-  Raw<WT> w[2][RT];
+  uint4 x[2][I];
+  uint4 w[2][WI];
   auto load = [&](int b, int64_t s) {
     s = s < end ? s : end - 1;
 #pragma unroll
-    for (int h = 0; h < 2; h++) x[b][h].template load<VEC>(a.x, xrow[h] + 32 * s);
+    for (int i = 0; i < I; i++) x[b][i] = load16<XT, VEC>(a.x, xrow[i] + 32 * s);
 #pragma unroll
-    for (int i = 0; i < RT; i++) w[b][i].template load<true>(t.a, arow[i] + 32 * s);
+    for (int i = 0; i < WI; i++) w[b][i] = load16<WT, true>(t.a, arow[i] + 32 * s);
   };
+  // products of pieces down to 2^-16 of the first (the next are under f32's half step)
   auto multiply = [&](int b) {
-    float xv[2][8];
 #pragma unroll
-    for (int h = 0; h < 2; h++) x[b][h].values(xv[h]);
+    for (int i = 0; i < I; i++) s_x[64 / C * i + lane / C][lane % C] = x[b][i];
+#pragma unroll
+    for (int i = 0; i < WI; i++) s_w[64 / WC * i + lane / WC][lane % WC] = w[b][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    b8v xp[2][kPieces<XT>];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      Raw<XT> r;
+#pragma unroll
+      for (int u = 0; u < C / 4; u++) r.u[u] = s_x[16 * h + col][C / 4 * g + u];
+      pieces_of<XT>(r, xp[h]);
+    }
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-      float wv[8];
-      w[b][i].values(wv);
+      Raw<WT> r;
 #pragma unroll
-      for (int q = 0; q < 8; q++)
+      for (int u = 0; u < WC / 4; u++) r.u[u] = s_w[16 * i + col][WC / 4 * g + u];
+      b8v wp[kPieces<WT>];
+      pieces_of<WT>(r, wp);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-          acc[h][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[q], xv[h][q], acc[h][i], 0, 0, 0);
+      for (int p = 0; p < kPieces<WT>; p++)
+#pragma unroll
+        for (int q = 0; q < kPieces<XT>; q++)
+          if (p + q < 3) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+              acc[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[p], xp[h][q], acc[h][i], 0, 0, 0);
+          }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  if (begin + wave < end) load(0, begin + wave);
-  for (int64_t s = begin + wave; s < end; s += 2 * W) {
+  const int64_t mine = begin + wave;
+  if (mine < end) load(0, mine);
+  for (int64_t s = mine; s < end; s += 2 * W) {
     load(1, s + W);
     multiply(0);
     load(0, s + 2 * W);
@@ -291,7 +403,7 @@ __global__ __launch_bounds__(64 * down_waves(RT)) void lora_down_kernel(LoraArgs
   }
 #pragma unroll
   for (int h = 0; h < 2; h++) {
-    if (h) __syncthreads();
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < RT; i++) *(f4v*)&s_part[wave][col][16 * i + 4 * g] = acc[h][i];
     __syncthreads();
@@ -301,7 +413,7 @@ __global__ __launch_bounds__(64 * down_waves(RT)) void lora_down_kernel(LoraArgs
         float v = s_part[0][r][j];
 #pragma unroll
         for (int q = 1; q < W; q++) v += s_part[q][r][j];
-        t.mid[(blockIdx.y * a.rows + row) * t.rank + j] = v;
+        t.mid[(part * a.rows + row) * t.rank + j] = v;
       }
     }
   }
@@ -318,10 +430,10 @@ __global__ __launch_bounds__(256) void lora_join_kernel(LoraArgs a) {
   *(f4v*)(t.mid + i) = v;
 }
 
-constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlocks = 2;
+constexpr int kUpWaves = 4, kUpTiles = 4, kUpOut = 16 * kUpTiles * kUpWaves;
 
 __device__ __forceinline__ f4v load_row4(const LoraTarget& t, const float* p, int64_t n) {
-  if (t.vec && n + 4 <= t.n) return *(const f4v*)(p + n);
+  if (t.vec && n + 4 <= t.n) return __builtin_nontemporal_load((const f4v*)(p + n));
   f4v y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int v = 0; v < 4; v++)
@@ -330,7 +442,7 @@ __device__ __forceinline__ f4v load_row4(const LoraTarget& t, const float* p, in
 }
 __device__ __forceinline__ void store_row4(const LoraTarget& t, float* p, int64_t n, f4v y) {
   if (t.vec && n + 4 <= t.n) {
-    *(f4v*)(p + n) = y;
+    __builtin_nontemporal_store(y, (f4v*)(p + n));
     return;
   }
 #pragma unroll
@@ -338,67 +450,86 @@ __device__ __forceinline__ void store_row4(const LoraTarget& t, float* p, int64_
     if (n + v < t.n) p[n + v] = y[v];
 }
 
-// A tile's rows x 64 outputs a wave at a time, kUpBlocks times: lane (row, g)
-// holds outputs 4 g .. 4 g + 3 of each 16 for rows `col` and 16 + col, and takes
-// the ranks U g .. U g + U - 1 of each of S runs of 4 U.
-template <int WT, int U, int S>
-__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a) {
-  const int who = a.whose[blockIdx.y];
+// A tile's rows x 256 outputs, 64 a wave: lane (row, g) holds outputs 4 g .. 4 g + 3
+// of each 16 for rows `col` and 16 + col, and takes the ranks 8 g .. 8 g + 7 of
+// each of S runs of 32. They pass through LDS, so that y and out are read and
+// written a row's 1 KiB at a time, past the caches. The workgroups of one
+// range of outputs follow each other on one XCD (tiles fastest, ranges dealt to
+// the XCDs), whose L2 then holds the range's B.
+template <int WT, int S>
+__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int tiles) {
+  constexpr int P = kTile / kUpWaves, MP = kPieces<QMM_X_F32>;
+  __shared__ float s_sum[kTile][kUpOut + 4];
   const LoraTarget& t = a.t[blockIdx.z];
-  if (who == kNoTile || (who < 0 && t.y == t.out)) return;
+  const int turn = blockIdx.x >> 3, tile = turn % tiles;
+  const int64_t n0 = (int64_t)kUpOut * ((blockIdx.x & 7) + 8 * (turn / tiles));
+  const int who = a.whose[tile];
+  if (who == kNoTile || (who < 0 && t.y == t.out) || n0 >= t.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int64_t first = ((int64_t)blockIdx.x * kUpBlocks * kUpWaves + wave) * 16 * kUpTiles;
-  const int32_t* rows = a.order + (int64_t)blockIdx.y * kTile;
-  const int64_t row[2] = {rows[col], rows[16 + col]};
-  const float scale = who >= 0 && t.scales ? t.scales[who] : 1.0f;
-  float m[2][S][U];
+  const int32_t* rows = a.order + (int64_t)tile * kTile;
+  f4v y[P];
 #pragma unroll
-  for (int h = 0; h < 2; h++)
+  for (int i = 0; i < P; i++) {
+    const int64_t row = rows[kUpWaves * i + wave];
+    y[i] = row >= 0 ? load_row4(t, t.y + row * t.ldy, n0 + 4 * lane) : f4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  if (who >= 0) {
+    Raw<WT> w[kUpTiles][S];
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      const int j = 4 * U * s + U * g;
-      if (who >= 0 && row[h] >= 0 && j < t.rank) {
-        load_values<QMM_X_F32, U, true>(t.mid, row[h] * t.rank + j, m[h][s]);
-      } else {
+    for (int c = 0; c < kUpTiles; c++) {
+      const int64_t n = n0 + 16 * (kUpTiles * wave + c) + col;
+      const int64_t at = ((int64_t)who * t.n + (n < t.n ? n : t.n - 1)) * t.rank;
 #pragma unroll
-        for (int q = 0; q < U; q++) m[h][s][q] = 0.0f;
+      for (int s = 0; s < S; s++) {
+        const int j = 32 * s + 8 * g;
+        w[c][s].zero();
+        if (j < t.rank) w[c][s].template load<true>(t.b, at + j);
       }
-#pragma unroll
-      for (int q = 0; q < U; q++) m[h][s][q] *= scale;
     }
-  for (int blk = 0; blk < kUpBlocks; blk++) {
-    const int64_t n0 = first + (int64_t)blk * kUpWaves * 16 * kUpTiles;
-    if (n0 >= t.n) break;
-    f4v y[2][kUpTiles];
+    const float scale = t.scales ? t.scales[who] : 1.0f;
+    b8v m[2][S][MP];
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < 2; h++) {
+      const int64_t row = max(0, rows[16 * h + col]);
 #pragma unroll
-      for (int c = 0; c < kUpTiles; c++)
-        y[h][c] = row[h] >= 0 ? load_row4(t, t.y + row[h] * t.ldy, n0 + 16 * c + 4 * g) : f4v{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < S; s++) {
+        const int j = 32 * s + 8 * g;
+        float v[8];
+        load_values<QMM_X_F32, 8, true>(t.mid, row * t.rank + (j < t.rank ? j : 0), v);
+#pragma unroll
+        for (int q = 0; q < 8; q++) v[q] = j < t.rank ? v[q] * scale : 0.0f;
+        pieces_of<MP>(v, m[h][s]);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < kUpTiles; c++) {
       f4v acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-      if (who >= 0) {
-        const int64_t n = n0 + 16 * c + col, at = ((int64_t)who * t.n + (n < t.n ? n : t.n - 1)) * t.rank;
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-          const int j = 4 * U * s + U * g;
-          float w[U];
-          load_values<WT, U, true>(t.b, at + (j < t.rank ? j : 0), w);
-          if (j >= t.rank) {
+      for (int s = 0; s < S; s++) {
+        b8v wp[kPieces<WT>];
+        pieces_of<WT>(w[c][s], wp);
 #pragma unroll
-            for (int q = 0; q < U; q++) w[q] = 0.0f;
-          }
+        for (int p = 0; p < kPieces<WT>; p++)
 #pragma unroll
-          for (int q = 0; q < U; q++)
+          for (int q = 0; q < MP; q++)
+            if (p + q < 3) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) acc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[q], m[h][s][q], acc[h], 0, 0, 0);
-        }
+              for (int h = 0; h < 2; h++)
+                acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[p], m[h][s][q], acc[h], 0, 0, 0);
+            }
       }
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-        if (row[h] >= 0) store_row4(t, t.out + row[h] * t.ldo, n0 + 16 * c + 4 * g, y[h][c] + acc[h]);
+      for (int h = 0; h < 2; h++) *(f4v*)&s_sum[16 * h + col][16 * (kUpTiles * wave + c) + 4 * g] = acc[h];
     }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int r = kUpWaves * i + wave;
+    const int64_t row = rows[r];
+    if (row < 0) continue;
+    if (who >= 0) y[i] += *(const f4v*)&s_sum[r][4 * lane];
+    store_row4(t, t.out + row * t.ldo, n0 + 4 * lane, y[i]);
   }
 }
 
@@ -417,27 +548,31 @@ Form form_of(const LoraArgs& a) {
   return rank * a.k <= (int64_t)1 << 17 ? kFused : kRows;
 }
 
-// Parts of k: until two workgroups a CU are there, of 4 steps a wave at least.
+// Parts of k: until the CUs have the 12 waves each that registers leave, of 4 steps
+// a wave at least.
 int splits_of(const LoraArgs& a, int cus) {
   if (form_of(a) != kTiles) return 1;
-  const int64_t groups = (a.rows + kTile - 1) / kTile * a.count, most = a.k / 1024;
-  int64_t s = 2 * cus / groups;
+  int rank = 0;
+  for (int i = 0; i < a.count; i++) rank = rank > a.t[i].rank ? rank : a.t[i].rank;
+  const int waves = down_waves((rank + 15) / 16, QMM_X_BF16);
+  const int64_t groups = (a.rows + kTile - 1) / kTile * a.count, most = a.k / (128 * waves);
+  int64_t s = 12 / waves * cus / groups;
   s = s < most ? s : most;
+  if (s > 8) s -= s % 8;  // parts that the XCDs share evenly
   return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
 template <int XT, int WT, int RT, bool VEC>
 hipError_t launch_tiles(const LoraArgs& a, int64_t widest, int64_t rank, hipStream_t st) {
-  const int64_t tiles = tiles_of(a), wide = 16 * kUpTiles * kUpWaves * kUpBlocks;
+  const int64_t tiles = tiles_of(a), ranges = (widest + kUpOut - 1) / kUpOut;
   int with_none = 0;
   for (int i = 0; i < a.count; i++) with_none |= a.t[i].y != a.t[i].out;
   lora_tiles_kernel<<<1, 1024, 2 * (a.slots + 1) * sizeof(int32_t), st>>>(a, (int)tiles, with_none);
-  lora_down_kernel<XT, WT, RT, VEC><<<dim3((unsigned)tiles, (unsigned)a.splits, (unsigned)a.count), 64 * down_waves(RT), 0, st>>>(a);
+  lora_down_kernel<XT, WT, RT, VEC><<<dim3((unsigned)(tiles * a.splits), (unsigned)a.count), 64 * down_waves(RT, WT), 0, st>>>(a, (int)tiles);
   if (a.splits > 1)
     lora_join_kernel<<<dim3((unsigned)((a.rows * rank + 1023) / 1024), (unsigned)a.count), 256, 0, st>>>(a);
-  constexpr int U = RT == 1 ? 4 : 8, S = RT == 1 ? 1 : RT / 2;
-  lora_up_kernel<WT, U, S><<<dim3((unsigned)((widest + wide - 1) / wide), (unsigned)tiles, (unsigned)a.count),
-                             64 * kUpWaves, 0, st>>>(a);
+  lora_up_kernel<WT, (RT + 1) / 2><<<dim3((unsigned)((ranges + 7) / 8 * 8 * tiles), 1, (unsigned)a.count), 64 * kUpWaves, 0,
+                                     st>>>(a, (int)tiles);
   return hipGetLastError();
 }
 
