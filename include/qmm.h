@@ -523,9 +523,9 @@ int qmm_adapters_add(int count, const qmm_adapter *adapters, int slots, int w_dt
  * A NaN logit counts as -inf, a logit of -inf is never drawn; a row of nothing
  * else gives -1 (qmm_gather_rows' "no row") and 0. Where a logit is +inf, those
  * alone are drawn, equally. Weights are relative to the largest, in 64 bits; weights
- * below 2^-60 may count as 0 where a setting is on. A row's token follows from
+ * below 2^-60 may count as 0 where a setting is on, and those below 2^-1000 do always. A row's token follows from
  * the row, its settings and vocab alone. Plan and
- * launch as qmm_forward (workspace 16-byte aligned). Two launches. At most 65535 rows. */
+ * launch as qmm_forward (workspace 16-byte aligned): the plan goes by which settings are given. At most 65535 rows. */
 int qmm_sample(const void *logits, int dtype, int64_t stride, const float *u, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *probs, int64_t vocab,
                int64_t rows, void *workspace, size_t workspace_bytes, size_t *need, int launch, int64_t stream);

@@ -1180,7 +1180,7 @@ int qmm_sample(const void* logits, int dtype, int64_t stride, const float* u, co
   a.logits = logits; a.u = u; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
   a.ids = ids; a.probs = probs; a.stride = stride; a.rows = (int)rows; a.vocab = (int)vocab;
   a.vec = (uintptr_t)logits % (4 * qmm::value_bytes(dtype)) == 0 && stride % 4 == 0;
-  *need = qmm::sample_plan(a, workspace);
+  *need = qmm::sample_plan(a, workspace, cu_count());
   if (!launch) return QMM_OK;
   if (g_fail_next.exchange(false)) return QMM_NO_ROOM;
   if (!logits || !u || !ids || !aligned16(workspace)) return QMM_UNSUPPORTED;

@@ -359,6 +359,16 @@ int lora_most_slots();
 size_t lora_plan(LoraArgs& a, void* ws, int cus);
 hipError_t launch_lora(const LoraArgs& a, int xdt, int wdt, hipStream_t st);
 
+// What one launch leaves to the next of a row with settings: mode 0, nothing.
+struct SampleState {
+  int32_t mode;
+  float top, lo;
+  int32_t ticket, listed, by_count;
+  double goal;    // the weight or the number of a prefix
+  uint64_t last;  // or the rank of its last value
+  double scale, floor;
+};
+
 // One token a row from its logits (sample.hip). Settings may be null (off).
 struct SampleArgs {
   const void* logits;
@@ -369,14 +379,21 @@ struct SampleArgs {
   const float* min_p;
   int32_t* ids;
   float* probs;  // may be null
-  float* maxima;   // workspace: [rows][4 chunks] the groups' largest logits
-  double* masses;  // and [rows][chunks] the chunks' weights
+  // workspace: the groups' largest logits [rows][4 chunks] and the chunks' weights [rows][chunks]
+  float* maxima;
+  double* masses;
+  // and with settings (null without): histograms [rows][slices][buckets], the
+  // weights that stay [rows][chunks], a border's values [rows][1024], the rows' states
+  double* parts;
+  double* kept;
+  uint64_t* lists;
+  SampleState* states;
   int64_t stride;
-  int rows, vocab;
+  int rows, vocab, slices;
   bool vec;  // the logits' rows lie at 4 values
 };
 int64_t sample_most_vocab();
-size_t sample_plan(SampleArgs& a, void* ws);
+size_t sample_plan(SampleArgs& a, void* ws, int cus);
 hipError_t launch_sample(const SampleArgs& a, int dtype, hipStream_t st);
 
 // Set-up a first launch would otherwise do (qmm_prepare): the LDS limit of

@@ -7,18 +7,25 @@
 // token is the first, by index, of the kept ones at which their running sum
 // passes u times their total.
 //
-// Two launches. The first reads the logits once: of every 1024 values (a wave's,
-// a chunk) the weight relative to the chunk's own largest, in 64 bits and one
-// order, and the largest of each 256 (16 lanes' values, a group). The second, a
-// workgroup a row, works from those: a row without settings draws a chunk by
-// the chunks' weights and reads that one again. Settings need the values past
-// a bound only: top_k the groups whose largest is among the k largest of the
-// groups (the k-th of them bounds the k-th value from below), min_p those past
-// its own line, top_p those past (1 - top_p) Z / n, which no value that ends
-// the run can be under (n values of at most that weight follow it). Up to 1024
-// values are sorted in LDS and every setting cut there; more are narrowed
-// down first by histograms of counts and weights, the weights as whole numbers
-// (2^S to the largest), so that no order of additions shows in them.
+// The first launch reads the logits once: of every 1024 values (a wave's, a chunk)
+// the weight relative to the chunk's own largest, in 64 bits and one order, and
+// the largest of each 256 (16 lanes' values, a group). Rows without settings then
+// draw a chunk by the chunks' weights and read that one again (sample_pick_kernel).
+//
+// Settings need the values past a bound only: top_k the groups whose largest is
+// among the k largest of the groups (the k-th of them bounds the k-th value from
+// below), min_p those past its own line, top_p those past (1 - top_p) Z / n, which
+// no value that ends the run can be under (n values of at most that weight
+// follow it). Up to 1024 values are sorted in LDS, or 64 in a wave, and every
+// setting cut there (sample_select_kernel, a workgroup a row).
+// A run by weight (or the k largest of very many) is narrowed down first: the row's
+// slices make histograms of counts and weights over the bound's range, the weights as
+// whole numbers (2^S to the largest), so that no order of additions shows in them;
+// sample_finish_kernel adds the slices', finds the bucket in which the run ends,
+// sums the weights above it chunk by chunk and lists the bucket's own values,
+// which the row's last workgroup sorts, cuts and draws from. More than 1024 values
+// at a border (equal logits) are narrowed down further by one workgroup, by their
+// bits and then by index.
 #include <cfloat>
 
 #include "../../include/qmm.h"
@@ -33,7 +40,9 @@ namespace {
 constexpr int kChunk = 1024, kGroups = 4;  // values a wave holds; groups in them
 constexpr int kMostVocab = 1 << 19;
 constexpr int kMostChunks = kMostVocab / kChunk;
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024;
+constexpr int kMostRows = 2048;  // of a launch: what the workspace holds
+enum { kHistogram = 1, kLine = 2 };  // what a row leaves to sample_finish_kernel
 constexpr int kList = 1024;     // values that are sorted
 constexpr int kBuckets = 2048;  // two a thread
 constexpr double kLog2e = 1.4426950408889634;
@@ -42,28 +51,58 @@ constexpr double kLog2e = 1.4426950408889634;
 // row, or NaN, is -inf.
 template <int T, bool VEC>
 __device__ __forceinline__ void load_chunk(const SampleArgs& a, int64_t row, int c, int lane, float v[16]) {
+  const int64_t at = row * a.stride + c * kChunk + 4 * lane;
+  if ((c + 1) * kChunk <= a.vocab) {
 #pragma unroll
-  for (int q = 0; q < 4; q++) {
-    const int i = c * kChunk + 256 * q + 4 * lane;
-    float* const o = v + 4 * q;
-    if (i + 4 <= a.vocab) {
-      load4<T, VEC>(a.logits, row * a.stride + i, o);
-    } else {
+    for (int q = 0; q < 4; q++) load4<T, VEC>(a.logits, at + 256 * q, v + 4 * q);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = i + e < a.vocab ? load1<T>(a.logits, row * a.stride + i + e) : -INFINITY;
+    for (int e = 0; e < 16; e++) {
+      const int i = 256 * (e >> 2) + (e & 3);
+      v[e] = c * kChunk + 4 * lane + i < a.vocab ? load1<T>(a.logits, at + i) : -INFINITY;
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = o[e] == o[e] ? o[e] : -INFINITY;
   }
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
 }
 __device__ __forceinline__ int index_of(int c, int lane, int e) { return c * kChunk + 256 * (e >> 2) + 4 * lane + (e & 3); }
 
-// exp((x - top) / T), scale = log2(e) / T; 0 for -inf. (x == top: 1, also where both are inf.)
-__device__ __forceinline__ double weight(float x, float top, double scale) {
-  if (x == top) return 1.0;
-  const double y = ((double)x - (double)top) * scale;
-  return y > -1074.0 ? exp2(y) : 0.0;
-}
+// 2^y by the nearest 64th below or above it, whose power is looked up (one of 64
+// in LDS, by its low six bits), and the Taylor polynomial of 2^r over what is
+// left: |r ln 2| <= 0.0055, whose sixth power over 6! is 2^-55. y in [-1000, 0];
+// under it 0.
+struct Powers {
+  double p[64];
+  // by the first 64 threads; a barrier follows
+  __device__ __forceinline__ void fill() {
+    if (threadIdx.x < 64) p[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  }
+  __device__ __forceinline__ double power(double y) const {
+    constexpr double kShift = 105553116266496.0;  // 1.5 * 2^46: its half step is 2^-7
+    const double t = y + kShift;
+    const uint32_t n = (uint32_t)__double2loint(t);  // 64 y, rounded
+    const double r = y - (t - kShift);
+    const double q = r * fma(r, fma(r, fma(r, fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3), 5.5504108664821580e-2),
+                                    2.4022650695910071e-1),
+                             6.9314718055994531e-1);
+    const double b = p[n & 63];
+    const double s = __hiloint2double(__double2hiint(b) + (int)((n & ~63u) << 14), __double2loint(b));
+    const double w = fma(s, q, s);
+    return y >= -1000.0 ? w : 0.0;
+  }
+};
+
+// A row's weights: exp((x - top) / T), scale = log2(e) / T; 0 for -inf. Where that
+// is no number (top or scale infinite) the largest values alone count.
+struct Weights {
+  const Powers* powers;
+  float top;
+  double scale;
+  __device__ __forceinline__ double operator()(float x) const {
+    if (top == INFINITY || scale == (double)INFINITY) return x == top ? 1.0 : 0.0;
+    return powers->power(((double)x - (double)top) * scale);
+  }
+};
 
 __device__ __forceinline__ double scale_of(const SampleArgs& a, int64_t row, bool& greedy) {
   const float t = a.temperature ? a.temperature[row] : 1.0f;
@@ -71,10 +110,17 @@ __device__ __forceinline__ double scale_of(const SampleArgs& a, int64_t row, boo
   return greedy ? 1.0 : kLog2e / (double)t;
 }
 
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
 template <int T, bool VEC>
 __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int chunks) {
+  __shared__ Powers powers;
   const int lane = threadIdx.x & 63, c = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t row = blockIdx.y;
+  powers.fill();
+  __syncthreads();
   if (c >= chunks) return;
   float v[16];
   load_chunk<T, VEC>(a, row, c, lane, v);
@@ -83,20 +129,41 @@ __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int ch
   float m = v[0];
 #pragma unroll
   for (int e = 1; e < 16; e++) m = fmaxf(m, v[e]);
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  // over 16 lanes, then over the four groups (the same for the wave)
+  m = fmaxf(m, __uint_as_float(dpp_u<0xB1>(__float_as_uint(m))));
+  m = fmaxf(m, __uint_as_float(dpp_u<0x4E>(__float_as_uint(m))));
+  m = fmaxf(m, __uint_as_float(dpp_u<0x141>(__float_as_uint(m))));
+  m = fmaxf(m, __uint_as_float(dpp_u<0x140>(__float_as_uint(m))));
   if ((lane & 15) == 0) a.maxima[(row * chunks + c) * kGroups + (lane >> 4)] = m;
-  m = fmaxf(m, __shfl_xor(m, 16, 64));
-  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  m = fmaxf(fmaxf(lane_value(m, 0), lane_value(m, 16)), fmaxf(lane_value(m, 32), lane_value(m, 48)));
   double s = 0.0;
   if (!greedy && m != -INFINITY) {
+    const Weights weight{&powers, m, scale};
+    if (m < INFINITY && scale < INFINITY) {
 #pragma unroll
-    for (int e = 0; e < 16; e++) s += weight(v[e], m, scale);
+      for (int e = 0; e < 16; e++) s += powers.power(((double)v[e] - (double)m) * scale);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s += weight(v[e]);
+    }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
   }
   if (lane == 0) a.masses[row * chunks + c] = s;
+  if (c == 0 && lane == 0 && a.states) a.states[row] = SampleState{};
 }
+
+// A weight as a whole number of units, 2^-bits of the largest weight each (bits at
+// most 52): the bits of its 53 that are left, cut off.
+struct Units {
+  int bits;
+  __device__ __forceinline__ uint64_t operator()(double w) const {
+    const uint64_t b = (uint64_t)__double_as_longlong(w);
+    const int shift = min(63, 1023 + 52 - bits - (int)(b >> 52));  // (0 and what is under a unit: all of them)
+    return ((b & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) >> shift;
+  }
+  __device__ __forceinline__ double size() const { return __hiloint2double((1023 + bits) << 20, 0); }
+};
 
 // Values in the order of their keys: key(x) < key(y) where x < y.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -111,6 +178,7 @@ __device__ __forceinline__ uint64_t rank_of(float x, int i) { return (uint64_t)k
 __device__ __forceinline__ float ranked_value(uint64_t r) { return value_of((uint32_t)(r >> 32)); }
 
 struct Shared {
+  Powers powers;
   float maxima[kMostChunks * kGroups];
   uint16_t active[kMostChunks * kGroups];
   union {
@@ -119,77 +187,137 @@ struct Shared {
       uint32_t count[kBuckets];
     } h;
     double group_mass[kMostChunks * kGroups];
+    double part[kBuckets];
   };
   uint64_t list[kList];
-  double sums[kWaves];
-  uint64_t sums64[kWaves];
-  uint32_t sums32[kWaves];
-  float tops[kWaves];
+  double sums[16];
+  uint64_t sums64[16];
+  uint32_t sums32[16];
   int n_active, n_list, found;
 };
 
-__device__ __forceinline__ float block_max(float v, Shared& s) {
+// The value of lane ^ M of the wave, on the vector unit (a shuffle goes through LDS: a
+// stage of a sort took 125 ns with it).
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (M == 1) return dpp_u<0xB1>(v);             // quad 1,0,3,2
+  if constexpr (M == 2) return dpp_u<0x4E>(v);             // quad 2,3,0,1
+  if constexpr (M == 4) return dpp_u<0x1B>(dpp_u<0x141>(v));  // 8 mirrored, each quad mirrored
+  if constexpr (M == 8) return dpp_u<0x128>(v);            // 16 turned by 8
+  if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  }
+  if constexpr (M == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+}
+template <int M>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return (uint64_t)lane_xor<M>((uint32_t)(v >> 32)) << 32 | lane_xor<M>((uint32_t)v);
+}
+
+// Running sums over the wave's lanes: within 16, then 15 -> the next 16, 31 -> the upper half.
+template <int CTL, int ROWS, typename T>
+__device__ __forceinline__ T lane_shift(T v) {
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); i++) w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[i], CTL, ROWS, 0xF, true);
+  __builtin_memcpy(&v, w, sizeof(T));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_sums(T v) {
+  v += lane_shift<0x111, 0xF>(v);
+  v += lane_shift<0x112, 0xF>(v);
+  v += lane_shift<0x114, 0xF>(v);
+  v += lane_shift<0x118, 0xF>(v);
+  v += lane_shift<0x142, 0xA>(v);
+  v += lane_shift<0x143, 0xC>(v);
+  return v;
+}
+
+// Of a workgroup of NT threads (NT / 64 waves).
+template <int NT>
+__device__ __forceinline__ float block_max(float v, double* waves) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  float* const w = (float*)waves;
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = v;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.tops[threadIdx.x >> 6] = v;
+  v = w[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; i++) v = fmaxf(v, w[i]);
   __syncthreads();
-  v = s.tops[0];
-  for (int w = 1; w < kWaves; w++) v = fmaxf(v, s.tops[w]);
   return v;
 }
 
 // The sum of the values of this thread and the ones before it, and all of them;
 // in one order, whatever the values.
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ T block_sums(T v, T* waves, T& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T up = __shfl_up(v, d, 64);
-    if (lane >= d) v += up;
-  }
-  __syncthreads();
+  v = wave_sums(v);
   if (lane == 63) waves[wave] = v;
   __syncthreads();
   T before = 0;
   total = 0;
-  for (int w = 0; w < kWaves; w++) {
+#pragma unroll
+  for (int w = 0; w < NT / 64; w++) {
     if (w == wave) before = total;
     total += waves[w];
   }
+  __syncthreads();
   return before + v;
 }
 
 // The least of the threads' numbers.
-__device__ __forceinline__ int block_least(int v, Shared& s) {
-  if (threadIdx.x == 0) s.found = INT32_MAX;
-  __syncthreads();
+__device__ __forceinline__ int block_least(int v, int* found) {
+  if (threadIdx.x == 0) *found = INT32_MAX;
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v = min(v, __shfl_xor(v, d, 64));
-  if ((threadIdx.x & 63) == 0) atomicMin(&s.found, v);
   __syncthreads();
-  v = s.found;
+  if ((threadIdx.x & 63) == 0 && v != INT32_MAX) atomicMin(found, v);
+  __syncthreads();
+  v = *found;
   __syncthreads();
   return v;
 }
 
-// One number a thread, sorted over the first n2 threads (a power of two, 64 at least), the least first.
+// The lesser of two lanes' numbers to the lower lane (up) or to the upper one.
+template <int M>
+__device__ __forceinline__ uint64_t sort_step(uint64_t v, bool up) {
+  const uint64_t o = lane_xor<M>(v);
+  return (((threadIdx.x & M) == 0) == up) == (o < v) ? o : v;
+}
+
+// One number a thread, sorted over the first n2 threads (a power of two, 64 at
+// least), the least first. The waves past them only meet the barriers.
 __device__ __forceinline__ uint64_t block_sort(uint64_t v, int n2, uint64_t* buf) {
   const int tid = threadIdx.x;
+  const bool in = tid < n2;  // the same for a wave
   for (int size = 2; size <= n2; size <<= 1) {
-    for (int stride = size >> 1; stride >= 1; stride >>= 1) {
-      uint64_t o;
-      if (stride >= 64) {
-        __syncthreads();
-        buf[tid] = v;
-        __syncthreads();
-        o = buf[tid ^ stride];
-      } else {
-        o = __shfl_xor((unsigned long long)v, stride, 64);
-      }
-      const bool low = (tid & stride) == 0, up = (tid & size) == 0;
-      if ((low == up) == (o < v)) v = o;
+    const bool up = (tid & size) == 0;
+    int stride = size >> 1;
+    for (; stride >= 64; stride >>= 1) {
+      __syncthreads();
+      if (in) buf[tid] = v;
+      __syncthreads();
+      if (!in) continue;
+      const uint64_t o = buf[tid ^ stride];
+      if (((tid & stride) == 0) == up ? o < v : o > v) v = o;
+    }
+    if (!in) continue;
+    switch (stride) {
+      case 32: v = sort_step<32>(v, up); [[fallthrough]];
+      case 16: v = sort_step<16>(v, up); [[fallthrough]];
+      case 8: v = sort_step<8>(v, up); [[fallthrough]];
+      case 4: v = sort_step<4>(v, up); [[fallthrough]];
+      case 2: v = sort_step<2>(v, up); [[fallthrough]];
+      default: v = sort_step<1>(v, up);
     }
   }
   return v;
@@ -214,50 +342,66 @@ __device__ __forceinline__ void each_value(const SampleArgs& a, int64_t row, con
   }
 }
 
-// The groups that hold a value of `lo` or more.
-__device__ __forceinline__ void activate(Shared& s, int groups, float lo) {
+// The groups from g0 to g1 whose largest value `in` takes.
+template <typename In>
+__device__ __forceinline__ void activate(Shared& s, int g0, int g1, In in) {
   __syncthreads();
   if (threadIdx.x == 0) s.n_active = 0;
   __syncthreads();
-  for (int g = threadIdx.x; g < groups; g += kThreads)
-    if (s.maxima[g] >= lo && s.maxima[g] != -INFINITY) s.active[atomicAdd(&s.n_active, 1)] = (uint16_t)g;
+  for (int g = g0 + (int)threadIdx.x; g < g1; g += kThreads)
+    if (s.maxima[g] != -INFINITY && in(s.maxima[g])) s.active[atomicAdd(&s.n_active, 1)] = (uint16_t)g;
   __syncthreads();
 }
 
 // The values that `in` takes into the list (the first kList that come), and how many there are.
 template <int T, bool VEC, typename In>
 __device__ __forceinline__ int collect(const SampleArgs& a, int64_t row, Shared& s, In in) {
-  __syncthreads();
   if (threadIdx.x == 0) s.n_list = 0;
   __syncthreads();
-  each_value<T, VEC>(a, row, s, [&](float x, int i) {
-    if (x != -INFINITY && in(x, i)) {
-      const int at = atomicAdd(&s.n_list, 1);
-      if (at < kList) s.list[at] = rank_of(x, i);
+  constexpr int kUnits = kThreads / 16;
+  const int n = s.n_active;
+  // two groups on their way at once; over once the list is
+  for (int k = threadIdx.x >> 4; k < n && *(volatile int*)&s.n_list <= kList; k += 2 * kUnits) {
+    float v[2][16];
+    int g[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      g[h] = s.active[min(k + h * kUnits, n - 1)];
+      load_chunk<T, VEC>(a, row, g[h] >> 2, (g[h] & 3) * 16 + (threadIdx.x & 15), v[h]);
     }
-  });
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (k + h * kUnits >= n) break;
+      uint32_t those = 0;
+#pragma unroll
+      for (int e = 0; e < 16; e++) those |= v[h][e] != -INFINITY && in(v[h][e]) ? 1u << e : 0u;
+      if (those == 0) continue;
+      int at = atomicAdd(&s.n_list, __popc(those));  // one addition a lane
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (those >> e & 1) {
+          if (at < kList) s.list[at] = rank_of(v[h][e], index_of(g[h] >> 2, (g[h] & 3) * 16 + (threadIdx.x & 15), e));
+          at++;
+        }
+    }
+  }
   __syncthreads();
   return s.n_list;
 }
 
-// What a row's settings ask of a prefix of the ordered values: `k` of them at
-// most, or their weight.
+// What a row's settings ask of a prefix of the ordered values: `want` of them
+// at most, or their weight.
 struct Goal {
   bool by_count;
   uint64_t want;
 };
 
 // A histogram over the values that `bucket` gives a bucket (the larger the
-// value, the lower), and the first bucket at which the goal is met: kBuckets
-// if none. Counts and weights of the buckets before it are added to above_*,
-// `inside` the bucket's own count.
+// value, the lower; -1: none).
 template <int T, bool VEC, typename B>
-__device__ __forceinline__ int narrow(const SampleArgs& a, int64_t row, Shared& s, const Goal& goal, float top,
-                                      double scale, double unit, uint64_t& above_count, uint64_t& above_mass,
-                                      uint32_t& inside, B bucket) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-  for (int b = tid; b < kBuckets; b += kThreads) {
+__device__ __forceinline__ void histogram(const SampleArgs& a, int64_t row, Shared& s, const Weights& weight, const Units& unit,
+                                          bool weights, B bucket) {
+  for (int b = threadIdx.x; b < kBuckets; b += kThreads) {
     s.h.mass[b] = 0;
     s.h.count[b] = 0;
   }
@@ -266,25 +410,31 @@ __device__ __forceinline__ int narrow(const SampleArgs& a, int64_t row, Shared& 
     const int b = x != -INFINITY ? bucket(x, i) : -1;
     if (b < 0) return;
     atomicAdd(&s.h.count[b], 1u);
-    atomicAdd((unsigned long long*)&s.h.mass[b], (unsigned long long)(weight(x, top, scale) * unit + 0.5));
+    if (weights) atomicAdd((unsigned long long*)&s.h.mass[b], (unsigned long long)unit(weight(x)));
   });
   __syncthreads();
-  const uint32_t c0 = s.h.count[2 * tid], c1 = s.h.count[2 * tid + 1];
-  const uint64_t m0 = s.h.mass[2 * tid], m1 = s.h.mass[2 * tid + 1];
+}
+
+// The first bucket at which the goal is met (kBuckets: none), from the counts and
+// weights of a thread's two buckets. Those of the buckets before it are added to
+// above_*, `inside` is the bucket's own count.
+__device__ __forceinline__ int first_met(Shared& s, const Goal& goal, const uint32_t c[2], const uint64_t m[2],
+                                         uint64_t& above_count, uint64_t& above_mass, uint32_t& inside) {
+  const int tid = threadIdx.x;
   uint32_t all_count;
   uint64_t all_mass;
-  const uint64_t count = above_count + block_sums<uint32_t>(c0 + c1, s.sums32, all_count);
-  const uint64_t mass = above_mass + block_sums<uint64_t>(m0 + m1, s.sums64, all_mass);
-  auto met = [&](uint64_t n, uint64_t m) { return n > 0 && (goal.by_count ? n : m) >= goal.want; };
+  const uint64_t count = above_count + block_sums<kThreads, uint32_t>(c[0] + c[1], s.sums32, all_count);
+  const uint64_t mass = above_mass + block_sums<kThreads, uint64_t>(m[0] + m[1], s.sums64, all_mass);
+  auto met = [&](uint64_t n, uint64_t w) { return n > 0 && (goal.by_count ? n : w) >= goal.want; };
   int b = INT32_MAX;
-  if (met(count, mass)) b = met(count - c1, mass - m1) ? 2 * tid : 2 * tid + 1;
-  b = block_least(b, s);
+  if (met(count, mass)) b = met(count - c[1], mass - m[1]) ? 2 * tid : 2 * tid + 1;
+  b = block_least(b, &s.found);
   if (b >= kBuckets) return kBuckets;
   // the sums before it are its thread's
   if (tid == b / 2) {
-    s.sums64[0] = (b & 1 ? count - c1 : count - c1 - c0);
-    s.sums64[1] = (b & 1 ? mass - m1 : mass - m1 - m0);
-    s.sums32[0] = b & 1 ? c1 : c0;
+    s.sums64[0] = count - c[1] - (b & 1 ? 0 : c[0]);
+    s.sums64[1] = mass - m[1] - (b & 1 ? 0 : m[0]);
+    s.sums32[0] = c[b & 1];
   }
   __syncthreads();
   above_count = s.sums64[0];
@@ -294,69 +444,96 @@ __device__ __forceinline__ int narrow(const SampleArgs& a, int64_t row, Shared& 
   return b;
 }
 
-// The rank of the last value of the prefix that meets the goal (0: all values
-// meet it together or not at all), `mass` the prefix's weight.
 template <int T, bool VEC, typename B>
+__device__ __forceinline__ int narrow(const SampleArgs& a, int64_t row, Shared& s, const Goal& goal, bool both,
+                                      const Weights& weight, const Units& unit, uint64_t& above_count, uint64_t& above_mass,
+                                      uint32_t& inside, B bucket) {
+  histogram<T, VEC>(a, row, s, weight, unit, both, bucket);
+  const uint32_t c[2] = {s.h.count[2 * threadIdx.x], s.h.count[2 * threadIdx.x + 1]};
+  const uint64_t m[2] = {s.h.mass[2 * threadIdx.x], s.h.mass[2 * threadIdx.x + 1]};
+  return first_met(s, goal, c, m, above_count, above_mass, inside);
+}
+
+// Buckets of equal width from a row's largest value down to its bound.
+struct Buckets {
+  float top, lo, inv;
+  __device__ __forceinline__ Buckets(float top, float lo) : top(top), lo(lo) {
+    const float width = top - lo;
+    inv = width > 0.0f && width < INFINITY ? (float)(kBuckets - 1) / width : 0.0f;
+  }
+  __device__ __forceinline__ int operator()(float x, int) const {
+    return x < lo ? -1 : x == top ? 0 : min(kBuckets - 1, (int)((top - x) * inv));
+  }
+};
+
+// The list's n values (all that lie in one bucket), sorted: the rank of the last
+// one of the prefix that meets the goal, and the prefix's weight.
+__device__ __forceinline__ uint64_t last_in_list(Shared& s, const Goal& goal, const Weights& weight, const Units& unit, int n,
+                                                 uint64_t above_count, uint64_t above_mass, uint64_t& mass) {
+  const int tid = threadIdx.x;
+  const uint64_t mine = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
+  const uint64_t w = tid < n ? unit(weight(ranked_value(mine))) : 0;
+  uint64_t total;
+  const uint64_t m = above_mass + block_sums<kThreads, uint64_t>(w, s.sums64, total);
+  const bool met = (goal.by_count ? above_count + tid + 1 : m) >= goal.want;
+  const int at = min(block_least(tid < n && met ? tid : INT32_MAX, &s.found), n - 1);
+  if (tid == at) {
+    s.sums64[0] = mine;
+    s.sums64[1] = m;
+  }
+  __syncthreads();
+  const uint64_t last = s.sums64[0];
+  mass = s.sums64[1];
+  __syncthreads();
+  return last;
+}
+
+// The same for a bucket of any number of values, over the active groups: by one workgroup.
+template <int T, bool VEC>
 __device__ __forceinline__ uint64_t last_of_prefix(const SampleArgs& a, int64_t row, Shared& s, const Goal& goal,
-                                                   float top, double scale, double unit, uint64_t& mass, B bucket,
-                                                   int first, uint64_t above_count, uint64_t above_mass, uint32_t inside) {
+                                                   const Weights& weight, const Units& unit, uint64_t& mass,
+                                                   const Buckets& bucket, int first, uint64_t above_count,
+                                                   uint64_t above_mass, uint32_t inside) {
   // the keys of the bucket, which falls as they rise: between the first with
   // bucket <= `first` and the last with bucket >= it
-  uint32_t lo = key_of(-FLT_MAX), hi = key_of(top);
+  uint32_t lo, hi = key_of(bucket.top);
   {
-    uint32_t l = lo, h = hi;
+    uint32_t l = key_of(-FLT_MAX), h = hi;
     while (l < h) {
       const uint32_t m = l + (h - l) / 2;
-      if (bucket(value_of(m), 0) <= first && bucket(value_of(m), 0) >= 0) h = m; else l = m + 1;
+      const int b = bucket(value_of(m), 0);
+      if (b <= first && b >= 0) h = m; else l = m + 1;
     }
-    const uint32_t from = l;
+    lo = l;
     h = hi;
     while (l < h) {
       const uint32_t m = l + (h - l + 1) / 2;
       if (bucket(value_of(m), 0) >= first) l = m; else h = m - 1;
     }
-    lo = from;
     hi = l;
   }
   while (inside > kList && lo < hi) {
     const uint32_t span = hi - lo, l = lo, h = hi;
     const int shift = span < (uint32_t)kBuckets ? 0 : 32 - __builtin_clz(span) - 11;
-    const int b = narrow<T, VEC>(a, row, s, goal, top, scale, unit, above_count, above_mass, inside,
-                                 [=](float x, int) {
-                                   const uint32_t k = key_of(x);
-                                   return k >= l && k <= h ? (int)((h - k) >> shift) : -1;
-                                 });
+    const int b = narrow<T, VEC>(a, row, s, goal, true, weight, unit, above_count, above_mass, inside, [=](float x, int) {
+      const uint32_t k = key_of(x);
+      return k >= l && k <= h ? (int)((h - k) >> shift) : -1;
+    });
     if (b >= kBuckets) break;  // (the bucket above met the goal: this is not reached)
     hi = h - ((uint32_t)b << shift);
     const uint32_t width = (1u << shift) - 1;
     lo = hi - l > width ? hi - width : l;
   }
-  uint64_t last;
   const uint32_t l = lo, h = hi;
   if (inside <= kList) {
-    const int n = min(kList, collect<T, VEC>(a, row, s, [=](float x, int) {
+    const int n = min(kList, collect<T, VEC>(a, row, s, [=](float x) {
                          const uint32_t k = key_of(x);
                          return k >= l && k <= h;
                        }));
-    const uint64_t r = ~block_sort(threadIdx.x < n ? ~s.list[threadIdx.x] : ~0ull, sort_size(n), s.list);
-    const uint64_t w = threadIdx.x < n ? (uint64_t)(weight(ranked_value(r), top, scale) * unit + 0.5) : 0;
-    uint64_t total;
-    const uint64_t m = above_mass + block_sums<uint64_t>(w, s.sums64, total);
-    const bool met = (goal.by_count ? above_count + threadIdx.x + 1 : m) >= goal.want;
-    int at = block_least(threadIdx.x < n && met ? (int)threadIdx.x : INT32_MAX, s);
-    at = min(at, n - 1);
-    if (threadIdx.x == at) {
-      s.sums64[0] = r;
-      s.sums64[1] = m;
-    }
-    __syncthreads();
-    last = s.sums64[0];
-    mass = s.sums64[1];
-    __syncthreads();
-    return last;
+    return last_in_list(s, goal, weight, unit, n, above_count, above_mass, mass);
   }
   // more equal values than the list holds: the first of them by index
-  const uint64_t w = (uint64_t)(weight(value_of(h), top, scale) * unit + 0.5);
+  const uint64_t w = unit(weight(value_of(h)));
   uint64_t n = goal.by_count ? goal.want - above_count : w ? (goal.want - above_mass + w - 1) / w : inside;
   if (n < 1 || (!goal.by_count && goal.want <= above_mass)) n = 1;
   if (n > inside) n = inside;
@@ -367,7 +544,7 @@ __device__ __forceinline__ uint64_t last_of_prefix(const SampleArgs& a, int64_t 
   int from = 0;
   for (int shift = 8; shift >= 0; shift -= 8) {  // 2^11 ranges of 2^8 places, then the place
     const int base = from, width = kBuckets << shift;
-    const int b = narrow<T, VEC>(a, row, s, nth, top, scale, 0.0, before, unused, within, [=](float x, int i) {
+    const int b = narrow<T, VEC>(a, row, s, nth, false, weight, unit, before, unused, within, [=](float x, int i) {
       return key_of(x) == h && i >= base && i - base < (shift ? width : 256) ? (i - base) >> shift : -1;
     });
     from = base + (min(b, kBuckets - 1) << shift);
@@ -380,252 +557,573 @@ __device__ __forceinline__ void answer(const SampleArgs& a, int64_t row, int id,
   if (a.probs) a.probs[row] = (float)p;
 }
 
+// Which values stay, of a row whose prefix is known: those of rank `last` or more
+// (and of `lo` or more), of weight `floor` or more.
+struct Stay {
+  float lo;
+  uint64_t last;
+  double floor;
+  __device__ __forceinline__ double operator()(const Weights& weight, float x, int i) const {
+    if (!(x >= lo && x != -INFINITY && rank_of(x, i) >= last)) return 0.0;
+    const double w = weight(x);
+    return w >= floor ? w : 0.0;
+  }
+};
+
+// The first by index of the values that stay at which their sum passes u of the
+// total: the chunk from the chunks' weights (thread c's of chunk c), the value
+// from the chunk.
+template <int NT, int T, bool VEC>
+__device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Weights& weight, const Stay& stay, double mass,
+                                     double u, int chunks, double* sums, int* found) {
+  const int tid = threadIdx.x;
+  double total;
+  const double upto = block_sums<NT, double>(mass, sums, total), r = u * total;
+  const bool some = tid < chunks && mass > 0.0;
+  int c = block_least(some && upto > r ? tid : INT32_MAX, found);
+  if (c == INT32_MAX) c = -block_least(some ? -tid : INT32_MAX, found);
+  if (tid == c) sums[0] = upto - mass;
+  __syncthreads();
+  if (tid >= 64) return;
+  double sum = sums[0], chosen = 0.0;
+  float v[16];
+  load_chunk<T, VEC>(a, row, c, tid, v);
+  double w[16], run[4];
+#pragma unroll
+  for (int e = 0; e < 16; e++) w[e] = stay(weight, v[e], index_of(c, tid, e));
+#pragma unroll
+  for (int q = 0; q < 4; q++) run[q] = wave_sums((w[4 * q] + w[4 * q + 1]) + (w[4 * q + 2] + w[4 * q + 3]));
+  int at = -1;
+  bool found_it = false;
+#pragma unroll
+  for (int q = 0; q < 4; q++) {
+    const double before = __shfl_up(run[q], 1, 64);
+    double upto = sum + (tid ? before : 0.0);
+    int place = -1, end = -1;
+    double pw = 0.0, ew = 0.0;
+#pragma unroll
+    for (int e = 4 * q; e < 4 * q + 4; e++) {
+      upto += w[e];
+      if (w[e] > 0.0) {
+        end = index_of(c, tid, e);
+        ew = w[e];
+        if (place < 0 && upto > r) {
+          place = end;
+          pw = w[e];
+        }
+      }
+    }
+    const uint64_t hits = __ballot(place >= 0), ends = __ballot(end >= 0);
+    if (!found_it && hits) {
+      const int l = __builtin_ctzll(hits);
+      at = __shfl(place, l, 64);
+      chosen = __shfl(pw, l, 64);
+      found_it = true;
+    } else if (!found_it && ends) {
+      // (the sums of the chunk, in another order, can end below r: the last value with a weight)
+      const int l = 63 - __builtin_clzll(ends);
+      at = __shfl(end, l, 64);
+      chosen = __shfl(ew, l, 64);
+    }
+    sum += __shfl(run[q], 63, 64);
+  }
+  if (tid == 0) answer(a, row, at, chosen / total);
+}
+
+__device__ __forceinline__ double number_of(const SampleArgs& a, int64_t row) {
+  return fmin(fmax((double)a.u[row], 0.0), 1.0);
+}
+
+// The first value, by index, of the row's largest ones.
 template <int T, bool VEC>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a, int chunks, int bits) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, groups = chunks * kGroups;
+__device__ __forceinline__ int first_largest(const SampleArgs& a, int64_t row, const float* maxima, int chunks, float top,
+                                             int* found) {
+  int mine = INT32_MAX;
+  for (int c = threadIdx.x >> 6; c < chunks; c += blockDim.x >> 6) {
+    const float* m = maxima + kGroups * c;
+    if (fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) != top) continue;
+    float v[16];
+    load_chunk<T, VEC>(a, row, c, threadIdx.x & 63, v);
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (v[e] == top) mine = min(mine, index_of(c, threadIdx.x & 63, e));
+    break;  // (a wave's later chunks come behind it)
+  }
+  return block_least(mine, found);
+}
+
+// The weights of the chunks relative to the row's largest value, thread c's of chunk c.
+__device__ __forceinline__ double chunk_weight(const SampleArgs& a, int64_t row, const float* maxima, int chunks,
+                                               const Weights& weight) {
+  const int c = threadIdx.x;
+  if (c >= chunks) return 0.0;
+  const float* m = maxima + kGroups * c;
+  const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  return top != -INFINITY ? a.masses[row * chunks + c] * weight(top) : 0.0;
+}
+
+// Rows without settings but the temperature.
+template <int T, bool VEC>
+__global__ __launch_bounds__(kMostChunks) void sample_pick_kernel(SampleArgs a, int chunks) {
+  constexpr int NT = kMostChunks;
+  __shared__ Powers powers;
+  __shared__ float maxima[kMostChunks * kGroups];
+  __shared__ double sums[NT / 64];
+  __shared__ int found;
   const int64_t row = blockIdx.x;
   bool greedy;
   const double scale = scale_of(a, row, greedy);
+  powers.fill();
+  float m = -INFINITY;
+  for (int g = threadIdx.x; g < chunks * kGroups; g += NT) {
+    const float v = a.maxima[row * chunks * kGroups + g];
+    maxima[g] = v;
+    m = fmaxf(m, v);
+  }
+  const float top = block_max<NT>(m, sums);
+  if (top == -INFINITY) {
+    if (threadIdx.x == 0) answer(a, row, -1, 0.0);
+  } else if (greedy) {
+    const int first = first_largest<T, VEC>(a, row, maxima, chunks, top, &found);
+    if (threadIdx.x == 0) answer(a, row, first, 1.0);
+  } else {
+    const Weights weight{&powers, top, scale};
+    draw<NT, T, VEC>(a, row, weight, Stay{-INFINITY, 0, 0.0}, chunk_weight(a, row, maxima, chunks, weight), number_of(a, row),
+                     chunks, sums, &found);
+  }
+}
+
+// What the settings leave of at most 64 values, the largest first, a lane each: a wave's.
+__device__ __forceinline__ void finish_wave(const SampleArgs& a, int64_t row, const Weights& weight, uint64_t r, int n, int k,
+                                            double p, double goal_of, double floor, double u) {
+  const int lane = threadIdx.x;
+  r = ~block_sort(lane < n ? ~r : ~0ull, 64, nullptr);
+  double w = lane < n && lane < k ? weight(ranked_value(r)) : 0.0;
+  const double sum = wave_sums(w);
+  const double goal = fmax(p, 0.0) * (goal_of > 0.0 ? goal_of : __shfl(sum, 63, 64));
+  const bool stays = lane < n && lane < k && (p >= 1.0 || lane == 0 || sum - w < goal) && w >= floor;
+  if (!stays) w = 0.0;
+  const uint64_t those = __ballot(stays);
+  // the sums by index, each in the order of the ranks
+  const int i = (int)(uint32_t)~r, m = 64 - __builtin_clzll(those);
+  double upto = 0.0, all = 0.0;
+  for (int j = 0; j < m; j++) {
+    const int ij = __builtin_amdgcn_readlane(i, j);
+    const double wj = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(w), j),
+                                       __builtin_amdgcn_readlane(__double2loint(w), j));
+    upto += ij <= i ? wj : 0.0;
+    all += wj;
+  }
+  // the least index whose sum passes the number (or the last one: u of 1)
+  const bool hit = stays && upto > u * all;
+  int best = hit ? i : INT32_MAX;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+  if (best == INT32_MAX) {
+    best = stays ? i : -1;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) best = max(best, __shfl_xor(best, d, 64));
+  }
+  if (stays && i == best) answer(a, row, best, w / all);
+}
+
+// The part of the row's chunks that a slice takes.
+__device__ __forceinline__ int slice_begin(int chunks, int slice, int slices) { return chunks * slice / slices; }
+
+template <int T, bool VEC>
+__global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, int chunks, int bits) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, groups = chunks * kGroups, slice = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const int k_set = a.top_k ? a.top_k[row] : 0, merged = min(groups, kThreads);
+  const bool k_on = k_set > 0 && k_set < a.vocab;
+  const int k = k_on ? k_set : a.vocab;
+  const double p = a.top_p ? (double)a.top_p[row] : 1.0;
+  const bool p_on = p < 1.0;
+  bool greedy;
+  const double scale = scale_of(a, row, greedy);
+  // rows that every slice makes a histogram of; the others are the first one's
+  const bool wide = !greedy && (k_on ? !p_on && k > merged : p_on);
+  if (!wide && slice > 0) return;
+  s.powers.fill();
   float m = -INFINITY;
   for (int g = tid; g < groups; g += kThreads) {
     const float v = a.maxima[row * groups + g];
     s.maxima[g] = v;
     m = fmaxf(m, v);
   }
-  const float top = block_max(m, s);
+  const float top = block_max<kThreads>(m, s.sums);
   if (top == -INFINITY) {  // no value left
-    if (tid == 0) answer(a, row, -1, 0.0);
+    if (tid == 0 && slice == 0) answer(a, row, -1, 0.0);
     return;
   }
   if (greedy) {
-    activate(s, groups, top);
-    int first = INT32_MAX;
-    each_value<T, VEC>(a, row, s, [&](float x, int i) {
-      if (x == top) first = min(first, i);
-    });
-    first = block_least(first, s);
+    const int first = first_largest<T, VEC>(a, row, s.maxima, chunks, top, &s.found);
     if (tid == 0) answer(a, row, first, 1.0);
     return;
   }
-
-  // the chunks' weights relative to the row's largest value
-  double mass = 0.0, total;
-  if (tid < chunks) {
-    float c = s.maxima[kGroups * tid];
-#pragma unroll
-    for (int g = 1; g < kGroups; g++) c = fmaxf(c, s.maxima[kGroups * tid + g]);
-    if (c != -INFINITY) mass = a.masses[row * chunks + tid] * weight(c, top, scale);
-  }
-  double upto = block_sums<double>(mass, s.sums, total);
-
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const bool k_on = k > 0 && k < a.vocab;
-  const double p = a.top_p ? (double)a.top_p[row] : 1.0;
-  const bool p_on = p < 1.0;
+  const Weights weight{&s.powers, top, scale};
+  const double mass = chunk_weight(a, row, s.maxima, chunks, weight);
   const double floor = a.min_p && a.min_p[row] > 0.0f ? fmin((double)a.min_p[row], 1.0) : 0.0;
-  const double unit = exp2((double)(63 - bits)), r_u = fmin(fmax((double)a.u[row], 0.0), 1.0);
+  const double u = number_of(a, row);
+  if (!k_on && !p_on && floor == 0.0) {
+    draw<kThreads, T, VEC>(a, row, weight, Stay{-INFINITY, 0, 0.0}, mass, u, chunks, s.sums, &s.found);
+    return;
+  }
+  double total;
+  (void)block_sums<kThreads, double>(mass, s.sums, total);
+  const Units unit{bits};
 
-  uint64_t last = 0;  // the rank of the last value kept
-  const bool cut = k_on || p_on || floor > 0.0;
-  if (cut) {
-    // no value under `line` is kept (in units of log2 w), nor counts for another's place: under 2^-60 none does
-    double line = -60.0;
-    if (p_on && !k_on) line = fmax(line, log2(fmin((1.0 - p) * total / a.vocab, 1.0)) - 1e-6);
-    if (floor > 0.0 && !(k_on && p_on)) line = fmax(line, log2(floor) - 1e-6);
-    const double at = (double)top + line / scale;
-    float lo = at >= (double)top ? top : (float)at;
-    if ((double)lo > at) lo = value_of(key_of(lo) - 1);
-    if (top == INFINITY) lo = top;
-    const int merged = min(groups, kThreads);
-    if (k_on && k <= merged) {
-      float g = tid < groups ? s.maxima[tid] : -INFINITY;
-      for (int j = tid + kThreads; j < groups; j += kThreads) g = fmaxf(g, s.maxima[j]);
-      const uint64_t sorted = ~block_sort(tid < merged ? ~((uint64_t)key_of(g) << 32) : ~0ull, sort_size(merged), s.list);
-      if (tid == k - 1) s.tops[0] = ranked_value(sorted);
-      __syncthreads();
-      lo = fmaxf(lo, s.tops[0]);
-    }
-    activate(s, groups, lo);
-    // a run by weight alone asks for more values than it ends up with
-    const bool narrow_first = p_on && !k_on;
-    int n = narrow_first ? kList + 1 : collect<T, VEC>(a, row, s, [=](float x, int) { return x >= lo; });
-    if (n > kList) {
-      // narrowed down along the values first
-      const float width = top - lo, inv = width > 0.0f && width < INFINITY ? (float)(kBuckets - 1) / width : 0.0f;
-      auto bucket = [=](float x, int) {
-        return x < lo ? -1 : x == top ? 0 : min(kBuckets - 1, (int)((top - x) * inv));
-      };
-      Goal goal{k_on, k_on ? (uint64_t)k : p_on ? (uint64_t)(fmax(p, 0.0) * total * unit) : ~0ull};
-      uint64_t above_count = 0, above_mass = 0, kept_mass = 0;
-      uint32_t inside = 0;
-      int b = narrow<T, VEC>(a, row, s, goal, top, scale, unit, above_count, above_mass, inside, bucket);
-      if (b < kBuckets && above_count + inside <= kList) {
-        const int edge = b;
-        n = collect<T, VEC>(a, row, s, [=](float x, int i) { return x >= lo && bucket(x, i) <= edge; });
-      } else {
-        if (b < kBuckets)
-          last = last_of_prefix<T, VEC>(a, row, s, goal, top, scale, unit, kept_mass, bucket, b, above_count, above_mass,
-                                        inside);
-        else if (k_on && p_on)
-          kept_mass = (uint64_t)(total * unit);  // fewer than k values have any weight
-        if (k_on && p_on) {
-          const Goal run{false, (uint64_t)(fmax(p, 0.0) * (double)kept_mass)};
-          above_count = above_mass = 0;
-          b = narrow<T, VEC>(a, row, s, run, top, scale, unit, above_count, above_mass, inside, bucket);
-          if (b < kBuckets) {
-            const uint64_t end = last_of_prefix<T, VEC>(a, row, s, run, top, scale, unit, kept_mass, bucket, b,
-                                                        above_count, above_mass, inside);
-            last = max(last, end);
-          }
-        }
-        n = kList + 1;
-      }
-    }
-    if (n <= kList) {
-      // every value that can stay, the largest first
-      uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
-      double w = tid < n && (!k_on || tid < k) ? weight(ranked_value(r), top, scale) : 0.0;
-      double all;
-      const double sum = block_sums<double>(w, s.sums, all);
-      const double goal = fmax(p, 0.0) * (k_on ? all : total);
-      const bool stays = tid < n && (!k_on || tid < k) && (!p_on || tid == 0 || sum - w < goal) && w >= floor;
-      // and those that stay, by index
-      __syncthreads();
-      r = block_sort(stays ? (uint64_t)(uint32_t)~r << 32 | r >> 32 : ~0ull, sort_size(n), s.list);
-      const bool there = r != ~0ull;
-      const float x = value_of((uint32_t)r);
-      w = there ? weight(x, top, scale) : 0.0;
-      const double upto_here = block_sums<double>(w, s.sums, all);
-      int hit = block_least(w > 0.0 && upto_here > r_u * all ? tid : INT32_MAX, s);
-      if (hit == INT32_MAX) hit = -block_least(w > 0.0 ? -tid : INT32_MAX, s);  // u of 1
-      if (tid == hit) answer(a, row, (int)(r >> 32), w / all);
+  // no value under `line` is kept (in units of log2 w), nor counts for another's place: under 2^-60 none does
+  double line = -60.0;
+  if (p_on && !k_on) line = fmax(line, log2(fmin((1.0 - p) * total / a.vocab, 1.0)) - 1e-6);
+  if (floor > 0.0 && !(k_on && p_on)) line = fmax(line, log2(floor) - 1e-6);
+  const double at = (double)top + line / scale;
+  float lo = at >= (double)top ? top : (float)at;
+  if ((double)lo > at) lo = value_of(key_of(lo) - 1);
+  if (top == INFINITY) lo = top;
+  const Goal goal{k_on, k_on ? (uint64_t)k : (uint64_t)(fmax(p, 0.0) * total * unit.size())};
+
+  if (wide) {
+    // the slice's part of the histogram: counts, or weights in 32 bits (they say where
+    // to look; the sums that decide are the next launch's)
+    activate(s, kGroups * slice_begin(chunks, slice, a.slices), kGroups * slice_begin(chunks, slice + 1, a.slices),
+             [=](float x) { return x >= lo; });
+    for (int b = tid; b < kBuckets; b += kThreads) s.part[b] = 0.0;
+    __syncthreads();
+    const Buckets bucket(top, lo);
+    const float scale32 = (float)scale;
+    const bool only_top = top == INFINITY || scale == (double)INFINITY;
+    each_value<T, VEC>(a, row, s, [&](float x, int i) {
+      if (!(x >= lo) || x == -INFINITY) return;
+      const float w = only_top ? (x == top ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f((x - top) * scale32);
+      atomicAdd(&s.part[bucket(x, i)], k_on ? 1.0 : (double)w);
+    });
+    __syncthreads();
+    double* const part = a.parts + (row * a.slices + slice) * kBuckets;
+    for (int b = tid; b < kBuckets; b += kThreads) part[b] = s.part[b];
+    if (tid == 0 && slice == 0)
+      a.states[row] = SampleState{kHistogram, top, lo, 0, 0, k_on, k_on ? (double)k : fmax(p, 0.0) * total, 0, scale, floor};
+    return;
+  }
+
+  const Buckets bucket(top, lo);
+  int deepest = kBuckets;  // the bucket past which no value of the k largest lies
+  if (k_on && k <= merged) {
+    // that of the k-th largest of the groups' maxima
+    for (int b = tid; b < kBuckets; b += kThreads) s.h.count[b] = 0;
+    __syncthreads();
+    float v = tid < groups ? s.maxima[tid] : -INFINITY;
+    if (tid + kThreads < groups) v = fmaxf(v, s.maxima[tid + kThreads]);
+    const int mine = v != -INFINITY ? bucket(v, 0) : -1;
+    if (mine >= 0) atomicAdd(&s.h.count[mine], 1u);
+    __syncthreads();
+    const uint32_t c1 = s.h.count[2 * tid + 1];
+    uint32_t all_count;
+    const uint32_t upto = block_sums<kThreads, uint32_t>(s.h.count[2 * tid] + c1, s.sums32, all_count);
+    const int b = block_least(upto >= (uint32_t)k ? 2 * tid + (upto - c1 < (uint32_t)k) : INT32_MAX, &s.found);
+    deepest = min(b, kBuckets);
+  }
+  // (its lower border, a bucket lower for the roundings)
+  if (deepest < kBuckets && bucket.inv > 0.0f) lo = fmaxf(lo, top - (float)(deepest + 2) / bucket.inv);
+  activate(s, 0, groups, [=](float x) { return x >= lo; });
+  // min_p alone, and most groups hold some of its values: more than the list does, as a rule
+  const bool many = !k_on && s.n_active > 3 * groups / 4 && groups >= 256;
+  int n = many ? kList + 1 : collect<T, VEC>(a, row, s, [=](float x) { return x >= lo; });
+  uint64_t last = 0;  // the rank of the last value of the prefix
+  if (n > kList) {
+    if (!k_on) {  // min_p alone: all the values past its line, which every slice then sums
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0.0, 0, scale, floor};
       return;
     }
-    // many values stay: their weight chunk by chunk
-    if (last) activate(s, groups, fmaxf(lo, ranked_value(last)));
-    for (int g = tid; g < groups; g += kThreads) s.group_mass[g] = 0.0;
-    __syncthreads();
-    for (int j = tid >> 4; j < s.n_active; j += kThreads / 16) {
-      const int g = s.active[j], lane = (g & 3) * 16 + (tid & 15);
-      float v[16];
-      load_chunk<T, VEC>(a, row, g >> 2, lane, v);
-      double sum = 0.0;
+    // very many values, or equal ones: narrowed down by this workgroup
+    const Buckets bucket(top, lo);
+    uint64_t above_count = 0, above_mass = 0, kept_mass = 0;
+    uint32_t inside = 0;
+    int b = narrow<T, VEC>(a, row, s, goal, true, weight, unit, above_count, above_mass, inside, bucket);
+    if (b < kBuckets && above_count + inside <= kList) {
+      const int edge = b;
+      n = collect<T, VEC>(a, row, s, [=](float x) { return x >= lo && bucket(x, 0) <= edge; });
+    } else {
+      if (b < kBuckets)
+        last = last_of_prefix<T, VEC>(a, row, s, goal, weight, unit, kept_mass, bucket, b, above_count, above_mass, inside);
+      else
+        kept_mass = (uint64_t)(total * unit.size());  // fewer than k values have any weight
+      if (p_on) {
+        const Goal run{false, (uint64_t)(fmax(p, 0.0) * (double)kept_mass)};
+        above_count = above_mass = 0;
+        b = narrow<T, VEC>(a, row, s, run, true, weight, unit, above_count, above_mass, inside, bucket);
+        if (b < kBuckets)
+          last = max(last, last_of_prefix<T, VEC>(a, row, s, run, weight, unit, kept_mass, bucket, b, above_count,
+                                                  above_mass, inside));
+      }
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0.0, last, scale, floor};
+      return;
+    }
+  }
+  // every value that can stay
+  const double goal_of = k_on ? 0.0 : total;
+  if (n <= 64) {
+    if (tid < 64) finish_wave(a, row, weight, tid < n ? s.list[tid] : 0, n, k, p, goal_of, floor, u);
+    return;
+  }
+  uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
+  double w = tid < n && tid < k ? weight(ranked_value(r)) : 0.0, all;
+  const double sum = block_sums<kThreads, double>(w, s.sums, all);
+  const double run = fmax(p, 0.0) * (k_on ? all : total);
+  const bool stays = tid < n && tid < k && (!p_on || tid == 0 || sum - w < run) && w >= floor;
+  // those that stay, by index
+  r = block_sort(stays ? (uint64_t)(uint32_t)~r << 32 | r >> 32 : ~0ull, sort_size(n), s.list);
+  const bool there = r != ~0ull;
+  w = there ? weight(value_of((uint32_t)r)) : 0.0;
+  const double upto = block_sums<kThreads, double>(w, s.sums, all);
+  int hit = block_least(w > 0.0 && upto > u * all ? tid : INT32_MAX, &s.found);
+  if (hit == INT32_MAX) hit = -block_least(w > 0.0 ? -tid : INT32_MAX, &s.found);  // u of 1
+  if (tid == hit) answer(a, row, (int)(r >> 32), w / all);
+}
+
+// Rows of which many values stay: sums by chunk, and the border's values sorted
+// by the last of the row's workgroups.
+template <int T, bool VEC>
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, int chunks, int bits) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, groups = chunks * kGroups, slice = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  SampleState* const state = a.states + row;
+  const int mode = state->mode;
+  if (mode == 0) return;
+  s.powers.fill();
+  for (int g = tid; g < groups; g += kThreads) s.maxima[g] = a.maxima[row * groups + g];
+  const float top = state->top, lo = state->lo;
+  const double floor = state->floor, goal = state->goal;
+  const bool by_count = state->by_count != 0;
+  const Weights weight{&s.powers, top, state->scale};
+  const Buckets bucket(top, lo);
+  uint64_t last = state->last;
+  double above = 0.0;                    // the values of the buckets before the border's
+  int from = kBuckets, to = kBuckets - 1;  // the buckets that hold the border
+  if (mode == kHistogram) {
+    double m[2] = {0.0, 0.0};
+#pragma unroll 8
+    for (int i = 0; i < a.slices; i++) {
+      const double2 p = *(const double2*)(a.parts + (row * a.slices + i) * kBuckets + 2 * tid);
+      m[0] += p.x;
+      m[1] += p.y;
+    }
+    double all;
+    const double upto = block_sums<kThreads, double>(m[0] + m[1], s.sums, all);
+    // 32-bit weights are off by 3e-6 of theirs at most (|y| <= 61, half a step of y)
+    const double off = by_count ? 0.0 : 1e-4 * goal;
+    auto first = [&](double want) {
+      const bool met = upto > 0.0 && upto >= want, sooner = upto - m[1] > 0.0 && upto - m[1] >= want;
+      return block_least(met ? 2 * tid + !sooner : INT32_MAX, &s.found);
+    };
+    from = min(first(goal - off), kBuckets);
+    to = off > 0.0 ? min(first(goal + off), kBuckets - 1) : min(from, kBuckets - 1);
+    if (by_count) {
+      if (tid == from / 2) s.sums[0] = upto - m[1] - (from & 1 ? 0.0 : m[0]);
+      __syncthreads();
+      above = s.sums[0];
+      __syncthreads();
+    }
+  }
+  const int c0 = slice_begin(chunks, slice, a.slices), c1 = slice_begin(chunks, slice + 1, a.slices);
+  const float least = last ? fmaxf(lo, ranked_value(last)) : lo;
+  activate(s, kGroups * c0, kGroups * c1, [=](float x) { return x >= least && bucket(x, 0) <= max(from, to); });
+  for (int g = kGroups * c0 + tid; g < kGroups * c1; g += kThreads) s.group_mass[g] = 0.0;
+  __syncthreads();
+  const int n_active = s.n_active;
+  for (int j = tid >> 4; j < n_active; j += kThreads / 16) {
+    const int g = s.active[j], lane = (g & 3) * 16 + (tid & 15);
+    float v[16];
+    load_chunk<T, VEC>(a, row, g >> 2, lane, v);
+    double sum = 0.0;
+    uint32_t border = 0;
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const double w = v[e] >= lo && rank_of(v[e], index_of(g >> 2, lane, e)) >= last ? weight(v[e], top, scale) : 0.0;
+    for (int e = 0; e < 16; e++) {
+      const int i = index_of(g >> 2, lane, e), b = v[e] >= lo && v[e] != -INFINITY ? bucket(v[e], i) : kBuckets + 1;
+      if (b < from && (last == 0 || rank_of(v[e], i) >= last)) {
+        const double w = weight(v[e]);
         sum += w >= floor ? w : 0.0;
       }
+      border |= b >= from && b <= to ? 1u << e : 0u;
+    }
+    if (border) {
+      int at = atomicAdd(&state->listed, __popc(border));
 #pragma unroll
-      for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-      if ((tid & 15) == 0) s.group_mass[g] = sum;
+      for (int e = 0; e < 16; e++)
+        if (border >> e & 1) {
+          if (at < kList) a.lists[row * kList + at] = rank_of(v[e], index_of(g >> 2, lane, e));
+          at++;
+        }
+    }
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if ((tid & 15) == 0) s.group_mass[g] = sum;
+  }
+  __syncthreads();
+  for (int c = c0 + tid; c < c1; c += kThreads) {
+    double sum = 0.0;
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) sum += s.group_mass[kGroups * c + g];
+    a.kept[row * chunks + c] = sum;
+  }
+  // the row's last workgroup goes on; what the others wrote is there for it
+  if (a.slices > 1) {
+    __syncthreads();  // the workgroup's stores have reached its L2
+    if (tid == 0) {
+      __threadfence();
+      s.found = atomicAdd(&state->ticket, 1);
+      __threadfence();
     }
     __syncthreads();
-    mass = 0.0;
-    if (tid < chunks)
-      for (int g = 0; g < kGroups; g++) mass += s.group_mass[kGroups * tid + g];
-    upto = block_sums<double>(mass, s.sums, total);
-    // (values that are not there do not stay below)
-    m = lo;
+    const bool final = s.found == a.slices - 1;
+    __syncthreads();
+    if (!final) return;
   } else {
-    m = -FLT_MAX;
+    __threadfence_block();
+    __syncthreads();
   }
-
-  // the chunk that the number falls into, and the place in it
-  const double r = r_u * total;
-  int c = block_least(tid < chunks && mass > 0.0 && upto > r ? tid : INT32_MAX, s);
-  if (c == INT32_MAX) c = -block_least(tid < chunks && mass > 0.0 ? -tid : INT32_MAX, s);
-  if (tid == c) s.sums[0] = upto - mass;
-  __syncthreads();
-  if (tid >= 64) return;
-  double sum = s.sums[0], chosen = 0.0;
-  float v[16];
-  load_chunk<T, VEC>(a, row, c, tid, v);
-  int at = -1;
-  for (int q = 0; q < 4; q++) {
-    double w[4], mine = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float x = q == 0 ? v[e] : q == 1 ? v[4 + e] : q == 2 ? v[8 + e] : v[12 + e];
-      const bool in = x != -INFINITY && (!cut || (x >= m && rank_of(x, index_of(c, tid, 4 * q + e)) >= last));
-      w[e] = in ? weight(x, top, scale) : 0.0;
-      if (cut && w[e] < floor) w[e] = 0.0;
-      mine += w[e];
-    }
-    double run = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double up = __shfl_up(run, d, 64);
-      if (tid >= d) run += up;
-    }
-    double before = sum + (run - mine);
-    int place = -1, end = -1;
-    double pw = 0.0, ew = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      before += w[e];
-      if (w[e] > 0.0) {
-        end = index_of(c, tid, 4 * q + e);
-        ew = w[e];
-        if (place < 0 && before > r) {
-          place = end;
-          pw = w[e];
-        }
+  double mass = tid < chunks ? ((const volatile double*)a.kept)[row * chunks + tid] : 0.0;
+  if (from < kBuckets) {
+    const int n = ((const volatile SampleState*)state)->listed;
+    bool sure = n <= kList;
+    if (sure) {
+      double all;
+      // (without what is under the floor: where some of it lies above the border, all of the border's values are under it)
+      if (!by_count) (void)block_sums<kThreads, double>(mass, s.sums, above);
+      if (tid < n) s.list[tid] = ((const volatile uint64_t*)a.lists)[row * kList + tid];
+      __syncthreads();
+      const uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
+      const double w = tid < n ? weight(ranked_value(r)) : 0.0;
+      const double upto = block_sums<kThreads, double>(w, s.sums, all);
+      // the border's prefix: its first value too where nothing lies above it
+      const bool in = tid < n && (by_count ? above + tid < goal : (tid == 0 && above == 0.0) || above + (upto - w) < goal);
+      const int m = min(block_least(in ? INT32_MAX : tid, &s.found), n);
+      // whether the border is where the 32-bit weights said
+      sure = by_count || ((above < goal || above == 0.0) && (above + all >= goal || to == kBuckets - 1));
+      if (sure) {
+        if (tid == m - 1) s.sums64[0] = r;
+        const int i = (int)(uint32_t)~r;
+        s.group_mass[tid] = in && w >= floor ? w : 0.0;
+        s.active[tid] = (uint16_t)(i >> 10);
+        __syncthreads();
+        last = m ? s.sums64[0] : 0;
+        if (tid < chunks)
+          for (int j = 0; j < m; j++) mass += s.active[j] == tid ? s.group_mass[j] : 0.0;
+        __syncthreads();
       }
     }
-    const uint64_t hits = __ballot(place >= 0);
-    if (hits) {
-      const int l = __builtin_ctzll(hits);
-      at = __shfl(place, l, 64);
-      chosen = __shfl(pw, l, 64);
-      break;
+    if (!sure) {
+      // more values than the list holds (equal ones, as a rule): narrowed down by this workgroup
+      const Units unit{bits};
+      const Goal exact{by_count, by_count ? (uint64_t)goal : (uint64_t)(goal * unit.size())};
+      uint64_t above_count = 0, above_mass = 0, unused = 0;
+      uint32_t inside = 0;
+      activate(s, 0, groups, [=](float x) { return x >= lo; });
+      const int b = narrow<T, VEC>(a, row, s, exact, true, weight, unit, above_count, above_mass, inside, bucket);
+      last = b < kBuckets ? last_of_prefix<T, VEC>(a, row, s, exact, weight, unit, unused, bucket, b, above_count, above_mass,
+                                                   inside)
+                          : 0;
+      __syncthreads();
+      for (int g = tid; g < groups; g += kThreads) s.group_mass[g] = 0.0;
+      __syncthreads();
+      for (int j = tid >> 4; j < s.n_active; j += kThreads / 16) {
+        const int g = s.active[j], lane = (g & 3) * 16 + (tid & 15);
+        float v[16];
+        load_chunk<T, VEC>(a, row, g >> 2, lane, v);
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 16; e++) sum += Stay{lo, last, floor}(weight, v[e], index_of(g >> 2, lane, e));
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if ((tid & 15) == 0) s.group_mass[g] = sum;
+      }
+      __syncthreads();
+      mass = 0.0;
+      if (tid < chunks)
+        for (int g = 0; g < kGroups; g++) mass += s.group_mass[kGroups * tid + g];
+      __syncthreads();
     }
-    // (the sums of the chunk, in another order, can end below r: the last value with a weight)
-    const uint64_t ends = __ballot(end >= 0);
-    if (ends) {
-      const int l = 63 - __builtin_clzll(ends);
-      at = __shfl(end, l, 64);
-      chosen = __shfl(ew, l, 64);
-    }
-    sum += __shfl(run, 63, 64);
   }
-  if (tid == 0) answer(a, row, at, chosen / total);
+  draw<kThreads, T, VEC>(a, row, weight, Stay{lo, last, floor}, mass, number_of(a, row), chunks, s.sums, &s.found);
+}
+
+// Slices of a row until two workgroups a CU are there, of 8 chunks at least.
+int slices_of(int64_t rows, int chunks, int cus) {
+  const int64_t want = 2 * cus / rows, most = chunks / 8;
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+
+template <int T, bool VEC>
+hipError_t launch_rows(const SampleArgs& a, hipStream_t st) {
+  const int chunks = (a.vocab + kChunk - 1) / kChunk;
+  int bits = 63;  // a row's weights add up to less than 2^64 units
+  while (((int64_t)1 << (63 - bits)) < a.vocab) bits--;
+  bits = bits < 52 ? bits : 52;
+  sample_chunks_kernel<T, VEC><<<dim3((unsigned)((chunks + 3) / 4), (unsigned)a.rows), 256, 0, st>>>(a, chunks);
+  if (!a.states) {
+    sample_pick_kernel<T, VEC><<<(unsigned)a.rows, kMostChunks, 0, st>>>(a, chunks);
+  } else {
+    const dim3 grid((unsigned)a.slices, (unsigned)a.rows);
+    sample_select_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, bits);
+    sample_finish_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, bits);
+  }
+  return hipGetLastError();
 }
 
 template <int T>
 hipError_t launch_type(const SampleArgs& a, hipStream_t st) {
-  const int chunks = (a.vocab + kChunk - 1) / kChunk;
-  int bits = 0;
-  while (((int64_t)1 << bits) < a.vocab) bits++;
-  const dim3 grid((unsigned)((chunks + 3) / 4), (unsigned)a.rows);
-  if (a.vec) {
-    sample_chunks_kernel<T, true><<<grid, 256, 0, st>>>(a, chunks);
-    sample_rows_kernel<T, true><<<(unsigned)a.rows, kThreads, 0, st>>>(a, chunks, bits);
-  } else {
-    sample_chunks_kernel<T, false><<<grid, 256, 0, st>>>(a, chunks);
-    sample_rows_kernel<T, false><<<(unsigned)a.rows, kThreads, 0, st>>>(a, chunks, bits);
-  }
-  return hipGetLastError();
+  return a.vec ? launch_rows<T, true>(a, st) : launch_rows<T, false>(a, st);
 }
 
 }  // namespace
 
 int64_t sample_most_vocab() { return kMostVocab; }
 
-size_t sample_plan(SampleArgs& a, void* ws) {
-  const size_t chunks = (size_t)a.rows * ((a.vocab + kChunk - 1) / kChunk);
-  a.masses = (double*)ws;
-  a.maxima = (float*)((uintptr_t)ws + chunks * sizeof(double));
-  return chunks * (sizeof(double) + kGroups * sizeof(float));
+size_t sample_plan(SampleArgs& a, void* ws, int cus) {
+  const int chunks = (a.vocab + kChunk - 1) / kChunk;
+  const size_t rows = a.rows < kMostRows ? a.rows : kMostRows;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const uintptr_t p = (uintptr_t)ws + at;  // (integers: a plan has no workspace)
+    at += align_up(bytes, 16);
+    return (void*)p;
+  };
+  a.masses = (double*)take(rows * chunks * sizeof(double));
+  a.maxima = (float*)take(rows * chunks * kGroups * sizeof(float));
+  if (a.top_k || a.top_p || a.min_p) {
+    a.slices = slices_of(rows, chunks, cus);
+    a.kept = (double*)take(rows * chunks * sizeof(double));
+    a.parts = (double*)take(rows * a.slices * kBuckets * sizeof(double));
+    a.lists = (uint64_t*)take(rows * kList * sizeof(uint64_t));
+    a.states = (SampleState*)take(rows * sizeof(SampleState));
+  }
+  return at;
 }
 
-hipError_t launch_sample(const SampleArgs& a, int dtype, hipStream_t st) {
+hipError_t launch_sample(const SampleArgs& all, int dtype, hipStream_t st) {
   QMM_NOTE_LAUNCH();
-  switch (dtype) {
-    case QMM_X_F16: return launch_type<QMM_X_F16>(a, st);
-    case QMM_X_BF16: return launch_type<QMM_X_BF16>(a, st);
-    default: return launch_type<QMM_X_F32>(a, st);
+  hipError_t e = hipSuccess;
+  for (int64_t r = 0; r < all.rows && e == hipSuccess; r += kMostRows) {
+    SampleArgs a = all;
+    a.rows = (int)(all.rows - r < kMostRows ? all.rows - r : kMostRows);
+    a.logits = (const char*)all.logits + r * all.stride * value_bytes(dtype);
+    a.u += r;
+    a.ids += r;
+    if (a.temperature) a.temperature += r;
+    if (a.top_k) a.top_k += r;
+    if (a.top_p) a.top_p += r;
+    if (a.min_p) a.min_p += r;
+    if (a.probs) a.probs += r;
+    switch (dtype) {
+      case QMM_X_F16: e = launch_type<QMM_X_F16>(a, st); break;
+      case QMM_X_BF16: e = launch_type<QMM_X_BF16>(a, st); break;
+      default: e = launch_type<QMM_X_F32>(a, st);
+    }
   }
+  return e;
 }
 
 }  // namespace qmm

@@ -59,7 +59,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     probs = torch.empty(rows, dtype=torch.float32, device=device)
     if rows:
         with on_device(device):
-            need = _need(vocab, rows)
+            need = _need(device.index, vocab, rows, top_k is not None or top_p is not None or min_p is not None)
             size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
             ws = torch.empty(need, dtype=torch.uint8, device=device)
@@ -70,9 +70,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
 
 
 @functools.lru_cache(maxsize=1024)
-def _need(vocab: int, rows: int) -> int:
-    """The workspace bytes that qmm_sample plans."""
-    need = ctypes.c_size_t(0)
-    check("qmm_sample", lib().qmm_sample(None, 0, vocab, None, None, None, None, None, None, None, vocab, rows, None, 0,
+def _need(device: int, vocab: int, rows: int, settings: bool) -> int:
+    """The workspace bytes that qmm_sample plans on the current device (`device`): by the sizes, and whether a setting
+    but the temperature is given."""
+    need, some = ctypes.c_size_t(0), 256 if settings else None  # any address: planning reads none
+    check("qmm_sample", lib().qmm_sample(None, 0, vocab, None, None, some, None, None, None, None, vocab, rows, None, 0,
                                          ctypes.byref(need), 0, 0))
     return need.value

@@ -164,6 +164,22 @@ def test_a_row_does_not_depend_on_its_place(dtype):
         assert torch.equal(got.ids, whole.ids[s]) and torch.equal(got.probs, whole.probs[s])
 
 
+def test_many_rows():
+    # more rows than a launch takes: every row as on its own
+    import swarmllm_amd as sa
+
+    few = logits(6, 25, 1300)
+    x = few.repeat(200, 1)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    u, t, p, m = (torch.rand(25, generator=g, device=DEV) for _ in range(4))
+    k = torch.randint(0, 1300, (25,), generator=g, device=DEV).to(torch.int32)
+    for settings in ((t, None, None, None), (t, None, p, None), (t, k, p, m * 0.1)):
+        want = sa.sample(few, u, *settings)
+        got = sa.sample(x, u.repeat(200), *(None if v is None else v.repeat(200) for v in settings))
+        assert torch.equal(got.ids.view(200, 25), want.ids.expand(200, 25))
+        assert torch.equal(got.probs.view(200, 25), want.probs.expand(200, 25))
+
+
 def test_captured_and_on_another_stream():
     import swarmllm_amd as sa
 
