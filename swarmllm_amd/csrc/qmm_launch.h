@@ -363,7 +363,7 @@ hipError_t launch_lora(const LoraArgs& a, int xdt, int wdt, hipStream_t st);
 struct SampleState {
   int32_t mode;
   float top, lo;
-  int32_t ticket, listed, by_count;
+  int32_t ticket, listed, by_count, above;
   double goal;    // the weight or the number of a prefix
   uint64_t last;  // or the rank of its last value
   double scale, floor;
@@ -384,7 +384,7 @@ struct SampleArgs {
   double* masses;
   // and with settings (null without): histograms [rows][slices][buckets], the
   // weights that stay [rows][chunks], a border's values [rows][1024], the rows' states
-  double* parts;
+  float* parts;
   double* kept;
   uint64_t* lists;
   SampleState* states;

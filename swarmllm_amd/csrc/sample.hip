@@ -48,7 +48,7 @@ constexpr int kBuckets = 2048;  // two a thread
 constexpr double kLog2e = 1.4426950408889634;
 
 // 16 values of chunk c at a lane's places 256 q + 4 lane + e; what is past the
-// row, or NaN, is -inf.
+// row is -inf.
 template <int T, bool VEC>
 __device__ __forceinline__ void load_chunk(const SampleArgs& a, int64_t row, int c, int lane, float v[16]) {
   const int64_t at = row * a.stride + c * kChunk + 4 * lane;
@@ -62,8 +62,6 @@ __device__ __forceinline__ void load_chunk(const SampleArgs& a, int64_t row, int
       v[e] = c * kChunk + 4 * lane + i < a.vocab ? load1<T>(a.logits, at + i) : -INFINITY;
     }
   }
-#pragma unroll
-  for (int e = 0; e < 16; e++) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
 }
 __device__ __forceinline__ int index_of(int c, int lane, int e) { return c * kChunk + 256 * (e >> 2) + 4 * lane + (e & 3); }
 
@@ -124,6 +122,8 @@ __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int ch
   if (c >= chunks) return;
   float v[16];
   load_chunk<T, VEC>(a, row, c, lane, v);
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e] = v[e] == v[e] ? v[e] : -INFINITY;
   bool greedy;
   const double scale = scale_of(a, row, greedy);
   float m = v[0];
@@ -193,7 +193,7 @@ struct Shared {
   double sums[16];
   uint64_t sums64[16];
   uint32_t sums32[16];
-  int n_active, n_list, found;
+  int n_active, n_list, found, found2;  // (the last two one after the other)
 };
 
 // The value of lane ^ M of the wave, on the vector unit (a shuffle goes through LDS: a
@@ -294,6 +294,25 @@ __device__ __forceinline__ uint64_t sort_step(uint64_t v, bool up) {
   return (((threadIdx.x & M) == 0) == up) == (o < v) ? o : v;
 }
 
+// The least of the threads' numbers a, and of b.
+__device__ __forceinline__ int2 block_least2(int a, int b, int* found) {
+  if (threadIdx.x < 2) found[threadIdx.x] = INT32_MAX;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    a = min(a, __shfl_xor(a, d, 64));
+    b = min(b, __shfl_xor(b, d, 64));
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    if (a != INT32_MAX) atomicMin(found, a);
+    if (b != INT32_MAX) atomicMin(found + 1, b);
+  }
+  __syncthreads();
+  const int2 r = make_int2(found[0], found[1]);
+  __syncthreads();
+  return r;
+}
+
 // One number a thread, sorted over the first n2 threads (a power of two, 64 at
 // least), the least first. The waves past them only meet the barriers.
 __device__ __forceinline__ uint64_t block_sort(uint64_t v, int n2, uint64_t* buf) {
@@ -353,12 +372,13 @@ __device__ __forceinline__ void activate(Shared& s, int g0, int g1, In in) {
   __syncthreads();
 }
 
-// The values that `in` takes into the list (the first kList that come), and how many there are.
+// The values from lo on that `in` takes into the list (the first kList that
+// come), and how many there are. lo is a number: NaN and -inf are not there.
 template <int T, bool VEC, typename In>
 __device__ __forceinline__ int collect(const SampleArgs& a, int64_t row, Shared& s, In in) {
+  constexpr int kUnits = kThreads / 16;
   if (threadIdx.x == 0) s.n_list = 0;
   __syncthreads();
-  constexpr int kUnits = kThreads / 16;
   const int n = s.n_active;
   // two groups on their way at once; over once the list is
   for (int k = threadIdx.x >> 4; k < n && *(volatile int*)&s.n_list <= kList; k += 2 * kUnits) {
@@ -372,14 +392,14 @@ __device__ __forceinline__ int collect(const SampleArgs& a, int64_t row, Shared&
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       if (k + h * kUnits >= n) break;
-      uint32_t those = 0;
+      int those = 0;
 #pragma unroll
-      for (int e = 0; e < 16; e++) those |= v[h][e] != -INFINITY && in(v[h][e]) ? 1u << e : 0u;
+      for (int e = 0; e < 16; e++) those += in(v[h][e]) ? 1 : 0;
       if (those == 0) continue;
-      int at = atomicAdd(&s.n_list, __popc(those));  // one addition a lane
+      int at = atomicAdd(&s.n_list, those);  // one addition a lane
 #pragma unroll
       for (int e = 0; e < 16; e++)
-        if (those >> e & 1) {
+        if (in(v[h][e])) {
           if (at < kList) s.list[at] = rank_of(v[h][e], index_of(g[h] >> 2, (g[h] & 3) * 16 + (threadIdx.x & 15), e));
           at++;
         }
@@ -407,7 +427,7 @@ __device__ __forceinline__ void histogram(const SampleArgs& a, int64_t row, Shar
   }
   __syncthreads();
   each_value<T, VEC>(a, row, s, [&](float x, int i) {
-    const int b = x != -INFINITY ? bucket(x, i) : -1;
+    const int b = x > -INFINITY ? bucket(x, i) : -1;
     if (b < 0) return;
     atomicAdd(&s.h.count[b], 1u);
     if (weights) atomicAdd((unsigned long long*)&s.h.mass[b], (unsigned long long)unit(weight(x)));
@@ -528,7 +548,7 @@ __device__ __forceinline__ uint64_t last_of_prefix(const SampleArgs& a, int64_t 
   if (inside <= kList) {
     const int n = min(kList, collect<T, VEC>(a, row, s, [=](float x) {
                          const uint32_t k = key_of(x);
-                         return k >= l && k <= h;
+                         return x == x && k >= l && k <= h;
                        }));
     return last_in_list(s, goal, weight, unit, n, above_count, above_mass, mass);
   }
@@ -564,7 +584,7 @@ struct Stay {
   uint64_t last;
   double floor;
   __device__ __forceinline__ double operator()(const Weights& weight, float x, int i) const {
-    if (!(x >= lo && x != -INFINITY && rank_of(x, i) >= last)) return 0.0;
+    if (!(x >= lo && x > -INFINITY && (last == 0 || rank_of(x, i) >= last))) return 0.0;
     const double w = weight(x);
     return w >= floor ? w : 0.0;
   }
@@ -573,7 +593,7 @@ struct Stay {
 // The first by index of the values that stay at which their sum passes u of the
 // total: the chunk from the chunks' weights (thread c's of chunk c), the value
 // from the chunk.
-template <int NT, int T, bool VEC>
+template <int NT, int T>
 __device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Weights& weight, const Stay& stay, double mass,
                                      double u, int chunks, double* sums, int* found) {
   const int tid = threadIdx.x;
@@ -584,50 +604,45 @@ __device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Wei
   if (c == INT32_MAX) c = -block_least(some ? -tid : INT32_MAX, found);
   if (tid == c) sums[0] = upto - mass;
   __syncthreads();
-  if (tid >= 64) return;
-  double sum = sums[0], chosen = 0.0;
-  float v[16];
-  load_chunk<T, VEC>(a, row, c, tid, v);
-  double w[16], run[4];
+  const double sum = sums[0];
+  __syncthreads();
+  constexpr int E = kChunk / NT;
+  double w[E], mine = 0.0, unused;
 #pragma unroll
-  for (int e = 0; e < 16; e++) w[e] = stay(weight, v[e], index_of(c, tid, e));
-#pragma unroll
-  for (int q = 0; q < 4; q++) run[q] = wave_sums((w[4 * q] + w[4 * q + 1]) + (w[4 * q + 2] + w[4 * q + 3]));
-  int at = -1;
-  bool found_it = false;
-#pragma unroll
-  for (int q = 0; q < 4; q++) {
-    const double before = __shfl_up(run[q], 1, 64);
-    double upto = sum + (tid ? before : 0.0);
-    int place = -1, end = -1;
-    double pw = 0.0, ew = 0.0;
-#pragma unroll
-    for (int e = 4 * q; e < 4 * q + 4; e++) {
-      upto += w[e];
-      if (w[e] > 0.0) {
-        end = index_of(c, tid, e);
-        ew = w[e];
-        if (place < 0 && upto > r) {
-          place = end;
-          pw = w[e];
-        }
-      }
-    }
-    const uint64_t hits = __ballot(place >= 0), ends = __ballot(end >= 0);
-    if (!found_it && hits) {
-      const int l = __builtin_ctzll(hits);
-      at = __shfl(place, l, 64);
-      chosen = __shfl(pw, l, 64);
-      found_it = true;
-    } else if (!found_it && ends) {
-      // (the sums of the chunk, in another order, can end below r: the last value with a weight)
-      const int l = 63 - __builtin_clzll(ends);
-      at = __shfl(end, l, 64);
-      chosen = __shfl(ew, l, 64);
-    }
-    sum += __shfl(run[q], 63, 64);
+  for (int e = 0; e < E; e++) {
+    const int i = c * kChunk + E * tid + e;
+    w[e] = i < a.vocab ? stay(weight, load1<T>(a.logits, row * a.stride + i), i) : 0.0;
+    mine += w[e];
   }
-  if (tid == 0) answer(a, row, at, chosen / total);
+  double before = sum + (block_sums<NT, double>(mine, sums, unused) - mine);
+  int place = INT32_MAX, end = -1;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    before += w[e];
+    if (w[e] > 0.0) {
+      end = E * tid + e;
+      if (place == INT32_MAX && before > r) place = end;
+    }
+  }
+  int at = block_least(place, found);
+  // (the sums of the chunk, in another order, can end below r: the last value with a weight)
+  if (at == INT32_MAX) at = -block_least(end >= 0 ? -end : INT32_MAX, found);
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    if (at == E * tid + e) answer(a, row, c * kChunk + at, w[e] / total);
+}
+
+// The weights of the values that stay, a thread each, added to their chunks:
+// thread c's of chunk c. As whole numbers of 2^-52, so in any order.
+__device__ __forceinline__ double to_chunks(Shared& s, int chunks, bool stays, uint64_t rank, double w) {
+  const Units unit{52};
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid < chunks) s.list[tid] = 0;
+  __syncthreads();
+  if (stays) atomicAdd((unsigned long long*)&s.list[(uint32_t)~rank >> 10], (unsigned long long)unit(w));
+  __syncthreads();
+  return tid < chunks ? (double)s.list[tid] / unit.size() : 0.0;
 }
 
 __device__ __forceinline__ double number_of(const SampleArgs& a, int64_t row) {
@@ -688,7 +703,7 @@ __global__ __launch_bounds__(kMostChunks) void sample_pick_kernel(SampleArgs a, 
     if (threadIdx.x == 0) answer(a, row, first, 1.0);
   } else {
     const Weights weight{&powers, top, scale};
-    draw<NT, T, VEC>(a, row, weight, Stay{-INFINITY, 0, 0.0}, chunk_weight(a, row, maxima, chunks, weight), number_of(a, row),
+    draw<NT, T>(a, row, weight, Stay{-INFINITY, 0, 0.0}, chunk_weight(a, row, maxima, chunks, weight), number_of(a, row),
                      chunks, sums, &found);
   }
 }
@@ -767,7 +782,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   const double floor = a.min_p && a.min_p[row] > 0.0f ? fmin((double)a.min_p[row], 1.0) : 0.0;
   const double u = number_of(a, row);
   if (!k_on && !p_on && floor == 0.0) {
-    draw<kThreads, T, VEC>(a, row, weight, Stay{-INFINITY, 0, 0.0}, mass, u, chunks, s.sums, &s.found);
+    draw<kThreads, T>(a, row, weight, Stay{-INFINITY, 0, 0.0}, mass, u, chunks, s.sums, &s.found);
     return;
   }
   double total;
@@ -782,6 +797,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   float lo = at >= (double)top ? top : (float)at;
   if ((double)lo > at) lo = value_of(key_of(lo) - 1);
   if (top == INFINITY) lo = top;
+  lo = fmaxf(lo, -FLT_MAX);  // -inf is never drawn
   const Goal goal{k_on, k_on ? (uint64_t)k : (uint64_t)(fmax(p, 0.0) * total * unit.size())};
 
   if (wide) {
@@ -795,15 +811,15 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
     const float scale32 = (float)scale;
     const bool only_top = top == INFINITY || scale == (double)INFINITY;
     each_value<T, VEC>(a, row, s, [&](float x, int i) {
-      if (!(x >= lo) || x == -INFINITY) return;
+      if (!(x >= lo)) return;
       const float w = only_top ? (x == top ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f((x - top) * scale32);
       atomicAdd(&s.part[bucket(x, i)], k_on ? 1.0 : (double)w);
     });
     __syncthreads();
-    double* const part = a.parts + (row * a.slices + slice) * kBuckets;
-    for (int b = tid; b < kBuckets; b += kThreads) part[b] = s.part[b];
+    float* const part = a.parts + (row * a.slices + slice) * kBuckets;  // (counts are whole in 32 bits too)
+    for (int b = tid; b < kBuckets; b += kThreads) part[b] = (float)s.part[b];
     if (tid == 0 && slice == 0)
-      a.states[row] = SampleState{kHistogram, top, lo, 0, 0, k_on, k_on ? (double)k : fmax(p, 0.0) * total, 0, scale, floor};
+      a.states[row] = SampleState{kHistogram, top, lo, 0, 0, k_on, 0, k_on ? (double)k : fmax(p, 0.0) * total, 0, scale, floor};
     return;
   }
 
@@ -828,12 +844,12 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   if (deepest < kBuckets && bucket.inv > 0.0f) lo = fmaxf(lo, top - (float)(deepest + 2) / bucket.inv);
   activate(s, 0, groups, [=](float x) { return x >= lo; });
   // min_p alone, and most groups hold some of its values: more than the list does, as a rule
-  const bool many = !k_on && s.n_active > 3 * groups / 4 && groups >= 256;
-  int n = many ? kList + 1 : collect<T, VEC>(a, row, s, [=](float x) { return x >= lo; });
+  const bool overfull = !k_on && s.n_active > 3 * groups / 4 && groups >= 256;
+  int n = overfull ? kList + 1 : collect<T, VEC>(a, row, s, [=](float x) { return x >= lo; });
   uint64_t last = 0;  // the rank of the last value of the prefix
   if (n > kList) {
     if (!k_on) {  // min_p alone: all the values past its line, which every slice then sums
-      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0.0, 0, scale, floor};
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, 0.0, 0, scale, floor};
       return;
     }
     // very many values, or equal ones: narrowed down by this workgroup
@@ -857,7 +873,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
           last = max(last, last_of_prefix<T, VEC>(a, row, s, run, weight, unit, kept_mass, bucket, b, above_count,
                                                   above_mass, inside));
       }
-      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0.0, last, scale, floor};
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, 0.0, last, scale, floor};
       return;
     }
   }
@@ -867,19 +883,16 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
     if (tid < 64) finish_wave(a, row, weight, tid < n ? s.list[tid] : 0, n, k, p, goal_of, floor, u);
     return;
   }
-  uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
-  double w = tid < n && tid < k ? weight(ranked_value(r)) : 0.0, all;
+  const uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
+  const double w = tid < n && tid < k ? weight(ranked_value(r)) : 0.0;
+  double all;
   const double sum = block_sums<kThreads, double>(w, s.sums, all);
   const double run = fmax(p, 0.0) * (k_on ? all : total);
   const bool stays = tid < n && tid < k && (!p_on || tid == 0 || sum - w < run) && w >= floor;
-  // those that stay, by index
-  r = block_sort(stays ? (uint64_t)(uint32_t)~r << 32 | r >> 32 : ~0ull, sort_size(n), s.list);
-  const bool there = r != ~0ull;
-  w = there ? weight(value_of((uint32_t)r)) : 0.0;
-  const double upto = block_sums<kThreads, double>(w, s.sums, all);
-  int hit = block_least(w > 0.0 && upto > u * all ? tid : INT32_MAX, &s.found);
-  if (hit == INT32_MAX) hit = -block_least(w > 0.0 ? -tid : INT32_MAX, &s.found);  // u of 1
-  if (tid == hit) answer(a, row, (int)(r >> 32), w / all);
+  const int staying = min(block_least(stays ? INT32_MAX : tid, &s.found), n);  // (they come first)
+  if (tid == staying - 1) s.sums64[0] = r;
+  const double kept = to_chunks(s, chunks, stays, r, w);
+  draw<kThreads, T>(a, row, weight, Stay{lo, s.sums64[0], floor}, kept, u, chunks, s.sums, &s.found);
 }
 
 // Rows of which many values stay: sums by chunk, and the border's values sorted
@@ -900,15 +913,14 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
   const Weights weight{&s.powers, top, state->scale};
   const Buckets bucket(top, lo);
   uint64_t last = state->last;
-  double above = 0.0;                    // the values of the buckets before the border's
   int from = kBuckets, to = kBuckets - 1;  // the buckets that hold the border
   if (mode == kHistogram) {
     double m[2] = {0.0, 0.0};
 #pragma unroll 8
     for (int i = 0; i < a.slices; i++) {
-      const double2 p = *(const double2*)(a.parts + (row * a.slices + i) * kBuckets + 2 * tid);
-      m[0] += p.x;
-      m[1] += p.y;
+      const float2 p = *(const float2*)(a.parts + (row * a.slices + i) * kBuckets + 2 * tid);
+      m[0] += (double)p.x;
+      m[1] += (double)p.y;
     }
     double all;
     const double upto = block_sums<kThreads, double>(m[0] + m[1], s.sums, all);
@@ -916,43 +928,46 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     const double off = by_count ? 0.0 : 1e-4 * goal;
     auto first = [&](double want) {
       const bool met = upto > 0.0 && upto >= want, sooner = upto - m[1] > 0.0 && upto - m[1] >= want;
-      return block_least(met ? 2 * tid + !sooner : INT32_MAX, &s.found);
+      return met ? 2 * tid + !sooner : INT32_MAX;
     };
-    from = min(first(goal - off), kBuckets);
-    to = off > 0.0 ? min(first(goal + off), kBuckets - 1) : min(from, kBuckets - 1);
-    if (by_count) {
-      if (tid == from / 2) s.sums[0] = upto - m[1] - (from & 1 ? 0.0 : m[0]);
-      __syncthreads();
-      above = s.sums[0];
-      __syncthreads();
-    }
+    const int2 both = block_least2(first(goal - off), first(goal + off), &s.found);
+    from = min(both.x, kBuckets);
+    to = min(both.y, kBuckets - 1);
   }
-  const int c0 = slice_begin(chunks, slice, a.slices), c1 = slice_begin(chunks, slice + 1, a.slices);
+  // the border's range of values: what is above it stays, what is in it is listed
   const float least = last ? fmaxf(lo, ranked_value(last)) : lo;
-  activate(s, kGroups * c0, kGroups * c1, [=](float x) { return x >= least && bucket(x, 0) <= max(from, to); });
+  float hi = least, low = least;
+  if (from < kBuckets) {
+    // (the step above the bucket's upper edge: what lies on it is listed)
+    hi = bucket.inv > 0.0f && from > 0 ? value_of(key_of(top - (float)from / bucket.inv) + 1) : INFINITY;
+    low = bucket.inv > 0.0f && to < kBuckets - 1 ? fmaxf(lo, top - (float)(to + 1) / bucket.inv) : lo;
+  }
+  const int slices = gridDim.x, c0 = slice_begin(chunks, slice, slices), c1 = slice_begin(chunks, slice + 1, slices);
+  activate(s, kGroups * c0, kGroups * c1, [=](float x) { return x >= low; });
   for (int g = kGroups * c0 + tid; g < kGroups * c1; g += kThreads) s.group_mass[g] = 0.0;
   __syncthreads();
   const int n_active = s.n_active;
+  int count = 0;
   for (int j = tid >> 4; j < n_active; j += kThreads / 16) {
     const int g = s.active[j], lane = (g & 3) * 16 + (tid & 15);
     float v[16];
     load_chunk<T, VEC>(a, row, g >> 2, lane, v);
     double sum = 0.0;
-    uint32_t border = 0;
+    int border = 0;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-      const int i = index_of(g >> 2, lane, e), b = v[e] >= lo && v[e] != -INFINITY ? bucket(v[e], i) : kBuckets + 1;
-      if (b < from && (last == 0 || rank_of(v[e], i) >= last)) {
+      if (v[e] >= hi && (last == 0 || rank_of(v[e], index_of(g >> 2, lane, e)) >= last)) {
         const double w = weight(v[e]);
         sum += w >= floor ? w : 0.0;
+        count++;
       }
-      border |= b >= from && b <= to ? 1u << e : 0u;
+      border += v[e] >= low && v[e] < hi ? 1 : 0;
     }
     if (border) {
-      int at = atomicAdd(&state->listed, __popc(border));
+      int at = atomicAdd(&state->listed, border);
 #pragma unroll
       for (int e = 0; e < 16; e++)
-        if (border >> e & 1) {
+        if (v[e] >= low && v[e] < hi) {
           if (at < kList) a.lists[row * kList + at] = rank_of(v[e], index_of(g >> 2, lane, e));
           at++;
         }
@@ -960,6 +975,11 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
     if ((tid & 15) == 0) s.group_mass[g] = sum;
+  }
+  if (by_count) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) count += __shfl_xor(count, d, 64);
+    if ((tid & 63) == 0 && count) atomicAdd(&state->above, count);
   }
   __syncthreads();
   for (int c = c0 + tid; c < c1; c += kThreads) {
@@ -969,7 +989,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     a.kept[row * chunks + c] = sum;
   }
   // the row's last workgroup goes on; what the others wrote is there for it
-  if (a.slices > 1) {
+  if (slices > 1) {
     __syncthreads();  // the workgroup's stores have reached its L2
     if (tid == 0) {
       __threadfence();
@@ -977,7 +997,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
       __threadfence();
     }
     __syncthreads();
-    const bool final = s.found == a.slices - 1;
+    const bool final = s.found == slices - 1;
     __syncthreads();
     if (!final) return;
   } else {
@@ -989,7 +1009,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     const int n = ((const volatile SampleState*)state)->listed;
     bool sure = n <= kList;
     if (sure) {
-      double all;
+      double all, above = (double)((const volatile SampleState*)state)->above;
       // (without what is under the floor: where some of it lies above the border, all of the border's values are under it)
       if (!by_count) (void)block_sums<kThreads, double>(mass, s.sums, above);
       if (tid < n) s.list[tid] = ((const volatile uint64_t*)a.lists)[row * kList + tid];
@@ -1000,17 +1020,12 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
       // the border's prefix: its first value too where nothing lies above it
       const bool in = tid < n && (by_count ? above + tid < goal : (tid == 0 && above == 0.0) || above + (upto - w) < goal);
       const int m = min(block_least(in ? INT32_MAX : tid, &s.found), n);
-      // whether the border is where the 32-bit weights said
-      sure = by_count || ((above < goal || above == 0.0) && (above + all >= goal || to == kBuckets - 1));
+      // whether the border is where the histogram said
+      sure = (above < goal || above == 0.0) && (above + (by_count ? n : all) >= goal || low <= lo);
       if (sure) {
         if (tid == m - 1) s.sums64[0] = r;
-        const int i = (int)(uint32_t)~r;
-        s.group_mass[tid] = in && w >= floor ? w : 0.0;
-        s.active[tid] = (uint16_t)(i >> 10);
-        __syncthreads();
+        mass += to_chunks(s, chunks, in && w >= floor, r, w);
         last = m ? s.sums64[0] : 0;
-        if (tid < chunks)
-          for (int j = 0; j < m; j++) mass += s.active[j] == tid ? s.group_mass[j] : 0.0;
         __syncthreads();
       }
     }
@@ -1046,7 +1061,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
       __syncthreads();
     }
   }
-  draw<kThreads, T, VEC>(a, row, weight, Stay{lo, last, floor}, mass, number_of(a, row), chunks, s.sums, &s.found);
+  draw<kThreads, T>(a, row, weight, Stay{lo, last, floor}, mass, number_of(a, row), chunks, s.sums, &s.found);
 }
 
 // Slices of a row until two workgroups a CU are there, of 8 chunks at least.
@@ -1066,9 +1081,9 @@ hipError_t launch_rows(const SampleArgs& a, hipStream_t st) {
   if (!a.states) {
     sample_pick_kernel<T, VEC><<<(unsigned)a.rows, kMostChunks, 0, st>>>(a, chunks);
   } else {
-    const dim3 grid((unsigned)a.slices, (unsigned)a.rows);
-    sample_select_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, bits);
-    sample_finish_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, bits);
+    sample_select_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
+    const int slices = chunks >= 16 * a.slices && a.rows <= 64 ? 2 * a.slices : a.slices;
+    sample_finish_kernel<T, VEC><<<dim3((unsigned)slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
   }
   return hipGetLastError();
 }
@@ -1096,7 +1111,7 @@ size_t sample_plan(SampleArgs& a, void* ws, int cus) {
   if (a.top_k || a.top_p || a.min_p) {
     a.slices = slices_of(rows, chunks, cus);
     a.kept = (double*)take(rows * chunks * sizeof(double));
-    a.parts = (double*)take(rows * a.slices * kBuckets * sizeof(double));
+    a.parts = (float*)take(rows * a.slices * kBuckets * sizeof(float));
     a.lists = (uint64_t*)take(rows * kList * sizeof(uint64_t));
     a.states = (SampleState*)take(rows * sizeof(SampleState));
   }
