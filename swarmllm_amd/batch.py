@@ -79,11 +79,10 @@ class PageTables:
         if tokens < 0 or tokens > 1 << 29:
             raise ValueError(f"PageTables.step: {tokens} tokens")
         device = self.device
-        q_starts = torch.empty(self.seqs + 1, dtype=torch.int32, device=device)
-        taken = torch.empty(self.seqs, dtype=torch.int32, device=device)
         slots = torch.empty(tokens, dtype=torch.int64, device=device)
-        positions = torch.empty(tokens, dtype=torch.int32, device=device)
-        seq = torch.empty(tokens, dtype=torch.int32, device=device)
+        # (two allocations for the five: a call is host time)
+        q_starts, taken, positions, seq = torch.empty(2 * (self.seqs + tokens) + 1, dtype=torch.int32, device=device) \
+            .split_with_sizes([self.seqs + 1, self.seqs, tokens, tokens])
         with on_device(device):
             check("qmm_pages_step", lib().qmm_pages_step(
                 self._ref, None if keep is None else keep.data_ptr(), None if new is None else new.data_ptr(), tokens,

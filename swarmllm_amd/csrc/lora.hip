@@ -621,6 +621,7 @@ int lora_most_slots() { return kMostSlots; }
 
 size_t lora_plan(LoraArgs& a, void* ws, int cus) {
   a.splits = splits_of(a, cus);
+  if (form_of(a) == kFused) return 0;
   size_t at = 0;
   for (int i = 0; i < a.count; i++) {
     a.t[i].mid = (float*)((uintptr_t)ws + at);

@@ -18,6 +18,7 @@
 
 #include "../../include/qmm.h"
 #include "mv_common.h"
+#include "wave_sums.h"
 
 namespace qmm {
 
@@ -29,12 +30,7 @@ constexpr int kMostThreads = 1024;
 template <typename T>
 __device__ __forceinline__ T block_sums(T v, T* wave_sums, T& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  T s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T up = __shfl_up(s, d, 64);
-    if (lane >= d) s += up;
-  }
+  const T s = qmm::wave_sums(v);
   __syncthreads();  // the sums of the call before are read
   if (lane == 63) wave_sums[wave] = s;
   __syncthreads();
@@ -48,27 +44,41 @@ __device__ __forceinline__ T block_sums(T v, T* wave_sums, T& total) {
   return before + s - v;
 }
 
-// The last b with starts[b] <= j (starts ascending, starts[0] = 0; j below starts[n]).
-__device__ __forceinline__ int owner(const int32_t* starts, int n, int32_t j) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= j)
-      lo = mid;
-    else
-      hi = mid;
+// The last b < n with starts[b] <= j, for N numbers at once (starts ascending,
+// starts[0] = 0; `top` the largest power of two below n, or 0).
+__device__ __forceinline__ int top_step(int n) { return n > 1 ? 1 << (31 - __builtin_clz(n - 1)) : 0; }
+template <int N>
+__device__ __forceinline__ void owners(const int32_t* starts, int n, int top, const int32_t j[N], int b[N]) {
+#pragma unroll
+  for (int u = 0; u < N; u++) b[u] = 0;
+  for (int step = top; step >= 1; step >>= 1) {
+    int32_t s[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) s[u] = starts[min(b[u] + step, n - 1)];
+#pragma unroll
+    for (int u = 0; u < N; u++)
+      if (b[u] + step < n && s[u] <= j[u]) b[u] += step;
   }
-  return lo;
+}
+__device__ __forceinline__ int owner(const int32_t* starts, int n, int top, int32_t j) {
+  int b[1];
+  owners<1>(starts, n, top, &j, b);
+  return b[0];
 }
 
-__device__ __forceinline__ void write_row(const PagesArgs& a, int64_t t, int b, int64_t pos) {
+// Pages that hold n positions (at most 2^30, so that nothing passes 32 bits).
+__device__ __forceinline__ int32_t pages_of(const PagesArgs& a, int32_t n) {
+  return (n + (1 << a.page_bits) - 1) >> a.page_bits;
+}
+
+__device__ __forceinline__ void write_row(const PagesArgs& a, int64_t t, int b, int32_t pos) {
   int64_t slot = -1;
   if (pos >= 0) {
-    const int32_t p = a.tables[b * a.table_stride + pos / a.page];
-    if (p >= 0) slot = (int64_t)p * a.page + pos % a.page;
+    const int32_t p = a.tables[b * (int32_t)a.table_stride + (pos >> a.page_bits)];
+    if (p >= 0) slot = ((int64_t)p << a.page_bits) + (pos & ((1 << a.page_bits) - 1));
   }
   a.slots[t] = slot;
-  if (a.positions) a.positions[t] = (int32_t)pos;
+  if (a.positions) a.positions[t] = pos;
   if (a.seq) a.seq[t] = b;
 }
 
@@ -83,7 +93,8 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
   int32_t* const s_need = s_freed + n + 1;    // [n + 1] pages taken before b
   int32_t* const s_rows = s_need + n + 1;     // [n + 1] rows before b
   int32_t* const s_took = s_rows + n + 1;     // [n] tokens taken, -1: refused
-  const int64_t cap = a.row_pages * a.page;
+  const int64_t cap = a.row_pages << a.page_bits;
+  const int top = top_step(n);
 
   int64_t freed_before = 0, rows_before = 0;
   for (int b0 = 0; b0 < n; b0 += threads) {
@@ -97,7 +108,7 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
       add = a.fresh ? max(0, a.fresh[b]) : 0;
       s_keep[b] = keep;
     }
-    const int32_t back = (len + a.page - 1) / a.page - (keep + a.page - 1) / a.page;
+    const int32_t back = pages_of(a, len) - pages_of(a, keep);
     int64_t total;
     const int64_t f = freed_before + block_sums<int64_t>(back, wave_sums, total);
     freed_before += total;
@@ -126,7 +137,7 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
       keep = s_keep[b];
       took = s_took[b];
     }
-    const int32_t want = took > 0 ? (int32_t)(((int64_t)keep + took + a.page - 1) / a.page) - (keep + a.page - 1) / a.page : 0;
+    const int32_t want = took > 0 ? pages_of(a, keep + took) - pages_of(a, keep) : 0;
     int64_t total;
     const int64_t before = need_before + block_sums<int64_t>(want, wave_sums, total);
     need_before += total;
@@ -140,23 +151,52 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
   if (tid == 0) s_need[n] = (int32_t)min(need_before, have);
   __syncthreads();
 
-  // the pages given back, on top of the stack, the first of them its end
-  for (int32_t j = tid; j < freed; j += threads) {
-    const int b = owner(s_freed, n, j);
-    const int32_t first = (s_keep[b] + a.page - 1) / a.page;
-    const int64_t at = have - 1 - j;
-    int32_t* const entry = a.tables + b * a.table_stride + first + (j - s_freed[b]);
-    if (at >= 0) a.free_pages[at] = *entry;
-    *entry = -1;
+  // the pages given back, on top of the stack, the first of them its end; four
+  // a thread at once, so that their loads overlap
+  for (int32_t j0 = tid; j0 < freed; j0 += 4 * threads) {
+    int32_t* entry[4];
+    int32_t p[4], j[4];
+    int of[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) j[u] = min(j0 + u * threads, freed - 1);
+    owners<4>(s_freed, n, top, j, of);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int b = of[u];
+      entry[u] = a.tables + b * (int32_t)a.table_stride + pages_of(a, s_keep[b]) + (j[u] - s_freed[b]);
+      p[u] = *entry[u];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t at = have - 1 - (j0 + u * threads);
+      if (j0 + u * threads >= freed) break;
+      if (at >= 0) a.free_pages[at] = p[u];
+      *entry[u] = -1;
+    }
   }
   __syncthreads();
   int32_t popped = 0;
-  for (int32_t j = tid; j < s_need[n]; j += threads) {
-    const int b = owner(s_need, n, j);
-    if (s_took[b] < 0) continue;
-    const int32_t first = (s_keep[b] + a.page - 1) / a.page;
-    a.tables[b * a.table_stride + first + (j - s_need[b])] = a.free_pages[have - 1 - j];
-    popped = j + 1;
+  const int32_t wanted = s_need[n];
+  for (int32_t j0 = tid; j0 < wanted; j0 += 4 * threads) {
+    int32_t* entry[4];
+    int32_t p[4], j[4];
+    int of[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) j[u] = min(j0 + u * threads, wanted - 1);
+    owners<4>(s_need, n, top, j, of);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int b = of[u];
+      const bool takes = j0 + u * threads < wanted && s_took[b] >= 0;
+      entry[u] = takes ? a.tables + b * (int32_t)a.table_stride + pages_of(a, s_keep[b]) + (j[u] - s_need[b]) : nullptr;
+      p[u] = a.free_pages[have - 1 - j[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (entry[u]) {
+        *entry[u] = p[u];
+        popped = j0 + u * threads + 1;
+      }
   }
   int64_t total;
   // (each thread's last page: the most of them is what left the stack)
@@ -178,8 +218,8 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
     if (t >= s_rows[n]) {
       write_row(a, t, -1, -1);
     } else {
-      const int b = owner(s_rows, n, (int32_t)t);
-      write_row(a, t, b, s_took[b] < 0 ? -1 : (int64_t)s_keep[b] + (t - s_rows[b]));
+      const int b = owner(s_rows, n, top, (int32_t)t);
+      write_row(a, t, b, s_took[b] < 0 ? -1 : s_keep[b] + ((int32_t)t - s_rows[b]));
     }
   }
 }
@@ -196,9 +236,9 @@ __global__ __launch_bounds__(256) void pages_rows_kernel(PagesArgs a) {
     write_row(a, t, -1, -1);
     return;
   }
-  const int b = owner(s_rows, a.seqs, (int32_t)t);
+  const int b = owner(s_rows, a.seqs, top_step(a.seqs), (int32_t)t);
   const int32_t took = a.taken[b];
-  write_row(a, t, b, took == 0 ? -1 : (int64_t)a.lens[b] - took + (t - s_rows[b]));
+  write_row(a, t, b, took == 0 ? -1 : a.lens[b] - took + ((int32_t)t - s_rows[b]));
 }
 
 }  // namespace

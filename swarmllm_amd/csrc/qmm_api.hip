@@ -1121,7 +1121,7 @@ int qmm_pages_step(const qmm_pages* pages, const int32_t* keep, const int32_t* f
       pages->page < 16 || pages->page > 256 || (pages->page & (pages->page - 1)) != 0 || pages->row_pages < 0 ||
       pages->table_stride < pages->row_pages || pages->pool < 0 || pages->pool > INT32_MAX ||
       pages->row_pages > ((int64_t)1 << 30) / pages->page ||
-      (int64_t)pages->seqs * pages->row_pages > INT32_MAX || !pages->free_count || !q_starts ||
+      pages->table_stride > INT32_MAX || (int64_t)pages->seqs * pages->table_stride > INT32_MAX || !pages->free_count || !q_starts ||
       (pages->row_pages > 0 && pages->seqs > 0 && !pages->tables) || (pages->pool > 0 && !pages->free_pages) ||
       (pages->seqs > 0 && (!pages->lens || !taken)) || (tokens > 0 && !slots))
     return QMM_UNSUPPORTED;
@@ -1129,7 +1129,7 @@ int qmm_pages_step(const qmm_pages* pages, const int32_t* keep, const int32_t* f
   a.tables = pages->tables; a.lens = pages->lens; a.free_pages = pages->free_pages; a.free_count = pages->free_count;
   a.keep = keep; a.fresh = fresh; a.q_starts = q_starts; a.taken = taken; a.slots = slots; a.positions = positions;
   a.seq = seq; a.table_stride = pages->table_stride; a.row_pages = pages->row_pages; a.pool = pages->pool;
-  a.tokens = tokens; a.seqs = pages->seqs; a.page = pages->page;
+  a.tokens = tokens; a.seqs = pages->seqs; a.page_bits = __builtin_ctz((unsigned)pages->page);
   clear_stale_error();
   return status_of(qmm::launch_pages_step(a, (hipStream_t)stream));
 }
@@ -1163,7 +1163,7 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
   if (!x || !ids || !aligned16(workspace)) return QMM_UNSUPPORTED;
   for (int i = 0; i < count; i++)
     if (!a.t[i].y || !a.t[i].out || (slots > 0 && (!a.t[i].a || !a.t[i].b))) return QMM_UNSUPPORTED;
-  if (workspace == nullptr || workspace_bytes < *need) return QMM_WORKSPACE_TOO_SMALL;
+  if (*need > 0 && (workspace == nullptr || workspace_bytes < *need)) return QMM_WORKSPACE_TOO_SMALL;
   clear_stale_error();
   return status_of(qmm::launch_lora(a, x_dtype, w_dtype, (hipStream_t)stream));
 }

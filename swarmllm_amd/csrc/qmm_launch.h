@@ -324,7 +324,7 @@ struct PagesArgs {
   int32_t* positions;
   int32_t* seq;
   int64_t table_stride, row_pages, pool, tokens;
-  int seqs, page;
+  int seqs, page_bits;
 };
 int pages_most_seqs();
 hipError_t launch_pages_step(const PagesArgs& a, hipStream_t st);

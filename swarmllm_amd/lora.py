@@ -88,10 +88,10 @@ class Adapters:
             need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             check("qmm_adapters_add", lib().qmm_adapters_add(
                 count, c, first.slots, _X_DTYPES[first.dtype], x.data_ptr(), x_type, xs, ids.data_ptr(), k, rows,
-                ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device)))
+                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device)))
         return outs
 
     def __repr__(self) -> str:
