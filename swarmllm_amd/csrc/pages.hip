@@ -25,6 +25,7 @@ namespace qmm {
 namespace {
 
 constexpr int kMostThreads = 1024;
+constexpr int kAtOnce = 2;  // pages a thread moves at once
 
 // Running sums over the workgroup's threads (in `v`'s own type), and the total.
 template <typename T>
@@ -151,23 +152,23 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
   if (tid == 0) s_need[n] = (int32_t)min(need_before, have);
   __syncthreads();
 
-  // the pages given back, on top of the stack, the first of them its end; four
-  // a thread at once, so that their loads overlap
-  for (int32_t j0 = tid; j0 < freed; j0 += 4 * threads) {
-    int32_t* entry[4];
-    int32_t p[4], j[4];
-    int of[4];
+  // the pages given back, on top of the stack, the first of them its end; two
+  // a thread at once, so that their searches and loads overlap (eight take no less: a search is 80 instructions)
+  for (int32_t j0 = tid; j0 < freed; j0 += kAtOnce * threads) {
+    int32_t* entry[kAtOnce];
+    int32_t p[kAtOnce], j[kAtOnce];
+    int of[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < 4; u++) j[u] = min(j0 + u * threads, freed - 1);
-    owners<4>(s_freed, n, top, j, of);
+    for (int u = 0; u < kAtOnce; u++) j[u] = min(j0 + u * threads, freed - 1);
+    owners<kAtOnce>(s_freed, n, top, j, of);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < kAtOnce; u++) {
       const int b = of[u];
       entry[u] = a.tables + b * (int32_t)a.table_stride + pages_of(a, s_keep[b]) + (j[u] - s_freed[b]);
       p[u] = *entry[u];
     }
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < kAtOnce; u++) {
       const int64_t at = have - 1 - (j0 + u * threads);
       if (j0 + u * threads >= freed) break;
       if (at >= 0) a.free_pages[at] = p[u];
@@ -177,22 +178,22 @@ __global__ __launch_bounds__(kMostThreads) void pages_plan_kernel(PagesArgs a, i
   __syncthreads();
   int32_t popped = 0;
   const int32_t wanted = s_need[n];
-  for (int32_t j0 = tid; j0 < wanted; j0 += 4 * threads) {
-    int32_t* entry[4];
-    int32_t p[4], j[4];
-    int of[4];
+  for (int32_t j0 = tid; j0 < wanted; j0 += kAtOnce * threads) {
+    int32_t* entry[kAtOnce];
+    int32_t p[kAtOnce], j[kAtOnce];
+    int of[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < 4; u++) j[u] = min(j0 + u * threads, wanted - 1);
-    owners<4>(s_need, n, top, j, of);
+    for (int u = 0; u < kAtOnce; u++) j[u] = min(j0 + u * threads, wanted - 1);
+    owners<kAtOnce>(s_need, n, top, j, of);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < kAtOnce; u++) {
       const int b = of[u];
       const bool takes = j0 + u * threads < wanted && s_took[b] >= 0;
       entry[u] = takes ? a.tables + b * (int32_t)a.table_stride + pages_of(a, s_keep[b]) + (j[u] - s_need[b]) : nullptr;
       p[u] = a.free_pages[have - 1 - j[u]];
     }
 #pragma unroll
-    for (int u = 0; u < 4; u++)
+    for (int u = 0; u < kAtOnce; u++)
       if (entry[u]) {
         *entry[u] = p[u];
         popped = j0 + u * threads + 1;
