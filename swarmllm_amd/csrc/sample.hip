@@ -789,10 +789,10 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
     __syncthreads();
     const Buckets bucket(top, lo);
     const float scale32 = (float)scale;
-    const bool only_top = top == INFINITY || scale == (double)INFINITY;
     each_value<T, VEC>(a, row, s, [&](float x, int i) {
       if (!(x >= lo)) return;
-      const float w = only_top ? (x == top ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f((x - top) * scale32);
+      // (no NaN: of an infinite scale, or of a difference past f32's range)
+      const float w = x == top ? 1.0f : __builtin_amdgcn_exp2f(fmaxf((x - top) * scale32, -200.0f));
       atomicAdd(&s.part[bucket(x, i)], k_on ? 1.0 : (double)w);
     });
     __syncthreads();

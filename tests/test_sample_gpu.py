@@ -134,6 +134,14 @@ def test_settings_past_their_range():
     check(x, u, temperature=[NAN, -1.0, INF, 1e-38, 1e-45, 1e30, 3e38, -0.0, 1e-6, 50.0, 1.0, -INF])
     check(x, u, temperature=[NAN, -1.0, INF, 1e-38, 1e-45, 1e30, 3e38, -0.0, 1e-6, 50.0, 1.0, -INF], top_k=[70, 2000] * 6,
           top_p=[0.9, 0.5, 1.0] * 4)
+    wild = [NAN, -1.0, INF, 1e-38, 1e-45, 1e30, 3e38, -0.0, 1e-6, 50.0, 1.0, -INF]
+    check(x, u, temperature=wild, top_p=[0.9, 0.5, 0.3] * 4)
+    check(x, u, temperature=wild, top_k=[3000] * 12)
+    huge = x.clone()
+    huge[:, ::3] = torch.finfo(torch.float32).max
+    huge[:, 1::3] = torch.finfo(torch.float32).min
+    check(huge, u, temperature=wild, top_p=[0.9, 0.5, 0.3] * 4)
+    check(huge, u, temperature=wild, top_k=[3000] * 12)
     check(x, u, top_k=[-2**31, -1, 0, 1, 4999, 5000, 5001, 2**31 - 1, 2, 1024, 1025, 4096])
     check(x, u, top_p=[NAN, -1.0, 0.0, 1e-30, 1.0, 2.0, INF, -INF, 1.0 - 2.0 ** -24, 0.5, 1e-3, 0.999])
     check(x, u, min_p=[NAN, -1.0, 0.0, 1e-30, 1.0, 2.0, INF, -INF, 1.0 - 2.0 ** -24, 0.5, 1e-3, 1e-45])
