@@ -619,6 +619,14 @@ hipError_t launch_x(const LoraArgs& a, int wdt, hipStream_t st) {
 int lora_most_rank() { return kMostRank; }
 int lora_most_slots() { return kMostSlots; }
 
+// A launch's threads in x stay below 2^32.
+bool lora_fits(const LoraArgs& a) {
+  if (form_of(a) != kTiles) return true;
+  int64_t widest = 0;
+  for (int i = 0; i < a.count; i++) widest = widest > a.t[i].n ? widest : a.t[i].n;
+  return (widest / kUpOut + 8) * tiles_of(a) < ((int64_t)1 << 32) / (64 * kUpWaves);
+}
+
 size_t lora_plan(LoraArgs& a, void* ws, int cus) {
   a.splits = splits_of(a, cus);
   if (form_of(a) == kFused) return 0;

@@ -1150,6 +1150,8 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
         d.y_stride < d.n || d.out_stride < d.n || (d.y == d.out && d.y && d.y_stride != d.out_stride) ||
         !aligned16(d.a) || !aligned16(d.b))
       return QMM_UNSUPPORTED;
+    for (int j = 0; j < i; j++)
+      if (d.out && d.out == adapters[j].out) return QMM_UNSUPPORTED;  // two projections in one place
     qmm::LoraTarget& t = a.t[i];
     t.a = d.a; t.b = d.b; t.scales = d.scales; t.y = d.y; t.out = d.out;
     t.n = d.n; t.ldy = d.y_stride; t.ldo = d.out_stride; t.rank = d.rank;
@@ -1157,6 +1159,7 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
   }
   *need = 0;
   if (rows == 0) return QMM_OK;
+  if (!qmm::lora_fits(a)) return QMM_UNSUPPORTED;
   *need = qmm::lora_plan(a, workspace, cu_count());
   if (!launch) return QMM_OK;
   if (g_fail_next.exchange(false)) return QMM_NO_ROOM;

@@ -356,6 +356,7 @@ struct LoraArgs {
 };
 int lora_most_rank();
 int lora_most_slots();
+bool lora_fits(const LoraArgs& a);
 size_t lora_plan(LoraArgs& a, void* ws, int cus);
 hipError_t launch_lora(const LoraArgs& a, int xdt, int wdt, hipStream_t st);
 

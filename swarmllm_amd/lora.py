@@ -84,6 +84,8 @@ class Adapters:
                            ad.rank)
         if rows == 0:
             return outs
+        if count > 1 and len({c[i].out for i in range(count)}) < count:
+            raise ValueError("Adapters.add_shared: one tensor for two projections")
         with on_device(device):
             need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)

@@ -33,7 +33,7 @@ def test_pages_refusals():
 
 def adapters_add(n=None, launch=0, count=1, slots=4, w=X_BF16, x=P, x_type=X_F32, x_stride=4096, ids=P, k=4096, rows=5,
                  ws=None, ws_bytes=0, **change):
-    c = (Adapter * 4)(*[Adapter(P, P, P, P, P, 1000, 1000, 1000, 16) for _ in range(4)])
+    c = (Adapter * 4)(*[Adapter(P, P, P, P, P + 4096 * i, 1000, 1000, 1000, 16) for i in range(4)])
     for key, v in change.items():
         setattr(c[0], key, v)
     n = n if n is not None else ctypes.c_size_t(7)
@@ -54,9 +54,17 @@ def test_adapters_plan_and_refusals():
     assert adapters_add(launch=1, ws=P + 4, ws_bytes=2 * need)[0] == QMM_UNSUPPORTED
     for bad in (dict(count=0), dict(count=5), dict(slots=-1), dict(slots=4097), dict(w=3), dict(x_type=-1), dict(x_stride=4095), dict(k=0),
                 dict(k=4080 + 8), dict(rows=-1), dict(rows=2**20 + 1), dict(n=ctypes.c_size_t(), rank=0), dict(rank=12),
-                dict(rank=136), dict(y_stride=999), dict(out_stride=999), dict(out_stride=1004), dict(a=P + 8),
+                dict(rank=136), dict(y_stride=999), dict(out_stride=999), dict(y=P, out=P, out_stride=1004), dict(a=P + 8),
                 dict(b=P + 4)):
         assert adapters_add(**bad)[0] == QMM_UNSUPPORTED, bad
+    # two projections into one place, and more workgroups than a launch takes
+    assert adapters_add(count=2)[0] == QMM_OK and adapters_add(count=2, out=2 * P)[0] == QMM_UNSUPPORTED
+    wide = dict(n=2**31 - 1, y_stride=2**31, out_stride=2**31)
+    c = (Adapter * 1)(Adapter(P, P, P, P, P, wide["n"], wide["y_stride"], wide["out_stride"], 16))
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 64, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+                                  0) == QMM_OK
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 100, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+                                  0) == QMM_UNSUPPORTED
     for null in (dict(x=None), dict(ids=None), dict(a=None), dict(b=None), dict(y=None), dict(out=None)):
         assert adapters_add(launch=1, ws=P, ws_bytes=2**20, **null)[0] == QMM_UNSUPPORTED, null
     st = lib().qmm_adapters_add(1, (Adapter * 1)(), 1, 0, P, 0, 4096, P, 4096, 1, None, 0, None, 0, 0)

@@ -187,6 +187,7 @@ def test_refusals():
                 lambda: ok.add(y.t().contiguous().t(), xs, ids), lambda: ok.add(y, xs, ids, out=y[:, :20]),
                 lambda: Adapters.add_shared([y, y], xs, [ok], ids), lambda: Adapters.add_shared([], xs, [], ids),
                 lambda: Adapters.add_shared([y, y], xs, [ok, other], ids),
-                lambda: Adapters.add_shared([y] * 5, xs, [ok] * 5, ids)):
+                lambda: Adapters.add_shared([y] * 5, xs, [ok] * 5, ids),
+                lambda: Adapters.add_shared([y, y], xs, [ok, ok], ids)):
         with pytest.raises(ValueError):
             bad()
