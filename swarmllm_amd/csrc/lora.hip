@@ -3,8 +3,11 @@
 // for A [slots][rank][k] and B [slots][n][rank] of up to four projections of
 // one activation; a row whose id names no slot keeps its y.
 //
-// Two launches: x against A into partial results in f32 (k in parts where the
-// rows alone do not fill the CUs), and those against B, y added.
+// Both products are bound by memory: of a row, A and B are read once and y goes in
+// and out, 2 operations a byte of adapter for a row alone; many rows of one adapter
+// share its A and B. So few rows are taken one by one on the vector units, and
+// many are sorted by their adapters into tiles of 32, whose products run on the
+// matrix cores (form_of, below). All sums are f32.
 #include "../../include/qmm.h"
 #include "qmm_device.h"
 #include "qmm_launch.h"
@@ -93,17 +96,13 @@ __device__ __forceinline__ void pieces_of(const Raw<T>& r, b8v out[kPieces<T>]) 
   }
 }
 
-// Values [i, i + N) of an array of type T, N 4 or 8. VEC: at an address that is
-// a multiple of their size (of 16 bytes at most); otherwise a value at a time.
-template <int T, int N, bool VEC>
+// 8 values from i on. VEC: at an address that is a multiple of 16 bytes;
+// otherwise a value at a time.
+template <int T, bool VEC>
 __device__ __forceinline__ void load_values(const void* p, int64_t i, float* v) {
-  if constexpr (N == 8) {
-    Raw<T> r;
-    r.template load<VEC>(p, i);
-    r.values(v);
-  } else {
-    load4<T, VEC>(p, i, v);
-  }
+  Raw<T> r;
+  r.template load<VEC>(p, i);
+  r.values(v);
 }
 
 // The adapter of row r, -1 without one.
@@ -124,11 +123,11 @@ __device__ __forceinline__ void dots(const void* x, int64_t xi, const void* w, i
 #pragma unroll 4
   for (int u = first; u < units; u += step) {
     float v[8];
-    load_values<XT, 8, VEC>(x, xi + 8 * u, v);
+    load_values<XT, VEC>(x, xi + 8 * u, v);
 #pragma unroll
     for (int j = 0; j < J; j++) {
       float a[8];
-      load_values<WT, 8, true>(w, wi + j * lda + 8 * u, a);
+      load_values<WT, true>(w, wi + j * lda + 8 * u, a);
 #pragma unroll
       for (int e = 0; e < 8; e++) sum[j] = fmaf(a[e], v[e], sum[j]);
     }
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(kRowThreads) void lora_row_kernel(LoraArgs a) {
 #pragma unroll 2
       for (int j = 0; j < t.rank; j += 8) {
         float b[8];
-        load_values<WT, 8, true>(t.b, at + j, b);
+        load_values<WT, true>(t.b, at + j, b);
 #pragma unroll
         for (int e = 0; e < 8; e++) sum = fmaf(b[e], s_mid[j + e], sum);
       }
@@ -495,7 +494,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int 
       for (int s = 0; s < S; s++) {
         const int j = 32 * s + 8 * g;
         float v[8];
-        load_values<QMM_X_F32, 8, true>(t.mid, row * t.rank + (j < t.rank ? j : 0), v);
+        load_values<QMM_X_F32, true>(t.mid, row * t.rank + (j < t.rank ? j : 0), v);
 #pragma unroll
         for (int q = 0; q < 8; q++) v[q] = j < t.rank ? v[q] * scale : 0.0f;
         pieces_of<MP>(v, m[h][s]);
@@ -538,14 +537,39 @@ int64_t tiles_of(const LoraArgs& a) {
   return (a.rows + kTile - 1) / kTile + (a.slots + 1 < a.rows ? a.slots + 1 : a.rows);
 }
 
-// How a call runs.
+// How a call runs, all times of calls in a replayed graph (bf16 adapters, f32 x).
+//
+// Rows one by one read A and B once a row, tiles once for 32 rows of one adapter,
+// but a tile is as dear for one row as for 32, and the rows have to be sorted
+// first. So rows one by one up to 64 of them, and while rows * rank, which their
+// work grows by, is at most 4096 (us one by one / in tiles; all rows with one
+// adapter, with 64 adapters in turn):
+//     64 rows, rank 64, 8192 to 8192        22 / 25     36 / 56
+//     128 rows, rank 32, 14336 to 4096      20 / 26     29 / 43
+//     256 rows, rank 16, 4096 to 2 x 14336  31 / 28     50 / 76
+//     128 rows, rank 64, 8192 to 8192       34 / 27     55 / 67
+//     512 rows, rank 16, 4096 to 2 x 14336  60 / 42     90 / 91
+//     512 rows, rank 64, 8192 to 8192       110 / 36    165 / 80
+//
+// Of rows one by one, the small ones in one launch: every workgroup of a row makes
+// the row's products with A for itself, which a second launch would hand it. That
+// is for an A of 2^16 values and while all workgroups together read at most 2^23
+// of them: then the one launch takes 1.5 to 2 us less or at most 3 more (one
+// launch / two: 1 row, rank 8, 896 to 896 4.7 / 6.7; 8 rows, rank 16, 4096 to
+// 4096 7.3 / 7.5; 16 rows, rank 16, 4096 to 6144 10.5 / 9.0), and a call that no
+// graph replays saves the host 4 us (8.4 / 12.3). Past it: 16 rows, rank 32, 4096
+// to 2 x 14336 19.9 / 12.6.
 enum Form { kFused, kRows, kTiles };
 
 Form form_of(const LoraArgs& a) {
   int rank = 0;
-  for (int i = 0; i < a.count; i++) rank = rank > a.t[i].rank ? rank : a.t[i].rank;
-  if (a.rows > 64) return kTiles;
-  return rank * a.k <= (int64_t)1 << 17 ? kFused : kRows;
+  int64_t groups = 0;
+  for (int i = 0; i < a.count; i++) {
+    rank = rank > a.t[i].rank ? rank : a.t[i].rank;
+    groups += a.rows * ((a.t[i].n + kRowOut - 1) / kRowOut);
+  }
+  if (a.rows > 64 && a.rows * rank > 4096) return kTiles;
+  return rank * a.k <= 1 << 16 && groups * rank * a.k <= 1 << 23 ? kFused : kRows;
 }
 
 // Parts of k: until the CUs have the 12 waves each that registers leave, of 4 steps

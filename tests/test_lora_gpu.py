@@ -33,7 +33,8 @@ CASES = [(1, 32, 1, 8, 1, "one"), (1, 4096, 4096, 16, 4, "one"), (2, 64, 17, 8, 
          (16, 512, 65, 16, 16, "mixed"), (17, 544, 129, 40, 5, "mixed"), (21, 4096, 1024, 16, 24, "mixed"),
          (33, 14336, 257, 64, 4, "runs"), (64, 2880, 300, 128, 40, "mixed"), (65, 1024, 1000, 16, 70, "mixed"),
          (77, 4096, 513, 32, 3, "runs"), (200, 8192, 96, 56, 2, "runs"), (513, 256, 777, 64, 6, "runs"),
-         (1000, 320, 64, 8, 100, "mixed"), (1300, 64, 3, 128, 2, "mixed")]
+         (1000, 320, 64, 8, 100, "mixed"), (1300, 64, 3, 128, 2, "mixed"),
+         (70, 1024, 1000, 64, 70, "mixed"), (300, 4096, 513, 16, 7, "mixed"), (300, 1024, 2100, 8, 40, "mixed")]
 
 
 @pytest.mark.parametrize("x,w", [("f32", "bf16"), ("f32", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"),
@@ -75,7 +76,7 @@ def test_whole_numbers_come_out_whole(rows, k, n, rank, slots, order, w):
     assert torch.equal(Adapters(a, b).add(y.clone(), xs, ids).double(), want)
 
 
-@pytest.mark.parametrize("rows", [1, 21, 100])
+@pytest.mark.parametrize("rows", [1, 21, 100, 300])
 def test_shared_projections_equal_their_own(rows):
     from swarmllm_amd import Adapters
 
@@ -98,7 +99,7 @@ def test_shared_projections_equal_their_own(rows):
 def test_strides_alignment_and_what_lies_between():
     from swarmllm_amd import Adapters
 
-    for rows in (3, 40, 90):
+    for rows in (3, 40, 270, 90):
         xs, a, b, scales, ids, y = make(rows, rows, 256, 50, 16, 3)
         wide = torch.full((rows, 400), 5.0, device=DEV)
         for off in (0, 1, 4):
@@ -117,7 +118,7 @@ def test_strides_alignment_and_what_lies_between():
     close(got.view(90, 50), want, bound)
 
 
-@pytest.mark.parametrize("rows", [16, 70])
+@pytest.mark.parametrize("rows", [16, 70, 300])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_an_adapter_reaches_its_own_rows_only(rows, bad):
     from swarmllm_amd import Adapters
@@ -146,7 +147,7 @@ def test_ids_outside_the_slots_and_no_slots():
     assert Adapters(a, b).add(y[:0], xs[:0], ids[:0]).shape == (0, 30)
 
 
-@pytest.mark.parametrize("rows", [4, 120])
+@pytest.mark.parametrize("rows", [4, 120, 300])
 def test_captured_and_on_another_stream(rows):
     from swarmllm_amd import Adapters
 
