@@ -14,6 +14,11 @@
 // pages needed) in LDS, then the pages that change hands, one a thread, each
 // finding its sequence by a binary search in those sums. Rows of a large batch
 // are a second launch over the CUs.
+//
+// A step moves a few KiB and computes next to nothing: what it takes is a launch (2.6 us
+// empty) and the latencies one after another of the loads, scans, searches and stores
+// (8 sequences of one new token each 4.2 us), and with hundreds of sequences the one
+// CU's instructions (256 sequences, 10240 rows 13.5 us).
 #include <hip/hip_runtime.h>
 
 #include "../../include/qmm.h"
@@ -253,6 +258,7 @@ hipError_t launch_pages_step(const PagesArgs& a, hipStream_t st) {
     const hipError_t e = set_max_dynamic_lds<pages_plan_kernel>();
     if (e != hipSuccess) return e;
   }
+  // (us in one launch / two: 1536 rows 10.4 / 12.4, 3840 12.4 / 12.5, 6400 14.6 / 12.7, 16384 30 / 16)
   const bool one = a.tokens <= 4 * kMostThreads;
   int64_t threads = one && a.tokens > a.seqs ? a.tokens : a.seqs;
   threads = threads > kMostThreads || !one ? kMostThreads : threads < 64 ? 64 : (threads + 63) / 64 * 64;

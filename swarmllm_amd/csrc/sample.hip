@@ -1,7 +1,8 @@
 // sample.hip — a token for each row of logits, from a given uniform number.
 //
 //   w_i = exp((x_i - max x) / T)
-// The values are ordered by x (equal ones by index, the lowest first). Of them
+// (64-bit weights and sums, of the logits as they are: the steps of w are far under
+// those of u). The values are ordered by x (equal ones by index, the lowest first). Of them
 // the first top_k are kept; of those the shortest run whose weight reaches
 // top_p of theirs (the first always); of those the ones with w >= min_p. The
 // token is the first, by index, of the kept ones at which their running sum
@@ -19,9 +20,9 @@
 // follow it). Up to 1024 values are sorted in LDS, or 64 in a wave, and every
 // setting cut there (sample_select_kernel, a workgroup a row).
 // A run by weight (or the k largest of very many) is narrowed down first: the row's
-// slices make histograms of counts and weights over the bound's range, the weights as
-// whole numbers (2^S to the largest), so that no order of additions shows in them;
-// sample_finish_kernel adds the slices', finds the bucket in which the run ends,
+// slices make histograms of counts or weights over the bound's range (a bucket's
+// weights are within 3% of each other and have 24 bits each, so that 64 bits add
+// up to 2^19 of them exactly, in any order); sample_finish_kernel adds the slices', finds the bucket in which the run ends,
 // sums the weights above it chunk by chunk and lists the bucket's own values,
 // which the row's last workgroup sorts, cuts and draws from. More than 1024 values
 // at a border (equal logits) are narrowed down further by one workgroup, by their
@@ -725,6 +726,13 @@ __device__ __forceinline__ void finish_wave(const SampleArgs& a, int64_t row, co
 // The part of the row's chunks that a slice takes.
 __device__ __forceinline__ int slice_begin(int chunks, int slice, int slices) { return chunks * slice / slices; }
 
+// Whether the k-th largest of the groups' maxima leaves few values past it to sort:
+// of values in any order, n over `groups` groups leave k of them with one when
+// k = groups (1 - exp(-n / groups)).
+__device__ __forceinline__ bool few_past(int k, int groups) {
+  return k < groups && -(float)groups * __logf(1.0f - (float)k / (float)groups) <= 0.75f * kList;
+}
+
 template <int T, bool VEC>
 __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, int chunks, int bits) {
   __shared__ Shared s;
@@ -737,8 +745,11 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   const bool p_on = p < 1.0;
   bool greedy;
   const double scale = scale_of(a, row, greedy);
-  // rows that every slice makes a histogram of; the others are the first one's
-  const bool wide = !greedy && (k_on ? !p_on && k > merged : p_on);
+  // rows that every slice makes a histogram of; the others are the first one's. (By
+  // count, us with the border sorted by one workgroup / narrowed down by all: 4 rows of
+  // 128256 f32 by top_k 100 22 / 30, 320 34 / 31, 400 37 / 31, 450, whose bound
+  // leaves more than the list holds, 76 / 31; 64 rows 33 / 50, 44 / 51, 48 / 51, 88 / 52)
+  const bool wide = !greedy && (k_on ? !p_on && !few_past(k, merged) : p_on);
   if (!wide && slice > 0) return;
   s.powers.fill();
   float m = -INFINITY;
@@ -823,7 +834,9 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   // (its lower border, a bucket lower for the roundings)
   if (deepest < kBuckets && bucket.inv > 0.0f) lo = fmaxf(lo, top - (float)(deepest + 2) / bucket.inv);
   activate(s, 0, groups, [=](float x) { return x >= lo; });
-  // min_p alone, and most groups hold some of its values: more than the list does, as a rule
+  // min_p alone, and most groups hold some of its values: more than the list does, as
+  // a rule, and to see that by listing costs more than it finds (16 rows by min_p 1e-5
+  // 28 us with this, 39 without; by 0.05 27, and 34 with a quarter for the three)
   const bool overfull = !k_on && s.n_active > 3 * groups / 4 && groups >= 256;
   int n = overfull ? kList + 1 : collect<T, VEC>(a, row, s, [=](float x) { return x >= lo; });
   uint64_t last = 0;  // the rank of the last value of the prefix
@@ -1044,9 +1057,12 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
   draw<kThreads, T>(a, row, weight, Stay{lo, last, floor}, mass, number_of(a, row), chunks, s.sums, &s.found);
 }
 
-// Slices of a row until two workgroups a CU are there, of 8 chunks at least.
+// Slices of a row until each CU has a workgroup (its registers hold one of 1024
+// threads), of 8 chunks at least, 8 at most (the finish reads all their parts). us by
+// top_p 0.9 of 128256 f32 values in 1, 2, 4 or 8 slices: 1 row 80, 54, 41, 34; 16 rows 85, 59,
+// 45, 41; 64 rows 92, 68, 59, and 90 in 8, twice what the CUs hold.
 int slices_of(int64_t rows, int chunks, int cus) {
-  const int64_t want = 2 * cus / rows, most = chunks / 8;
+  const int64_t want = cus / rows, most = chunks / 8;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
 }
@@ -1062,8 +1078,7 @@ hipError_t launch_rows(const SampleArgs& a, hipStream_t st) {
     sample_pick_kernel<T, VEC><<<(unsigned)a.rows, kMostChunks, 0, st>>>(a, chunks);
   } else {
     sample_select_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
-    const int slices = chunks >= 16 * a.slices && a.rows <= 64 ? 2 * a.slices : a.slices;
-    sample_finish_kernel<T, VEC><<<dim3((unsigned)slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
+    sample_finish_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
   }
   return hipGetLastError();
 }
