@@ -458,6 +458,10 @@ __device__ __forceinline__ void store_row4(const LoraTarget& t, float* p, int64_
 template <int WT, int S>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int tiles) {
   constexpr int P = kTile / kUpWaves, MP = kPieces<QMM_X_F32>;
+  // at ranks past 32 y comes after the products, whose registers it then takes: four workgroups a CU
+  // for three (2000 rows of 8192 to 28672 by rank 64 166 us, 189 with y first; rank
+  // 32 47 and 44, rank 128, which two fill either way, 173 and 169)
+  constexpr bool LATE = S == 2;
   __shared__ float s_sum[kTile][kUpOut + 4];
   const LoraTarget& t = a.t[blockIdx.z];
   const int turn = blockIdx.x >> 3, tile = turn % tiles;
@@ -467,11 +471,14 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int32_t* rows = a.order + (int64_t)tile * kTile;
   f4v y[P];
+  auto load_y = [&]() {
 #pragma unroll
-  for (int i = 0; i < P; i++) {
-    const int64_t row = rows[kUpWaves * i + wave];
-    y[i] = row >= 0 ? load_row4(t, t.y + row * t.ldy, n0 + 4 * lane) : f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+    for (int i = 0; i < P; i++) {
+      const int64_t row = rows[kUpWaves * i + wave];
+      y[i] = row >= 0 ? load_row4(t, t.y + row * t.ldy, n0 + 4 * lane) : f4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  };
+  if (!LATE || who < 0) load_y();
   if (who >= 0) {
     Raw<WT> w[kUpTiles][S];
 #pragma unroll
@@ -520,6 +527,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int 
 #pragma unroll
       for (int h = 0; h < 2; h++) *(f4v*)&s_sum[16 * h + col][16 * (kUpTiles * wave + c) + 4 * g] = acc[h];
     }
+    if (LATE) load_y();
     __syncthreads();
   }
 #pragma unroll
