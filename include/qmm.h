@@ -489,11 +489,17 @@ int qmm_pages_step(const qmm_pages *pages, const int32_t *keep, const int32_t *f
  * 32); a [slots][rank][k] and b [slots][n][rank] of w_dtype (qmm_x_dtype), each
  * 16-byte aligned, rank a multiple of 8 up to 128 (an adapter of a lower rank
  * has zeros); scales [slots] f32 (NULL: 1); y and out f32. out may be y itself
- * (the same pointer and stride); otherwise nothing overlaps. Values of x and of
- * the adapters enter as they are, sums are f32. Where x's sums are split, and
- * so a row's last bits, follows from rows, k and count. An adapter's values reach its own
- * rows only. Plan (launch == 0) and launch as qmm_forward: the workspace
- * (16-byte aligned) holds x's products with a. Two launches. At most 2^20 rows. */
+ * (the same pointer and stride); otherwise nothing overlaps. two projections have
+ * two outs. Values of x and of the adapters enter as they are, sums are f32
+ * (products of many rows leave out parts under 2^-24 of each; an infinite value
+ * makes its row's results infinite or NaN). In which order the sums are taken,
+ * and so a row's last bits, follows from rows, k, count and the projections' n
+ * and ranks; a batch's bits are the same each time. An adapter's values reach
+ * its own rows only. Plan (launch == 0) and launch as qmm_forward: the workspace
+ * (16-byte aligned) holds x's products with a; small calls need none. One launch
+ * for few rows of small adapters, two for more, three or four for many (rows *
+ * rank past 4096). At most 2^20 rows; an n of many millions beside many rows is
+ * QMM_UNSUPPORTED. */
 typedef struct qmm_adapter {
     const void *a, *b;
     const float *scales;
@@ -524,8 +530,9 @@ int qmm_adapters_add(int count, const qmm_adapter *adapters, int slots, int w_dt
  * else gives -1 (qmm_gather_rows' "no row") and 0. Where a logit is +inf, those
  * alone are drawn, equally. Weights are relative to the largest, in 64 bits; weights
  * below 2^-60 may count as 0 where a setting is on, and those below 2^-1000 do always. A row's token follows from
- * the row, its settings and vocab alone. Plan and
- * launch as qmm_forward (workspace 16-byte aligned): the plan goes by which settings are given. At most 65535 rows. */
+ * the row, its settings and vocab alone, where the 64-bit sums' last bits do not
+ * decide. Plan and launch as qmm_forward (workspace 16-byte aligned): the plan
+ * goes by which settings are given. At most 65535 rows. */
 int qmm_sample(const void *logits, int dtype, int64_t stride, const float *u, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *probs, int64_t vocab,
                int64_t rows, void *workspace, size_t workspace_bytes, size_t *need, int launch, int64_t stream);
