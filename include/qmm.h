@@ -451,7 +451,7 @@ int qmm_attend(const qmm_cache *cache, const void *q, int q_dtype, int64_t q_str
  *               lies past its count has no meaning
  *   free_count  int32 [1]
  * page: positions of a page (16, 32, 64, 128 or 256). A page is one sequence's.
- * At most 4096 sequences, fewer than 2^31 entries of tables (seqs * table_stride), 2^30 positions a
+ * At most 4096 sequences, 2^30 entries of tables (seqs * table_stride), 2^30 positions a
  * sequence. */
 typedef struct qmm_pages {
     int32_t *tables, *lens, *free_pages, *free_count;

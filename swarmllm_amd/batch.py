@@ -43,10 +43,10 @@ class PageTables:
                     or t.device != self.device:
                 raise ValueError(f"PageTables: {name} must be contiguous int32 {shape} on one GPU, not {t.dtype} "
                                  f"{tuple(t.shape)} on {t.device}")
-        if page < 16 or page > 256 or page & (page - 1) or seqs > 4096 or row * page > 1 << 30 or seqs * row >= 1 << 31 \
+        if page < 16 or page > 256 or page & (page - 1) or seqs > 4096 or row * page > 1 << 30 or seqs * row > 1 << 30 \
                 or free.numel() >= 1 << 31:
             raise ValueError(f"PageTables: {seqs} sequences of {row} pages of {page}: at most 4096, pages of 16 to 256 "
-                             "positions (a power of two), 2^30 positions a sequence, fewer than 2^31 entries")
+                             "positions (a power of two), 2^30 positions a sequence, 2^30 entries, fewer than 2^31 pages")
         self.tables, self.lens, self.free, self.free_count = tables, lens, free, free_count
         self.seqs, self.row_pages, self.page = seqs, row, page
         self._c = Pages(tables.data_ptr(), lens.data_ptr(), free.data_ptr(), free_count.data_ptr(), row, row, free.numel(),

@@ -1121,7 +1121,7 @@ int qmm_pages_step(const qmm_pages* pages, const int32_t* keep, const int32_t* f
       pages->page < 16 || pages->page > 256 || (pages->page & (pages->page - 1)) != 0 || pages->row_pages < 0 ||
       pages->table_stride < pages->row_pages || pages->pool < 0 || pages->pool > INT32_MAX ||
       pages->row_pages > ((int64_t)1 << 30) / pages->page ||
-      pages->table_stride > INT32_MAX || (int64_t)pages->seqs * pages->table_stride > INT32_MAX || !pages->free_count || !q_starts ||
+      pages->table_stride > INT32_MAX || (int64_t)pages->seqs * pages->table_stride > (int64_t)1 << 30 || !pages->free_count || !q_starts ||
       (pages->row_pages > 0 && pages->seqs > 0 && !pages->tables) || (pages->pool > 0 && !pages->free_pages) ||
       (pages->seqs > 0 && (!pages->lens || !taken)) || (tokens > 0 && !slots))
     return QMM_UNSUPPORTED;

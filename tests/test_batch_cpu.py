@@ -24,7 +24,8 @@ def pages_step(tokens=10, q=P, taken=P, slots=P, **change):
 def test_pages_refusals():
     for bad in (dict(seqs=-1), dict(seqs=4097), dict(page=8), dict(page=48), dict(page=512), dict(page=0),
                 dict(row_pages=-1), dict(table_stride=19), dict(pool=-1), dict(pool=2**31), dict(row_pages=2**24 + 1,
-                table_stride=2**40), dict(seqs=4096, row_pages=2**19, table_stride=2**19), dict(tables=None),
+                table_stride=2**40), dict(seqs=4096, row_pages=2**19, table_stride=2**19),
+                dict(seqs=1024, row_pages=2**10, table_stride=2**20 + 1), dict(tables=None),
                 dict(lens=None), dict(free_pages=None), dict(free_count=None), dict(q=None), dict(taken=None),
                 dict(slots=None), dict(tokens=-1), dict(tokens=2**29 + 1)):
         assert pages_step(**bad) == QMM_UNSUPPORTED, bad
