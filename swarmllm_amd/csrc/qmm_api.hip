@@ -1150,8 +1150,9 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
         d.y_stride < d.n || d.out_stride < d.n || (d.y == d.out && d.y && d.y_stride != d.out_stride) ||
         !aligned16(d.a) || !aligned16(d.b))
       return QMM_UNSUPPORTED;
+    // two projections in one place, or one in the place that another reads
     for (int j = 0; j < i; j++)
-      if (d.out && d.out == adapters[j].out) return QMM_UNSUPPORTED;  // two projections in one place
+      if (d.out && (d.out == adapters[j].out || d.out == adapters[j].y || d.y == adapters[j].out)) return QMM_UNSUPPORTED;
     qmm::LoraTarget& t = a.t[i];
     t.a = d.a; t.b = d.b; t.scales = d.scales; t.y = d.y; t.out = d.out;
     t.n = d.n; t.ldy = d.y_stride; t.ldo = d.out_stride; t.rank = d.rank;

@@ -84,8 +84,8 @@ class Adapters:
                            ad.rank)
         if rows == 0:
             return outs
-        if count > 1 and len({c[i].out for i in range(count)}) < count:
-            raise ValueError("Adapters.add_shared: one tensor for two projections")
+        if any(c[i].out in (c[j].out, c[j].y) for i in range(count) for j in range(count) if i != j):
+            raise ValueError("Adapters.add_shared: one projection's out is another's out or y")
         with on_device(device):
             need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)

@@ -177,7 +177,7 @@ def test_refusals():
 
     xs, a, b, scales, ids, y = make(1, 10, 64, 30, 8, 3)
     ok = Adapters(a, b, scales)
-    other = Adapters(a[:2].contiguous(), b[:2].contiguous())
+    other, other_y = Adapters(a[:2].contiguous(), b[:2].contiguous()), y.clone()
     for bad in (lambda: Adapters(a[0], b), lambda: Adapters(a, b[:2]), lambda: Adapters(a, b.float()),
                 lambda: Adapters(a[:, :4].contiguous(), b[:, :, :4].contiguous()), lambda: Adapters(a.cpu(), b.cpu()),
                 lambda: Adapters(a, b.transpose(1, 2)), lambda: Adapters(a[:, :, :40].contiguous(), b),
@@ -189,6 +189,64 @@ def test_refusals():
                 lambda: Adapters.add_shared([y, y], xs, [ok], ids), lambda: Adapters.add_shared([], xs, [], ids),
                 lambda: Adapters.add_shared([y, y], xs, [ok, other], ids),
                 lambda: Adapters.add_shared([y] * 5, xs, [ok] * 5, ids),
-                lambda: Adapters.add_shared([y, y], xs, [ok, ok], ids)):
+                lambda: Adapters.add_shared([y, y], xs, [ok, ok], ids),
+                lambda: Adapters.add_shared([y, other_y], xs, [ok, ok], ids, outs=[other_y, y]),
+                lambda: Adapters.add_shared([y, other_y], xs, [ok, ok], ids, outs=[torch.empty_like(y), y])):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("rows,rank", [(3, 16), (20, 64), (90, 64)])
+def test_rows_far_apart(rows, rank):
+    # x, y and out reach past 2^31 values (and 2^32 bytes)
+    from swarmllm_amd import Adapters
+
+    xs, a, b, scales, ids, y = make(5, rows, 1056, 72, rank, 3, "bf16")
+    want, bound = ref.adapters(y, xs, ids, a, b, scales)
+    step = (2 ** 31 // (rows - 1) + 64) // 8 * 8
+    far_x = torch.empty(step * (rows - 1) + 1056, dtype=torch.bfloat16, device=DEV).as_strided((rows, 1056), (step, 1))
+    far_y = torch.empty(step * (rows - 1) + 72, device=DEV).as_strided((rows, 72), (step, 1))
+    far_x.copy_(xs)
+    far_y.copy_(y)
+    ad = Adapters(a, b, scales)
+    close(ad.add(far_y, far_x, ids, out=torch.empty_like(y)), want, bound)
+    assert torch.equal(ad.add(far_y, far_x, ids), ad.add(y, xs, ids))
+
+
+def test_adapters_past_2_31_values():
+    from swarmllm_amd import Adapters
+
+    g = torch.Generator(device=DEV).manual_seed(8)
+    slots, rank, k, n = 4096, 128, 4128, 2
+    a = torch.empty(slots, rank, k, dtype=torch.bfloat16, device=DEV)
+    b = torch.empty(slots, n, rank, dtype=torch.bfloat16, device=DEV)
+    used = torch.tensor([0, 1, 4094, 4095], device=DEV)
+    for i in used.tolist():
+        a[i] = (torch.randn(rank, k, generator=g, device=DEV) / 64).bfloat16()
+        b[i] = torch.randn(n, rank, generator=g, device=DEV).bfloat16()
+    for rows in (2, 70, 4100):
+        x = torch.randn(rows, k, generator=g, device=DEV)
+        ids = used[torch.randint(4, (rows,), generator=g, device=DEV)].to(torch.int32)
+        y = torch.randn(rows, n, generator=g, device=DEV)
+        want, bound = ref.adapters(y, x, ids, a, b, None)
+        close(Adapters(a, b).add(y, x, ids), want, bound)
+
+
+def test_two_calls_at_once():
+    from swarmllm_amd import Adapters
+
+    sets = []
+    for rows, k, rank in ((30, 2048, 64), (400, 2048, 64), (8, 4096, 16)):
+        xs, a, b, scales, ids, y = make(rows, rows, k, 600, rank, 6)
+        sets.append((Adapters(a, b, scales), xs, ids, y))
+    want = [ad.add(y.clone(), xs, ids) for ad, xs, ids, y in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = [[] for _ in sets]
+    torch.cuda.synchronize()
+    for turn in range(5):
+        for s, (ad, xs, ids, y), out in zip(streams, sets, outs):
+            with torch.cuda.stream(s):
+                out.append(ad.add(y.clone(), xs, ids))
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert all(torch.equal(o, w) for o in out)

@@ -164,3 +164,33 @@ def test_refusals():
                 lambda: ok.step(i32([1] * 4), -1), lambda: ok.step(i32([1] * 4), 5, keep=i32([1] * 4).cpu())):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_large_page_numbers_and_arrays_not_wanted():
+    import ctypes
+
+    from swarmllm_amd import PageTables
+    from swarmllm_amd._lib import lib
+
+    base = 2 ** 31 - 1 - 40
+    for tokens in (90, 5000):
+        pages = PageTables.alloc(3, 10, 40, page=256)
+        pages.free += base
+        rows = pages.step(i32([300, 256, 20]), 576 + 20)
+        want = [[base, base + 1], [base + 2], [base + 3]]
+        assert [[p for p in t if p >= 0] for t in pages.tables.tolist()] == want
+        assert rows.slots[[0, 299, 300, 575]].tolist() == [base * 256, (base + 1) * 256 + 43, (base + 2) * 256, (base + 3) * 256 + 19]
+        # only what is wanted: no keep, no positions, no sequences
+        new = i32([40, 30, 20])
+        q, taken = torch.empty(4, dtype=torch.int32, device=DEV), torch.empty(3, dtype=torch.int32, device=DEV)
+        slots = torch.full((tokens + 8,), -7, dtype=torch.int64, device=DEV)
+        assert lib().qmm_pages_step(ctypes.byref(pages._c), None, new.data_ptr(), tokens, q.data_ptr(), taken.data_ptr(),
+                                    slots.data_ptr(), None, None, torch.cuda.current_stream().cuda_stream) == 0
+        assert q.tolist() == [0, 40, 70, 90] and taken.tolist() == [40, 30, 20] and pages.lens.tolist() == [340, 286, 40]
+        got = slots.tolist()
+        assert got[:40] == [(base + 1) * 256 + 44 + i for i in range(40)] and got[40:70] == [(base + 4) * 256 + i for i in range(30)]
+        assert got[70:90] == [(base + 3) * 256 + 20 + i for i in range(20)] and got[90:] == [-1] * (tokens - 90) + [-7] * 8
+    rows = pages.step()  # nothing wanted
+    assert rows.q_starts.tolist() == [0] * 4 and rows.slots.numel() == 0 and pages.lens.tolist() == [340, 286, 40]
+    rows = pages.step(tokens=7)
+    assert rows.q_starts.tolist() == [0] * 4 and rows.slots.tolist() == rows.seq.tolist() == rows.positions.tolist() == [-1] * 7

@@ -227,3 +227,60 @@ def test_refusals():
                 lambda: sa.sample(torch.empty(3, 2 ** 19 + 1, device=DEV), u)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_rows_far_apart():
+    import swarmllm_amd as sa
+
+    x = logits(11, 4, 20011).bfloat16()
+    step = 2 ** 30 + 3
+    far = torch.empty(3 * step + 20011, dtype=torch.bfloat16, device=DEV).as_strided((4, 20011), (step, 1))
+    far.copy_(x)
+    u = vec([0.1, 0.5, 0.9, 0.99])
+    k, p = vec([0, 30, 5000, 0], torch.int32), vec([0.9, 1.0, 0.99, 0.5])
+    for settings in ((None, None, None), (None, k, None), (None, None, p), (u, k, p)):
+        got, want = sa.sample(far, u, *settings), sa.sample(x, u, *settings)
+        assert torch.equal(got.ids, want.ids) and torch.equal(got.probs, want.probs)
+
+
+def test_two_calls_at_once():
+    import swarmllm_amd as sa
+
+    sets = []
+    for rows, vocab in ((40, 30000), (3, 128256), (300, 5000)):
+        x = logits(rows, rows, vocab)
+        g = torch.Generator(device=DEV).manual_seed(rows)
+        u, t = (torch.rand(rows, generator=g, device=DEV) for _ in range(2))
+        k = torch.randint(0, 900, (rows,), generator=g, device=DEV).to(torch.int32)
+        sets.append((x, u, t, k * (k % 3 == 0), 0.9 * torch.ones_like(u)))
+    want = [sa.sample(*s) for s in sets]
+    streams, outs = [torch.cuda.Stream() for _ in sets], [[] for _ in sets]
+    torch.cuda.synchronize()
+    for turn in range(5):
+        for stream, s, out in zip(streams, sets, outs):
+            with torch.cuda.stream(stream):
+                out.append(sa.sample(*s))
+    torch.cuda.synchronize()
+    for out, w in zip(outs, want):
+        assert all(torch.equal(o.ids, w.ids) and torch.equal(o.probs, w.probs) for o in out)
+
+
+def test_without_chances():
+    import ctypes
+
+    import swarmllm_amd as sa
+    from swarmllm_amd._lib import X_F32, lib
+
+    x, u = logits(12, 9, 9000), vec([0.05 + 0.1 * i for i in range(9)])
+    t, k, p = vec([1.0, 0.0, 0.5] * 3), vec([0, 0, 0, 5, 80, 2000, 0, 0, 1], torch.int32), vec([0.9, 0.9, 1.0] * 3)
+    for settings in ((None, None, None), (t, None, None), (t, k, p)):
+        want = sa.sample(x, u, *settings).ids
+        ids, need = torch.full((9,), -7, dtype=torch.int32, device=DEV), ctypes.c_size_t()
+        ptrs = [None if v is None else v.data_ptr() for v in settings] + [None]
+        call = lambda ws, size, launch: lib().qmm_sample(x.data_ptr(), X_F32, 9000, u.data_ptr(), *ptrs, ids.data_ptr(), None, 9000,
+                                                         9, ws, size, ctypes.byref(need), launch,
+                                                         torch.cuda.current_stream().cuda_stream)
+        assert call(None, 0, 0) == 0
+        ws = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+        assert call(ws.data_ptr(), need.value, 1) == 0
+        assert torch.equal(ids, want)
