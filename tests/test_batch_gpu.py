@@ -186,3 +186,62 @@ def test_a_batch_without_pages_left_stands_still():
     rows = pages.step(torch.tensor([0, 0, 4], dtype=torch.int32, device=DEV), 4,
                       keep=torch.tensor([-1, 10, -1], dtype=torch.int32, device=DEV))
     assert rows.taken.tolist() == [0, 0, 4] and pages.lens.tolist() == [16, 10, 4]
+
+
+FIRST_UNDER_CAPTURE = """
+import sys
+sys.path[:0] = ["."]
+import torch
+from swarmllm_amd import Adapters, PageTables, sample
+
+g = torch.Generator(device="cuda").manual_seed(1)
+ad = [Adapters((torch.randn(3, r, k, generator=g, device="cuda") / 64).bfloat16(),
+               torch.randn(3, 100, r, generator=g, device="cuda").bfloat16()) for r, k in ((16, 512), (64, 2048))]
+xs = [torch.randn(rows, a.k, generator=g, device="cuda") for a, rows in ((ad[0], 9), (ad[1], 30), (ad[1], 200))]
+ids = [(torch.arange(len(x), device="cuda") % 4 - 1).to(torch.int32) for x in xs]
+logits, u = 3 * torch.randn(20, 40000, generator=g, device="cuda"), torch.rand(20, generator=g, device="cuda")
+k = torch.tensor([0, 0, 50, 3000] * 5, dtype=torch.int32, device="cuda")
+p = torch.tensor([0.9, 1.0, 0.8, 1.0, 1.0] * 4, device="cuda")
+new = torch.ones(4096, dtype=torch.int32, device="cuda")
+new[::2] = 3
+pages = [PageTables.alloc(n, 8, 20000, page=16) for n in (5, 4096)]
+
+
+def steps():
+    outs = [s for n, t in ((5, 20), (4096, 9000)) for s in pages[n > 5].step(new[:n], t)]
+    outs += [a.add(torch.zeros(len(x), 100, device="cuda"), x, i) for a, x, i in zip((ad[0], ad[1], ad[1]), xs, ids)]
+    return outs + [*sample(logits, u), *sample(logits, u, top_k=k, top_p=p)]
+
+
+torch.cuda.synchronize()
+state = [[t.clone() for t in (q.tables, q.lens, q.free, q.free_count)] for q in pages]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = steps()
+for turn in range(4):
+    graph.replay()
+    got = [o.clone() for o in outs] + [t.clone() for q in pages for t in (q.tables, q.lens, q.free_count)]
+    after = [[t.clone() for t in (q.tables, q.lens, q.free, q.free_count)] for q in pages]
+    for q, s in zip(pages, state):
+        for t, v in zip((q.tables, q.lens, q.free, q.free_count), s):
+            t.copy_(v)
+    want = steps() + [t.clone() for q in pages for t in (q.tables, q.lens, q.free_count)]
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want)), turn
+    for q, s in zip(pages, after):
+        for t, v in zip((q.tables, q.lens, q.free, q.free_count), s):
+            t.copy_(v)
+    state = after
+    xs[0].mul_(0.5), xs[2].mul_(-0.5), logits.mul_(0.9)
+torch.cuda.synchronize()
+print("equal")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_UNDER_CAPTURE], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip().endswith("equal"), r.stdout[-500:] + r.stderr[-2000:]
