@@ -924,8 +924,11 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
     }
     double all;
     const double upto = block_sums<kThreads, double>(m[0] + m[1], s.sums, all);
-    // 32-bit weights are off by 3e-6 of theirs at most (|y| <= 61, half a step of y)
-    const double off = by_count ? 0.0 : 1e-4 * goal;
+    // the exponents of 32-bit weights are off by three half steps, 2^-22.4 of theirs; over
+    // the weights' sum they are 20 in the mean at most (2^19 values): 2.5e-6 of it, and
+    // 1e-7 of exp2 (a wider range has the border's many small values in it: top_p 0.999 of
+    // 16 rows 158 us with 1e-4 here, 48 with this). Where it does not hold the exact sums show it.
+    const double off = by_count ? 0.0 : 4e-6 * goal;
     auto first = [&](double want) {
       const bool met = upto > 0.0 && upto >= want, sooner = upto - m[1] > 0.0 && upto - m[1] >= want;
       return met ? 2 * tid + !sooner : INT32_MAX;
