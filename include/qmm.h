@@ -497,8 +497,8 @@ int qmm_pages_step(const qmm_pages *pages, const int32_t *keep, const int32_t *f
  * and ranks; a batch's bits are the same each time. An adapter's values reach
  * its own rows only. Plan (launch == 0) and launch as qmm_forward: the workspace
  * (16-byte aligned) holds x's products with a; small calls need none. One launch
- * for few rows of small adapters, two for more, three or four for many (rows *
- * rank past 4096). At most 2^20 rows; an n of many millions beside many rows is
+ * for few rows of small adapters, two for more, three or four for many (past 1024,
+ * or reading more than 3 * 2^25 values of a and b one by one). At most 2^20 rows; an n of many millions beside many rows is
  * QMM_UNSUPPORTED. */
 typedef struct qmm_adapter {
     const void *a, *b;

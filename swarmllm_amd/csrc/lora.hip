@@ -562,17 +562,20 @@ int64_t tiles_of(const LoraArgs& a) {
 
 // How a call runs, all times of calls in a replayed graph (bf16 adapters, f32 x).
 //
-// Rows one by one read A and B once a row, tiles once for 32 rows of one adapter,
-// but a tile is as dear for one row as for 32, and the rows have to be sorted
-// first. So rows one by one up to 64 of them, and while rows * rank, which their
-// work grows by, is at most 4096 (us one by one / in tiles; all rows with one
-// adapter, with 64 adapters in turn):
-//     64 rows, rank 64, 8192 to 8192        22 / 25     36 / 56
-//     128 rows, rank 32, 14336 to 4096      20 / 26     29 / 43
-//     256 rows, rank 16, 4096 to 2 x 14336  31 / 28     50 / 76
-//     128 rows, rank 64, 8192 to 8192       34 / 27     55 / 67
-//     512 rows, rank 16, 4096 to 2 x 14336  60 / 42     90 / 91
-//     512 rows, rank 64, 8192 to 8192       110 / 36    165 / 80
+// Rows one by one read their A and B once a row, tiles once for 32 rows of one
+// adapter, but a tile is as dear for one row as for 32, and the rows have to be sorted
+// first. So rows one by one while all of them together read at most 3 * 2^25 values
+// of A and B (and up to 1024 rows; us one by one / in tiles, a row's place by n and k; all rows
+// with 1 adapter, or each with one of 64 in turn):
+//     64 rows, rank 16, 4096 to 2 x 14336    38M values   14 / 23     20 / 48
+//     32 rows, rank 64, 4096 to 2 x 14336    75M          28 / 26     48 / 53
+//     128 rows, rank 32, 14336 to 4096       75M          20 / 26     29 / 43
+//     16 rows, rank 128, 4096 to 2 x 14336   75M          28 / 30     50 / 67
+//     128 rows, rank 64, 8192 to 8192        134M         34 / 27     55 / 67
+//     256 rows, rank 16, 4096 to 2 x 14336   151M         31 / 28     50 / 76
+//     64 rows, rank 64, 4096 to 2 x 14336    151M         44 / 28     80 / 81
+//     128 rows, rank 64, 4096 to 2 x 14336   302M         77 / 32     144 / 106
+//     512 rows, rank 64, 8192 to 8192        537M         110 / 36    165 / 80
 //
 // Of rows one by one, the small ones in one launch: every workgroup of a row makes
 // the row's products with A for itself, which a second launch would hand it. That
@@ -586,12 +589,13 @@ enum Form { kFused, kRows, kTiles };
 
 Form form_of(const LoraArgs& a) {
   int rank = 0;
-  int64_t groups = 0;
+  int64_t groups = 0, values = 0;
   for (int i = 0; i < a.count; i++) {
     rank = rank > a.t[i].rank ? rank : a.t[i].rank;
     groups += a.rows * ((a.t[i].n + kRowOut - 1) / kRowOut);
+    values += a.rows * a.t[i].rank * (a.k + a.t[i].n);
   }
-  if (a.rows > 64 && a.rows * rank > 4096) return kTiles;
+  if (a.rows > 1024 || values > (int64_t)3 << 25) return kTiles;
   return rank * a.k <= 1 << 16 && groups * rank * a.k <= 1 << 23 ? kFused : kRows;
 }
 

@@ -44,14 +44,14 @@ def adapters_add(n=None, launch=0, count=1, slots=4, w=X_BF16, x=P, x_type=X_F32
 
 def test_adapters_plan_and_refusals():
     assert adapters_add() == (QMM_OK, 0)  # few rows of a short k: in one launch, nothing between
-    st, need = adapters_add(rows=300)
-    assert st == QMM_OK and need >= 300 * 16 * 4
+    st, need = adapters_add(rows=3000)
+    assert st == QMM_OK and need >= 3000 * 16 * 4
     assert adapters_add(k=28672, x_stride=28672)[1] >= 5 * 16 * 4
-    many = [adapters_add(rows=500, slots=s)[1] for s in (1, 4, 100)]
-    assert 500 * 16 * 4 <= many[0] < many[1] < many[2]  # whole tiles, and one begun for each adapter
+    many = [adapters_add(rows=2000, slots=s)[1] for s in (1, 4, 100)]
+    assert 2000 * 16 * 4 <= many[0] < many[1] < many[2]  # whole tiles, and one begun for each adapter
     assert adapters_add(rows=0) == (QMM_OK, 0) and adapters_add(rows=0, launch=1) == (QMM_OK, 0)
-    assert adapters_add(rows=300, launch=1, ws=P, ws_bytes=need - 1) == (QMM_WORKSPACE_TOO_SMALL, need)
-    assert adapters_add(rows=300, launch=1)[0] == QMM_WORKSPACE_TOO_SMALL
+    assert adapters_add(rows=3000, launch=1, ws=P, ws_bytes=need - 1) == (QMM_WORKSPACE_TOO_SMALL, need)
+    assert adapters_add(rows=3000, launch=1)[0] == QMM_WORKSPACE_TOO_SMALL
     assert adapters_add(launch=1, ws=P + 4, ws_bytes=2 * need)[0] == QMM_UNSUPPORTED
     for bad in (dict(count=0), dict(count=5), dict(slots=-1), dict(slots=4097), dict(w=3), dict(x_type=-1), dict(x_stride=4095), dict(k=0),
                 dict(k=4080 + 8), dict(rows=-1), dict(rows=2**20 + 1), dict(n=ctypes.c_size_t(), rank=0), dict(rank=12),
@@ -61,11 +61,11 @@ def test_adapters_plan_and_refusals():
     # two projections into one place, and more workgroups than a launch takes
     assert adapters_add(count=2)[0] == QMM_OK and adapters_add(count=2, out=2 * P)[0] == QMM_UNSUPPORTED
     assert adapters_add(count=2, out=10 * P)[0] == QMM_UNSUPPORTED and adapters_add(count=2, y=2 * P)[0] == QMM_UNSUPPORTED
-    wide = dict(n=2**31 - 1, y_stride=2**31, out_stride=2**31)
+    wide = dict(n=2**30, y_stride=2**31, out_stride=2**31)
     c = (Adapter * 1)(Adapter(P, P, P, P, P, wide["n"], wide["y_stride"], wide["out_stride"], 16))
-    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 64, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 1, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
                                   0) == QMM_OK
-    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 300, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 64, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
                                   0) == QMM_UNSUPPORTED
     for null in (dict(x=None), dict(ids=None), dict(a=None), dict(b=None), dict(y=None), dict(out=None)):
         assert adapters_add(launch=1, ws=P, ws_bytes=2**20, **null)[0] == QMM_UNSUPPORTED, null
@@ -100,7 +100,7 @@ def test_injected_failure_is_one_call_s():
     assert sample(launch=1, ws=P, ws_bytes=0)[0] == QMM_WORKSPACE_TOO_SMALL
     lib().qmm_fail_next_launch()
     assert adapters_add(launch=1, ws=P, ws_bytes=2**20)[0] == QMM_NO_ROOM
-    assert adapters_add(rows=300, launch=1)[0] == QMM_WORKSPACE_TOO_SMALL
+    assert adapters_add(rows=3000, launch=1)[0] == QMM_WORKSPACE_TOO_SMALL
 
 
 def test_reference_step_by_hand():

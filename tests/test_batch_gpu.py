@@ -11,10 +11,10 @@ VOCAB, HIDDEN, HEADS, KV, HD, FFN, LAYERS, PAGE, RANK, SLOTS = 1000, 256, 4, 2, 
 class Tiny:
     """A small decoder of Q8_0 weights with adapters at q, k, v and o."""
 
-    def __init__(self):
+    def __init__(self, seed=1):
         from swarmllm_amd import Adapters, GgmlDType, QMatMul, QTensor, fill_normal
 
-        seeds = iter(range(1, 1000))
+        seeds, g = iter(range(1000 * seed, 1000 * seed + 1000)), torch.Generator(device=DEV).manual_seed(seed)
 
         def weight(n, k, std=0.05):
             return QTensor.quantize(fill_normal(n * k, seed=next(seeds), std=std).view(n, k), GgmlDType.Q8_0)
@@ -22,7 +22,7 @@ class Tiny:
         def adapters(n, k):
             a = fill_normal(SLOTS * RANK * k, seed=next(seeds), std=k ** -0.5).view(SLOTS, RANK, k)
             b = fill_normal(SLOTS * n * RANK, seed=next(seeds), std=0.3).view(SLOTS, n, RANK)
-            return Adapters(a.bfloat16(), b.bfloat16(), torch.rand(SLOTS, device=DEV) + 0.5)
+            return Adapters(a.bfloat16(), b.bfloat16(), torch.rand(SLOTS, generator=g, device=DEV) + 0.5)
 
         self.embed, self.head = weight(VOCAB, HIDDEN, 1.0), QMatMul(weight(VOCAB, HIDDEN, 0.3))
         self.layers = []
@@ -96,11 +96,15 @@ def requests():
     return prompts, adapter, temperature, top_k, top_p, u
 
 
-def tokens_of(loop, prompts, u, steps, capture=False):
-    """The tokens of each step [steps + 1, places]."""
+def tokens_of(loop, prompts, u, steps, capture=False, like=None):
+    """The tokens of each step [steps + 1, places]. The prompts' batch is padded to the rows of the prompts `like`:
+    products and attention choose their kernels, and so a row's last bits, by a batch's rows."""
+    like = prompts if like is None else like
+    ids = torch.cat(prompts)
+    ids = torch.nn.functional.pad(ids, (0, sum(len(p) for p in like) - ids.numel()))
     loop.new.copy_(torch.tensor([len(p) for p in prompts]))
     loop.u.copy_(u[0])
-    loop.step(torch.cat(prompts), max(len(p) for p in prompts))
+    loop.step(ids, max(len(p) for p in like))
     out = [loop.token.clone()]
     loop.new.fill_(1)
     graph = None
@@ -135,7 +139,8 @@ def test_requests_together_as_alone_and_captured():
     assert torch.equal(captured, together)
     for b in range(4):
         s = slice(b, b + 1)
-        alone = tokens_of(Loop(model, 1, adapter[s], temperature[s], top_k[s], top_p[s]), [prompts[b]], u[:, s].contiguous(), 10)
+        alone = tokens_of(Loop(model, 1, adapter[s], temperature[s], top_k[s], top_p[s]), [prompts[b]], u[:, s].contiguous(), 10,
+                          like=prompts)
         assert torch.equal(alone[:, 0], together[:, b]), b
 
 
@@ -197,7 +202,7 @@ from swarmllm_amd import Adapters, PageTables, sample
 g = torch.Generator(device="cuda").manual_seed(1)
 ad = [Adapters((torch.randn(3, r, k, generator=g, device="cuda") / 64).bfloat16(),
                torch.randn(3, 100, r, generator=g, device="cuda").bfloat16()) for r, k in ((16, 512), (64, 2048))]
-xs = [torch.randn(rows, a.k, generator=g, device="cuda") for a, rows in ((ad[0], 9), (ad[1], 30), (ad[1], 200))]
+xs = [torch.randn(rows, a.k, generator=g, device="cuda") for a, rows in ((ad[0], 9), (ad[1], 30), (ad[1], 1200))]
 ids = [(torch.arange(len(x), device="cuda") % 4 - 1).to(torch.int32) for x in xs]
 logits, u = 3 * torch.randn(20, 40000, generator=g, device="cuda"), torch.rand(20, generator=g, device="cuda")
 k = torch.tensor([0, 0, 50, 3000] * 5, dtype=torch.int32, device="cuda")

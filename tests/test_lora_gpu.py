@@ -34,7 +34,11 @@ CASES = [(1, 32, 1, 8, 1, "one"), (1, 4096, 4096, 16, 4, "one"), (2, 64, 17, 8, 
          (33, 14336, 257, 64, 4, "runs"), (64, 2880, 300, 128, 40, "mixed"), (65, 1024, 1000, 16, 70, "mixed"),
          (77, 4096, 513, 32, 3, "runs"), (200, 8192, 96, 56, 2, "runs"), (513, 256, 777, 64, 6, "runs"),
          (1000, 320, 64, 8, 100, "mixed"), (1300, 64, 3, 128, 2, "mixed"),
-         (70, 1024, 1000, 64, 70, "mixed"), (300, 4096, 513, 16, 7, "mixed"), (300, 1024, 2100, 8, 40, "mixed")]
+         (70, 1024, 1000, 64, 70, "mixed"), (300, 4096, 513, 16, 7, "mixed"), (300, 1024, 2100, 8, 40, "mixed"),
+         (1025, 32, 1, 8, 1, "one"), (1030, 96, 63, 24, 2, "mixed"), (1100, 544, 129, 40, 5, "mixed"),
+         (2100, 4096, 513, 16, 24, "mixed"), (1500, 256, 777, 64, 70, "mixed"), (1040, 320, 64, 8, 1100, "mixed"),
+         (64, 14336, 2100, 128, 40, "mixed"), (20, 8192, 40000, 128, 3, "mixed"), (9, 28672, 8192, 128, 2, "runs"),
+         (70, 8192, 8192, 96, 70, "mixed")]
 
 
 @pytest.mark.parametrize("x,w", [("f32", "bf16"), ("f32", "f16"), ("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"),
@@ -76,7 +80,7 @@ def test_whole_numbers_come_out_whole(rows, k, n, rank, slots, order, w):
     assert torch.equal(Adapters(a, b).add(y.clone(), xs, ids).double(), want)
 
 
-@pytest.mark.parametrize("rows", [1, 21, 100, 300])
+@pytest.mark.parametrize("rows", [1, 21, 100, 300, 1100])
 def test_shared_projections_equal_their_own(rows):
     from swarmllm_amd import Adapters
 
@@ -99,7 +103,7 @@ def test_shared_projections_equal_their_own(rows):
 def test_strides_alignment_and_what_lies_between():
     from swarmllm_amd import Adapters
 
-    for rows in (3, 40, 270, 90):
+    for rows in (3, 40, 270, 1050, 90):
         xs, a, b, scales, ids, y = make(rows, rows, 256, 50, 16, 3)
         wide = torch.full((rows, 400), 5.0, device=DEV)
         for off in (0, 1, 4):
@@ -118,7 +122,7 @@ def test_strides_alignment_and_what_lies_between():
     close(got.view(90, 50), want, bound)
 
 
-@pytest.mark.parametrize("rows", [16, 70, 300])
+@pytest.mark.parametrize("rows", [16, 70, 300, 1100])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_an_adapter_reaches_its_own_rows_only(rows, bad):
     from swarmllm_amd import Adapters
@@ -147,7 +151,7 @@ def test_ids_outside_the_slots_and_no_slots():
     assert Adapters(a, b).add(y[:0], xs[:0], ids[:0]).shape == (0, 30)
 
 
-@pytest.mark.parametrize("rows", [4, 120, 300])
+@pytest.mark.parametrize("rows", [4, 120, 300, 1100])
 def test_captured_and_on_another_stream(rows):
     from swarmllm_amd import Adapters
 
@@ -196,7 +200,7 @@ def test_refusals():
             bad()
 
 
-@pytest.mark.parametrize("rows,rank", [(3, 16), (20, 64), (90, 64)])
+@pytest.mark.parametrize("rows,rank", [(3, 16), (20, 64), (1090, 64)])
 def test_rows_far_apart(rows, rank):
     # x, y and out reach past 2^31 values (and 2^32 bytes)
     from swarmllm_amd import Adapters
@@ -236,7 +240,7 @@ def test_two_calls_at_once():
     from swarmllm_amd import Adapters
 
     sets = []
-    for rows, k, rank in ((30, 2048, 64), (400, 2048, 64), (8, 4096, 16)):
+    for rows, k, rank in ((30, 2048, 64), (400, 8192, 64), (8, 4096, 16)):
         xs, a, b, scales, ids, y = make(rows, rows, k, 600, rank, 6)
         sets.append((Adapters(a, b, scales), xs, ids, y))
     want = [ad.add(y.clone(), xs, ids) for ad, xs, ids, y in sets]
