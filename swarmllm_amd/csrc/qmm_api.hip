@@ -1150,6 +1150,7 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
         d.y_stride < d.n || d.out_stride < d.n || (d.y == d.out && d.y && d.y_stride != d.out_stride) ||
         !aligned16(d.a) || !aligned16(d.b))
       return QMM_UNSUPPORTED;
+    if (d.out && d.out == x) return QMM_UNSUPPORTED;  // one in the place that all read
     // two projections in one place, or one in the place that another reads
     for (int j = 0; j < i; j++)
       if (d.out && (d.out == adapters[j].out || d.out == adapters[j].y || d.y == adapters[j].out)) return QMM_UNSUPPORTED;

@@ -48,7 +48,7 @@ class Adapters:
         """out = y + scales[i] * (x a[i]^T) b[i]^T row by row, i = ids[row]; a row
         whose id is outside [0, slots) is y's. y [..., n] f32 is the projection's
         product of x [..., k] (f32, f16 or bf16), ids int32 one a row; out: by
-        default y itself, which is added to. The products are of x's and the
+        default y itself, which is added to; it shares memory with nothing else. The products are of x's and the
         adapters' own values, with f32 sums."""
         return Adapters.add_shared([y], x, [self], ids, None if out is None else [out])[0]
 
@@ -86,6 +86,8 @@ class Adapters:
             return outs
         if any(c[i].out in (c[j].out, c[j].y) for i in range(count) for j in range(count) if i != j):
             raise ValueError("Adapters.add_shared: one projection's out is another's out or y")
+        if any(c[i].out == x.data_ptr() for i in range(count)):
+            raise ValueError("Adapters.add: out is x")
         with on_device(device):
             need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)

@@ -32,7 +32,7 @@ def test_pages_refusals():
     assert lib().qmm_pages_step(None, None, None, 0, P, P, P, None, None, 0) == QMM_UNSUPPORTED
 
 
-def adapters_add(n=None, launch=0, count=1, slots=4, w=X_BF16, x=P, x_type=X_F32, x_stride=4096, ids=P, k=4096, rows=5,
+def adapters_add(n=None, launch=0, count=1, slots=4, w=X_BF16, x=17 * P, x_type=X_F32, x_stride=4096, ids=P, k=4096, rows=5,
                  ws=None, ws_bytes=0, **change):
     c = (Adapter * 4)(*[Adapter(P, P, P, 9 * P + 4096 * i, P + 4096 * i, 1000, 1000, 1000, 16) for i in range(4)])
     for key, v in change.items():
@@ -61,11 +61,12 @@ def test_adapters_plan_and_refusals():
     # two projections into one place, and more workgroups than a launch takes
     assert adapters_add(count=2)[0] == QMM_OK and adapters_add(count=2, out=2 * P)[0] == QMM_UNSUPPORTED
     assert adapters_add(count=2, out=10 * P)[0] == QMM_UNSUPPORTED and adapters_add(count=2, y=2 * P)[0] == QMM_UNSUPPORTED
+    assert adapters_add(x=5 * P, out=5 * P)[0] == QMM_UNSUPPORTED
     wide = dict(n=2**30, y_stride=2**31, out_stride=2**31)
     c = (Adapter * 1)(Adapter(P, P, P, P, P, wide["n"], wide["y_stride"], wide["out_stride"], 16))
-    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 1, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, 17 * P, X_F32, 4096, P, 4096, 1, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
                                   0) == QMM_OK
-    assert lib().qmm_adapters_add(1, c, 4, X_BF16, P, X_F32, 4096, P, 4096, 64, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
+    assert lib().qmm_adapters_add(1, c, 4, X_BF16, 17 * P, X_F32, 4096, P, 4096, 64, None, 0, ctypes.byref(ctypes.c_size_t()), 0,
                                   0) == QMM_UNSUPPORTED
     for null in (dict(x=None), dict(ids=None), dict(a=None), dict(b=None), dict(y=None), dict(out=None)):
         assert adapters_add(launch=1, ws=P, ws_bytes=2**20, **null)[0] == QMM_UNSUPPORTED, null

@@ -195,6 +195,7 @@ def test_refusals():
                 lambda: Adapters.add_shared([y] * 5, xs, [ok] * 5, ids),
                 lambda: Adapters.add_shared([y, y], xs, [ok, ok], ids),
                 lambda: Adapters.add_shared([y, other_y], xs, [ok, ok], ids, outs=[other_y, y]),
+                lambda: Adapters(a, torch.zeros(3, 64, 8, device=DEV, dtype=a.dtype)).add(xs, xs, ids),
                 lambda: Adapters.add_shared([y, other_y], xs, [ok, ok], ids, outs=[torch.empty_like(y), y])):
         with pytest.raises(ValueError):
             bad()
