@@ -730,13 +730,13 @@ __device__ __forceinline__ int slice_begin(int chunks, int slice, int slices) { 
 
 // A row, or a slice of one, is a chain of short passes over what the CU holds (maxima,
 // a scan, the groups past the bound, a sort), each waiting for the one before:
-// 1 row of 128256 by top_k 40 and top_p 9 us, 64 rows of mixed settings 28.
+// 1 row of 128256 by top_k 40 and top_p 9 us, 64 rows of mixed settings 22.
 //
-// Whether the k-th largest of the groups' maxima leaves few values past it to sort:
-// of values in any order, n over `groups` groups leave k of them with one when
+// Whether the k-th largest of the groups' maxima leaves few values (`few`) past it to
+// sort: of values in any order, n over `groups` groups leave k of them with one when
 // k = groups (1 - exp(-n / groups)).
-__device__ __forceinline__ bool few_past(int k, int groups) {
-  return k < groups && -(float)groups * __logf(1.0f - (float)k / (float)groups) <= 0.75f * kList;
+__device__ __forceinline__ bool few_past(int k, int groups, float few) {
+  return k < groups && -(float)groups * __logf(1.0f - (float)k / (float)groups) <= few;
 }
 
 template <int T, bool VEC>
@@ -754,8 +754,11 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   // rows that every slice makes a histogram of; the others are the first one's. (By
   // count, us with the border sorted by one workgroup / narrowed down by all: 4 rows of
   // 128256 f32 by top_k 100 22 / 30, 320 34 / 31, 400 37 / 31, 450, whose bound
-  // leaves more than the list holds, 76 / 31; 64 rows 33 / 50, 44 / 51, 48 / 51, 88 / 52)
-  const bool wide = !greedy && (k_on ? !p_on && !few_past(k, merged) : p_on);
+  // leaves more than the list holds, 76 / 31; 64 rows 33 / 50, 44 / 51, 48 / 51, 88 / 52.
+  // Beside rows by top_p, which wait for all slices anyway, sooner: 21 rows of mixed
+  // settings with top_k to 320 55 / 45, 64 70 / 64; 8 of which none is by top_p alone 33 / 40)
+  const float few = (a.top_p ? 0.4f : 0.75f) * kList;
+  const bool wide = !greedy && (k_on ? !p_on && !few_past(k, merged, few) : p_on);
   if (!wide && slice > 0) return;
   s.powers.fill();
   float m = -INFINITY;
@@ -896,7 +899,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
 
 // Rows of which many values stay: sums by chunk, and the border's values sorted
 // by the last of the row's workgroups: again a chain of passes, and the 64-bit weights of
-// the values that stay (64 rows of mixed settings 31 us).
+// the values that stay (64 rows of mixed settings 29 us).
 template <int T, bool VEC>
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, int chunks, int bits) {
   __shared__ Shared s;

@@ -9,7 +9,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import Adapter, check, lib
+from ._lib import QMM_OK, Adapter, check, lib
 from .qtensor import _X_DTYPES, on_device, raw_stream
 
 _MOST = 4  # projections a call
@@ -48,8 +48,8 @@ class Adapters:
         """out = y + scales[i] * (x a[i]^T) b[i]^T row by row, i = ids[row]; a row
         whose id is outside [0, slots) is y's. y [..., n] f32 is the projection's
         product of x [..., k] (f32, f16 or bf16), ids int32 one a row; out: by
-        default y itself, which is added to; it shares memory with nothing else. The products are of x's and the
-        adapters' own values, with f32 sums."""
+        default y itself, which is added to; it shares memory with nothing else.
+        The products are of x's and the adapters' own values, with f32 sums."""
         return Adapters.add_shared([y], x, [self], ids, None if out is None else [out])[0]
 
     @staticmethod
@@ -84,18 +84,19 @@ class Adapters:
                            ad.rank)
         if rows == 0:
             return outs
-        if any(c[i].out in (c[j].out, c[j].y) for i in range(count) for j in range(count) if i != j):
-            raise ValueError("Adapters.add_shared: one projection's out is another's out or y")
-        if any(c[i].out == x.data_ptr() for i in range(count)):
-            raise ValueError("Adapters.add: out is x")
         with on_device(device):
             need = _need(device.index, first.slots, k, rows, tuple((ad.n, ad.rank) for ad in adapters))
             size = ctypes.c_size_t(need)
             # a buffer a call: stream-ordered, and under capture the graph's own
             ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            check("qmm_adapters_add", lib().qmm_adapters_add(
+            status = lib().qmm_adapters_add(
                 count, c, first.slots, _X_DTYPES[first.dtype], x.data_ptr(), x_type, xs, ids.data_ptr(), k, rows,
-                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device)))
+                None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device))
+        if status != QMM_OK:  # (the arrays' places are the library's to check: a call is host time)
+            if any(c[i].out in (x.data_ptr(), *(p for j in range(count) if i != j for p in (c[j].out, c[j].y)))
+                   for i in range(count)):
+                raise ValueError("Adapters.add: an out that is x, or another projection's out or y")
+            check("qmm_adapters_add", status)
         return outs
 
     def __repr__(self) -> str:
