@@ -70,14 +70,14 @@ __device__ __forceinline__ int index_of(int c, int lane, int e) { return c * kCh
 // 2^y by the nearest 64th below or above it, whose power is looked up (one of 64
 // in LDS, by its low six bits), and the Taylor polynomial of 2^r over what is
 // left: |r ln 2| <= 0.0055, whose sixth power over 6! is 2^-55. y in [-1000, 0];
-// under it 0.
+// under it 0 (power; near takes none such).
 struct Powers {
   double p[64];
   // by the first 64 threads; a barrier follows
   __device__ __forceinline__ void fill() {
     if (threadIdx.x < 64) p[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
   }
-  __device__ __forceinline__ double power(double y) const {
+  __device__ __forceinline__ double near(double y) const {
     constexpr double kShift = 105553116266496.0;  // 1.5 * 2^46: its half step is 2^-7
     const double t = y + kShift;
     const uint32_t n = (uint32_t)__double2loint(t);  // 64 y, rounded
@@ -87,7 +87,11 @@ struct Powers {
                              6.9314718055994531e-1);
     const double b = p[n & 63];
     const double s = __hiloint2double(__double2hiint(b) + (int)((n & ~63u) << 14), __double2loint(b));
-    const double w = fma(s, q, s);
+    return fma(s, q, s);
+  }
+  // for any y <= 0: what is under 2^-1000 (-inf too) is 0
+  __device__ __forceinline__ double power(double y) const {
+    const double w = near(y);
     return y >= -1000.0 ? w : 0.0;
   }
 };
@@ -115,7 +119,7 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 }
 
 // Bound by the logits' bytes and by the 64-bit arithmetic of a weight, 17 instructions:
-// 512 rows of 128256 f32 values in 69 us, 263 MB at 3.8 TB/s; 1 row 3.9 us.
+// 512 rows of 128256 f32 values in 65 us, 263 MB at 4.0 TB/s; 1 row 3.9 us.
 template <int T, bool VEC>
 __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int chunks) {
   __shared__ Powers powers;
@@ -144,8 +148,9 @@ __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int ch
   if (!greedy && m != -INFINITY) {
     const Weights weight{&powers, m, scale};
     if (m < INFINITY && scale < INFINITY) {
+      // (2^-1000 for what is under it: beside the largest's 1 no sum sees it)
 #pragma unroll
-      for (int e = 0; e < 16; e++) s += powers.power(((double)v[e] - (double)m) * scale);
+      for (int e = 0; e < 16; e++) s += powers.near(fmax(((double)v[e] - (double)m) * scale, -1000.0));
     } else {
 #pragma unroll
       for (int e = 0; e < 16; e++) s += weight(v[e]);
