@@ -752,7 +752,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   const int k_set = a.top_k ? a.top_k[row] : 0, merged = min(groups, kThreads);
   const bool k_on = k_set > 0 && k_set < a.vocab;
   const int k = k_on ? k_set : a.vocab;
-  const double p = a.top_p ? (double)a.top_p[row] : 1.0;
+  const double p_set = a.top_p ? (double)a.top_p[row] : 1.0, p = p_set < 1.0 ? p_set : 1.0;  // (NaN too is off)
   const bool p_on = p < 1.0;
   bool greedy;
   const double scale = scale_of(a, row, greedy);
