@@ -529,9 +529,11 @@ int qmm_adapters_add(int count, const qmm_adapter *adapters, int slots, int w_dt
  * A NaN logit counts as -inf, a logit of -inf is never drawn; a row of nothing
  * else gives -1 (qmm_gather_rows' "no row") and 0. Where a logit is +inf, those
  * alone are drawn, equally. Weights are relative to the largest, in 64 bits; weights
- * below 2^-60 may count as 0 where a setting is on, and those below 2^-1000 do always. A row's token follows from
- * the row, its settings and vocab alone, where the 64-bit sums' last bits do not
- * decide. Plan and launch as qmm_forward (workspace 16-byte aligned): the plan
+ * below 2^-60, or below 2^-62 of the row's total, may count as 0 where a setting is on,
+ * and those below 2^-1000 do always. Where more than 1024 values lie at the border of a run by
+ * weight, the weights that decide it are cut to whole numbers of 2^-62 of the row's total. A row's
+ * token follows from the row, its settings and vocab alone, where the 64-bit sums' last
+ * bits (or that cut) do not decide. Plan and launch as qmm_forward (workspace 16-byte aligned): the plan
  * goes by which settings are given. At most 65535 rows. */
 int qmm_sample(const void *logits, int dtype, int64_t stride, const float *u, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *probs, int64_t vocab,

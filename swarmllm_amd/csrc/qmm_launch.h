@@ -365,6 +365,7 @@ struct SampleState {
   int32_t mode;
   float top, lo;
   int32_t ticket, listed, by_count, above;
+  int32_t bits;   // the unit of whole-number weights: 2^-bits
   double goal;    // the weight or the number of a prefix
   uint64_t last;  // or the rank of its last value
   double scale, floor;

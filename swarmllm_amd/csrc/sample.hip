@@ -163,13 +163,15 @@ __global__ __launch_bounds__(256) void sample_chunks_kernel(SampleArgs a, int ch
 }
 
 // A weight as a whole number of units, 2^-bits of the largest weight each (bits at
-// most 52): the bits of its 53 that are left, cut off.
+// most 62): the bits past them are cut off.
 struct Units {
   int bits;
+  // Of a row whose weights add up to total (1 at least): 2^62 to 2^63 of them, a unit at most 2^-62 of it.
+  static __device__ __forceinline__ Units of(double total) { return Units{62 - ((__double2hiint(total) >> 20) - 1023)}; }
   __device__ __forceinline__ uint64_t operator()(double w) const {
     const uint64_t b = (uint64_t)__double_as_longlong(w);
-    const int shift = min(63, 1023 + 52 - bits - (int)(b >> 52));  // (0 and what is under a unit: all of them)
-    return ((b & 0xFFFFFFFFFFFFFull) | 0x10000000000000ull) >> shift;
+    const int shift = min(63, 1023 + 62 - bits - (int)(b >> 52));  // (0 and what is under a unit: all of them)
+    return ((b << 10 & 0x3FFFFFFFFFFFFC00ull) | 0x4000000000000000ull) >> shift;
   }
   __device__ __forceinline__ double size() const { return __hiloint2double((1023 + bits) << 20, 0); }
 };
@@ -621,9 +623,10 @@ __device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Wei
 }
 
 // The weights of the values that stay, a thread each, added to their chunks:
-// thread c's of chunk c. As whole numbers of 2^-52, so in any order.
-__device__ __forceinline__ double to_chunks(Shared& s, int chunks, bool stays, uint64_t rank, double w) {
-  const Units unit{52};
+// thread c's of chunk c. As whole numbers, so in any order (of 2^-52 at least, of which
+// a chunk's 1024 values add up to 2^62).
+__device__ __forceinline__ double to_chunks(Shared& s, const Units& row_unit, int chunks, bool stays, uint64_t rank, double w) {
+  const Units unit{max(52, row_unit.bits)};
   const int tid = threadIdx.x;
   __syncthreads();
   if (tid < chunks) s.list[tid] = 0;
@@ -745,7 +748,7 @@ __device__ __forceinline__ bool few_past(int k, int groups, float few) {
 }
 
 template <int T, bool VEC>
-__global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, int chunks, int bits) {
+__global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, int chunks) {
   __shared__ Shared s;
   const int tid = threadIdx.x, groups = chunks * kGroups, slice = blockIdx.x;
   const int64_t row = blockIdx.y;
@@ -792,7 +795,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   }
   double total;
   (void)block_sums<kThreads, double>(mass, s.sums, total);
-  const Units unit{bits};
+  const Units unit = Units::of(total);
 
   // no value under `line` is kept (in units of log2 w), nor counts for another's place: under 2^-60 none does
   double line = -60.0;
@@ -824,7 +827,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
     float* const part = a.parts + (row * a.slices + slice) * kBuckets;  // (counts are whole in 32 bits too)
     for (int b = tid; b < kBuckets; b += kThreads) part[b] = (float)s.part[b];
     if (tid == 0 && slice == 0)
-      a.states[row] = SampleState{kHistogram, top, lo, 0, 0, k_on, 0, k_on ? (double)k : fmax(p, 0.0) * total, 0, scale, floor};
+      a.states[row] = SampleState{kHistogram, top, lo, 0, 0, k_on, 0, unit.bits, k_on ? (double)k : fmax(p, 0.0) * total, 0, scale, floor};
     return;
   }
 
@@ -856,7 +859,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   uint64_t last = 0;  // the rank of the last value of the prefix
   if (n > kList) {
     if (!k_on) {  // min_p alone: all the values past its line, which every slice then sums
-      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, 0.0, 0, scale, floor};
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, unit.bits, 0.0, 0, scale, floor};
       return;
     }
     // very many values, or equal ones: narrowed down by this workgroup
@@ -880,7 +883,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
           last = max(last, last_of_prefix<T, VEC>(a, row, s, run, weight, unit, kept_mass, bucket, b, above_count,
                                                   above_mass, inside));
       }
-      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, 0.0, last, scale, floor};
+      if (tid == 0) a.states[row] = SampleState{kLine, top, lo, 0, 0, 0, 0, unit.bits, 0.0, last, scale, floor};
       return;
     }
   }
@@ -898,7 +901,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   const bool stays = tid < n && tid < k && (!p_on || tid == 0 || sum - w < run) && w >= floor;
   const int staying = min(block_least(stays ? INT32_MAX : tid, &s.found), n);  // (they come first)
   if (tid == staying - 1) s.sums64[0] = r;
-  const double kept = to_chunks(s, chunks, stays, r, w);
+  const double kept = to_chunks(s, unit, chunks, stays, r, w);
   draw<kThreads, T>(a, row, weight, Stay{lo, s.sums64[0], floor}, kept, u, chunks, s.sums, &s.found);
 }
 
@@ -906,7 +909,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
 // by the last of the row's workgroups: again a chain of passes, and the 64-bit weights of
 // the values that stay (64 rows of mixed settings 29 us).
 template <int T, bool VEC>
-__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, int chunks, int bits) {
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, int chunks) {
   __shared__ Shared s;
   const int tid = threadIdx.x, groups = chunks * kGroups, slice = blockIdx.x;
   const int64_t row = blockIdx.y;
@@ -920,6 +923,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
   const bool by_count = state->by_count != 0;
   const Weights weight{&s.powers, top, state->scale};
   const Buckets bucket(top, lo);
+  const Units unit{state->bits};
   uint64_t last = state->last;
   int from = kBuckets, to = kBuckets - 1;  // the buckets that hold the border
   if (mode == kHistogram) {
@@ -1036,14 +1040,13 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, i
       sure = (above < goal || above == 0.0) && (above + (by_count ? n : all) >= goal || low <= lo);
       if (sure) {
         if (tid == m - 1) s.sums64[0] = r;
-        mass += to_chunks(s, chunks, in && w >= floor, r, w);
+        mass += to_chunks(s, unit, chunks, in && w >= floor, r, w);
         last = m ? s.sums64[0] : 0;
         __syncthreads();
       }
     }
     if (!sure) {
       // more values than the list holds (equal ones, as a rule): narrowed down by this workgroup
-      const Units unit{bits};
       const Goal exact{by_count, by_count ? (uint64_t)goal : (uint64_t)(goal * unit.size())};
       uint64_t above_count = 0, above_mass = 0, unused = 0;
       uint32_t inside = 0;
@@ -1089,15 +1092,12 @@ int slices_of(int64_t rows, int chunks, int cus) {
 template <int T, bool VEC>
 hipError_t launch_rows(const SampleArgs& a, hipStream_t st) {
   const int chunks = (a.vocab + kChunk - 1) / kChunk;
-  int bits = 63;  // a row's weights add up to less than 2^64 units
-  while (((int64_t)1 << (63 - bits)) < a.vocab) bits--;
-  bits = bits < 52 ? bits : 52;
   sample_chunks_kernel<T, VEC><<<dim3((unsigned)((chunks + 3) / 4), (unsigned)a.rows), 256, 0, st>>>(a, chunks);
   if (!a.states) {
     sample_pick_kernel<T, VEC><<<(unsigned)a.rows, kMostChunks, 0, st>>>(a, chunks);
   } else {
-    sample_select_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
-    sample_finish_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks, bits);
+    sample_select_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks);
+    sample_finish_kernel<T, VEC><<<dim3((unsigned)a.slices, (unsigned)a.rows), kThreads, 0, st>>>(a, chunks);
   }
   return hipGetLastError();
 }
