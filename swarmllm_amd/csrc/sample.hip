@@ -699,14 +699,14 @@ __global__ __launch_bounds__(kMostChunks) void sample_pick_kernel(SampleArgs a, 
   }
 }
 
-// What the settings leave of at most 64 values, the largest first, a lane each: a wave's.
+// What the settings leave of at most 64 values (top_p only beside top_k), the largest first, a lane each: a wave's.
 __device__ __forceinline__ void finish_wave(const SampleArgs& a, int64_t row, const Weights& weight, uint64_t r, int n, int k,
-                                            double p, double goal_of, double floor, double u) {
+                                            double p, double floor, double u) {
   const int lane = threadIdx.x;
   r = ~block_sort(lane < n ? ~r : ~0ull, 64, nullptr);
   double w = lane < n && lane < k ? weight(ranked_value(r)) : 0.0;
   const double sum = wave_sums(w);
-  const double goal = fmax(p, 0.0) * (goal_of > 0.0 ? goal_of : __shfl(sum, 63, 64));
+  const double goal = fmax(p, 0.0) * __shfl(sum, 63, 64);
   const bool stays = lane < n && lane < k && (p >= 1.0 || lane == 0 || sum - w < goal) && w >= floor;
   if (!stays) w = 0.0;
   const uint64_t those = __ballot(stays);
@@ -806,7 +806,6 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
   if ((double)lo > at) lo = value_of(key_of(lo) - 1);
   if (top == INFINITY) lo = top;
   lo = fmaxf(lo, -FLT_MAX);  // -inf is never drawn
-  const Goal goal{k_on, k_on ? (uint64_t)k : (uint64_t)(fmax(p, 0.0) * total * unit.size())};
 
   if (wide) {
     // the slice's part of the histogram: counts, or weights in 32 bits (they say where
@@ -864,6 +863,7 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
     }
     // very many values, or equal ones: narrowed down by this workgroup
     const Buckets bucket(top, lo);
+    const Goal goal{true, (uint64_t)k};
     uint64_t above_count = 0, above_mass = 0, kept_mass = 0;
     uint32_t inside = 0;
     int b = narrow<T, VEC>(a, row, s, goal, true, weight, unit, above_count, above_mass, inside, bucket);
@@ -887,17 +887,16 @@ __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a, i
       return;
     }
   }
-  // every value that can stay
-  const double goal_of = k_on ? 0.0 : total;
+  // every value that can stay (by top_p beside top_k only: the others by it are wide)
   if (n <= 64) {
-    if (tid < 64) finish_wave(a, row, weight, tid < n ? s.list[tid] : 0, n, k, p, goal_of, floor, u);
+    if (tid < 64) finish_wave(a, row, weight, tid < n ? s.list[tid] : 0, n, k, p, floor, u);
     return;
   }
   const uint64_t r = ~block_sort(tid < n ? ~s.list[tid] : ~0ull, sort_size(n), s.list);
   const double w = tid < n && tid < k ? weight(ranked_value(r)) : 0.0;
   double all;
   const double sum = block_sums<kThreads, double>(w, s.sums, all);
-  const double run = fmax(p, 0.0) * (k_on ? all : total);
+  const double run = fmax(p, 0.0) * all;
   const bool stays = tid < n && tid < k && (!p_on || tid == 0 || sum - w < run) && w >= floor;
   const int staying = min(block_least(stays ? INT32_MAX : tid, &s.found), n);  // (they come first)
   if (tid == staying - 1) s.sums64[0] = r;
