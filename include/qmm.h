@@ -491,8 +491,9 @@ int qmm_pages_step(const qmm_pages *pages, const int32_t *keep, const int32_t *f
  * has zeros); scales [slots] f32 (NULL: 1); y and out f32. out may be y itself
  * (the same pointer and stride); otherwise nothing overlaps. two projections have
  * two outs. Values of x and of the adapters enter as they are, sums are f32
- * (products of many rows leave out parts under 2^-24 of each; an infinite value
- * makes its row's results infinite or NaN). In which order the sums are taken,
+ * (in many rows a product of two f32 values may leave out parts under 2^-23 of it, one of
+ * an f16 and an f32 value parts under 2^-24, the products with b taking f32 values; an infinite
+ * value makes its row's results infinite or NaN). In which order the sums are taken,
  * and so a row's last bits, follows from rows, k, count and the projections' n
  * and ranks; a batch's bits are the same each time. An adapter's values reach
  * its own rows only. Plan (launch == 0) and launch as qmm_forward: the workspace

@@ -62,26 +62,47 @@ struct Raw {
   }
 };
 
-// A value as a sum of bf16 ones, each the leading 8 bits of what those before it
-// leave: 1 for a bf16 value, 2 for f16, 3 for f32, and nothing left.
+// A value as a sum of bf16 ones, and nothing left: 1 for a bf16 value, 2 for f16, 3
+// for f32. The first is the nearest, so that what it leaves has no sign of its
+// own: of a value of 2^e at least and under 2^(e+1) 2^(e-8) at most, of which the second leaves
+// the third under 2^(e-16). (With the first cut off, the products that are left out reach
+// 2^-21 of a product, all of one sign.) The second of three is cut off, not rounded:
+// it cannot carry a sum of the two past the value, f32's largest among them.
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef float f2v __attribute__((ext_vector_type(2)));
 template <int T>
 constexpr int kPieces = T == QMM_X_BF16 ? 1 : T == QMM_X_F16 ? 2 : 3;
-// the upper halves of a and b, side by side
+// the nearest of a and b, side by side (one instruction)
+__device__ __forceinline__ uint32_t nearest(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v{a, b}), b2v));
+}
+// their upper halves
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) {
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 template <int N>
 __device__ __forceinline__ void pieces_of(float v[8], b8v out[N]) {
+  constexpr float kMost = 0x1.fep127f;  // the largest bf16 value: f32 ones past it would round to infinity
 #pragma unroll
   for (int p = 0; p < N; p++) {
     uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) w[e] = upper_halves(v[2 * e], v[2 * e + 1]);
+    for (int e = 0; e < 4; e++) {
+      float a = v[2 * e], b = v[2 * e + 1];
+      if (N == 3 && p == 0) {
+        a = __builtin_amdgcn_fmed3f(a, -kMost, kMost);
+        b = __builtin_amdgcn_fmed3f(b, -kMost, kMost);
+      }
+      w[e] = N == 3 && p == 1 ? upper_halves(a, b) : nearest(a, b);
+    }
     out[p] = __builtin_bit_cast(b8v, make_uint4(w[0], w[1], w[2], w[3]));
     if (p + 1 < N) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+      for (int e = 0; e < 4; e++) {
+        v[2 * e] -= __uint_as_float(w[e] << 16);
+        v[2 * e + 1] -= __uint_as_float(w[e] & 0xFFFF0000u);
+      }
     }
   }
 }
@@ -369,7 +390,9 @@ __global__ __launch_bounds__(64 * down_waves(RT, WT)) void lora_down_kernel(Lora
 #pragma unroll
     for (int i = 0; i < WI; i++) w[b][i] = load16<WT, true>(t.a, arow[i] + 32 * s);
   };
-  // products of pieces down to 2^-16 of the first (the next are under f32's half step)
+  // products of pieces down to 2^-16 of the first; of the next ones two f32 values have two,
+  // f16 and f32 one, under 2^-24 of the product each. The larger ones first: in an
+  // instruction a product's low bits are lost where larger ones stand beside it
   auto multiply = [&](int b) {
 #pragma unroll
     for (int i = 0; i < I; i++) s_x[64 / C * i + lane / C][lane % C] = x[b][i];
@@ -392,14 +415,16 @@ __global__ __launch_bounds__(64 * down_waves(RT, WT)) void lora_down_kernel(Lora
       b8v wp[kPieces<WT>];
       pieces_of<WT>(r, wp);
 #pragma unroll
-      for (int p = 0; p < kPieces<WT>; p++)
+      for (int d = 0; d < 3; d++)
 #pragma unroll
-        for (int q = 0; q < kPieces<XT>; q++)
-          if (p + q < 3) {
+        for (int p = 0; p < kPieces<WT>; p++) {
+          const int q = d - p;
+          if (q >= 0 && q < kPieces<XT>) {
 #pragma unroll
             for (int h = 0; h < 2; h++)
               acc[h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[p], xp[h][q], acc[h][i], 0, 0, 0);
           }
+        }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -530,14 +555,16 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs a, int 
         b8v wp[kPieces<WT>];
         pieces_of<WT>(w[c][s], wp);
 #pragma unroll
-        for (int p = 0; p < kPieces<WT>; p++)
+        for (int d = 0; d < 3; d++)
 #pragma unroll
-          for (int q = 0; q < MP; q++)
-            if (p + q < 3) {
+          for (int p = 0; p < kPieces<WT>; p++) {
+            const int q = d - p;
+            if (q >= 0 && q < MP) {
 #pragma unroll
               for (int h = 0; h < 2; h++)
                 acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wp[p], m[h][s][q], acc[h], 0, 0, 0);
             }
+          }
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) *(f4v*)&s_sum[16 * h + col][16 * (kUpTiles * wave + c) + 4 * g] = acc[h];
