@@ -489,8 +489,9 @@ int qmm_pages_step(const qmm_pages *pages, const int32_t *keep, const int32_t *f
  * 32); a [slots][rank][k] and b [slots][n][rank] of w_dtype (qmm_x_dtype), each
  * 16-byte aligned, rank a multiple of 8 up to 128 (an adapter of a lower rank
  * has zeros); scales [slots] f32 (NULL: 1); y and out f32. out may be y itself
- * (the same pointer and stride); otherwise nothing overlaps. two projections have
- * two outs. Values of x and of the adapters enter as they are, sums are f32
+ * (the same pointer and stride); otherwise an out shares no byte with anything else that
+ * the call takes (rows between its rows share none), nor does the workspace: the launch
+ * refuses that as QMM_UNSUPPORTED. Values of x and of the adapters enter as they are, sums are f32
  * (in many rows a product of two f32 values may leave out parts under 2^-23 of it, one of
  * an f16 and an f32 value parts under 2^-24, the products with b taking f32 values; an infinite
  * value makes its row's results infinite or NaN). In which order the sums are taken,

@@ -68,6 +68,65 @@ bool shape_ok(int type, int64_t k, int64_t n, int64_t rows) {
 // As the planes of an activation or a cache, or partial results, have to lie.
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// Rows of `width` bytes, `stride` (at least that) apart.
+typedef __int128 wide;  // (a stride can be any number)
+struct Region {
+  const void* at;
+  int64_t rows, width;
+  wide stride;
+};
+
+// Whether two of them have a byte in common (rows between the other's rows have none).
+bool overlap(const Region& a, const Region& b) {
+  if (!a.at || !b.at || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+  const wide pa = (uintptr_t)a.at, pb = (uintptr_t)b.at;
+  if (pa + (wide)(a.rows - 1) * a.stride + a.width <= pb || pb + (wide)(b.rows - 1) * b.stride + b.width <= pa) return false;
+  if (a.rows > b.rows) return overlap(b, a);
+  auto floor_div = [](wide n, wide d) { return n / d - (n % d < 0 ? 1 : 0); };
+  if (a.rows == 1 || a.stride == b.stride) {
+    // b's row j lies pb - pa + m stride behind a's row i, m = j - i: the least m at which it ends behind its start
+    const wide first = floor_div(pa - pb - b.width, b.stride) + 1, least = 1 - (wide)a.rows, m = first > least ? first : least;
+    return m < b.rows && pb - pa + m * b.stride < a.width;
+  }
+  for (wide i = 0; i < a.rows; i++) {
+    const wide at = pa + i * a.stride, first = floor_div(at - pb - b.width, b.stride) + 1, j = first > 0 ? first : 0;
+    if (j < b.rows && pb + j * b.stride < at + a.width) return true;
+  }
+  return false;
+}
+
+// Whether an output (or the workspace) shares memory with an array that the call reads or writes, but for an
+// output in its own y's place.
+bool adapters_overlap(const qmm::LoraArgs& a, int x_dtype, int w_dtype, const void* workspace, size_t bytes) {
+  const int64_t wb = qmm::value_bytes(w_dtype), slots = a.slots;
+  auto whole = [](const void* p, int64_t n) { return Region{p, 1, n, n}; };
+  auto rows = [&](const void* p, int64_t n, int64_t stride, int64_t size) { return Region{p, a.rows, n * size, (wide)stride * size}; };
+  Region read[2 + 3 * qmm::kMaxTargets], out[qmm::kMaxTargets];
+  int n = 0;
+  read[n++] = rows(a.x, a.k, a.xs, qmm::value_bytes(x_dtype));
+  read[n++] = whole(a.ids, 4 * a.rows);
+  for (int i = 0; i < a.count; i++) {
+    const qmm::LoraTarget& t = a.t[i];
+    out[i] = rows(t.out, t.n, t.ldo, 4);
+    read[n++] = whole(t.a, slots * t.rank * a.k * wb);
+    read[n++] = whole(t.b, slots * t.n * t.rank * wb);
+    read[n++] = whole(t.scales, 4 * slots);
+  }
+  const Region ws = whole(workspace, (int64_t)bytes);
+  for (int i = 0; i < n; i++) {
+    if (overlap(ws, read[i])) return true;
+    for (int j = 0; j < a.count; j++)
+      if (overlap(out[j], read[i])) return true;
+  }
+  for (int i = 0; i < a.count; i++) {
+    const Region y = rows(a.t[i].y, a.t[i].n, a.t[i].ldy, 4);
+    if (overlap(ws, out[i]) || overlap(ws, y)) return true;
+    for (int j = 0; j < a.count; j++)
+      if ((i < j && overlap(out[i], out[j])) || ((i != j || a.t[i].y != a.t[i].out) && overlap(y, out[j]))) return true;
+  }
+  return false;
+}
+
 // A paged cache's sizes: pages of 16 to 256 positions (a power of two), heads
 // of a dim the attention kernels are built for, planes inside an int64.
 bool cache_shape_ok(int64_t pages, int kv_heads, int head_dim, int page) {
@@ -1169,6 +1228,7 @@ int qmm_adapters_add(int count, const qmm_adapter* adapters, int slots, int w_dt
   for (int i = 0; i < count; i++)
     if (!a.t[i].y || !a.t[i].out || (slots > 0 && (!a.t[i].a || !a.t[i].b))) return QMM_UNSUPPORTED;
   if (*need > 0 && (workspace == nullptr || workspace_bytes < *need)) return QMM_WORKSPACE_TOO_SMALL;
+  if (adapters_overlap(a, x_dtype, w_dtype, workspace, *need)) return QMM_UNSUPPORTED;
   clear_stale_error();
   return status_of(qmm::launch_lora(a, x_dtype, w_dtype, (hipStream_t)stream));
 }

@@ -9,7 +9,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import QMM_OK, Adapter, check, lib
+from ._lib import QMM_OK, QMM_UNSUPPORTED, Adapter, check, lib
 from .qtensor import _X_DTYPES, on_device, raw_stream
 
 _MOST = 4  # projections a call
@@ -48,8 +48,9 @@ class Adapters:
         """out = y + scales[i] * (x a[i]^T) b[i]^T row by row, i = ids[row]; a row
         whose id is outside [0, slots) is y's. y [..., n] f32 is the projection's
         product of x [..., k] (f32, f16 or bf16), ids int32 one a row; out: by
-        default y itself, which is added to; it shares memory with nothing else.
-        The products are of x's and the adapters' own values, with f32 sums."""
+        default y itself, which is added to; otherwise it shares no memory with
+        what the call reads (other columns of one wide array share none). The
+        products are of x's and the adapters' own values, with f32 sums."""
         return Adapters.add_shared([y], x, [self], ids, None if out is None else [out])[0]
 
     @staticmethod
@@ -92,10 +93,10 @@ class Adapters:
             status = lib().qmm_adapters_add(
                 count, c, first.slots, _X_DTYPES[first.dtype], x.data_ptr(), x_type, xs, ids.data_ptr(), k, rows,
                 None if ws is None else ws.data_ptr(), need, ctypes.byref(size), 1, raw_stream(device))
-        if status != QMM_OK:  # (the arrays' places are the library's to check: a call is host time)
-            if any(c[i].out in (x.data_ptr(), *(p for j in range(count) if i != j for p in (c[j].out, c[j].y)))
-                   for i in range(count)):
-                raise ValueError("Adapters.add: an out that is x, or another projection's out or y")
+        if status == QMM_UNSUPPORTED:  # (the arrays' places are the library's to check: a call is host time)
+            raise ValueError("Adapters.add: an out that shares memory with x, ids, an adapter, another projection's y or "
+                             "out, or with its own y without being it")
+        if status != QMM_OK:
             check("qmm_adapters_add", status)
         return outs
 
