@@ -603,6 +603,9 @@ int64_t tiles_of(const LoraArgs& a) {
 //     64 rows, rank 64, 4096 to 2 x 14336    151M         44 / 28     80 / 81
 //     128 rows, rank 64, 4096 to 2 x 14336   302M         77 / 32     144 / 106
 //     512 rows, rank 64, 8192 to 8192        537M         110 / 36    165 / 80
+// Where the line lies is a choice between the two columns: with many adapters it
+// would lie higher (256 rows of 64 adapters lose some 25 us past it), with one lower. The
+// table is of bf16 adapters, and so are its bytes: f32 ones read twice as many.
 //
 // Of rows one by one, the small ones in one launch: every workgroup of a row makes
 // the row's products with A for itself, which a second launch would hand it. That
